@@ -228,6 +228,110 @@ lgx_status lgx_gqa_prefill_attn_fast(lgx_ctx* ctx, const float* q, const uint16_
                                      int32_t hkv, int32_t d, int32_t maxp, int32_t num_pages,
                                      int32_t max_seq_len, float* out, void* stream);
 
+/* ---- 8-bit KV cache ----
+ * A paged cache of int8 quants with one binary32 scale for each block of 16
+ * tokens (a page) and KV head: value = scale * quant.  K pages are
+ * [num_pages][hkv][16][d] (token by token), V pages [num_pages][hkv][d][16]
+ * (dimension by dimension: the order in which the attention reads them), both
+ * 16-byte aligned; the scales are [num_pages][hkv].  d is 64 or 128.  Half the
+ * memory and half the traffic of the binary16 cache.  No counterpart in the
+ * reference, which has no attention. */
+typedef struct lgx_kv_i8 {
+    int8_t* k;
+    int8_t* v;
+    float* k_scale;
+    float* v_scale;
+    int32_t num_pages, hkv, d;
+} lgx_kv_i8;
+
+/* Rotation of query and key heads: the first `rot` dimensions (even, 0..d) in
+ * pairs, (i, i + rot/2), or (2i, 2i + 1) when interleaved; pair i of position p
+ * turns by the angle whose cosine and sine stand at [p][i] of the tables (device
+ * memory, [max_pos][rot/2]; NULL with rot 0).  Positions at or past max_pos use the
+ * last row. */
+typedef struct lgx_rope {
+    const float* cos_t;
+    const float* sin_t;
+    int32_t rot, interleaved, max_pos;
+} lgx_rope;
+
+/* Scaled positions for contexts longer than a model was trained on.
+ * LGX_ROPE_LINEAR: every angle divided by `factor`.  LGX_ROPE_BASE: theta times
+ * factor^(rot / (rot - 2)), so that the slowest pair turns `factor` times slower
+ * and the fastest as before.  LGX_ROPE_PARTS: a pair that makes t turns over
+ * original_len positions keeps its angle from t = fast on, has it divided by
+ * `factor` up to t = slow, and a mixture linear in t between them; cosines and
+ * sines are multiplied by 0.1 ln(factor) + 1. */
+enum { LGX_ROPE_PLAIN = 0, LGX_ROPE_LINEAR = 1, LGX_ROPE_BASE = 2, LGX_ROPE_PARTS = 3 };
+typedef struct lgx_rope_scaling {
+    int32_t kind;
+    int32_t original_len; /* LGX_ROPE_PARTS */
+    double factor;        /* >= 1 */
+    double slow, fast;    /* LGX_ROPE_PARTS, 0 <= slow < fast (1 and 32 as published) */
+} lgx_rope_scaling;
+/* cos_t / sin_t (host memory, [max_pos][rot/2]) of the angles p * theta^(-2i /
+ * rot), in binary64, rounded once.  scaling NULL: plain. */
+lgx_status lgx_rope_tables(int32_t max_pos, int32_t rot, double theta, const lgx_rope_scaling* scaling,
+                           float* cos_t, float* sin_t);
+
+/* Appends up to P rows to each of B sequences.  Row b*P + j of qkv
+ * ([B*P][(hq + 2 hkv) d]: q heads | k heads | v heads), plus bias (nullable), is
+ * token seq_len[b] + j; rows j >= n_new[b] (device int32 [B], nullable: P) are
+ * padding, and nothing is read or written for them.  q and k heads are rotated;
+ * q goes to q_out [B*P][hq][d]; k and v are quantised into slot t % 16 of page
+ * page_table[b][t / 16].  Everything between the inputs and the rounded results is
+ * computed in binary64.  For each block touched, with a the largest magnitude of
+ * its new values (0 if below 2^-119: scales are normal numbers):
+ *   a new block (its slot 0 is among the new tokens): scale = a / 127 (binary32);
+ *   one that holds tokens: its scale stays while it is >= a / 127, else it is
+ *   doubled until it is, and the old quants are halved as often (one rounding,
+ *   halves away from zero); a scale of 0 becomes a / 127;
+ *   quant = the nearest integer to value / scale, halves away from zero, within
+ *   +-127; a new value that is infinite or NaN makes the block's scale NaN until
+ *   the block is begun again (so attention to it gives NaN, not a wrong number).
+ * An old value is therefore never off by more than one step of its block's scale.
+ * Slots not appended to keep their quants.  seq_len is not advanced; lengths are
+ * clamped to [0, 16 maxp]; tokens past 16 maxp and pages outside [0, num_pages)
+ * are not written.  A page may belong to several sequences while none of them
+ * appends to it; two sequences that append to one page in a call race. */
+lgx_status lgx_rope_kv_append_i8(lgx_ctx* ctx, const float* qkv, const float* bias, const lgx_rope* rope,
+                                 const int32_t* seq_len, const int32_t* n_new, const int32_t* page_table,
+                                 const lgx_kv_i8* kv, float* q_out, int32_t B, int32_t P, int32_t hq,
+                                 int32_t maxp, void* stream);
+/* k_out / v_out [B][n][hkv][d] = the values of tokens start[b] .. + n of every
+ * sequence; zeros past 16 maxp.  start is clamped to [0, 16 maxp], page ids to
+ * [0, num_pages). */
+lgx_status lgx_kv_read_i8(lgx_ctx* ctx, const lgx_kv_i8* kv, const int32_t* page_table, const int32_t* start,
+                          int32_t B, int32_t n, int32_t maxp, float* k_out, float* v_out, void* stream);
+
+/* Options of the attention calls below (NULL: none).  The score of a query at
+ * position p and a key at t is
+ *   s = scale * q.k (scale 0: 1/sqrt(d));  s = softcap * tanh(s / softcap) if
+ *   softcap > 0;  s -= slopes[h] * (p - t) if slopes (device binary32 [hq]);
+ * with window > 0 only the last `window` tokens up to and with p are seen. */
+typedef struct lgx_attn_opts {
+    float scale, softcap;
+    int32_t window;
+    const float* slopes;
+} lgx_attn_opts;
+/* lgx_gqa_decode_attn over the 8-bit cache: out[b][h] over the first seq_len[b]
+ * tokens of sequence b (the query is at position seq_len[b] - 1), lengths clamped
+ * to [0, max_seq_len], page ids to [0, num_pages); seq_len 0 gives zeros.
+ * hq/hkv in 1..16.  Not the canonical schedule: scores from int8 products with q
+ * in 24 bits, weights in 22 bits, binary32 sums (about 1e-6 of the 64-bit result
+ * over the cache's values); the same inputs give the same bits.  Partial results
+ * of long contexts live in the ctx workspace. */
+lgx_status lgx_gqa_decode_attn_i8(lgx_ctx* ctx, const float* q, const lgx_kv_i8* kv, const int32_t* page_table,
+                                  const int32_t* seq_len, int32_t B, int32_t hq, int32_t maxp,
+                                  int32_t max_seq_len, const lgx_attn_opts* opts, float* out, void* stream);
+/* The same for P causal rows per sequence, as lgx_gqa_prefill_attn: row b*P + j is
+ * the query at position seq_len[b] + j, its K and V already cached.  Rows j >=
+ * n_new[b] (nullable: P) are padding: their rows of out are left as they are. */
+lgx_status lgx_gqa_prefill_attn_i8(lgx_ctx* ctx, const float* q, const lgx_kv_i8* kv, const int32_t* page_table,
+                                   const int32_t* seq_len, const int32_t* n_new, int32_t B, int32_t P,
+                                   int32_t hq, int32_t maxp, int32_t max_seq_len, const lgx_attn_opts* opts,
+                                   float* out, void* stream);
+
 /* ---- range partials (for consumers that fuse the range tree) ---- */
 /* Number of canonical 32-block ranges of K = the partial count of a product. */
 int32_t lgx_q8_range_count(int32_t k);

@@ -98,6 +98,11 @@ SIGNATURES = {
     "lgx_qwen_generate": (C.c_int, [_P, _I32, _P, _I32, _P, _P]),
     "lgx_model_tensor": (C.c_int, [_P, _I32, _I32, C.POINTER(_P), C.POINTER(C.c_size_t)]),
     "lgx_qwen_logits": (C.c_int, [_P, _I32, _P, _P]),
+    "lgx_rope_tables": (C.c_int, [_I32, _I32, C.c_double, _P, _P, _P]),
+    "lgx_rope_kv_append_i8": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _P]),
+    "lgx_kv_read_i8": (C.c_int, [_P, _P, _P, _P, _I32, _I32, _I32, _P, _P, _P]),
+    "lgx_gqa_decode_attn_i8": (C.c_int, [_P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _P, _P, _P]),
+    "lgx_gqa_prefill_attn_i8": (C.c_int, [_P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _P]),
 }
 
 # Model shapes of the decode benchmarks (random-init Qwen2.5-0.5B / -7B shaped
@@ -219,6 +224,28 @@ class QwenConfigC(C.Structure):
                 ("rms_eps", C.c_float), ("rope_theta", C.c_double), ("emb_sigma", C.c_double)]
 
 
+class KvI8C(C.Structure):
+    """lgx_kv_i8."""
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("num_pages", _I32),
+                ("hkv", _I32), ("d", _I32)]
+
+
+class RopeC(C.Structure):
+    """lgx_rope."""
+    _fields_ = [("cos_t", _P), ("sin_t", _P), ("rot", _I32), ("interleaved", _I32), ("max_pos", _I32)]
+
+
+class RopeScalingC(C.Structure):
+    """lgx_rope_scaling."""
+    _fields_ = [("kind", _I32), ("original_len", _I32), ("factor", C.c_double), ("slow", C.c_double),
+                ("fast", C.c_double)]
+
+
+class AttnOptsC(C.Structure):
+    """lgx_attn_opts."""
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("window", _I32), ("slopes", _P)]
+
+
 _lib = None
 
 
@@ -270,6 +297,83 @@ class Q8Matrix:
     @property
     def nbytes(self) -> int:
         return self.qs.numel() + 2 * self.d.numel()
+
+
+def _tensor(name, x, dtype: str, shape):
+    """x, refused unless it is a contiguous device tensor of that type and shape
+    (None: any extent)."""
+    if str(x.dtype) != "torch." + dtype or not x.is_contiguous() or not x.is_cuda:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor on the device")
+    if len(x.shape) != len(shape) or any(w is not None and w != n for w, n in zip(shape, x.shape)):
+        raise ValueError(f"{name} has shape {tuple(x.shape)}, expected {tuple(shape)}")
+    return x
+
+
+class KvCacheI8:
+    """An 8-bit paged KV cache (lgx_kv_i8): int8 K pages [pages][hkv][16][d] and V
+    pages [pages][hkv][d][16], float32 scales [pages][hkv] for each."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        n, hkv, _, d = k.shape
+        _tensor("k", k, "int8", (n, hkv, 16, d))
+        _tensor("v", v, "int8", (n, hkv, d, 16))
+        _tensor("k_scale", k_scale, "float32", (n, hkv))
+        _tensor("v_scale", v_scale, "float32", (n, hkv))
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.num_pages, self.hkv, self.d, self.device = n, hkv, d, k.device
+        self._c = KvI8C(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, hkv, d)
+        self.cstruct = C.byref(self._c)
+
+    @classmethod
+    def empty(cls, ctx: "Context", num_pages: int, hkv: int, d: int) -> "KvCacheI8":
+        """A cache of zeros on ctx's device."""
+        t = ctx.torch
+        return cls(t.zeros((num_pages, hkv, 16, d), dtype=t.int8, device=ctx.dev),
+                   t.zeros((num_pages, hkv, d, 16), dtype=t.int8, device=ctx.dev),
+                   t.zeros((num_pages, hkv), dtype=t.float32, device=ctx.dev),
+                   t.zeros((num_pages, hkv), dtype=t.float32, device=ctx.dev))
+
+
+class Rope:
+    """Rotation of query and key heads (lgx_rope): cos / sin are float32 device
+    tensors [positions][rot / 2], the first rot dimensions of a head are turned in
+    pairs (i, i + rot / 2), or (2i, 2i + 1) when interleaved."""
+
+    def __init__(self, cos, sin, interleaved: bool = False):
+        n, half = cos.shape
+        _tensor("cos", cos, "float32", (n, half))
+        _tensor("sin", sin, "float32", (n, half))
+        self.cos, self.sin = cos, sin
+        self._c = RopeC(cos.data_ptr(), sin.data_ptr(), 2 * half, int(interleaved), n)
+        self.cstruct = C.byref(self._c)
+
+    @classmethod
+    def tables(cls, ctx: "Context", max_pos: int, rot: int, theta: float = 1e6, interleaved: bool = False,
+               scaling: str = "plain", factor: float = 1.0, original_len: int = 0, slow: float = 1.0,
+               fast: float = 32.0) -> "Rope":
+        """Tables of lgx_rope_tables on ctx's device; scaling: "plain", "linear",
+        "base" or "parts"."""
+        t = ctx.torch
+        kinds = ("plain", "linear", "base", "parts")
+        if scaling not in kinds:
+            raise ValueError(f"scaling {scaling!r} is none of {kinds}")
+        sc = RopeScalingC(kinds.index(scaling), original_len, factor, slow, fast)
+        shape = (max(max_pos, 0), max(rot, 0) // 2)
+        cos, sin = t.empty(shape, dtype=t.float32), t.empty(shape, dtype=t.float32)
+        _check(lib().lgx_rope_tables(max_pos, rot, theta, C.byref(sc), cos.data_ptr(), sin.data_ptr()))
+        return cls(cos.to(ctx.dev), sin.to(ctx.dev), interleaved)
+
+
+class AttnOpts:
+    """Options of the 8-bit cache's attention (lgx_attn_opts): scale 0 is
+    1 / sqrt(d); softcap 0 and window 0 are none; slopes: float32 [hq]."""
+
+    def __init__(self, scale: float = 0.0, softcap: float = 0.0, window: int = 0, slopes=None):
+        if slopes is not None:
+            _tensor("slopes", slopes, "float32", (None,))
+        self.slopes = slopes
+        self._c = AttnOptsC(scale, softcap, window, _ptr_or_none(slopes))
+        self.cstruct = C.byref(self._c)
 
 
 class Context:
@@ -488,6 +592,85 @@ class Context:
                   page_table.data_ptr(), seq_len.data_ptr(), B, P, hq, hkv, d, maxp, num_pages,
                   max_seq_len, out.data_ptr(), self._s()))
         return out
+
+    # ---- 8-bit KV cache --------------------------------------------------
+    def rope_kv_append_i8(self, qkv, bias, rope: Rope, seq_len, page_table, kv: KvCacheI8, P: int = 1,
+                          n_new=None, q_out=None):
+        """Rotates and appends rows [B*P][(hq + 2 hkv) d] (row b*P + j: token
+        seq_len[b] + j, j < n_new[b]) to the cache; returns the rotated queries
+        [B*P][hq][d]."""
+        t = self.torch
+        B, maxp = page_table.shape
+        d, hkv = kv.d, kv.hkv
+        rows, width = qkv.shape
+        hq = width // d - 2 * hkv
+        if rows != B * P or hq < 1 or width % d:
+            raise ValueError(f"qkv {tuple(qkv.shape)} is not [{B * P}][(hq + {2 * hkv}) * {d}]")
+        _tensor("qkv", qkv, "float32", (rows, width))
+        if bias is not None:
+            _tensor("bias", bias, "float32", (width,))
+        self._lengths(seq_len, n_new, page_table, kv, B)
+        q_out = t.empty((rows, hq, d), dtype=t.float32, device=self.dev) if q_out is None else \
+            _tensor("q_out", q_out, "float32", (rows, hq, d))
+        _check(lib().lgx_rope_kv_append_i8(
+            self.handle, qkv.data_ptr(), _ptr_or_none(bias), rope.cstruct, seq_len.data_ptr(),
+            _ptr_or_none(n_new), page_table.data_ptr(), kv.cstruct, q_out.data_ptr(), B, P, hq, maxp, self._s()))
+        return q_out
+
+    def kv_read_i8(self, kv: KvCacheI8, page_table, start, n: int, k_out=None, v_out=None):
+        """(K, V) of tokens start[b] .. + n of every sequence, float32 [B][n][hkv][d]."""
+        t = self.torch
+        B, maxp = page_table.shape
+        self._lengths(start, None, page_table, kv, B)
+        shape = (B, n, kv.hkv, kv.d)
+        k_out = t.empty(shape, dtype=t.float32, device=self.dev) if k_out is None else \
+            _tensor("k_out", k_out, "float32", shape)
+        v_out = t.empty(shape, dtype=t.float32, device=self.dev) if v_out is None else \
+            _tensor("v_out", v_out, "float32", shape)
+        _check(lib().lgx_kv_read_i8(self.handle, kv.cstruct, page_table.data_ptr(), start.data_ptr(), B, n, maxp,
+                                    k_out.data_ptr(), v_out.data_ptr(), self._s()))
+        return k_out, v_out
+
+    def _lengths(self, seq_len, n_new, page_table, kv, B):
+        if kv.device != self.dev:
+            raise ValueError(f"the cache is on {kv.device}, the context on {self.dev}")
+        _tensor("page_table", page_table, "int32", (B, None))
+        _tensor("lengths", seq_len, "int32", (B,))
+        if n_new is not None:
+            _tensor("n_new", n_new, "int32", (B,))
+
+    def gqa_decode_attn_i8(self, q, kv: KvCacheI8, page_table, seq_len, max_seq_len: int, opts: AttnOpts = None,
+                           out=None):
+        """q [B][hq][d] over the first seq_len[b] tokens of the 8-bit cache."""
+        B, hq = q.shape[0], q.shape[1]
+        _tensor("q", q, "float32", (B, None, kv.d))
+        self._lengths(seq_len, None, page_table, kv, B)
+        out = self._attn_out(q, opts, out)
+        _check(lib().lgx_gqa_decode_attn_i8(
+            self.handle, q.data_ptr(), kv.cstruct, page_table.data_ptr(), seq_len.data_ptr(), B, hq,
+            page_table.shape[1], max_seq_len, opts.cstruct if opts is not None else None, out.data_ptr(), self._s()))
+        return out
+
+    def gqa_prefill_attn_i8(self, q, kv: KvCacheI8, page_table, seq_len, P: int, max_seq_len: int, n_new=None,
+                            opts: AttnOpts = None, out=None):
+        """q [B*P][hq][d]: row b*P + j (j < n_new[b]) is the query at position
+        seq_len[b] + j, causal over the 8-bit cache."""
+        B, hq = page_table.shape[0], q.shape[1]
+        _tensor("q", q, "float32", (B * P, None, kv.d))
+        self._lengths(seq_len, n_new, page_table, kv, B)
+        out = self._attn_out(q, opts, out)
+        _check(lib().lgx_gqa_prefill_attn_i8(
+            self.handle, q.data_ptr(), kv.cstruct, page_table.data_ptr(), seq_len.data_ptr(), _ptr_or_none(n_new),
+            B, P, hq, page_table.shape[1], max_seq_len, opts.cstruct if opts is not None else None, out.data_ptr(),
+            self._s()))
+        return out
+
+    def _attn_out(self, q, opts, out):
+        if opts is not None and opts.slopes is not None and opts.slopes.numel() != q.shape[1]:
+            raise ValueError(f"{opts.slopes.numel()} slopes for {q.shape[1]} query heads")
+        if out is None:
+            return self.torch.empty_like(q)
+        return _tensor("out", out, "float32", q.shape)
 
     def q8_gemm(self, W: Q8Matrix, xq, xd, y=None):
         t = self.torch

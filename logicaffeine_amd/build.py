@@ -49,7 +49,7 @@ def build_kernels() -> str:
 
 
 HOST_SOURCES = ["lgx_host.cpp", "lgx_glue.cpp", "lgx_model.cpp", "lgx_gen.cpp", "lgx_gguf.cpp",
-                "lgx_f16gemm.cpp"]
+                "lgx_f16gemm.cpp", "lgx_kv8.cpp"]
 BUILD_DIR = os.path.join(HERE, "_build")
 
 

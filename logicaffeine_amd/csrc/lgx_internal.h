@@ -169,6 +169,14 @@ enum Kern {
     K_NORM_QKV_D64,
     K_NORM_QKV_D128,
     K_GEMM_GRPM16,
+    K_KV8_APPEND_D64,
+    K_KV8_APPEND_D128,
+    K_KV8_READ_D64,
+    K_KV8_READ_D128,
+    K_ATTN8_D64,     // 16 columns; + 1: with caps, distances or a window; + 2: 128 columns
+    K_ATTN8_D128 = K_ATTN8_D64 + 4,
+    K_ATTN8_MERGE_D64 = K_ATTN8_D128 + 4,
+    K_ATTN8_MERGE_D128,
     K_COUNT
 };
 inline const char* const kKernelNames[] = {
@@ -217,6 +225,10 @@ inline const char* const kKernelNames[] = {
     "lgx_k_attn_prefill_fast_d128_g7", "lgx_k_attn_prefill_fast_d128_g8",
     "lgx_k_attn_merge_o_d64", "lgx_k_attn_merge_o_d128", "lgx_k_norm_qkv_d64", "lgx_k_norm_qkv_d128",
     "lgx_k_q8_gemm_grpm16",
+    "lgx_k_kv8_append_d64", "lgx_k_kv8_append_d128", "lgx_k_kv8_read_d64", "lgx_k_kv8_read_d128",
+    "lgx_k_attn8_d64_c16", "lgx_k_attn8x_d64_c16", "lgx_k_attn8_d64_c128", "lgx_k_attn8x_d64_c128",
+    "lgx_k_attn8_d128_c16", "lgx_k_attn8x_d128_c16", "lgx_k_attn8_d128_c128", "lgx_k_attn8x_d128_c128",
+    "lgx_k_attn8_merge_d64", "lgx_k_attn8_merge_d128",
 };
 
 static_assert(sizeof(kKernelNames) / sizeof(kKernelNames[0]) == K_COUNT,

@@ -423,3 +423,56 @@ typedef struct {
     int8_t* dst;
     int32_t rows, k;
 } lgx_act_t16_args;
+
+// ---- 8-bit KV cache (lgx_kv8.hip) ----
+// Pages: K int8 [num_pages][hkv][16][d], V int8 [num_pages][hkv][d][16], one
+// binary32 scale per (page, KV head) for each: ks, vs [num_pages][hkv].
+typedef struct {
+    const float* x;            // [B*P][(hq + 2 hkv) d]
+    const float* bias;         // [(hq + 2 hkv) d], nullable
+    const float* cos_t;        // [max_pos][rot / 2]
+    const float* sin_t;
+    const int32_t* seq_len;    // [B] tokens before the call
+    const int32_t* n_new;      // [B] rows of each sequence, nullable: P
+    const int32_t* page_table; // [B][maxp]
+    int8_t* k;
+    int8_t* v;
+    float* ks;
+    float* vs;
+    float* q_out;              // [B*P][hq][d]
+    int32_t P, hq, hkv, maxp, num_pages, max_pos, rot, interleaved;
+    int32_t nblk;              // pages that P rows can touch
+} lgx_kv8_append_args;
+
+typedef struct {
+    const int8_t* k;
+    const int8_t* v;
+    const float* ks;
+    const float* vs;
+    const int32_t* page_table; // [B][maxp]
+    const int32_t* start;      // [B] first token of each sequence
+    float* k_out;              // [B][n][hkv][d]
+    float* v_out;
+    int32_t n, hkv, maxp, num_pages, nblk;
+} lgx_kv8_read_args;
+
+typedef struct {
+    const float* q;            // [B*P][hq][d]
+    const int8_t* k;
+    const int8_t* v;
+    const float* ks;
+    const float* vs;
+    const int32_t* page_table; // [B][maxp]
+    const int32_t* seq_len;    // [B]
+    const int32_t* n_new;      // [B], nullable: P
+    const float* slopes;       // [hq], nullable
+    float* out;                // [B*P][hq][d]
+    float* part;               // nsplit > 1: [B*P*hq][nsplit][d], then (m, l) pairs [B*P*hq][nsplit]
+    int32_t P, hq, hkv, maxp, num_pages, maxlen;
+    int32_t len_add;           // row j sees seq_len + j + len_add tokens
+    int32_t window;            // 0: all
+    int32_t nsplit, cps, ncb;  // splits of the tiles, tiles per split, column blocks
+    int32_t rows;              // B*P
+    float scale, softcap;
+} lgx_attn8_args;
+#define LGX_A8_TILE 64         // tokens of a tile: four pages

@@ -5424,3 +5424,5 @@ LGX_FPA_KERNELS(128, 5)
 LGX_FPA_KERNELS(128, 6)
 LGX_FPA_KERNELS(128, 7)
 LGX_FPA_KERNELS(128, 8)
+
+#include "lgx_kv8.hip"

@@ -1,0 +1,540 @@
+// lgx_kv8.hip -- the 8-bit KV cache: append with rotation, read-back, and the
+// attention of decode and prefill rows over it.  Part of lgx_kernels.hip (one
+// code object).
+//
+// Format.  A block is the 16 tokens of a page for one KV head; K and V blocks
+// hold int8 quants and one binary32 scale each, value = scale * quant.  K lies
+// token by token ([16][d]); V dimension by dimension ([d][16]), the order in
+// which the PV product takes it: 16 tokens of a dimension are one 16-byte load.
+
+// ---------------------------------------------------------------------------
+// Append.  Workgroup (block of 16 token slots of sequence b, head of the row):
+// thread (slot, c) holds the d / 16 elements from c d / 16 on of the slot's row.
+// q heads: rotate, write binary32.  K / V heads: rotate (K), the block's largest
+// magnitude, the scale, the quants.  All arithmetic between the binary32 input
+// and the rounded result is binary64, so a quant next to a rounding border does
+// not depend on how the products were formed.
+// A block that already holds tokens keeps its scale unless a new value exceeds
+// 127 of it; then the scale doubles until it does not and the old quants are
+// halved as often, rounded once: an old value is off by less than one step of
+// the final scale however often its block grew (1/2 + 1/4 + ...).
+// ---------------------------------------------------------------------------
+template <int D>
+__device__ __forceinline__ void kv8_append_body(const lgx_kv8_append_args& a) {
+    constexpr int E = D / 16;
+    __shared__ double am_s[4];
+    __shared__ int bad_s[4];
+    __shared__ __align__(16) int8_t v_s[D * LGX_PAGE];
+    const int tid = threadIdx.x, slot = tid >> 4, e0 = (tid & 15) * E;
+    const int b = blockIdx.x / a.nblk, hh = blockIdx.y;
+    const int sl = min(max(a.seq_len[b], 0), a.maxp * LGX_PAGE);
+    const int nn = a.n_new ? min(max(a.n_new[b], 0), a.P) : a.P;
+    const int pb = sl / LGX_PAGE + (blockIdx.x - b * a.nblk), t0 = pb * LGX_PAGE;
+    if (t0 >= sl + nn) return;                    // uniform: no new row in this block
+    const int j = t0 + slot - sl;                 // row of this slot
+    const bool is_new = j >= 0 && j < nn;
+    double y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = 0.0;
+    const bool turn = hh < a.hq + a.hkv;
+    if (is_new) {
+        const float* xr = a.x + ((int64_t)b * a.P + j) * ((int64_t)(a.hq + 2 * a.hkv) * D) + (int64_t)hh * D;
+        const float* br = a.bias ? a.bias + hh * D : nullptr;
+        const int half = a.rot / 2;
+        const int64_t pos = min(t0 + slot, a.max_pos - 1);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int i = e0 + e;
+            double x = xr[i];
+            if (br) x += br[i];
+            if (turn && i < a.rot) {
+                // the pair's other element, its index in the tables, and on
+                // which side of the pair this one is
+                const int o = a.interleaved ? i ^ 1 : i < half ? i + half : i - half;
+                const int p = a.interleaved ? i >> 1 : i < half ? i : i - half;
+                const bool first = a.interleaved ? (i & 1) == 0 : i < half;
+                double z = xr[o];
+                if (br) z += br[o];
+                const double c = a.cos_t[pos * half + p], s = a.sin_t[pos * half + p];
+                x = first ? x * c - z * s : x * c + z * s;
+            }
+            y[e] = x;
+        }
+    }
+    if (hh < a.hq) {
+        if (is_new) {
+            float* q = a.q_out + (((int64_t)b * a.P + j) * a.hq + hh) * D + e0;
+#pragma unroll
+            for (int e = 0; e < E; e += 4)
+                *(float4*)(q + e) = make_float4((float)y[e], (float)y[e + 1], (float)y[e + 2], (float)y[e + 3]);
+        }
+        return;
+    }
+    if (pb >= a.maxp) return;                     // uniform: past the sequence's pages
+    const int page = a.page_table[(int64_t)b * a.maxp + pb];
+    if (page < 0 || page >= a.num_pages) return;  // uniform
+    double am = 0.0;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        am = fmax(am, fabs(y[e]));
+        bad = bad || !(fabs(y[e]) < __builtin_inf());
+    }
+#pragma unroll
+    for (int s = 32; s; s >>= 1) am = fmax(am, __shfl_xor(am, s, 64));
+    const bool wave_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+    if ((tid & 63) == 0) {
+        am_s[tid >> 6] = am;
+        bad_s[tid >> 6] = wave_bad;
+    }
+    __syncthreads();
+    am = fmax(fmax(am_s[0], am_s[1]), fmax(am_s[2], am_s[3]));
+    bad = bad_s[0] || bad_s[1] || bad_s[2] || bad_s[3];
+    const bool isv = hh >= a.hq + a.hkv;
+    const int g = hh - a.hq - (isv ? a.hkv : 0);
+    const int64_t blk = (int64_t)page * a.hkv + g;
+    float* sp = (isv ? a.vs : a.ks) + blk;
+    const int s0 = max(sl - t0, 0);               // the first new slot
+    const float old = s0 ? *sp : 0.0f;
+    // a block whose values are all below 2^-119 is zero: scales are normal numbers
+    float scale = am < 0x1p-119 ? 0.0f : (float)(am / 127.0);
+    int grow = 0;
+    if (bad || !(old >= 0.0f && old < __builtin_inff())) scale = __builtin_nanf("");
+    else if (old > 0.0f) {
+        const float need = scale;
+        scale = old;
+        while (scale < need) {
+            scale *= 2.0f;
+            ++grow;
+        }
+    }
+    __syncthreads();                              // every wave has read the old scale
+    if (tid == 0) *sp = scale;
+    const double inv = scale > 0.0f ? 1.0 / (double)scale : 0.0;
+    int q[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int m = (int)fmin(floor(fabs(y[e]) * inv + 0.5), 127.0);
+        q[e] = bad ? 0 : y[e] < 0.0 ? -m : m;
+    }
+    const bool again = slot < s0 && grow > 0;     // an old token whose quants shrink
+    auto shrink = [&](int v) {
+        const int m = grow > 8 ? 0 : ((v < 0 ? -v : v) + (1 << (grow - 1))) >> grow;
+        return v < 0 ? -m : m;
+    };
+    if (!isv) {
+        int8_t* kr = a.k + (blk * LGX_PAGE + slot) * D + e0;
+        if (again) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) q[e] = shrink(kr[e]);
+        }
+        if (is_new || again) {
+#pragma unroll
+            for (int e = 0; e < E; e += 4)
+                *(uint32_t*)(kr + e) = (q[e] & 255) | (q[e + 1] & 255) << 8 | (q[e + 2] & 255) << 16 | (uint32_t)q[e + 3] << 24;
+        }
+        return;
+    }
+    int8_t* vb = a.v + blk * LGX_PAGE * D;
+    if (s0 == 0 && t0 + LGX_PAGE <= sl + nn) {    // uniform: a whole block
+#pragma unroll
+        for (int e = 0; e < E; ++e) v_s[(e0 + e) * LGX_PAGE + slot] = (int8_t)q[e];
+        __syncthreads();
+        if (tid < D) *(uint4*)(vb + tid * LGX_PAGE) = *(const uint4*)(v_s + tid * LGX_PAGE);
+        return;
+    }
+    if (again) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) q[e] = shrink(vb[(e0 + e) * LGX_PAGE + slot]);
+    }
+    if (is_new || again) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) vb[(e0 + e) * LGX_PAGE + slot] = (int8_t)q[e];
+    }
+}
+extern "C" __global__ __launch_bounds__(256) void lgx_k_kv8_append_d64(const lgx_kv8_append_args a) { kv8_append_body<64>(a); }
+extern "C" __global__ __launch_bounds__(256) void lgx_k_kv8_append_d128(const lgx_kv8_append_args a) { kv8_append_body<128>(a); }
+
+// ---------------------------------------------------------------------------
+// Read-back: tokens start[b] .. + n of every sequence as binary32.  Workgroup
+// (block of 16 token slots of sequence b, KV head); V's block passes through LDS
+// to come out token by token.
+// ---------------------------------------------------------------------------
+template <int D>
+__device__ __forceinline__ void kv8_read_body(const lgx_kv8_read_args& a) {
+    constexpr int E = D / 16;
+    __shared__ __align__(16) int8_t v_s[D * LGX_PAGE];
+    const int tid = threadIdx.x, slot = tid >> 4, e0 = (tid & 15) * E;
+    const int b = blockIdx.x / a.nblk, g = blockIdx.y;
+    const int st = min(max(a.start[b], 0), a.maxp * LGX_PAGE);
+    const int pb = st / LGX_PAGE + (blockIdx.x - b * a.nblk);
+    const int64_t row = (int64_t)pb * LGX_PAGE + slot - st;
+    const bool has = pb < a.maxp;                 // uniform
+    const int page = has ? min(max(a.page_table[(int64_t)b * a.maxp + pb], 0), a.num_pages - 1) : 0;
+    const int64_t blk = (int64_t)page * a.hkv + g;
+    if (tid < D) *(uint4*)(v_s + tid * LGX_PAGE) = *(const uint4*)(a.v + (blk * D + tid) * LGX_PAGE);
+    __syncthreads();
+    if (row < 0 || row >= a.n) return;
+    const float ks = has ? a.ks[blk] : 0.0f, vs = has ? a.vs[blk] : 0.0f;
+    const int8_t* kr = a.k + (blk * LGX_PAGE + slot) * D + e0;
+    const int64_t o = (((int64_t)b * a.n + row) * a.hkv + g) * D + e0;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+        float kf[4], vf[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            kf[i] = has ? ks * (float)kr[e + i] : 0.0f;
+            vf[i] = has ? vs * (float)v_s[(e0 + e + i) * LGX_PAGE + slot] : 0.0f;
+        }
+        *(float4*)(a.k_out + o + e) = make_float4(kf[0], kf[1], kf[2], kf[3]);
+        *(float4*)(a.v_out + o + e) = make_float4(vf[0], vf[1], vf[2], vf[3]);
+    }
+}
+extern "C" __global__ __launch_bounds__(256) void lgx_k_kv8_read_d64(const lgx_kv8_read_args a) { kv8_read_body<64>(a); }
+extern "C" __global__ __launch_bounds__(256) void lgx_k_kv8_read_d128(const lgx_kv8_read_args a) { kv8_read_body<128>(a); }
+
+// ---------------------------------------------------------------------------
+// Attention.  The (row, query head) pairs of one KV head are the columns of the
+// products, 16 to a matrix instruction; a tile is 64 tokens, four pages.
+//   scores   S^T[token][column] = K . Q^T on v_mfma_i32_16x16x64_i8, K quants as
+//            they lie in memory.  q is an integer of 24 bits (its row scaled by a
+//            power of two) in three signed base-256 digits: three exact int32
+//            products, joined in binary32.
+//   softmax  running maximum and sum per column, in base 2.
+//   PV       O^T[dim][column] += V^T . P^T on v_mfma_f32_16x16x32_f16: V quants are
+//            binary16 numbers, a weight (times its page's V scale) is the sum of
+//            two binary16 numbers, 22 bits.  Accumulation in binary32.
+// Row 4 p + v of score sub-tile u is token 4 u + v of page p, so that lane (column,
+// kg) ends up with all 16 scores of page kg: its scales are one value per lane,
+// and its weights are the PV operand as they stand (V's 16-byte loads give lane
+// (dim, kg) the 16 tokens of page kg).  Nothing passes through LDS or across
+// lanes but the column maximum.
+// ---------------------------------------------------------------------------
+
+// Four int8 quants as binary16: the byte of v + 128 under the exponent of 1024
+// is 1152 + v.
+__device__ __forceinline__ void i8_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    const uint32_t x = w ^ 0x80808080u;
+    const v2h off = {(_Float16)1152.0f, (_Float16)1152.0f};
+    const v2h l = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) - off;
+    const v2h h = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) - off;
+    lo = __builtin_bit_cast(uint32_t, l);
+    hi = __builtin_bit_cast(uint32_t, h);
+}
+
+// tanh: below 0.35 the odd series (the term after the last is under 1.3e-8 of
+// the result), else (1 - t) / (1 + t), t = exp(-2 |x|), where 1 - t > 0.5.
+__device__ __forceinline__ float a8_tanh(float x) {
+    const float ax = fabsf(x), t = __builtin_amdgcn_exp2f(-2.8853900817779268f * ax);
+    const float big = copysignf((1.0f - t) / (1.0f + t), x);
+    const float y = x * x;
+    float p = fmaf(y, -1382.0f / 155925.0f, 62.0f / 2835.0f);
+    p = fmaf(y, p, -17.0f / 315.0f);
+    p = fmaf(y, p, 2.0f / 15.0f);
+    p = fmaf(y, p, -1.0f / 3.0f);
+    return ax < 0.35f ? fmaf(x * y, p, x) : big;
+}
+
+// Maximum over the four lanes of a column.
+__device__ __forceinline__ float col_max(float v) {
+    v = fmaxf(v, shfl_xor_f(v, 16));
+    return fmaxf(v, shfl_xor_f(v, 32));
+}
+__device__ __forceinline__ float col_sum(float v) {
+    v = v + shfl_xor_f(v, 16);
+    return v + shfl_xor_f(v, 32);
+}
+
+// Four waves: WC of them side by side over the columns (16 NT each), the others
+// over the tiles.  X: capped scores, distance bias or a window.
+template <int D, int NT, int WC, bool X>
+__device__ __forceinline__ void attn8_body(const lgx_attn8_args& a) {
+    constexpr int WT = 4 / WC, NC = 16 * NT * WC, NS = D / 64, ND = D / 16;
+    constexpr float kLog2e = 1.44269504088896341f, kUp = 8192.0f;
+    __shared__ v4f o_s[WT > 1 ? WC * (WT / 2) * NT * ND * 64 : 1];
+    __shared__ float ml_s[WT > 1 ? WC * (WT / 2) * NT * 3 * 64 : 1];
+    const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wc = wave % WC, wt = wave / WC;
+    const int cb = blockIdx.x % a.ncb, rest = blockIdx.x / a.ncb;
+    const int sp = rest % a.nsplit, bg = rest / a.nsplit;
+    const int b = bg / a.hkv, g = bg - b * a.hkv;
+    const int G = a.hq / a.hkv;
+    const int nn = a.n_new ? min(max(a.n_new[b], 0), a.P) : a.P;
+    const int ncols = nn * G, c0 = cb * NC;
+    if (c0 >= ncols) return;                      // uniform
+    const int sl = max(a.seq_len[b], 0);
+    // tokens that the row of column c sees: [first(c), last(c))
+    auto last = [&](int c) { return (int)min((int64_t)sl + c / G + a.len_add, (int64_t)a.maxlen); };
+    auto first = [&](int c) { return X && a.window ? max(last(c) - a.window, 0) : 0; };
+    // the split's tiles
+    const int tb0 = first(c0) / LGX_A8_TILE + sp * a.cps;
+    const int tb1 = min((last(min(c0 + NC, ncols) - 1) + LGX_A8_TILE - 1) / LGX_A8_TILE, tb0 + a.cps);
+
+    const int wcol = c0 + wc * 16 * NT;           // the wave's first column
+    int L[NT], lo[NT];
+    int64_t orow[NT];                             // (row, head) of the lane's column
+    float f[NT], slope[NT];
+    v4i qd[NT][3][NS];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int c = wcol + 16 * n + col;
+        const bool ok = c < ncols;
+        const int cc = ok ? c : ncols - 1;
+        L[n] = ok ? last(cc) : 0;
+        lo[n] = ok ? first(cc) : 0;
+        orow[n] = ((int64_t)b * a.P + cc / G) * a.hq + g * G + cc % G;
+        slope[n] = X && a.slopes ? a.slopes[g * G + cc % G] : 0.0f;
+        const float* qr = a.q + orow[n] * D + 16 * kg;
+        float x[NS][16], am = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const float4 v = *(const float4*)(qr + 64 * s + e);
+                x[s][e] = v.x;
+                x[s][e + 1] = v.y;
+                x[s][e + 2] = v.z;
+                x[s][e + 3] = v.w;
+            }
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                am = fmaxf(am, fabsf(x[s][e]));
+                bad = bad || !(fabsf(x[s][e]) < __builtin_inff());
+            }
+        am = col_max(am);
+        const float isbad = col_max(bad ? 1.0f : 0.0f);
+        // the largest power of two that keeps every |q| within 127 * 65536, the
+        // range of three balanced digits
+        const float up = __uint_as_float(__float_as_uint(fminf(8323072.0f / am, 0x1p100f)) & 0x7f800000u);
+        f[n] = isbad != 0.0f ? __builtin_nanf("") : a.scale / up;
+        if (!X) f[n] *= kLog2e;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float y = isbad != 0.0f ? 0.0f : x[s][4 * w + e] * up;
+                    v[e] = ((uint32_t)(int)rintf(y) + 0x808080u) ^ 0x808080u;
+                }
+                // byte i of the four numbers is digit i
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    const uint32_t sel = 0x0c0c0000u | (uint32_t)(4 + i) << 8 | (uint32_t)i;
+                    const uint32_t p01 = __builtin_amdgcn_perm(v[1], v[0], sel);
+                    const uint32_t p23 = __builtin_amdgcn_perm(v[3], v[2], sel);
+                    qd[n][i][s][w] = (int)(p01 | p23 << 16);
+                }
+            }
+    }
+    float m[NT], l[NT], vref = 0x1p-126f;
+    v4f o[NT][ND];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        m[n] = -__builtin_inff();
+        l[n] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[n][i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // the wave's own tiles: those that its columns see
+    const int wlast = min(wcol + 16 * NT, ncols) - 1;
+    const int wt0 = wcol < ncols ? first(wcol) / LGX_A8_TILE : 0;
+    const int wt1 = wcol < ncols ? min(tb1, (last(wlast) + LGX_A8_TILE - 1) / LGX_A8_TILE) : 0;
+    const int wend = wcol < ncols ? last(wlast) : 0, wbeg = wcol < ncols ? first(wcol) : 0;
+    const int32_t* ptab = a.page_table + (int64_t)b * a.maxp;
+    auto page_of = [&](int i) { return (int64_t)min(max(ptab[min(i, a.maxp - 1)], 0), a.num_pages - 1) * a.hkv + g; };
+#pragma unroll 1
+    for (int t = max(tb0, wt0) + wt; t < wt1; t += WT) {
+        const int t0 = t * LGX_A8_TILE;
+        const int64_t pk = page_of(4 * t + (col >> 2)), pv = page_of(4 * t + kg);
+        uint4 kw[4][NS], vw[ND];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+                kw[u][s] = *(const uint4*)(a.k + (pk * LGX_PAGE + 4 * u + (col & 3)) * D + 64 * s + 16 * kg);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) vw[i] = *(const uint4*)(a.v + (pv * D + 16 * i + col) * LGX_PAGE);
+        // a page outside the wave's tokens may hold anything
+        const int pt = t0 + 16 * kg;
+        const bool live = pt < wend && pt + LGX_PAGE > wbeg;
+        const float ks = a.ks[pv], vsc = live ? a.vs[pv] : 0.0f;
+        // weights are in units of the largest V scale so far, rounded down to a
+        // power of two, times 2^-13 (they stay below 2^14, and their second
+        // binary16 part is not subnormal where it matters)
+        const float vtop = col_max(vsc < __builtin_inff() ? vsc : 0.0f);
+        const float vnew = fmaxf(vref, __uint_as_float(__float_as_uint(vtop) & 0x7f800000u));
+        const float r = vsc * (1.0f / vnew) * kUp, vdown = vref / vnew;
+        vref = vnew;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float z[16];
+            const float fk = f[n] * ks;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                v4i c2 = {0, 0, 0, 0}, c1 = {0, 0, 0, 0}, c0_ = {0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    const v4i kv = __builtin_bit_cast(v4i, kw[u][s]);
+                    c2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv, qd[n][2][s], c2, 0, 0, 0);
+                    c1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv, qd[n][1][s], c1, 0, 0, 0);
+                    c0_ = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv, qd[n][0][s], c0_, 0, 0, 0);
+                }
+                // |c1| 256 + |c0| < 2^30
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    z[4 * u + v] = fmaf((float)c2[v], 65536.0f, (float)(c1[v] * 256 + c0_[v])) * fk;
+            }
+            const bool edge = __builtin_amdgcn_ballot_w64(t0 + LGX_A8_TILE > L[n] || t0 < lo[n]) != 0;
+            if constexpr (X) {
+                if (a.softcap > 0.0f) {
+                    const float inv = 1.0f / a.softcap;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) z[e] = a.softcap * a8_tanh(z[e] * inv);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    z[e] = (z[e] - slope[n] * (float)(L[n] - 1 - (pt + e))) * kLog2e;
+            }
+            if (edge) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (pt + e >= L[n] || pt + e < lo[n]) z[e] = -__builtin_inff();
+            }
+            float mt = z[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) mt = fmaxf(mt, z[e]);
+            const float mn = fmaxf(m[n], col_max(mt));
+            const bool none = mn == -__builtin_inff();   // nothing seen yet
+            const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
+            const float mref = none ? 0.0f : mn;
+            m[n] = mn;
+            float ps = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                z[e] = __builtin_amdgcn_exp2f(z[e] - mref);
+                ps += z[e];
+            }
+            l[n] = l[n] * alpha + ps;
+            const float down = alpha * vdown;
+            if (__builtin_amdgcn_ballot_w64(down != 1.0f)) {
+#pragma unroll
+                for (int i = 0; i < ND; ++i) o[n][i] *= down;
+            }
+            v8h ph[2], pl[2];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                // a weight of 0 meets no scale (a later row's page may hold NaN)
+                const float w = z[e] == 0.0f ? 0.0f : z[e] * r;
+                ph[e >> 3][e & 7] = (_Float16)w;
+                pl[e >> 3][e & 7] = (_Float16)(w - (float)ph[e >> 3][e & 7]);
+            }
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
+                uint4 h0, h1;
+                i8_to_f16(vw[i].x, h0.x, h0.y);
+                i8_to_f16(vw[i].y, h0.z, h0.w);
+                i8_to_f16(vw[i].z, h1.x, h1.y);
+                i8_to_f16(vw[i].w, h1.z, h1.w);
+                o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h0), ph[0], o[n][i], 0, 0, 0);
+                o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h1), ph[1], o[n][i], 0, 0, 0);
+                o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h0), pl[0], o[n][i], 0, 0, 0);
+                o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h1), pl[1], o[n][i], 0, 0, 0);
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) l[n] = col_sum(l[n]);
+    // join the waves that share columns, halving their number
+    if constexpr (WT > 1) {
+#pragma unroll
+        for (int h = WT / 2; h; h >>= 1) {
+            const int at = (wc * (WT / 2) + wt % h) * NT;
+            if (wt >= h && wt < 2 * h) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    ml_s[((at + n) * 3 + 0) * 64 + lane] = m[n];
+                    ml_s[((at + n) * 3 + 1) * 64 + lane] = l[n];
+                    ml_s[((at + n) * 3 + 2) * 64 + lane] = vref;
+#pragma unroll
+                    for (int i = 0; i < ND; ++i) o_s[((at + n) * ND + i) * 64 + lane] = o[n][i];
+                }
+            }
+            __syncthreads();
+            if (wt < h) {
+                const float vo = ml_s[(at * 3 + 2) * 64 + lane];
+                const float vn = fmaxf(vref, vo);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float mo = ml_s[((at + n) * 3 + 0) * 64 + lane], lo_ = ml_s[((at + n) * 3 + 1) * 64 + lane];
+                    const float mn = fmaxf(m[n], mo);
+                    const float w0 = m[n] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[n] - mn);
+                    const float w1 = mo == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mo - mn);
+                    l[n] = l[n] * w0 + lo_ * w1;
+                    m[n] = mn;
+#pragma unroll
+                    for (int i = 0; i < ND; ++i)
+                        o[n][i] = o[n][i] * (w0 * (vref / vn)) + o_s[((at + n) * ND + i) * 64 + lane] * (w1 * (vo / vn));
+                }
+                vref = vn;
+            }
+            __syncthreads();
+        }
+        if (wt) return;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        if (wcol + 16 * n + col >= ncols) continue;
+        // NaN sums stay NaN; nothing seen gives zeros
+        const float unit = vref * (1.0f / kUp);
+        const float s = a.nsplit > 1 ? unit : l[n] == 0.0f ? 0.0f : unit / l[n];
+        float* dst = a.nsplit > 1 ? a.part + (orow[n] * a.nsplit + sp) * D : a.out + orow[n] * D;
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+            *(float4*)(dst + 16 * i + 4 * kg) = make_float4(o[n][i][0] * s, o[n][i][1] * s, o[n][i][2] * s, o[n][i][3] * s);
+        if (a.nsplit > 1 && kg == 0) {
+            float2* ml = (float2*)(a.part + (int64_t)a.rows * a.hq * a.nsplit * D) + orow[n] * a.nsplit + sp;
+            *ml = make_float2(m[n], l[n]);
+        }
+    }
+}
+
+// Joins the splits of one (row, head).
+template <int D>
+__device__ __forceinline__ void attn8_merge_body(const lgx_attn8_args& a) {
+    const int64_t rh = blockIdx.x;
+    const int row = (int)(rh / a.hq), b = row / a.P, j = row - b * a.P;
+    if (a.n_new && j >= a.n_new[b]) return;
+    const float2* ml = (const float2*)(a.part + (int64_t)a.rows * a.hq * a.nsplit * D) + rh * a.nsplit;
+    const float* p = a.part + rh * a.nsplit * D + threadIdx.x;
+    float m = -__builtin_inff(), l = 0.0f, o = 0.0f;
+    for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, ml[s].x);
+    for (int s = 0; s < a.nsplit; ++s) {
+        const float2 x = ml[s];
+        // an empty split's maximum is -inf
+        const float w = x.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x.x - m);
+        l = fmaf(w, x.y, l);
+        o = fmaf(w, p[(int64_t)s * D], o);
+    }
+    a.out[rh * D + threadIdx.x] = l == 0.0f ? 0.0f : o / l;
+}
+extern "C" __global__ __launch_bounds__(64) void lgx_k_attn8_merge_d64(const lgx_attn8_args a) { attn8_merge_body<64>(a); }
+extern "C" __global__ __launch_bounds__(128) void lgx_k_attn8_merge_d128(const lgx_attn8_args a) { attn8_merge_body<128>(a); }
+
+#define LGX_A8_KERNELS(D, C, NT, WC)                                                                           \
+    extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_d##D##_c##C(const lgx_attn8_args a) {        \
+        attn8_body<D, NT, WC, false>(a);                                                                       \
+    }                                                                                                          \
+    extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8x_d##D##_c##C(const lgx_attn8_args a) {       \
+        attn8_body<D, NT, WC, true>(a);                                                                        \
+    }
+LGX_A8_KERNELS(64, 16, 1, 1)
+LGX_A8_KERNELS(128, 16, 1, 1)
+LGX_A8_KERNELS(64, 128, 2, 4)
+LGX_A8_KERNELS(128, 128, 2, 4)
