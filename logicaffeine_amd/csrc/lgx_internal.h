@@ -171,6 +171,8 @@ enum Kern {
     K_GEMM_GRPM16,
     K_KV8_APPEND_D64,
     K_KV8_APPEND_D128,
+    K_KV8_APPEND1_D64,
+    K_KV8_APPEND1_D128,
     K_KV8_READ_D64,
     K_KV8_READ_D128,
     K_ATTN8_D64,     // 16 columns; + 1: with caps, distances or a window; + 2: 128 columns
@@ -225,7 +227,8 @@ inline const char* const kKernelNames[] = {
     "lgx_k_attn_prefill_fast_d128_g7", "lgx_k_attn_prefill_fast_d128_g8",
     "lgx_k_attn_merge_o_d64", "lgx_k_attn_merge_o_d128", "lgx_k_norm_qkv_d64", "lgx_k_norm_qkv_d128",
     "lgx_k_q8_gemm_grpm16",
-    "lgx_k_kv8_append_d64", "lgx_k_kv8_append_d128", "lgx_k_kv8_read_d64", "lgx_k_kv8_read_d128",
+    "lgx_k_kv8_append_d64", "lgx_k_kv8_append_d128",
+    "lgx_k_kv8_append1_d64", "lgx_k_kv8_append1_d128", "lgx_k_kv8_read_d64", "lgx_k_kv8_read_d128",
     "lgx_k_attn8_d64_c16", "lgx_k_attn8x_d64_c16", "lgx_k_attn8_d64_c128", "lgx_k_attn8x_d64_c128",
     "lgx_k_attn8_d128_c16", "lgx_k_attn8x_d128_c16", "lgx_k_attn8_d128_c128", "lgx_k_attn8x_d128_c128",
     "lgx_k_attn8_merge_d64", "lgx_k_attn8_merge_d128",

@@ -425,6 +425,7 @@ typedef struct {
 } lgx_act_t16_args;
 
 // ---- 8-bit KV cache (lgx_kv8.hip) ----
+#define LGX_KV8_QH 4           // query heads per workgroup of the append of several rows
 // Pages: K int8 [num_pages][hkv][16][d], V int8 [num_pages][hkv][d][16], one
 // binary32 scale per (page, KV head) for each: ks, vs [num_pages][hkv].
 typedef struct {
@@ -442,6 +443,7 @@ typedef struct {
     float* q_out;              // [B*P][hq][d]
     int32_t P, hq, hkv, maxp, num_pages, max_pos, rot, interleaved;
     int32_t nblk;              // pages that P rows can touch
+    int32_t vec;               // runs of d / 32 pairs are aligned and of one kind
 } lgx_kv8_append_args;
 
 typedef struct {

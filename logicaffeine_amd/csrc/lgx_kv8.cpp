@@ -163,9 +163,16 @@ lgx_status lgx_rope_kv_append_i8(lgx_ctx* c, const float* qkv, const float* bias
             return fail(LGX_OUT_OF_BOUNDS, "append of %d x %d rows, %lld heads", B, P, (long long)heads);
         lgx_kv8_append_args a{qkv, bias, rope->cos_t, rope->sin_t, seq_len, n_new, page_table, kv->k, kv->v,
                               kv->k_scale, kv->v_scale, q_out, P, hq, kv->hkv, maxp, kv->num_pages, rope->max_pos,
-                              rope->rot, rope->interleaved, (int32_t)nblk};
-        return launch(c, kv->d == 64 ? K_KV8_APPEND_D64 : K_KV8_APPEND_D128, dim3((unsigned)(B * nblk), (unsigned)heads),
-                      dim3(256), a, stream);
+                              rope->rot, rope->interleaved, (int32_t)nblk, 0};
+        const bool d64 = kv->d == 64;
+        if (P == 1)
+            return launch(c, d64 ? K_KV8_APPEND1_D64 : K_KV8_APPEND1_D128, dim3((unsigned)B, cdiv(heads, 4)), dim3(256), a,
+                          stream);
+        // a thread's d / 32 pairs in 16- or 8-byte pieces
+        a.vec = rope->rot / 2 % (kv->d / 32) == 0 && aligned16(qkv) && aligned16(bias) && aligned16(rope->cos_t) &&
+                aligned16(rope->sin_t);
+        return launch(c, d64 ? K_KV8_APPEND_D64 : K_KV8_APPEND_D128,
+                      dim3((unsigned)(B * nblk), cdiv(hq, LGX_KV8_QH) + 2 * kv->hkv), dim3(256), a, stream);
     });
 }
 

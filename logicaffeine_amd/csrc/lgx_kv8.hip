@@ -8,152 +8,385 @@
 // which the PV product takes it: 16 tokens of a dimension are one 16-byte load.
 
 // ---------------------------------------------------------------------------
-// Append.  Workgroup (block of 16 token slots of sequence b, head of the row):
-// thread (slot, c) holds the d / 16 elements from c d / 16 on of the slot's row.
-// q heads: rotate, write binary32.  K / V heads: rotate (K), the block's largest
-// magnitude, the scale, the quants.  All arithmetic between the binary32 input
-// and the rounded result is binary64, so a quant next to a rounding border does
-// not depend on how the products were formed.
+// Append.  All arithmetic between the binary32 input and the rounded result is
+// binary64, so a quant next to a rounding border does not depend on how the
+// products were formed.
 // A block that already holds tokens keeps its scale unless a new value exceeds
 // 127 of it; then the scale doubles until it does not and the old quants are
 // halved as often, rounded once: an old value is off by less than one step of
 // the final scale however often its block grew (1/2 + 1/4 + ...).
+//
+// A head is D / 2 pairs: pair p < rot / 2 is (p, p + rot / 2), or (2p, 2p + 1)
+// when interleaved, and turns; the others are (2p, 2p + 1) and do not.  A thread
+// holds E / 2 consecutive pairs as two runs of E / 2 dimensions (Pairs): the two
+// members of its turning pairs, or E neighbours.
 // ---------------------------------------------------------------------------
+template <int H>
+struct Pairs {
+    int ia, ib;        // first dimension of each run
+    int p;             // first pair
+    bool apart, turn;  // members half a rotation apart; any of the pairs turns
+};
+// Runs of H pairs from pair p on of a head with `rot` turning dimensions; `vec`:
+// rot / 2 is a multiple of H, so that the pairs of a run are all of one kind.
+template <int H>
+__device__ __forceinline__ Pairs<H> pairs_of(int p, int rot, bool inter, bool vec) {
+    Pairs<H> r;
+    r.p = p;
+    r.turn = p < rot / 2;
+    r.apart = vec && r.turn && !inter;
+    r.ia = r.apart ? p : 2 * p;
+    r.ib = r.apart ? p + rot / 2 : 2 * p + H;
+    return r;
+}
+// Dimensions of pair p + k, one by one (rot / 2 not a multiple of H).
+__device__ __forceinline__ void pair_dims(int p, int rot, bool inter, int& i0, int& i1) {
+    const bool apart = p < rot / 2 && !inter;
+    i0 = apart ? p : 2 * p;
+    i1 = apart ? p + rot / 2 : 2 * p + 1;
+}
+template <int H>
+struct RunT;
+template <>
+struct RunT<1> { typedef float type __attribute__((ext_vector_type(1))); };
+template <>
+struct RunT<2> { typedef float type __attribute__((ext_vector_type(2))); };
+template <>
+struct RunT<4> { typedef float type __attribute__((ext_vector_type(4))); };
+
+// The head row's values at the thread's pairs: x[k], z[k] the members of pair k
+// (runs that are neighbours come out as (2k, 2k + 1) too), bias added.
+template <int H>
+__device__ __forceinline__ void load_pairs(const float* xr, const float* br, const Pairs<H>& w, int rot, bool inter, bool vec,
+                                           double (&x)[H], double (&z)[H]) {
+    typedef typename RunT<H>::type V;
+    if (vec) {                                    // uniform
+        float v[2 * H], o[2 * H];
+        *(V*)v = *(const V*)(xr + w.ia);
+        *(V*)(v + H) = *(const V*)(xr + w.ib);
+        if (br) {
+            *(V*)o = *(const V*)(br + w.ia);
+            *(V*)(o + H) = *(const V*)(br + w.ib);
+        }
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+            x[k] = w.apart ? v[k] : v[2 * k];
+            z[k] = w.apart ? v[H + k] : v[2 * k + 1];
+            if (br) {
+                x[k] += w.apart ? o[k] : o[2 * k];
+                z[k] += w.apart ? o[H + k] : o[2 * k + 1];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+            int i0, i1;
+            pair_dims(w.p + k, rot, inter, i0, i1);
+            x[k] = xr[i0];
+            z[k] = xr[i1];
+            if (br) {
+                x[k] += br[i0];
+                z[k] += br[i1];
+            }
+        }
+    }
+}
+// The tables' values of the thread's pairs at a position; (1, 0) where a pair
+// does not turn.
+template <int H>
+__device__ __forceinline__ void load_turns(const lgx_kv8_append_args& a, const Pairs<H>& w, int64_t pos, bool vec, float (&c)[H],
+                                           float (&s)[H]) {
+    typedef typename RunT<H>::type V;
+    const int64_t at = pos * (a.rot / 2) + w.p;
+    if (vec) {
+        if (w.turn) {
+            *(V*)c = *(const V*)(a.cos_t + at);
+            *(V*)s = *(const V*)(a.sin_t + at);
+        } else {
+#pragma unroll
+            for (int k = 0; k < H; ++k) c[k] = 1.0f, s[k] = 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+            const bool on = w.p + k < a.rot / 2;
+            c[k] = on ? a.cos_t[at + k] : 1.0f;
+            s[k] = on ? a.sin_t[at + k] : 0.0f;
+        }
+    }
+}
+// The pair's rotation; one that does not turn keeps its bits (an infinite member
+// would meet the other's 0).
+template <int H>
+__device__ __forceinline__ void turn_pairs(const float (&c)[H], const float (&s)[H], const Pairs<H>& w, int rot, double (&x)[H],
+                                           double (&z)[H]) {
+#pragma unroll
+    for (int k = 0; k < H; ++k) {
+        const double y0 = x[k] * (double)c[k] - z[k] * (double)s[k], y1 = z[k] * (double)c[k] + x[k] * (double)s[k];
+        const bool on = w.p + k < rot / 2;
+        x[k] = on ? y0 : x[k];
+        z[k] = on ? y1 : z[k];
+    }
+}
+template <int H>
+__device__ __forceinline__ void store_q(float* q, const Pairs<H>& w, int rot, bool inter, bool vec, const double (&x)[H],
+                                        const double (&z)[H]) {
+    typedef typename RunT<H>::type V;
+    if (vec) {
+        float v[2 * H];
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+            // runs of one member, or neighbours in turn
+            v[k] = (float)(w.apart ? x[k] : k & 1 ? z[k / 2] : x[k / 2]);
+            v[H + k] = (float)(w.apart ? z[k] : k & 1 ? z[(H + k) / 2] : x[(H + k) / 2]);
+        }
+        *(V*)(q + w.ia) = *(const V*)v;
+        *(V*)(q + w.ib) = *(const V*)(v + H);
+    } else {
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+            int i0, i1;
+            pair_dims(w.p + k, rot, inter, i0, i1);
+            q[i0] = (float)x[k];
+            q[i1] = (float)z[k];
+        }
+    }
+}
+// The scale of a block: `need` of its new values (NaN where one is not finite),
+// `old` the scale of the tokens it holds (0 for a new block); grow: doublings.
+__device__ __forceinline__ float block_scale(double am, bool bad, float old, int& grow) {
+    // a block whose values are all below 2^-119 is zero: scales are normal numbers
+    const float need = am < 0x1p-119 ? 0.0f : (float)(am / 127.0);
+    grow = 0;
+    if (bad || !(old >= 0.0f && old < __builtin_inff())) return __builtin_nanf("");
+    if (!(old > 0.0f)) return need;
+    float scale = old;
+    while (scale < need) {
+        scale *= 2.0f;
+        ++grow;
+    }
+    return scale;
+}
+__device__ __forceinline__ int quant8(double y, double inv) {
+    const int m = (int)fmin(floor(fabs(y) * inv + 0.5), 127.0);
+    return y < 0.0 ? -m : m;
+}
+__device__ __forceinline__ int halve8(int v, int grow) {
+    const int m = grow > 8 ? 0 : ((v < 0 ? -v : v) + (1 << (grow - 1))) >> grow;
+    return v < 0 ? -m : m;
+}
+
+// Workgroup (block of 16 token slots of sequence b; QH query heads, or a K or V
+// head): thread (slot, c) holds D / 32 pairs of the slot's row.  Query heads share
+// the thread's cosines and sines.
+#define KV8_QH LGX_KV8_QH
 template <int D>
 __device__ __forceinline__ void kv8_append_body(const lgx_kv8_append_args& a) {
-    constexpr int E = D / 16;
+    constexpr int H = D / 32;
     __shared__ double am_s[4];
     __shared__ int bad_s[4];
     __shared__ __align__(16) int8_t v_s[D * LGX_PAGE];
-    const int tid = threadIdx.x, slot = tid >> 4, e0 = (tid & 15) * E;
-    const int b = blockIdx.x / a.nblk, hh = blockIdx.y;
+    const int tid = threadIdx.x, slot = tid >> 4;
+    const int b = blockIdx.x / a.nblk, nqg = (a.hq + KV8_QH - 1) / KV8_QH;
+    const bool isq = (int)blockIdx.y < nqg, isv = (int)blockIdx.y >= nqg + a.hkv;
     const int sl = min(max(a.seq_len[b], 0), a.maxp * LGX_PAGE);
     const int nn = a.n_new ? min(max(a.n_new[b], 0), a.P) : a.P;
     const int pb = sl / LGX_PAGE + (blockIdx.x - b * a.nblk), t0 = pb * LGX_PAGE;
     if (t0 >= sl + nn) return;                    // uniform: no new row in this block
     const int j = t0 + slot - sl;                 // row of this slot
     const bool is_new = j >= 0 && j < nn;
-    double y[E];
+    const int rot = isv ? 0 : a.rot;
+    const bool inter = a.interleaved != 0, vec = a.vec != 0;
+    const Pairs<H> w = pairs_of<H>((tid & 15) * H, rot, inter, vec);
+    const int64_t row = (int64_t)b * a.P + j;
+    const float* xr = a.x + row * ((int64_t)(a.hq + 2 * a.hkv) * D);
+    float c[H], s[H];
+    if (is_new && !isv) load_turns<H>(a, w, min(t0 + slot, a.max_pos - 1), vec, c, s);
+    if (isq) {
+        if (!is_new) return;
+        const int h0 = blockIdx.y * KV8_QH;
+        double x[KV8_QH][H], z[KV8_QH][H];
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = 0.0;
-    const bool turn = hh < a.hq + a.hkv;
-    if (is_new) {
-        const float* xr = a.x + ((int64_t)b * a.P + j) * ((int64_t)(a.hq + 2 * a.hkv) * D) + (int64_t)hh * D;
-        const float* br = a.bias ? a.bias + hh * D : nullptr;
-        const int half = a.rot / 2;
-        const int64_t pos = min(t0 + slot, a.max_pos - 1);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int i = e0 + e;
-            double x = xr[i];
-            if (br) x += br[i];
-            if (turn && i < a.rot) {
-                // the pair's other element, its index in the tables, and on
-                // which side of the pair this one is
-                const int o = a.interleaved ? i ^ 1 : i < half ? i + half : i - half;
-                const int p = a.interleaved ? i >> 1 : i < half ? i : i - half;
-                const bool first = a.interleaved ? (i & 1) == 0 : i < half;
-                double z = xr[o];
-                if (br) z += br[o];
-                const double c = a.cos_t[pos * half + p], s = a.sin_t[pos * half + p];
-                x = first ? x * c - z * s : x * c + z * s;
-            }
-            y[e] = x;
+        for (int i = 0; i < KV8_QH; ++i) {
+            const int h = min(h0 + i, a.hq - 1);
+            load_pairs<H>(xr + h * D, a.bias ? a.bias + h * D : nullptr, w, rot, inter, vec, x[i], z[i]);
         }
-    }
-    if (hh < a.hq) {
-        if (is_new) {
-            float* q = a.q_out + (((int64_t)b * a.P + j) * a.hq + hh) * D + e0;
 #pragma unroll
-            for (int e = 0; e < E; e += 4)
-                *(float4*)(q + e) = make_float4((float)y[e], (float)y[e + 1], (float)y[e + 2], (float)y[e + 3]);
+        for (int i = 0; i < KV8_QH; ++i) {
+            if (h0 + i >= a.hq) break;            // uniform
+            turn_pairs<H>(c, s, w, rot, x[i], z[i]);
+            store_q<H>(a.q_out + (row * a.hq + h0 + i) * D, w, rot, inter, vec, x[i], z[i]);
         }
         return;
     }
     if (pb >= a.maxp) return;                     // uniform: past the sequence's pages
     const int page = a.page_table[(int64_t)b * a.maxp + pb];
     if (page < 0 || page >= a.num_pages) return;  // uniform
+    const int g = blockIdx.y - nqg - (isv ? a.hkv : 0), hh = a.hq + (isv ? a.hkv : 0) + g;
+    double y[2 * H];
+    {
+        double x[H], z[H];
+#pragma unroll
+        for (int k = 0; k < H; ++k) x[k] = z[k] = 0.0;
+        if (is_new) {
+            load_pairs<H>(xr + hh * D, a.bias ? a.bias + hh * D : nullptr, w, rot, inter, vec, x, z);
+            if (!isv) turn_pairs<H>(c, s, w, rot, x, z);
+        }
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+            y[k] = x[k];
+            y[H + k] = z[k];
+        }
+    }
+    // dimension of y[e]
+    auto dim = [&](int e) {
+        if (vec) return w.apart ? (e < H ? w.ia + e : w.ib + e - H) : 2 * (w.p + e % H) + e / H;
+        int i0, i1;
+        pair_dims(w.p + e % H, rot, inter, i0, i1);
+        return e < H ? i0 : i1;
+    };
     double am = 0.0;
     bool bad = false;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
+    for (int e = 0; e < 2 * H; ++e) {
         am = fmax(am, fabs(y[e]));
         bad = bad || !(fabs(y[e]) < __builtin_inf());
     }
 #pragma unroll
-    for (int s = 32; s; s >>= 1) am = fmax(am, __shfl_xor(am, s, 64));
+    for (int m = 32; m; m >>= 1) am = fmax(am, __shfl_xor(am, m, 64));
     const bool wave_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
     if ((tid & 63) == 0) {
         am_s[tid >> 6] = am;
         bad_s[tid >> 6] = wave_bad;
     }
-    __syncthreads();
-    am = fmax(fmax(am_s[0], am_s[1]), fmax(am_s[2], am_s[3]));
-    bad = bad_s[0] || bad_s[1] || bad_s[2] || bad_s[3];
-    const bool isv = hh >= a.hq + a.hkv;
-    const int g = hh - a.hq - (isv ? a.hkv : 0);
     const int64_t blk = (int64_t)page * a.hkv + g;
     float* sp = (isv ? a.vs : a.ks) + blk;
     const int s0 = max(sl - t0, 0);               // the first new slot
     const float old = s0 ? *sp : 0.0f;
-    // a block whose values are all below 2^-119 is zero: scales are normal numbers
-    float scale = am < 0x1p-119 ? 0.0f : (float)(am / 127.0);
-    int grow = 0;
-    if (bad || !(old >= 0.0f && old < __builtin_inff())) scale = __builtin_nanf("");
-    else if (old > 0.0f) {
-        const float need = scale;
-        scale = old;
-        while (scale < need) {
-            scale *= 2.0f;
-            ++grow;
-        }
-    }
+    __syncthreads();
+    am = fmax(fmax(am_s[0], am_s[1]), fmax(am_s[2], am_s[3]));
+    bad = bad_s[0] || bad_s[1] || bad_s[2] || bad_s[3];
+    int grow;
+    const float scale = block_scale(am, bad, old, grow);
     __syncthreads();                              // every wave has read the old scale
     if (tid == 0) *sp = scale;
     const double inv = scale > 0.0f ? 1.0 / (double)scale : 0.0;
-    int q[E];
+    int q[2 * H];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int m = (int)fmin(floor(fabs(y[e]) * inv + 0.5), 127.0);
-        q[e] = bad ? 0 : y[e] < 0.0 ? -m : m;
-    }
+    for (int e = 0; e < 2 * H; ++e) q[e] = bad ? 0 : quant8(y[e], inv);
     const bool again = slot < s0 && grow > 0;     // an old token whose quants shrink
-    auto shrink = [&](int v) {
-        const int m = grow > 8 ? 0 : ((v < 0 ? -v : v) + (1 << (grow - 1))) >> grow;
-        return v < 0 ? -m : m;
-    };
     if (!isv) {
-        int8_t* kr = a.k + (blk * LGX_PAGE + slot) * D + e0;
+        int8_t* kr = a.k + (blk * LGX_PAGE + slot) * D;
         if (again) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) q[e] = shrink(kr[e]);
+            for (int e = 0; e < 2 * H; ++e) q[e] = halve8(kr[dim(e)], grow);
         }
         if (is_new || again) {
+            if (vec) {
+                // the runs' bytes in one store each
+                uint32_t ra = 0, rb = 0;
 #pragma unroll
-            for (int e = 0; e < E; e += 4)
-                *(uint32_t*)(kr + e) = (q[e] & 255) | (q[e + 1] & 255) << 8 | (q[e + 2] & 255) << 16 | (uint32_t)q[e + 3] << 24;
+                for (int k = 0; k < H; ++k) {
+                    const int ea = w.apart ? q[k] : q[(k & 1) * H + k / 2];
+                    const int eb = w.apart ? q[H + k] : q[(k & 1) * H + (H + k) / 2];
+                    ra |= (uint32_t)(ea & 255) << (8 * k);
+                    rb |= (uint32_t)(eb & 255) << (8 * k);
+                }
+                if (H == 4) {
+                    *(uint32_t*)(kr + w.ia) = ra;
+                    *(uint32_t*)(kr + w.ib) = rb;
+                } else {
+                    *(uint16_t*)(kr + w.ia) = (uint16_t)ra;
+                    *(uint16_t*)(kr + w.ib) = (uint16_t)rb;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 2 * H; ++e) kr[dim(e)] = (int8_t)q[e];
+            }
         }
         return;
     }
     int8_t* vb = a.v + blk * LGX_PAGE * D;
     if (s0 == 0 && t0 + LGX_PAGE <= sl + nn) {    // uniform: a whole block
 #pragma unroll
-        for (int e = 0; e < E; ++e) v_s[(e0 + e) * LGX_PAGE + slot] = (int8_t)q[e];
+        for (int e = 0; e < 2 * H; ++e) v_s[dim(e) * LGX_PAGE + slot] = (int8_t)q[e];
         __syncthreads();
         if (tid < D) *(uint4*)(vb + tid * LGX_PAGE) = *(const uint4*)(v_s + tid * LGX_PAGE);
         return;
     }
     if (again) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) q[e] = shrink(vb[(e0 + e) * LGX_PAGE + slot]);
+        for (int e = 0; e < 2 * H; ++e) q[e] = halve8(vb[dim(e) * LGX_PAGE + slot], grow);
     }
     if (is_new || again) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) vb[(e0 + e) * LGX_PAGE + slot] = (int8_t)q[e];
+        for (int e = 0; e < 2 * H; ++e) vb[dim(e) * LGX_PAGE + slot] = (int8_t)q[e];
     }
 }
 extern "C" __global__ __launch_bounds__(256) void lgx_k_kv8_append_d64(const lgx_kv8_append_args a) { kv8_append_body<64>(a); }
 extern "C" __global__ __launch_bounds__(256) void lgx_k_kv8_append_d128(const lgx_kv8_append_args a) { kv8_append_body<128>(a); }
+
+// One new row per sequence (a decode step): a wave per head, a pair per lane (with
+// D = 64 the upper half of the wave idles).  The row does not depend on the
+// length, so its loads are in flight together with the length's, and the cosines
+// with the page's.
+template <int D>
+__device__ __forceinline__ void kv8_append1_body(const lgx_kv8_append_args& a) {
+    const int p = threadIdx.x & 63, b = blockIdx.x;
+    const int hh = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + (threadIdx.x >> 6));
+    const bool on = p < D / 2, isv = hh >= a.hq + a.hkv, inter = a.interleaved != 0;
+    if (hh >= a.hq + 2 * a.hkv || (a.n_new && a.n_new[b] < 1)) return;   // uniform per wave
+    const int rot = isv ? 0 : a.rot;
+    int i0, i1;
+    pair_dims(on ? p : 0, rot, inter, i0, i1);
+    const int64_t at = (int64_t)b * (a.hq + 2 * a.hkv) * D + hh * D;
+    double x[1] = {a.x[at + i0]}, z[1] = {a.x[at + i1]};
+    const int sl = min(max(a.seq_len[b], 0), a.maxp * LGX_PAGE);
+    const int pb = sl / LGX_PAGE;
+    if (a.bias) {
+        x[0] += a.bias[hh * D + i0];
+        z[0] += a.bias[hh * D + i1];
+    }
+    const int page = pb < a.maxp ? a.page_table[(int64_t)b * a.maxp + pb] : -1;
+    const Pairs<1> w = {i0, i1, p, false, p < rot / 2};
+    if (!isv) {
+        float c[1], s[1];
+        load_turns<1>(a, w, min(sl, a.max_pos - 1), false, c, s);
+        turn_pairs<1>(c, s, w, rot, x, z);
+    }
+    if (hh < a.hq) {
+        if (on) store_q<1>(a.q_out + ((int64_t)b * a.hq + hh) * D, w, rot, inter, false, x, z);
+        return;
+    }
+    if (page < 0 || page >= a.num_pages) return;
+    const int g = hh - a.hq - (isv ? a.hkv : 0), s0 = sl % LGX_PAGE;
+    const int64_t blk = (int64_t)page * a.hkv + g;
+    float* sp = (isv ? a.vs : a.ks) + blk;
+    const float old = s0 ? *sp : 0.0f;
+    double am = on ? fmax(fabs(x[0]), fabs(z[0])) : 0.0;
+    const bool bad = __builtin_amdgcn_ballot_w64(on && !(fabs(x[0]) < __builtin_inf() && fabs(z[0]) < __builtin_inf())) != 0;
+#pragma unroll
+    for (int m = 32; m; m >>= 1) am = fmax(am, __shfl_xor(am, m, 64));
+    int grow;
+    const float scale = block_scale(am, bad, old, grow);
+    if (p == 0) *sp = scale;
+    if (!on) return;
+    const double inv = scale > 0.0f ? 1.0 / (double)scale : 0.0;
+    const int q0 = bad ? 0 : quant8(x[0], inv), q1 = bad ? 0 : quant8(z[0], inv);
+    // K: slot s0 of 16 rows; V: column s0
+    int8_t* base = (isv ? a.v : a.k) + blk * LGX_PAGE * D;
+    const int ds = isv ? LGX_PAGE : 1, ts = isv ? 1 : D;
+    if (grow > 0)
+        for (int t = 0; t < s0; ++t) {
+            int8_t *e0 = base + i0 * ds + t * ts, *e1 = base + i1 * ds + t * ts;
+            *e0 = (int8_t)halve8(*e0, grow);
+            *e1 = (int8_t)halve8(*e1, grow);
+        }
+    base[i0 * ds + s0 * ts] = (int8_t)q0;
+    base[i1 * ds + s0 * ts] = (int8_t)q1;
+}
+extern "C" __global__ __launch_bounds__(256) void lgx_k_kv8_append1_d64(const lgx_kv8_append_args a) { kv8_append1_body<64>(a); }
+extern "C" __global__ __launch_bounds__(256) void lgx_k_kv8_append1_d128(const lgx_kv8_append_args a) { kv8_append1_body<128>(a); }
 
 // ---------------------------------------------------------------------------
 // Read-back: tokens start[b] .. + n of every sequence as binary32.  Workgroup
