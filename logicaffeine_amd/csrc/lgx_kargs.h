@@ -478,3 +478,4 @@ typedef struct {
     float scale, softcap;
 } lgx_attn8_args;
 #define LGX_A8_TILE 64         // tokens of a tile: four pages
+#define LGX_A8_SPLITS 512      // splits at most

@@ -26,19 +26,19 @@ lgx_status check_kv(const lgx_kv_i8* kv, int32_t maxp) {
 int pages_touched(int n) { return (int)(((int64_t)n + LGX_PAGE - 2) / LGX_PAGE + 1); }
 
 // (row, head) pairs of a workgroup.
-int attn8_cols(int64_t cols) { return cols <= 16 ? 16 : 128; }
+int attn8_cols(const lgx_ctx* c, int64_t cols) { return cols <= c->attn8_narrow ? 16 : 128; }
 
 // Splits of the visible tiles: two workgroups per compute unit, a tile per wave
 // at least.
 lgx_status run_attn8(lgx_ctx* c, lgx_attn8_args& a, int B, int d, bool x, void* stream) {
     const int64_t cols = (int64_t)a.P * (a.hq / a.hkv);
-    const int nc = attn8_cols(cols), wt = nc == 16 ? 4 : 1;
+    const int nc = attn8_cols(c, cols), wt = nc == 16 ? 4 : 1;
     const int64_t ncb = (cols + nc - 1) / nc, blocks = (int64_t)B * a.hkv * ncb;
     // a block's rows are at most nc apart
     int64_t tiles = cdiv(a.maxlen, LGX_A8_TILE);
     if (a.window) tiles = std::min<int64_t>(tiles, ((int64_t)a.window + nc) / LGX_A8_TILE + 2);
-    const int64_t want = std::max<int64_t>(1, 2 * (int64_t)c->ncu / blocks);
-    const int64_t cps = std::max<int64_t>((tiles + want - 1) / want + wt - 1, wt) / wt * wt;
+    const int64_t want = std::min<int64_t>(std::max<int64_t>(1, (int64_t)c->attn8_wgs * c->ncu / blocks), LGX_A8_SPLITS);
+    const int64_t cps = ((tiles + want - 1) / want + wt - 1) / wt * wt;
     a.ncb = (int)ncb;
     a.cps = (int)cps;
     a.nsplit = (int)((tiles + cps - 1) / cps);
@@ -51,7 +51,7 @@ lgx_status run_attn8(lgx_ctx* c, lgx_attn8_args& a, int B, int d, bool x, void* 
         return st;
     const int k = (d == 64 ? K_ATTN8_D64 : K_ATTN8_D128) + (nc == 16 ? 0 : 2) + (x ? 1 : 0);
     if ((st = launch(c, (Kern)k, dim3((unsigned)grid), dim3(256), a, stream)) != LGX_OK || a.nsplit == 1) return st;
-    return launch(c, d == 64 ? K_ATTN8_MERGE_D64 : K_ATTN8_MERGE_D128, dim3((unsigned)rh), dim3(d), a, stream);
+    return launch(c, d == 64 ? K_ATTN8_MERGE_D64 : K_ATTN8_MERGE_D128, dim3((unsigned)rh), dim3(256), a, stream);
 }
 
 lgx_status attn8(lgx_ctx* c, const float* q, const lgx_kv_i8* kv, const int32_t* page_table,
@@ -96,7 +96,7 @@ lgx_status attn8(lgx_ctx* c, const float* q, const lgx_kv_i8* kv, const int32_t*
     a.maxlen = max_seq_len;
     a.len_add = len_add;
     a.rows = B * P;
-    return run_attn8(c, a, B, kv->d, a.softcap > 0.0f || a.window > 0 || a.slopes != nullptr, stream);
+    return run_attn8(c, a, B, kv->d, a.softcap > 0.0f || a.window > 0 || a.slopes != nullptr || a.scale < 0.0f, stream);
 }
 
 }  // namespace

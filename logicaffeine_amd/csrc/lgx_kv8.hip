@@ -390,38 +390,45 @@ extern "C" __global__ __launch_bounds__(256) void lgx_k_kv8_append1_d128(const l
 
 // ---------------------------------------------------------------------------
 // Read-back: tokens start[b] .. + n of every sequence as binary32.  Workgroup
-// (block of 16 token slots of sequence b, KV head); V's block passes through LDS
-// to come out token by token.
+// (block of 16 token slots of sequence b, KV head).  K: thread (slot, c) has d / 16
+// neighbouring values.  V: a thread has a run of tokens of one dimension, so that
+// neighbouring threads write neighbouring dimensions of a row.
 // ---------------------------------------------------------------------------
 template <int D>
 __device__ __forceinline__ void kv8_read_body(const lgx_kv8_read_args& a) {
-    constexpr int E = D / 16;
-    __shared__ __align__(16) int8_t v_s[D * LGX_PAGE];
+    constexpr int E = D / 16, NT = LGX_PAGE * D / 256;   // tokens of a thread's V run: 8 or 4
     const int tid = threadIdx.x, slot = tid >> 4, e0 = (tid & 15) * E;
     const int b = blockIdx.x / a.nblk, g = blockIdx.y;
     const int st = min(max(a.start[b], 0), a.maxp * LGX_PAGE);
     const int pb = st / LGX_PAGE + (blockIdx.x - b * a.nblk);
-    const int64_t row = (int64_t)pb * LGX_PAGE + slot - st;
-    const bool has = pb < a.maxp;                 // uniform
+    const int64_t row0 = (int64_t)pb * LGX_PAGE - st;    // row of slot 0, possibly before the first
+    const bool has = pb < a.maxp;                        // uniform
     const int page = has ? min(max(a.page_table[(int64_t)b * a.maxp + pb], 0), a.num_pages - 1) : 0;
     const int64_t blk = (int64_t)page * a.hkv + g;
-    if (tid < D) *(uint4*)(v_s + tid * LGX_PAGE) = *(const uint4*)(a.v + (blk * D + tid) * LGX_PAGE);
-    __syncthreads();
-    if (row < 0 || row >= a.n) return;
     const float ks = has ? a.ks[blk] : 0.0f, vs = has ? a.vs[blk] : 0.0f;
-    const int8_t* kr = a.k + (blk * LGX_PAGE + slot) * D + e0;
-    const int64_t o = (((int64_t)b * a.n + row) * a.hkv + g) * D + e0;
-#pragma unroll
-    for (int e = 0; e < E; e += 4) {
-        float kf[4], vf[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            kf[i] = has ? ks * (float)kr[e + i] : 0.0f;
-            vf[i] = has ? vs * (float)v_s[(e0 + e + i) * LGX_PAGE + slot] : 0.0f;
-        }
-        *(float4*)(a.k_out + o + e) = make_float4(kf[0], kf[1], kf[2], kf[3]);
-        *(float4*)(a.v_out + o + e) = make_float4(vf[0], vf[1], vf[2], vf[3]);
+    int8_t kq[E], vq[NT];
+    const int dim = tid % D, t0 = tid / D * NT;
+    if (E == 8) {
+        *(uint2*)kq = *(const uint2*)(a.k + (blk * LGX_PAGE + slot) * D + e0);
+        *(uint2*)vq = *(const uint2*)(a.v + (blk * D + dim) * LGX_PAGE + t0);
+    } else {
+        *(uint32_t*)kq = *(const uint32_t*)(a.k + (blk * LGX_PAGE + slot) * D + e0);
+        *(uint32_t*)vq = *(const uint32_t*)(a.v + (blk * D + dim) * LGX_PAGE + t0);
     }
+    auto at = [&](int64_t row) { return (((int64_t)b * a.n + row) * a.hkv + g) * D; };
+    auto on = [&](int64_t row) { return row >= 0 && row < a.n; };
+    if (on(row0 + slot)) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = has ? ks * (float)kq[e + i] : 0.0f;
+            *(float4*)(a.k_out + at(row0 + slot) + e0 + e) = make_float4(f[0], f[1], f[2], f[3]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+        if (on(row0 + t0 + t)) a.v_out[at(row0 + t0 + t) + dim] = has ? vs * (float)vq[t] : 0.0f;
 }
 extern "C" __global__ __launch_bounds__(256) void lgx_k_kv8_read_d64(const lgx_kv8_read_args a) { kv8_read_body<64>(a); }
 extern "C" __global__ __launch_bounds__(256) void lgx_k_kv8_read_d128(const lgx_kv8_read_args a) { kv8_read_body<128>(a); }
@@ -469,305 +476,569 @@ __device__ __forceinline__ float a8_tanh(float x) {
     return ax < 0.35f ? fmaf(x * y, p, x) : big;
 }
 
-// Maximum over the four lanes of a column.
+// Joins over the four lanes of a column: the swaps leave a row of 16 lanes beside
+// its neighbour's, then half a wave beside the other.
+__device__ __forceinline__ float col_join16(float v, float& other) {
+    typedef unsigned v2u __attribute__((ext_vector_type(2)));
+    const unsigned x = __float_as_uint(v);
+    const v2u r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    other = __uint_as_float(r[1]);
+    return __uint_as_float(r[0]);
+}
+__device__ __forceinline__ float col_join32(float v, float& other) {
+    typedef unsigned v2u __attribute__((ext_vector_type(2)));
+    const unsigned x = __float_as_uint(v);
+    const v2u r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    other = __uint_as_float(r[1]);
+    return __uint_as_float(r[0]);
+}
 __device__ __forceinline__ float col_max(float v) {
-    v = fmaxf(v, shfl_xor_f(v, 16));
-    return fmaxf(v, shfl_xor_f(v, 32));
+    float w;
+    v = col_join16(v, w);
+    v = fmaxf(v, w);
+    v = col_join32(v, w);
+    return fmaxf(v, w);
 }
 __device__ __forceinline__ float col_sum(float v) {
-    v = v + shfl_xor_f(v, 16);
-    return v + shfl_xor_f(v, 32);
+    float w;
+    v = col_join16(v, w);
+    v = v + w;
+    v = col_join32(v, w);
+    return v + w;
 }
 
-// Four waves: WC of them side by side over the columns (16 NT each), the others
-// over the tiles.  X: capped scores, distance bias or a window.
-template <int D, int NT, int WC, bool X>
-__device__ __forceinline__ void attn8_body(const lgx_attn8_args& a) {
-    constexpr int WT = 4 / WC, NC = 16 * NT * WC, NS = D / 64, ND = D / 16;
-    constexpr float kLog2e = 1.44269504088896341f, kUp = 8192.0f;
-    __shared__ v4f o_s[WT > 1 ? WC * (WT / 2) * NT * ND * 64 : 1];
-    __shared__ float ml_s[WT > 1 ? WC * (WT / 2) * NT * 3 * 64 : 1];
-    const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wc = wave % WC, wt = wave / WC;
-    const int cb = blockIdx.x % a.ncb, rest = blockIdx.x / a.ncb;
-    const int sp = rest % a.nsplit, bg = rest / a.nsplit;
-    const int b = bg / a.hkv, g = bg - b * a.hkv;
-    const int G = a.hq / a.hkv;
-    const int nn = a.n_new ? min(max(a.n_new[b], 0), a.P) : a.P;
-    const int ncols = nn * G, c0 = cb * NC;
-    if (c0 >= ncols) return;                      // uniform
-    const int sl = max(a.seq_len[b], 0);
+// What a workgroup of NC columns sees: its sequence, rows, tiles.
+struct A8Block {
+    int b, g, G, sp, c0, ncols, sl;
+    int tb0, tb1;      // tiles of the split
+};
+template <int NC, bool X>
+struct A8 {
+    const lgx_attn8_args& a;
+    A8Block k;
     // tokens that the row of column c sees: [first(c), last(c))
-    auto last = [&](int c) { return (int)min((int64_t)sl + c / G + a.len_add, (int64_t)a.maxlen); };
-    auto first = [&](int c) { return X && a.window ? max(last(c) - a.window, 0) : 0; };
-    // the split's tiles
-    const int tb0 = first(c0) / LGX_A8_TILE + sp * a.cps;
-    const int tb1 = min((last(min(c0 + NC, ncols) - 1) + LGX_A8_TILE - 1) / LGX_A8_TILE, tb0 + a.cps);
+    __device__ __forceinline__ int last(int c) const {
+        return (int)min((int64_t)k.sl + c / k.G + a.len_add, (int64_t)a.maxlen);
+    }
+    __device__ __forceinline__ int first(int c) const { return X && a.window ? max(last(c) - a.window, 0) : 0; }
+    // false: no column
+    __device__ __forceinline__ bool place() {
+        const int cb = blockIdx.x % a.ncb, rest = blockIdx.x / a.ncb;
+        k.sp = rest % a.nsplit;
+        const int bg = __builtin_amdgcn_readfirstlane(rest / a.nsplit);
+        k.b = __builtin_amdgcn_readfirstlane(bg / a.hkv);
+        k.g = bg - k.b * a.hkv;
+        k.G = a.hq / a.hkv;
+        const int nn = a.n_new ? min(max(a.n_new[k.b], 0), a.P) : a.P;
+        k.ncols = nn * k.G;
+        k.c0 = cb * NC;
+        if (k.c0 >= k.ncols) return false;
+        k.sl = max(a.seq_len[k.b], 0);
+        k.tb0 = first(k.c0) / LGX_A8_TILE + k.sp * a.cps;
+        k.tb1 = min((last(min(k.c0 + NC, k.ncols) - 1) + LGX_A8_TILE - 1) / LGX_A8_TILE, k.tb0 + a.cps);
+        return true;
+    }
+};
 
-    const int wcol = c0 + wc * 16 * NT;           // the wave's first column
-    int L[NT], lo[NT];
-    int64_t orow[NT];                             // (row, head) of the lane's column
-    float f[NT], slope[NT];
-    v4i qd[NT][3][NS];
+// The query of a lane's column: its digits as B operands, the factor that turns
+// an integer score (times the page's K scale) into a score (in base 2 unless X).
+template <int D, bool X>
+__device__ __forceinline__ float a8_query(const lgx_attn8_args& a, const float* qr, v4i (&qd)[3][D / 64]) {
+    constexpr int NS = D / 64;
+    float x[NS][16], am = 0.0f;
+    bool bad = false;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int c = wcol + 16 * n + col;
-        const bool ok = c < ncols;
-        const int cc = ok ? c : ncols - 1;
-        L[n] = ok ? last(cc) : 0;
-        lo[n] = ok ? first(cc) : 0;
-        orow[n] = ((int64_t)b * a.P + cc / G) * a.hq + g * G + cc % G;
-        slope[n] = X && a.slopes ? a.slopes[g * G + cc % G] : 0.0f;
-        const float* qr = a.q + orow[n] * D + 16 * kg;
-        float x[NS][16], am = 0.0f;
-        bool bad = false;
+    for (int s = 0; s < NS; ++s)
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+        for (int e = 0; e < 16; e += 4) {
+            const float4 v = *(const float4*)(qr + 64 * s + e);
+            x[s][e] = v.x;
+            x[s][e + 1] = v.y;
+            x[s][e + 2] = v.z;
+            x[s][e + 3] = v.w;
+        }
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const float4 v = *(const float4*)(qr + 64 * s + e);
-                x[s][e] = v.x;
-                x[s][e + 1] = v.y;
-                x[s][e + 2] = v.z;
-                x[s][e + 3] = v.w;
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            am = fmaxf(am, fabsf(x[s][e]));
+            bad = bad || !(fabsf(x[s][e]) < __builtin_inff());
+        }
+    am = col_max(am);
+    const bool isbad = col_max(bad ? 1.0f : 0.0f) != 0.0f;
+    // the largest power of two that keeps every |q| within 127 * 65536, the
+    // range of three balanced digits
+    const float up = __uint_as_float(__float_as_uint(fminf(8323072.0f / am, 0x1p100f)) & 0x7f800000u);
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float y = isbad ? 0.0f : x[s][4 * w + e] * up;
+                v[e] = ((uint32_t)(int)rintf(y) + 0x808080u) ^ 0x808080u;
             }
+            // byte i of the four numbers is digit i
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                am = fmaxf(am, fabsf(x[s][e]));
-                bad = bad || !(fabsf(x[s][e]) < __builtin_inff());
+            for (int i = 0; i < 3; ++i) {
+                const uint32_t sel = 0x0c0c0000u | (uint32_t)(4 + i) << 8 | (uint32_t)i;
+                const uint32_t p01 = __builtin_amdgcn_perm(v[1], v[0], sel);
+                const uint32_t p23 = __builtin_amdgcn_perm(v[3], v[2], sel);
+                qd[i][s][w] = (int)(p01 | p23 << 16);
             }
-        am = col_max(am);
-        const float isbad = col_max(bad ? 1.0f : 0.0f);
-        // the largest power of two that keeps every |q| within 127 * 65536, the
-        // range of three balanced digits
-        const float up = __uint_as_float(__float_as_uint(fminf(8323072.0f / am, 0x1p100f)) & 0x7f800000u);
-        f[n] = isbad != 0.0f ? __builtin_nanf("") : a.scale / up;
-        if (!X) f[n] *= kLog2e;
+        }
+    return isbad ? __builtin_nanf("") : a.scale / up * (X ? 1.0f : 1.44269504088896341f);
+}
+
+// Integer scores of a tile for one column tile: S[4 u + v] is token 4 u + v of
+// page kg.  kf(u, s): K fragment of sub-tile u, dimensions 64 s ..
+template <int NS, class KF>
+__device__ __forceinline__ void a8_scores(const KF& kf, const v4i (&qd)[3][NS], float (&S)[16]) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+    for (int u = 0; u < 4; ++u) {
+        v4i c2 = {0, 0, 0, 0}, c1 = {0, 0, 0, 0}, c0 = {0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                uint32_t v[4];
+        for (int s = 0; s < NS; ++s) {
+            const v4i kv = __builtin_bit_cast(v4i, kf(u, s));
+            c2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv, qd[2][s], c2, 0, 0, 0);
+            c1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv, qd[1][s], c1, 0, 0, 0);
+            c0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv, qd[0][s], c0, 0, 0, 0);
+        }
+        // |c1| 256 + |c0| < 2^30
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float y = isbad != 0.0f ? 0.0f : x[s][4 * w + e] * up;
-                    v[e] = ((uint32_t)(int)rintf(y) + 0x808080u) ^ 0x808080u;
-                }
-                // byte i of the four numbers is digit i
-#pragma unroll
-                for (int i = 0; i < 3; ++i) {
-                    const uint32_t sel = 0x0c0c0000u | (uint32_t)(4 + i) << 8 | (uint32_t)i;
-                    const uint32_t p01 = __builtin_amdgcn_perm(v[1], v[0], sel);
-                    const uint32_t p23 = __builtin_amdgcn_perm(v[3], v[2], sel);
-                    qd[n][i][s][w] = (int)(p01 | p23 << 16);
-                }
-            }
+        for (int v = 0; v < 4; ++v) S[4 * u + v] = fmaf((float)c2[v], 65536.0f, (float)(c1[v] * 256 + c0[v]));
     }
-    float m[NT], l[NT], vref = 0x1p-126f;
-    v4f o[NT][ND];
+}
+
+// One column's running softmax; L, lo: the tokens it sees.
+struct A8Col {
+    float f, slope, m, l;
+    int L, lo;
+};
+// From integer scores to the tile's weights as two binary16 parts.  pt: the first
+// token of the lane's page, t0 of the tile; r: the page's V scale in units of the
+// running reference.  Returns the factor of what was summed before.
+template <bool X>
+__device__ __forceinline__ float a8_weights(const lgx_attn8_args& a, float (&S)[16], A8Col& c, float ks, float r, int t0, int pt,
+                                            v8h (&ph)[2], v8h (&pl)[2]) {
+    constexpr float kLog2e = 1.44269504088896341f;
+    const float fk = c.f * ks;
+    float mt;
+    // uniform: some column does not see the whole tile
+    const bool edge = __builtin_amdgcn_ballot_w64(t0 + LGX_A8_TILE > c.L || t0 < c.lo) != 0;
+    if (X || edge) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        m[n] = -__builtin_inff();
-        l[n] = 0.0f;
+        for (int e = 0; e < 16; ++e) S[e] *= fk;
+        if constexpr (X) {
+            if (a.softcap > 0.0f) {
+                const float inv = 1.0f / a.softcap;
 #pragma unroll
-        for (int i = 0; i < ND; ++i) o[n][i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+                for (int e = 0; e < 16; ++e) S[e] = a.softcap * a8_tanh(S[e] * inv);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) S[e] = (S[e] - c.slope * (float)(c.L - 1 - (pt + e))) * kLog2e;
+        }
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (pt + e >= c.L || pt + e < c.lo) S[e] = -__builtin_inff();
+        }
     }
-    // the wave's own tiles: those that its columns see
-    const int wlast = min(wcol + 16 * NT, ncols) - 1;
-    const int wt0 = wcol < ncols ? first(wcol) / LGX_A8_TILE : 0;
-    const int wt1 = wcol < ncols ? min(tb1, (last(wlast) + LGX_A8_TILE - 1) / LGX_A8_TILE) : 0;
-    const int wend = wcol < ncols ? last(wlast) : 0, wbeg = wcol < ncols ? first(wcol) : 0;
+    mt = S[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mt = fmaxf(mt, S[e]);
+    if (!(X || edge)) mt *= fk;                   // scales are not negative
+    const float mn = fmaxf(c.m, col_max(mt));
+    const bool none = mn == -__builtin_inff();    // nothing seen yet
+    const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(c.m - mn);
+    const float mref = none ? 0.0f : mn;
+    c.m = mn;
+    float w[16], ps = 0.0f;
+    if (X || edge) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) S[e] = __builtin_amdgcn_exp2f(S[e] - mref);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) S[e] = __builtin_amdgcn_exp2f(fmaf(S[e], fk, -mref));
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        ps += S[e];
+        w[e] = S[e] * r;
+    }
+    if (edge) {
+        // a weight of 0 meets no scale (a later row's page may hold NaN)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = S[e] == 0.0f ? 0.0f : w[e];
+    }
+    c.l = c.l * alpha + ps;
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+        // the first part rounded toward zero, the second holds the rest
+        typedef __fp16 v2f __attribute__((ext_vector_type(2)));
+        const v2f hi = __builtin_amdgcn_cvt_pkrtz(w[e], w[e + 1]);
+        const _Float16 h0 = (_Float16)hi[0], h1 = (_Float16)hi[1];
+        const v2f lo = __builtin_amdgcn_cvt_pkrtz(fmaf((float)h0, -1.0f, w[e]), fmaf((float)h1, -1.0f, w[e + 1]));
+        ph[e >> 3][e & 7] = h0;
+        ph[e >> 3][(e & 7) + 1] = h1;
+        pl[e >> 3][e & 7] = (_Float16)lo[0];
+        pl[e >> 3][(e & 7) + 1] = (_Float16)lo[1];
+    }
+    return alpha;
+}
+
+// The V scale of a lane's page in units of the wave's reference: the largest
+// scale so far rounded down to a power of two, times 2^-13 (weights stay below
+// 2^14, and their second binary16 part is not subnormal where it matters).  down:
+// the old unit in the new one.
+#define A8_UP 8192.0f
+__device__ __forceinline__ float a8_vscale(float vs, float& vref, float& down) {
+    const float top = col_max(vs < __builtin_inff() ? vs : 0.0f);
+    const float vn = fmaxf(vref, __uint_as_float(__float_as_uint(top) & 0x7f800000u));
+    const float inv = __builtin_amdgcn_rcpf(vn);  // of a power of two: exact
+    down = vref * inv;
+    vref = vn;
+    return vs * inv * A8_UP;
+}
+
+// o += V^T . P^T for N column tiles; vf(i): V fragment of dimensions 16 i ..
+template <int ND, int N, class VF>
+__device__ __forceinline__ void a8_pv(const VF& vf, const v8h (&ph)[N][2], const v8h (&pl)[N][2], v4f (&o)[N][ND]) {
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+        const uint4 v = vf(i);
+        uint4 h0, h1;
+        i8_to_f16(v.x, h0.x, h0.y);
+        i8_to_f16(v.y, h0.z, h0.w);
+        i8_to_f16(v.z, h1.x, h1.y);
+        i8_to_f16(v.w, h1.z, h1.w);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h0), ph[n][0], o[n][i], 0, 0, 0);
+            o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h1), ph[n][1], o[n][i], 0, 0, 0);
+            o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h0), pl[n][0], o[n][i], 0, 0, 0);
+            o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h1), pl[n][1], o[n][i], 0, 0, 0);
+        }
+    }
+}
+
+// A column's result, or its split's: unit: the wave's V reference.
+template <int ND>
+__device__ __forceinline__ void a8_store(const lgx_attn8_args& a, int64_t orow, int sp, const A8Col& c, float vref, int kg,
+                                         const v4f (&o)[ND]) {
+    constexpr int D = 16 * ND;
+    const float unit = vref * (1.0f / A8_UP);
+    // NaN sums stay NaN; nothing seen gives zeros
+    const float s = a.nsplit > 1 ? unit : c.l == 0.0f ? 0.0f : unit / c.l;
+    float* dst = a.nsplit > 1 ? a.part + (orow * a.nsplit + sp) * D : a.out + orow * D;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+        *(float4*)(dst + 16 * i + 4 * kg) = make_float4(o[i][0] * s, o[i][1] * s, o[i][2] * s, o[i][3] * s);
+    if (a.nsplit > 1 && kg == 0) {
+        float2* ml = (float2*)(a.part + (int64_t)a.rows * a.hq * a.nsplit * D) + orow * a.nsplit + sp;
+        *ml = make_float2(c.m, c.l);
+    }
+}
+
+// Few columns (a decode row's heads): 16 per workgroup, its four waves take the
+// tiles in turn, K and V straight into registers, the next tile's in flight during
+// the current one's products; at the end the waves' results are joined in LDS.
+template <int D, bool X>
+__device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
+    constexpr int WT = 4, NS = D / 64, ND = D / 16;
+    __shared__ v4f o_s[WT / 2 * ND * 64];
+    __shared__ float ml_s[WT / 2 * 3 * 64];
+    const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
+    const int wt = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    A8<16, X> w{a, {}};
+    if (!w.place()) return;                       // uniform
+    const int b = w.k.b, g = w.k.g, G = w.k.G;
+    const int c = w.k.c0 + col, cc = min(c, w.k.ncols - 1);
+    const bool ok = c < w.k.ncols;
+    const int64_t orow = ((int64_t)b * a.P + cc / G) * a.hq + g * G + cc % G;
+    const int wlast = min(w.k.c0 + 16, w.k.ncols) - 1;
+    const int wend = w.last(wlast), wbeg = w.first(w.k.c0);
     const int32_t* ptab = a.page_table + (int64_t)b * a.maxp;
-    auto page_of = [&](int i) { return (int64_t)min(max(ptab[min(i, a.maxp - 1)], 0), a.num_pages - 1) * a.hkv + g; };
-#pragma unroll 1
-    for (int t = max(tb0, wt0) + wt; t < wt1; t += WT) {
-        const int t0 = t * LGX_A8_TILE;
-        const int64_t pk = page_of(4 * t + (col >> 2)), pv = page_of(4 * t + kg);
-        uint4 kw[4][NS], vw[ND];
+    struct Pages {
+        int k, v;
+    };
+    struct Tile {
+        uint4 k[4][NS], v[ND];
+        float ks, vs;
+    };
+    auto pages = [&](int t) {
+        Pages p;
+        p.k = ptab[min(4 * t + (col >> 2), a.maxp - 1)];
+        p.v = ptab[min(4 * t + kg, a.maxp - 1)];
+        return p;
+    };
+    auto load = [&](Tile& x, int t, const Pages& p) __attribute__((always_inline)) {
+        const int64_t pk = (int64_t)min(max(p.k, 0), a.num_pages - 1) * a.hkv + g;
+        const int64_t pv = (int64_t)min(max(p.v, 0), a.num_pages - 1) * a.hkv + g;
+        x.ks = a.ks[pv];
+        x.vs = a.vs[pv];
+        const int8_t* kp = a.k + (pk * LGX_PAGE + (col & 3)) * D + 16 * kg;
+        const int8_t* vp = a.v + (pv * D + col) * LGX_PAGE;
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int s = 0; s < NS; ++s)
-                kw[u][s] = *(const uint4*)(a.k + (pk * LGX_PAGE + 4 * u + (col & 3)) * D + 64 * s + 16 * kg);
+            for (int s = 0; s < NS; ++s) x.k[u][s] = *(const uint4*)(kp + 4 * u * D + 64 * s);
 #pragma unroll
-        for (int i = 0; i < ND; ++i) vw[i] = *(const uint4*)(a.v + (pv * D + 16 * i + col) * LGX_PAGE);
-        // a page outside the wave's tokens may hold anything
-        const int pt = t0 + 16 * kg;
+        for (int i = 0; i < ND; ++i) x.v[i] = *(const uint4*)(vp + 16 * i * LGX_PAGE);
+    };
+    float vref = 0x1p-126f;
+    v4f o[1][ND];
+#pragma unroll
+    for (int i = 0; i < ND; ++i) o[0][i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    A8Col k;
+    k.m = -__builtin_inff();
+    k.l = 0.0f;
+    k.L = ok ? w.last(cc) : 0;
+    k.lo = ok ? w.first(cc) : 0;
+    k.slope = X && a.slopes ? a.slopes[g * G + cc % G] : 0.0f;
+    v4i qd[3][NS];
+    auto run = [&](const Tile& x, int t) __attribute__((always_inline)) {
+        const int t0 = t * LGX_A8_TILE, pt = t0 + 16 * kg;
+        float S[16], vdown;
+        a8_scores<NS>([&](int u, int s) { return x.k[u][s]; }, qd, S);
+        // a page outside the tokens seen may hold anything
         const bool live = pt < wend && pt + LGX_PAGE > wbeg;
-        const float ks = a.ks[pv], vsc = live ? a.vs[pv] : 0.0f;
-        // weights are in units of the largest V scale so far, rounded down to a
-        // power of two, times 2^-13 (they stay below 2^14, and their second
-        // binary16 part is not subnormal where it matters)
-        const float vtop = col_max(vsc < __builtin_inff() ? vsc : 0.0f);
-        const float vnew = fmaxf(vref, __uint_as_float(__float_as_uint(vtop) & 0x7f800000u));
-        const float r = vsc * (1.0f / vnew) * kUp, vdown = vref / vnew;
-        vref = vnew;
+        const float r = a8_vscale(live ? x.vs : 0.0f, vref, vdown);
+        v8h ph[1][2], pl[1][2];
+        const float down = a8_weights<X>(a, S, k, x.ks, r, t0, pt, ph[0], pl[0]) * vdown;
+        if (__builtin_amdgcn_ballot_w64(down != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < ND; ++i) o[0][i] *= down;
+        }
+        a8_pv<ND, 1>([&](int i) { return x.v[i]; }, ph, pl, o);
+    };
+    int t = w.k.tb0 + wt;
+    const int end = w.k.tb1;
+    Tile x, y;
+    if (t < end) load(x, t, pages(t));
+    Pages p = pages(t + WT);                      // indexes are clamped
+    k.f = a8_query<D, X>(a, a.q + orow * D + 16 * kg, qd);
+#pragma unroll 1
+    for (; t < end; t += 2 * WT) {
+        if (t + WT < end) load(y, t + WT, p);
+        p = pages(t + 2 * WT);
+        run(x, t);
+        if (t + WT >= end) break;
+        if (t + 2 * WT < end) load(x, t + 2 * WT, p);
+        p = pages(t + 3 * WT);
+        run(y, t + WT);
+    }
+    k.l = col_sum(k.l);
+    // join the waves, halving their number
+#pragma unroll
+    for (int h = WT / 2; h; h >>= 1) {
+        const int at = wt % h;
+        if (wt >= h && wt < 2 * h) {
+            ml_s[(at * 3 + 0) * 64 + lane] = k.m;
+            ml_s[(at * 3 + 1) * 64 + lane] = k.l;
+            ml_s[(at * 3 + 2) * 64 + lane] = vref;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) o_s[(at * ND + i) * 64 + lane] = o[0][i];
+        }
+        __syncthreads();
+        if (wt < h) {
+            const float mo = ml_s[(at * 3 + 0) * 64 + lane], lo = ml_s[(at * 3 + 1) * 64 + lane];
+            const float vo = ml_s[(at * 3 + 2) * 64 + lane], vn = fmaxf(vref, vo), mn = fmaxf(k.m, mo);
+            const float w0 = k.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(k.m - mn);
+            const float w1 = mo == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mo - mn);
+            k.l = k.l * w0 + lo * w1;
+            k.m = mn;
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+                o[0][i] = o[0][i] * (w0 * (vref / vn)) + o_s[(at * ND + i) * 64 + lane] * (w1 * (vo / vn));
+            vref = vn;
+        }
+        __syncthreads();
+    }
+    if (wt == 0 && ok) a8_store<ND>(a, orow, w.k.sp, k, vref, kg, o[0]);
+}
+
+// Many columns (prefill): 128 per workgroup, 32 per wave; every tile passes through
+// LDS once for all of them, by direct global->LDS loads into two buffers, each wave
+// instruction bringing one operand fragment (1 KiB) in the order of the lanes.
+template <int D, bool X>
+__device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
+    constexpr int NT = 2, NS = D / 64, ND = D / 16, NF = 4 * NS + ND, FW = NF / 4;
+    static_assert(4 * NS == ND, "waves 0 and 1 bring K, 2 and 3 bring V");
+    typedef __attribute__((address_space(3))) const uint4 lds_c4;
+    // two variables: a direct load into one is known not to alias reads of the other
+    __shared__ __align__(16) uint4 b0_s[NF * 64], b1_s[NF * 64];
+    const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    A8<64 * NT, X> w{a, {}};
+    if (!w.place()) return;                       // uniform
+    const int b = w.k.b, g = w.k.g, G = w.k.G;
+    const int wcol = w.k.c0 + wave * 16 * NT;     // the wave's first column
+    const bool any = wcol < w.k.ncols;            // uniform per wave
+    const int wlast = min(wcol + 16 * NT, w.k.ncols) - 1;
+    const int wend = any ? w.last(wlast) : 0, wbeg = any ? w.first(wcol) : 0;
+    A8Col k[NT];
+    v4i qd[NT][3][NS];
+    int64_t orow[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int c = wcol + 16 * n + col, cc = min(c, w.k.ncols - 1);
+        const bool ok = c < w.k.ncols;
+        orow[n] = ((int64_t)b * a.P + cc / G) * a.hq + g * G + cc % G;
+        k[n].m = -__builtin_inff();
+        k[n].l = 0.0f;
+        k[n].L = ok ? w.last(cc) : 0;
+        k[n].lo = ok ? w.first(cc) : 0;
+        k[n].slope = X && a.slopes ? a.slopes[g * G + cc % G] : 0.0f;
+        k[n].f = a8_query<D, X>(a, a.q + orow[n] * D + 16 * kg, qd[n]);
+    }
+    const int32_t* ptab = a.page_table + (int64_t)b * a.maxp;
+    // the page of the wave's direct loads, and of the lane's scales
+    struct Pages {
+        int ld, sc;
+    };
+    auto pages = [&](int t) {
+        Pages p;
+        p.ld = ptab[min(4 * t + (wave < 2 ? col >> 2 : kg), a.maxp - 1)];
+        p.sc = ptab[min(4 * t + kg, a.maxp - 1)];
+        return p;
+    };
+    auto block = [&](int p) { return (int64_t)min(max(p, 0), a.num_pages - 1) * a.hkv + g; };
+    auto stage = [&](uint4* buf, int p) __attribute__((always_inline)) {
+        const int64_t blk = block(p);
+        const int8_t* src = wave < 2 ? a.k + (blk * LGX_PAGE + (col & 3)) * D + 16 * kg : a.v + (blk * D + col) * LGX_PAGE;
+#pragma unroll
+        for (int j = 0; j < FW; ++j) {
+            const int f = (wave & 1) * FW + j;
+            const int off = wave < 2 ? 4 * (f / NS) * D + 64 * (f % NS) : 16 * f * LGX_PAGE;
+            load_lds_16(src + off, (lds_void*)(buf + (wave * FW + j) * 64));
+        }
+    };
+    float vref = 0x1p-126f;
+    v4f o[NT][ND];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[n][i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    struct Scales {
+        float k, v;
+    };
+    auto scales = [&](int p) {
+        const int64_t blk = block(p);
+        return Scales{a.ks[blk], a.vs[blk]};
+    };
+    const int end = w.k.tb1;
+    // tile t from buf (landed), the next one's loads into nbuf
+    auto run = [&](const uint4* buf, uint4* nbuf, int t, Scales& sc, Pages& p) __attribute__((always_inline)) {
+        publish_lds_loads();                      // tile t landed; tile t - 1 read
+        const Scales now = sc;
+        if (t + 1 < end) {
+            stage(nbuf, p.ld);
+            sc = scales(p.sc);
+            p = pages(t + 2);
+        }
+        const int t0 = t * LGX_A8_TILE, pt = t0 + 16 * kg;
+        if (t0 >= wend || t0 + LGX_A8_TILE <= wbeg) return;   // uniform per wave
+        lds_c4* fr = (lds_c4*)buf + lane;
+        // a page outside the tokens seen may hold anything
+        const bool live = pt < wend && pt + LGX_PAGE > wbeg;
+        float vdown;
+        const float r = a8_vscale(live ? now.v : 0.0f, vref, vdown);
+        v8h ph[NT][2], pl[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float z[16];
-            const float fk = f[n] * ks;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                v4i c2 = {0, 0, 0, 0}, c1 = {0, 0, 0, 0}, c0_ = {0, 0, 0, 0};
-#pragma unroll
-                for (int s = 0; s < NS; ++s) {
-                    const v4i kv = __builtin_bit_cast(v4i, kw[u][s]);
-                    c2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv, qd[n][2][s], c2, 0, 0, 0);
-                    c1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv, qd[n][1][s], c1, 0, 0, 0);
-                    c0_ = __builtin_amdgcn_mfma_i32_16x16x64_i8(kv, qd[n][0][s], c0_, 0, 0, 0);
-                }
-                // |c1| 256 + |c0| < 2^30
-#pragma unroll
-                for (int v = 0; v < 4; ++v)
-                    z[4 * u + v] = fmaf((float)c2[v], 65536.0f, (float)(c1[v] * 256 + c0_[v])) * fk;
-            }
-            const bool edge = __builtin_amdgcn_ballot_w64(t0 + LGX_A8_TILE > L[n] || t0 < lo[n]) != 0;
-            if constexpr (X) {
-                if (a.softcap > 0.0f) {
-                    const float inv = 1.0f / a.softcap;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) z[e] = a.softcap * a8_tanh(z[e] * inv);
-                }
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    z[e] = (z[e] - slope[n] * (float)(L[n] - 1 - (pt + e))) * kLog2e;
-            }
-            if (edge) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (pt + e >= L[n] || pt + e < lo[n]) z[e] = -__builtin_inff();
-            }
-            float mt = z[0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) mt = fmaxf(mt, z[e]);
-            const float mn = fmaxf(m[n], col_max(mt));
-            const bool none = mn == -__builtin_inff();   // nothing seen yet
-            const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
-            const float mref = none ? 0.0f : mn;
-            m[n] = mn;
-            float ps = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                z[e] = __builtin_amdgcn_exp2f(z[e] - mref);
-                ps += z[e];
-            }
-            l[n] = l[n] * alpha + ps;
-            const float down = alpha * vdown;
+            float S[16];
+            a8_scores<NS>([&](int u, int s) -> uint4 { return fr[(u * NS + s) * 64]; }, qd[n], S);
+            const float down = a8_weights<X>(a, S, k[n], now.k, r, t0, pt, ph[n], pl[n]) * vdown;
             if (__builtin_amdgcn_ballot_w64(down != 1.0f)) {
 #pragma unroll
                 for (int i = 0; i < ND; ++i) o[n][i] *= down;
             }
-            v8h ph[2], pl[2];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                // a weight of 0 meets no scale (a later row's page may hold NaN)
-                const float w = z[e] == 0.0f ? 0.0f : z[e] * r;
-                ph[e >> 3][e & 7] = (_Float16)w;
-                pl[e >> 3][e & 7] = (_Float16)(w - (float)ph[e >> 3][e & 7]);
-            }
-#pragma unroll
-            for (int i = 0; i < ND; ++i) {
-                uint4 h0, h1;
-                i8_to_f16(vw[i].x, h0.x, h0.y);
-                i8_to_f16(vw[i].y, h0.z, h0.w);
-                i8_to_f16(vw[i].z, h1.x, h1.y);
-                i8_to_f16(vw[i].w, h1.z, h1.w);
-                o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h0), ph[0], o[n][i], 0, 0, 0);
-                o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h1), ph[1], o[n][i], 0, 0, 0);
-                o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h0), pl[0], o[n][i], 0, 0, 0);
-                o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h1), pl[1], o[n][i], 0, 0, 0);
-            }
         }
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) l[n] = col_sum(l[n]);
-    // join the waves that share columns, halving their number
-    if constexpr (WT > 1) {
-#pragma unroll
-        for (int h = WT / 2; h; h >>= 1) {
-            const int at = (wc * (WT / 2) + wt % h) * NT;
-            if (wt >= h && wt < 2 * h) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    ml_s[((at + n) * 3 + 0) * 64 + lane] = m[n];
-                    ml_s[((at + n) * 3 + 1) * 64 + lane] = l[n];
-                    ml_s[((at + n) * 3 + 2) * 64 + lane] = vref;
-#pragma unroll
-                    for (int i = 0; i < ND; ++i) o_s[((at + n) * ND + i) * 64 + lane] = o[n][i];
-                }
-            }
-            __syncthreads();
-            if (wt < h) {
-                const float vo = ml_s[(at * 3 + 2) * 64 + lane];
-                const float vn = fmaxf(vref, vo);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float mo = ml_s[((at + n) * 3 + 0) * 64 + lane], lo_ = ml_s[((at + n) * 3 + 1) * 64 + lane];
-                    const float mn = fmaxf(m[n], mo);
-                    const float w0 = m[n] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[n] - mn);
-                    const float w1 = mo == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mo - mn);
-                    l[n] = l[n] * w0 + lo_ * w1;
-                    m[n] = mn;
-#pragma unroll
-                    for (int i = 0; i < ND; ++i)
-                        o[n][i] = o[n][i] * (w0 * (vref / vn)) + o_s[((at + n) * ND + i) * 64 + lane] * (w1 * (vo / vn));
-                }
-                vref = vn;
-            }
-            __syncthreads();
+        a8_pv<ND, NT>([&](int i) -> uint4 { return fr[(4 * NS + i) * 64]; }, ph, pl, o);
+    };
+    if (w.k.tb0 < end) {
+        Pages p = pages(w.k.tb0);
+        stage(b0_s, p.ld);
+        Scales sc = scales(p.sc);
+        p = pages(w.k.tb0 + 1);
+#pragma unroll 1
+        for (int t = w.k.tb0; t < end; t += 2) {
+            run(b0_s, b1_s, t, sc, p);
+            if (t + 1 < end) run(b1_s, b0_s, t + 1, sc, p);
         }
-        if (wt) return;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        if (wcol + 16 * n + col >= ncols) continue;
-        // NaN sums stay NaN; nothing seen gives zeros
-        const float unit = vref * (1.0f / kUp);
-        const float s = a.nsplit > 1 ? unit : l[n] == 0.0f ? 0.0f : unit / l[n];
-        float* dst = a.nsplit > 1 ? a.part + (orow[n] * a.nsplit + sp) * D : a.out + orow[n] * D;
-#pragma unroll
-        for (int i = 0; i < ND; ++i)
-            *(float4*)(dst + 16 * i + 4 * kg) = make_float4(o[n][i][0] * s, o[n][i][1] * s, o[n][i][2] * s, o[n][i][3] * s);
-        if (a.nsplit > 1 && kg == 0) {
-            float2* ml = (float2*)(a.part + (int64_t)a.rows * a.hq * a.nsplit * D) + orow[n] * a.nsplit + sp;
-            *ml = make_float2(m[n], l[n]);
-        }
+        k[n].l = col_sum(k[n].l);
+        if (wcol + 16 * n + col < w.k.ncols) a8_store<ND>(a, orow[n], w.k.sp, k[n], vref, kg, o[n]);
     }
 }
 
-// Joins the splits of one (row, head).
+// Joins the splits of one (row, head): the splits' weights into LDS, then D / 4
+// threads per split, 1024 / D splits at a time.
 template <int D>
 __device__ __forceinline__ void attn8_merge_body(const lgx_attn8_args& a) {
+    constexpr int Q = D / 4, NG = 256 / Q;
+    __shared__ float w_s[LGX_A8_SPLITS], red_s[4];
+    __shared__ v4f o_s[256];
+    const int tid = threadIdx.x;
     const int64_t rh = blockIdx.x;
     const int row = (int)(rh / a.hq), b = row / a.P, j = row - b * a.P;
     if (a.n_new && j >= a.n_new[b]) return;
     const float2* ml = (const float2*)(a.part + (int64_t)a.rows * a.hq * a.nsplit * D) + rh * a.nsplit;
-    const float* p = a.part + rh * a.nsplit * D + threadIdx.x;
-    float m = -__builtin_inff(), l = 0.0f, o = 0.0f;
-    for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, ml[s].x);
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float2 x = ml[s];
+    static_assert(LGX_A8_SPLITS == 512, "two splits per thread");
+    float2 x[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        x[i] = tid + 256 * i < a.nsplit ? ml[tid + 256 * i] : make_float2(-__builtin_inff(), 0.0f);
+    float m = wave_max(fmaxf(x[0].x, x[1].x));
+    if ((tid & 63) == 0) red_s[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red_s[0], red_s[1]), fmaxf(red_s[2], red_s[3]));
+    __syncthreads();
+    float l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
         // an empty split's maximum is -inf
-        const float w = x.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x.x - m);
-        l = fmaf(w, x.y, l);
-        o = fmaf(w, p[(int64_t)s * D], o);
+        const float w = x[i].x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x[i].x - m);
+        w_s[tid + 256 * i] = w;
+        l = fmaf(w, x[i].y, l);
     }
-    a.out[rh * D + threadIdx.x] = l == 0.0f ? 0.0f : o / l;
+#pragma unroll
+    for (int s = 32; s; s >>= 1) l += __shfl_xor(l, s, 64);
+    if ((tid & 63) == 0) red_s[tid >> 6] = l;
+    __syncthreads();
+    l = (red_s[0] + red_s[1]) + (red_s[2] + red_s[3]);
+    const int q = tid % Q, sg = tid / Q;
+    const v4f* p = (const v4f*)(a.part + rh * a.nsplit * D) + q;
+    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int s = sg; s < a.nsplit; s += NG) o += p[(int64_t)s * Q] * w_s[s];
+    o_s[tid] = o;
+    __syncthreads();
+    if (tid >= Q) return;
+#pragma unroll
+    for (int i = 1; i < NG; ++i) o += o_s[tid + i * Q];
+    const float s = l == 0.0f ? 0.0f : 1.0f / l;
+    *((v4f*)(a.out + rh * D) + q) = o * s;
 }
-extern "C" __global__ __launch_bounds__(64) void lgx_k_attn8_merge_d64(const lgx_attn8_args a) { attn8_merge_body<64>(a); }
-extern "C" __global__ __launch_bounds__(128) void lgx_k_attn8_merge_d128(const lgx_attn8_args a) { attn8_merge_body<128>(a); }
+extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_merge_d64(const lgx_attn8_args a) { attn8_merge_body<64>(a); }
+extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_merge_d128(const lgx_attn8_args a) { attn8_merge_body<128>(a); }
 
-#define LGX_A8_KERNELS(D, C, NT, WC)                                                                           \
-    extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_d##D##_c##C(const lgx_attn8_args a) {        \
-        attn8_body<D, NT, WC, false>(a);                                                                       \
-    }                                                                                                          \
-    extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8x_d##D##_c##C(const lgx_attn8_args a) {       \
-        attn8_body<D, NT, WC, true>(a);                                                                        \
+#define LGX_A8_KERNELS(D)                                                                                              \
+    extern "C" __global__ __launch_bounds__(256, 2) void lgx_k_attn8_d##D##_c16(const lgx_attn8_args a) {              \
+        attn8_narrow_body<D, false>(a);                                                                                \
+    }                                                                                                                  \
+    extern "C" __global__ __launch_bounds__(256, 2) void lgx_k_attn8x_d##D##_c16(const lgx_attn8_args a) {             \
+        attn8_narrow_body<D, true>(a);                                                                                 \
+    }                                                                                                                  \
+    extern "C" __global__ __launch_bounds__(256, 2) void lgx_k_attn8_d##D##_c128(const lgx_attn8_args a) {             \
+        attn8_wide_body<D, false>(a);                                                                                  \
+    }                                                                                                                  \
+    extern "C" __global__ __launch_bounds__(256, 2) void lgx_k_attn8x_d##D##_c128(const lgx_attn8_args a) {            \
+        attn8_wide_body<D, true>(a);                                                                                   \
     }
-LGX_A8_KERNELS(64, 16, 1, 1)
-LGX_A8_KERNELS(128, 16, 1, 1)
-LGX_A8_KERNELS(64, 128, 2, 4)
-LGX_A8_KERNELS(128, 128, 2, 4)
+LGX_A8_KERNELS(64)
+LGX_A8_KERNELS(128)
