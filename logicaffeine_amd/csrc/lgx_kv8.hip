@@ -463,6 +463,15 @@ __device__ __forceinline__ void i8_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi
     hi = __builtin_bit_cast(uint32_t, h);
 }
 
+// w minus the low (hi = 0) or high half of a pair of binary16 numbers, exact.
+template <int HI>
+__device__ __forceinline__ float minus_half(float w, uint32_t pair) {
+    float r;
+    if (HI) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(pair), "v"(w));
+    else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(pair), "v"(w));
+    return r;
+}
+
 // tanh: below 0.35 the odd series (the term after the last is under 1.3e-8 of
 // the result), else (1 - t) / (1 + t), t = exp(-2 |x|), where 1 - t > 0.5.
 __device__ __forceinline__ float a8_tanh(float x) {
@@ -611,124 +620,137 @@ __device__ __forceinline__ void a8_scores(const KF& kf, const v4i (&qd)[3][NS], 
     }
 }
 
-// One column's running softmax; L, lo: the tokens it sees.
+// One column's running softmax.  L, lo: the tokens it sees; m, l: maximum and sum;
+// e: V scales are taken in units of 2^e, that of the largest one seen so far
+// rounded down, and weights carry 2^13 (they stay below 2^14, and their second
+// binary16 part is not subnormal where it matters).
+#define A8_UP 13
 struct A8Col {
     float f, slope, m, l;
-    int L, lo;
+    int L, lo, e;
 };
-// From integer scores to the tile's weights as two binary16 parts.  pt: the first
-// token of the lane's page, t0 of the tile; r: the page's V scale in units of the
-// running reference.  Returns the factor of what was summed before.
-template <bool X>
-__device__ __forceinline__ float a8_weights(const lgx_attn8_args& a, float (&S)[16], A8Col& c, float ks, float r, int t0, int pt,
-                                            v8h (&ph)[2], v8h (&pl)[2]) {
+__device__ __forceinline__ void a8_reset(A8Col& c) {
+    c.m = -__builtin_inff();
+    c.l = 0.0f;
+    c.e = -126;
+}
+__device__ __forceinline__ int a8_exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 127; }
+__device__ __forceinline__ float a8_unit(const A8Col& c) { return ldexpf(1.0f, c.e - A8_UP); }
+
+// From integer scores to the tile's weights, each times its page's V scale, as two
+// binary16 parts, for N column tiles.  EDGE: some column does not see the whole
+// tile, or the scores are capped, biased or windowed (X).  ks, vs: the scales of
+// the lane's page; pt: its first token.  down[n]: the factor of what was summed
+// before.
+template <bool X, bool EDGE, int N>
+__device__ __forceinline__ void a8_weights(const lgx_attn8_args& a, float (&S)[N][16], A8Col (&c)[N], float ks, float vs, int pt,
+                                           v8h (&ph)[N][2], v8h (&pl)[N][2], float (&down)[N]) {
+    static_assert(EDGE || !X, "other scores are formed ahead of the maximum");
     constexpr float kLog2e = 1.44269504088896341f;
-    const float fk = c.f * ks;
-    float mt;
-    // uniform: some column does not see the whole tile
-    const bool edge = __builtin_amdgcn_ballot_w64(t0 + LGX_A8_TILE > c.L || t0 < c.lo) != 0;
-    if (X || edge) {
+    const float inf = __builtin_inff();
+    float off[N], fk[N], r[N];
+    int top = 0;
+    if (!EDGE) top = a8_exponent(col_max(vs < inf ? vs : 0.0f));
 #pragma unroll
-        for (int e = 0; e < 16; ++e) S[e] *= fk;
-        if constexpr (X) {
-            if (a.softcap > 0.0f) {
-                const float inv = 1.0f / a.softcap;
+    for (int n = 0; n < N; ++n) {
+        fk[n] = c[n].f * ks;
+        bool page = true;
+        if (EDGE) {
+            const int hi = c[n].L - pt, lo = c[n].lo - pt;       // what the column sees of the page
 #pragma unroll
-                for (int e = 0; e < 16; ++e) S[e] = a.softcap * a8_tanh(S[e] * inv);
+            for (int e = 0; e < 16; ++e) S[n][e] *= fk[n];
+            if constexpr (X) {
+                if (a.softcap > 0.0f) {
+                    const float inv = 1.0f / a.softcap;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) S[n][e] = a.softcap * a8_tanh(S[n][e] * inv);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) S[n][e] = (S[n][e] - c[n].slope * (float)(hi - 1 - e)) * kLog2e;
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) S[e] = (S[e] - c.slope * (float)(c.L - 1 - (pt + e))) * kLog2e;
-        }
-        if (edge) {
-#pragma unroll
             for (int e = 0; e < 16; ++e)
-                if (pt + e >= c.L || pt + e < c.lo) S[e] = -__builtin_inff();
+                if (e >= hi || e < lo) S[n][e] = -inf;
+            // a page that the column does not see may hold anything
+            page = hi > 0 && lo < LGX_PAGE;
+            top = a8_exponent(col_max(page && vs < inf ? vs : 0.0f));
+        }
+        float mt = fmaxf(fmaxf(S[n][0], S[n][1]), S[n][2]);
+#pragma unroll
+        for (int e = 3; e < 15; e += 2) mt = fmaxf(fmaxf(mt, S[n][e]), S[n][e + 1]);
+        mt = fmaxf(mt, S[n][15]);
+        const float mn = fmaxf(c[n].m, col_max(EDGE ? mt : mt * fk[n]));   // scales are not negative
+        const bool none = mn == -inf;             // nothing seen yet
+        const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(c[n].m - mn);
+        const int en = max(c[n].e, top);
+        down[n] = ldexpf(alpha, c[n].e - en);
+        c[n].l *= alpha;
+        c[n].m = mn;
+        c[n].e = en;
+        off[n] = none ? 0.0f : -mn;
+        r[n] = page ? ldexpf(vs, A8_UP - en) : 0.0f;
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        float ps = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            S[n][e] = __builtin_amdgcn_exp2f(EDGE ? S[n][e] + off[n] : fmaf(S[n][e], fk[n], off[n]));
+            ps += S[n][e];
+            S[n][e] *= r[n];
+        }
+        c[n].l += ps;
+        uint32_t hw[8], lw[8];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+            // the first part rounded toward zero, the second holds the rest
+            const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(S[n][e], S[n][e + 1]));
+            hw[e >> 1] = h;
+            lw[e >> 1] =
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(minus_half<0>(S[n][e], h), minus_half<1>(S[n][e + 1], h)));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            ph[n][i] = as_v8h(make_uint4(hw[4 * i], hw[4 * i + 1], hw[4 * i + 2], hw[4 * i + 3]));
+            pl[n][i] = as_v8h(make_uint4(lw[4 * i], lw[4 * i + 1], lw[4 * i + 2], lw[4 * i + 3]));
         }
     }
-    mt = S[0];
-#pragma unroll
-    for (int e = 1; e < 16; ++e) mt = fmaxf(mt, S[e]);
-    if (!(X || edge)) mt *= fk;                   // scales are not negative
-    const float mn = fmaxf(c.m, col_max(mt));
-    const bool none = mn == -__builtin_inff();    // nothing seen yet
-    const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(c.m - mn);
-    const float mref = none ? 0.0f : mn;
-    c.m = mn;
-    float w[16], ps = 0.0f;
-    if (X || edge) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) S[e] = __builtin_amdgcn_exp2f(S[e] - mref);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) S[e] = __builtin_amdgcn_exp2f(fmaf(S[e], fk, -mref));
-    }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        ps += S[e];
-        w[e] = S[e] * r;
-    }
-    if (edge) {
-        // a weight of 0 meets no scale (a later row's page may hold NaN)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = S[e] == 0.0f ? 0.0f : w[e];
-    }
-    c.l = c.l * alpha + ps;
-#pragma unroll
-    for (int e = 0; e < 16; e += 2) {
-        // the first part rounded toward zero, the second holds the rest
-        typedef __fp16 v2f __attribute__((ext_vector_type(2)));
-        const v2f hi = __builtin_amdgcn_cvt_pkrtz(w[e], w[e + 1]);
-        const _Float16 h0 = (_Float16)hi[0], h1 = (_Float16)hi[1];
-        const v2f lo = __builtin_amdgcn_cvt_pkrtz(fmaf((float)h0, -1.0f, w[e]), fmaf((float)h1, -1.0f, w[e + 1]));
-        ph[e >> 3][e & 7] = h0;
-        ph[e >> 3][(e & 7) + 1] = h1;
-        pl[e >> 3][e & 7] = (_Float16)lo[0];
-        pl[e >> 3][(e & 7) + 1] = (_Float16)lo[1];
-    }
-    return alpha;
 }
+struct A8Edge { static constexpr bool value = true; };
+struct A8Whole { static constexpr bool value = false; };
 
-// The V scale of a lane's page in units of the wave's reference: the largest
-// scale so far rounded down to a power of two, times 2^-13 (weights stay below
-// 2^14, and their second binary16 part is not subnormal where it matters).  down:
-// the old unit in the new one.
-#define A8_UP 8192.0f
-__device__ __forceinline__ float a8_vscale(float vs, float& vref, float& down) {
-    const float top = col_max(vs < __builtin_inff() ? vs : 0.0f);
-    const float vn = fmaxf(vref, __uint_as_float(__float_as_uint(top) & 0x7f800000u));
-    const float inv = __builtin_amdgcn_rcpf(vn);  // of a power of two: exact
-    down = vref * inv;
-    vref = vn;
-    return vs * inv * A8_UP;
+// Sixteen quants (16 dimensions of a K row, 16 tokens of a V dimension) as two
+// binary16 operands.
+__device__ __forceinline__ void i8_to_v8h(const uint4& v, uint4& h0, uint4& h1) {
+    i8_to_f16(v.x, h0.x, h0.y);
+    i8_to_f16(v.y, h0.z, h0.w);
+    i8_to_f16(v.z, h1.x, h1.y);
+    i8_to_f16(v.w, h1.z, h1.w);
 }
-
-// o += V^T . P^T for N column tiles; vf(i): V fragment of dimensions 16 i ..
+// o += V^T . P^T for N column tiles; vf(i, h0, h1): V operands of dimensions 16 i ..
 template <int ND, int N, class VF>
 __device__ __forceinline__ void a8_pv(const VF& vf, const v8h (&ph)[N][2], const v8h (&pl)[N][2], v4f (&o)[N][ND]) {
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
-        const uint4 v = vf(i);
         uint4 h0, h1;
-        i8_to_f16(v.x, h0.x, h0.y);
-        i8_to_f16(v.y, h0.z, h0.w);
-        i8_to_f16(v.z, h1.x, h1.y);
-        i8_to_f16(v.w, h1.z, h1.w);
+        vf(i, h0, h1);
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h0), ph[n][0], o[n][i], 0, 0, 0);
-            o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h1), ph[n][1], o[n][i], 0, 0, 0);
-            o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h0), pl[n][0], o[n][i], 0, 0, 0);
-            o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h1), pl[n][1], o[n][i], 0, 0, 0);
-        }
+        for (int n = 0; n < N; ++n) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h0), ph[n][0], o[n][i], 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < N; ++n) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h1), ph[n][1], o[n][i], 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < N; ++n) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h0), pl[n][0], o[n][i], 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < N; ++n) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h1), pl[n][1], o[n][i], 0, 0, 0);
     }
 }
 
-// A column's result, or its split's: unit: the wave's V reference.
+// A column's result, or its split's.
 template <int ND>
-__device__ __forceinline__ void a8_store(const lgx_attn8_args& a, int64_t orow, int sp, const A8Col& c, float vref, int kg,
+__device__ __forceinline__ void a8_store(const lgx_attn8_args& a, int64_t orow, int sp, const A8Col& c, int kg,
                                          const v4f (&o)[ND]) {
     constexpr int D = 16 * ND;
-    const float unit = vref * (1.0f / A8_UP);
+    const float unit = a8_unit(c);
     // NaN sums stay NaN; nothing seen gives zeros
     const float s = a.nsplit > 1 ? unit : c.l == 0.0f ? 0.0f : unit / c.l;
     float* dst = a.nsplit > 1 ? a.part + (orow * a.nsplit + sp) * D : a.out + orow * D;
@@ -742,8 +764,9 @@ __device__ __forceinline__ void a8_store(const lgx_attn8_args& a, int64_t orow, 
 }
 
 // Few columns (a decode row's heads): 16 per workgroup, its four waves take the
-// tiles in turn, K and V straight into registers, the next tile's in flight during
-// the current one's products; at the end the waves' results are joined in LDS.
+// tiles in turn, K and V straight into registers: the next tile's K is in flight
+// from the end of the scores on, its V from the end of the PV product; at the end
+// the waves' results are joined in LDS.
 template <int D, bool X>
 __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
     constexpr int WT = 4, NS = D / 64, ND = D / 16;
@@ -757,15 +780,9 @@ __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
     const int c = w.k.c0 + col, cc = min(c, w.k.ncols - 1);
     const bool ok = c < w.k.ncols;
     const int64_t orow = ((int64_t)b * a.P + cc / G) * a.hq + g * G + cc % G;
-    const int wlast = min(w.k.c0 + 16, w.k.ncols) - 1;
-    const int wend = w.last(wlast), wbeg = w.first(w.k.c0);
     const int32_t* ptab = a.page_table + (int64_t)b * a.maxp;
     struct Pages {
         int k, v;
-    };
-    struct Tile {
-        uint4 k[4][NS], v[ND];
-        float ks, vs;
     };
     auto pages = [&](int t) {
         Pages p;
@@ -773,102 +790,149 @@ __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
         p.v = ptab[min(4 * t + kg, a.maxp - 1)];
         return p;
     };
-    auto load = [&](Tile& x, int t, const Pages& p) __attribute__((always_inline)) {
-        const int64_t pk = (int64_t)min(max(p.k, 0), a.num_pages - 1) * a.hkv + g;
-        const int64_t pv = (int64_t)min(max(p.v, 0), a.num_pages - 1) * a.hkv + g;
-        x.ks = a.ks[pv];
-        x.vs = a.vs[pv];
-        const int8_t* kp = a.k + (pk * LGX_PAGE + (col & 3)) * D + 16 * kg;
-        const int8_t* vp = a.v + (pv * D + col) * LGX_PAGE;
+    auto block = [&](int p) { return (int64_t)min(max(p, 0), a.num_pages - 1) * a.hkv + g; };
+    uint4 kw[4][NS], vw[ND];
+    auto load_k = [&](const Pages& p) __attribute__((always_inline)) {
+        const int8_t* kp = a.k + (block(p.k) * LGX_PAGE + (col & 3)) * D + 16 * kg;
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int s = 0; s < NS; ++s) x.k[u][s] = *(const uint4*)(kp + 4 * u * D + 64 * s);
-#pragma unroll
-        for (int i = 0; i < ND; ++i) x.v[i] = *(const uint4*)(vp + 16 * i * LGX_PAGE);
+            for (int s = 0; s < NS; ++s) kw[u][s] = *(const uint4*)(kp + 4 * u * D + 64 * s);
     };
-    float vref = 0x1p-126f;
-    v4f o[1][ND];
+    auto load_v = [&](const Pages& p) __attribute__((always_inline)) {
+        const int8_t* vp = a.v + (block(p.v) * D + col) * LGX_PAGE;
 #pragma unroll
-    for (int i = 0; i < ND; ++i) o[0][i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-    A8Col k;
-    k.m = -__builtin_inff();
-    k.l = 0.0f;
-    k.L = ok ? w.last(cc) : 0;
-    k.lo = ok ? w.first(cc) : 0;
-    k.slope = X && a.slopes ? a.slopes[g * G + cc % G] : 0.0f;
-    v4i qd[3][NS];
-    auto run = [&](const Tile& x, int t) __attribute__((always_inline)) {
-        const int t0 = t * LGX_A8_TILE, pt = t0 + 16 * kg;
-        float S[16], vdown;
-        a8_scores<NS>([&](int u, int s) { return x.k[u][s]; }, qd, S);
-        // a page outside the tokens seen may hold anything
-        const bool live = pt < wend && pt + LGX_PAGE > wbeg;
-        const float r = a8_vscale(live ? x.vs : 0.0f, vref, vdown);
-        v8h ph[1][2], pl[1][2];
-        const float down = a8_weights<X>(a, S, k, x.ks, r, t0, pt, ph[0], pl[0]) * vdown;
-        if (__builtin_amdgcn_ballot_w64(down != 1.0f)) {
-#pragma unroll
-            for (int i = 0; i < ND; ++i) o[0][i] *= down;
-        }
-        a8_pv<ND, 1>([&](int i) { return x.v[i]; }, ph, pl, o);
+        for (int i = 0; i < ND; ++i) vw[i] = *(const uint4*)(vp + 16 * i * LGX_PAGE);
     };
     int t = w.k.tb0 + wt;
     const int end = w.k.tb1;
-    Tile x, y;
-    if (t < end) load(x, t, pages(t));
-    Pages p = pages(t + WT);                      // indexes are clamped
-    k.f = a8_query<D, X>(a, a.q + orow * D + 16 * kg, qd);
+    // Loads are issued whether or not there is such a tile (the wave's last one's
+    // again, from the cache): a conditional load's registers would be copied, and so
+    // waited for, where the branches meet.
+    const int mine = end - 1 - t >= 0 ? t + (end - 1 - t) / WT * WT : t;   // the wave's last tile
+    Pages p = pages(t);
+    load_k(p);
+    float ks = a.ks[block(p.v)], vs = a.vs[block(p.v)];
+    load_v(p);
+    p = pages(min(t + WT, mine));
+    v4f o[1][ND];
+#pragma unroll
+    for (int i = 0; i < ND; ++i) o[0][i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    A8Col k[1];
+    a8_reset(k[0]);
+    k[0].L = w.last(cc);                          // columns past the last repeat it
+    k[0].lo = w.first(cc);
+    k[0].slope = X && a.slopes ? a.slopes[g * G + cc % G] : 0.0f;
+    v4i qd[3][NS];
+    k[0].f = a8_query<D, X>(a, a.q + orow * D + 16 * kg, qd);
+    auto tile = [&](auto form) __attribute__((always_inline)) {
+        constexpr bool edge = decltype(form)::value;
+        const int pt = t * LGX_A8_TILE + 16 * kg;
+        const float ksn = ks, vsn = vs;
+        float S[1][16], down[1];
+        a8_scores<NS>([&](int u, int s) { return kw[u][s]; }, qd, S[0]);
+        const Pages pn = p;
+        load_k(pn);
+        ks = a.ks[block(pn.v)];
+        vs = a.vs[block(pn.v)];
+        p = pages(min(t + 2 * WT, mine));
+        v8h ph[1][2], pl[1][2];
+        a8_weights<X, edge, 1>(a, S, k, ksn, vsn, pt, ph, pl, down);
+        if (__builtin_amdgcn_ballot_w64(down[0] != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < ND; ++i) o[0][i] *= down[0];
+        }
+        a8_pv<ND, 1>([&](int i, uint4& h0, uint4& h1) { i8_to_v8h(vw[i], h0, h1); }, ph, pl, o);
+        load_v(pn);
+    };
+    // the tiles that every column sees whole, then the others
+    if constexpr (!X) {
 #pragma unroll 1
-    for (; t < end; t += 2 * WT) {
-        if (t + WT < end) load(y, t + WT, p);
-        p = pages(t + 2 * WT);
-        run(x, t);
-        if (t + WT >= end) break;
-        if (t + 2 * WT < end) load(x, t + 2 * WT, p);
-        p = pages(t + 3 * WT);
-        run(y, t + WT);
+        for (const int whole = min(end, w.last(w.k.c0) / LGX_A8_TILE); t < whole; t += WT) tile(A8Whole());
     }
-    k.l = col_sum(k.l);
+#pragma unroll 1
+    for (; t < end; t += WT) tile(A8Edge());
+    k[0].l = col_sum(k[0].l);
     // join the waves, halving their number
 #pragma unroll
     for (int h = WT / 2; h; h >>= 1) {
         const int at = wt % h;
         if (wt >= h && wt < 2 * h) {
-            ml_s[(at * 3 + 0) * 64 + lane] = k.m;
-            ml_s[(at * 3 + 1) * 64 + lane] = k.l;
-            ml_s[(at * 3 + 2) * 64 + lane] = vref;
+            ml_s[(at * 3 + 0) * 64 + lane] = k[0].m;
+            ml_s[(at * 3 + 1) * 64 + lane] = k[0].l;
+            ml_s[(at * 3 + 2) * 64 + lane] = (float)k[0].e;
 #pragma unroll
             for (int i = 0; i < ND; ++i) o_s[(at * ND + i) * 64 + lane] = o[0][i];
         }
         __syncthreads();
         if (wt < h) {
             const float mo = ml_s[(at * 3 + 0) * 64 + lane], lo = ml_s[(at * 3 + 1) * 64 + lane];
-            const float vo = ml_s[(at * 3 + 2) * 64 + lane], vn = fmaxf(vref, vo), mn = fmaxf(k.m, mo);
-            const float w0 = k.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(k.m - mn);
+            const int eo = (int)ml_s[(at * 3 + 2) * 64 + lane], en = max(k[0].e, eo);
+            const float mn = fmaxf(k[0].m, mo);
+            const float w0 = k[0].m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(k[0].m - mn);
             const float w1 = mo == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mo - mn);
-            k.l = k.l * w0 + lo * w1;
-            k.m = mn;
+            const float u0 = ldexpf(w0, k[0].e - en), u1 = ldexpf(w1, eo - en);
+            k[0].l = k[0].l * w0 + lo * w1;
+            k[0].m = mn;
+            k[0].e = en;
 #pragma unroll
-            for (int i = 0; i < ND; ++i)
-                o[0][i] = o[0][i] * (w0 * (vref / vn)) + o_s[(at * ND + i) * 64 + lane] * (w1 * (vo / vn));
-            vref = vn;
+            for (int i = 0; i < ND; ++i) o[0][i] = o[0][i] * u0 + o_s[(at * ND + i) * 64 + lane] * u1;
         }
         __syncthreads();
     }
-    if (wt == 0 && ok) a8_store<ND>(a, orow, w.k.sp, k, vref, kg, o[0]);
+    if (wt == 0 && ok) a8_store<ND>(a, orow, w.k.sp, k[0], kg, o[0]);
 }
 
-// Many columns (prefill): 128 per workgroup, 32 per wave; every tile passes through
-// LDS once for all of them, by direct global->LDS loads into two buffers, each wave
-// instruction bringing one operand fragment (1 KiB) in the order of the lanes.
+// The query of a lane's column as two binary16 parts per operand (22 bits under the
+// row's largest magnitude, which a power of two brings to 2^14 .. 2^15), dimensions
+// 64 s + 16 kg + 8 h .. in step 2 s + h.
+template <int D, bool X>
+__device__ __forceinline__ float a8_query16(const lgx_attn8_args& a, const float* qr, v8h (&qh)[2][D / 32]) {
+    constexpr int NH = D / 32;
+    float x[NH][8], am = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            const float4 v = *(const float4*)(qr + 64 * (h >> 1) + 8 * (h & 1) + e);
+            x[h][e] = v.x;
+            x[h][e + 1] = v.y;
+            x[h][e + 2] = v.z;
+            x[h][e + 3] = v.w;
+        }
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            am = fmaxf(am, fabsf(x[h][e]));
+            bad = bad || !(fabsf(x[h][e]) < __builtin_inff());
+        }
+    am = col_max(am);
+    const bool isbad = col_max(bad ? 1.0f : 0.0f) != 0.0f;
+    const float up = __uint_as_float(__float_as_uint(fminf(32768.0f / am, 0x1p100f)) & 0x7f800000u);
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float y = isbad ? 0.0f : x[h][e] * up;
+            qh[0][h][e] = (_Float16)y;
+            qh[1][h][e] = (_Float16)(y - (float)qh[0][h][e]);
+        }
+    return isbad ? __builtin_nanf("") : a.scale / up * (X ? 1.0f : 1.44269504088896341f);
+}
+
+// Many columns (prefill): 128 per workgroup, 32 per wave.  Every tile is converted to
+// binary16 once for all of them: each wave brings a quarter of its quants into LDS
+// (two waves K, two V; a direct load brings one 1 KiB fragment in the order of the
+// lanes), a tile ahead, and then turns them into operands in one of two LDS buffers
+// while the other's tile is in use.  With K in binary16 the scores need no joining of digits: two products,
+// one accumulator.
 template <int D, bool X>
 __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
-    constexpr int NT = 2, NS = D / 64, ND = D / 16, NF = 4 * NS + ND, FW = NF / 4;
+    constexpr int NT = 2, NS = D / 64, NH = D / 32, ND = D / 16, NF = 4 * NS + ND, FW = NF / 4;
     static_assert(4 * NS == ND, "waves 0 and 1 bring K, 2 and 3 bring V");
-    typedef __attribute__((address_space(3))) const uint4 lds_c4;
-    // two variables: a direct load into one is known not to alias reads of the other
-    __shared__ __align__(16) uint4 b0_s[NF * 64], b1_s[NF * 64];
+    __shared__ __align__(16) uint4 f_s[2][2 * NF * 64], raw_s[NF * 64];
     const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     A8<64 * NT, X> w{a, {}};
@@ -878,101 +942,162 @@ __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
     const bool any = wcol < w.k.ncols;            // uniform per wave
     const int wlast = min(wcol + 16 * NT, w.k.ncols) - 1;
     const int wend = any ? w.last(wlast) : 0, wbeg = any ? w.first(wcol) : 0;
-    A8Col k[NT];
-    v4i qd[NT][3][NS];
-    int64_t orow[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int c = wcol + 16 * n + col, cc = min(c, w.k.ncols - 1);
-        const bool ok = c < w.k.ncols;
-        orow[n] = ((int64_t)b * a.P + cc / G) * a.hq + g * G + cc % G;
-        k[n].m = -__builtin_inff();
-        k[n].l = 0.0f;
-        k[n].L = ok ? w.last(cc) : 0;
-        k[n].lo = ok ? w.first(cc) : 0;
-        k[n].slope = X && a.slopes ? a.slopes[g * G + cc % G] : 0.0f;
-        k[n].f = a8_query<D, X>(a, a.q + orow[n] * D + 16 * kg, qd[n]);
-    }
     const int32_t* ptab = a.page_table + (int64_t)b * a.maxp;
-    // the page of the wave's direct loads, and of the lane's scales
-    struct Pages {
-        int ld, sc;
-    };
-    auto pages = [&](int t) {
-        Pages p;
-        p.ld = ptab[min(4 * t + (wave < 2 ? col >> 2 : kg), a.maxp - 1)];
-        p.sc = ptab[min(4 * t + kg, a.maxp - 1)];
-        return p;
-    };
+    const int end = w.k.tb1;
+    // Loads are issued whether or not there is such a tile (the last one's again,
+    // from the cache): a conditional load's register would be copied, and so waited
+    // for, where the branches meet.
+    auto page_ld = [&](int t) { return ptab[min(4 * max(min(t, end - 1), 0) + (wave < 2 ? col >> 2 : kg), a.maxp - 1)]; };
+    auto page_sc = [&](int t) { return ptab[min(4 * max(min(t, end - 1), 0) + kg, a.maxp - 1)]; };
     auto block = [&](int p) { return (int64_t)min(max(p, 0), a.num_pages - 1) * a.hkv + g; };
-    auto stage = [&](uint4* buf, int p) __attribute__((always_inline)) {
+    uint4* const raw = raw_s + wave * FW * 64;
+    // the wave's fragments of a tile, p its page
+    auto load = [&](int p) __attribute__((always_inline)) {
         const int64_t blk = block(p);
         const int8_t* src = wave < 2 ? a.k + (blk * LGX_PAGE + (col & 3)) * D + 16 * kg : a.v + (blk * D + col) * LGX_PAGE;
 #pragma unroll
         for (int j = 0; j < FW; ++j) {
             const int f = (wave & 1) * FW + j;
-            const int off = wave < 2 ? 4 * (f / NS) * D + 64 * (f % NS) : 16 * f * LGX_PAGE;
-            load_lds_16(src + off, (lds_void*)(buf + (wave * FW + j) * 64));
+            load_lds_16(src + (wave < 2 ? 4 * (f / NS) * D + 64 * (f % NS) : 16 * f * LGX_PAGE), (lds_void*)(raw + j * 64));
         }
     };
-    float vref = 0x1p-126f;
+    // them as operands: 2 f and 2 f + 1 of fragment f
+    auto convert = [&](uint4* buf) __attribute__((always_inline)) {
+        uint4* dst = buf + wave * 2 * FW * 64 + lane;
+#pragma unroll
+        for (int j = 0; j < FW; ++j) {
+            uint4 h0, h1;
+            i8_to_v8h(raw[j * 64 + lane], h0, h1);
+            dst[2 * j * 64] = h0;
+            dst[(2 * j + 1) * 64] = h1;
+        }
+    };
+    load(page_ld(w.k.tb0));
+    int pl_ = page_ld(w.k.tb0 + 1), ps_ = page_sc(w.k.tb0 + 1);
+    float ks, vs;
+    {
+        const int64_t sb = block(page_sc(w.k.tb0));
+        ks = a.ks[sb];
+        vs = a.vs[sb];
+    }
+    A8Col k[NT];
+    v8h qh[NT][2][NH];
+    auto orow = [&](int c) { return ((int64_t)b * a.P + c / G) * a.hq + g * G + c % G; };
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int c = wcol + 16 * n + col, cc = min(c, w.k.ncols - 1);
+        a8_reset(k[n]);
+        k[n].L = w.last(cc);                      // columns past the last repeat it
+        k[n].lo = w.first(cc);
+        k[n].slope = X && a.slopes ? a.slopes[g * G + cc % G] : 0.0f;
+        k[n].f = a8_query16<D, X>(a, a.q + orow(cc) * D + 16 * kg, qh[n]);
+    }
     v4f o[NT][ND];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < ND; ++i) o[n][i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-    struct Scales {
-        float k, v;
-    };
-    auto scales = [&](int p) {
-        const int64_t blk = block(p);
-        return Scales{a.ks[blk], a.vs[blk]};
-    };
-    const int end = w.k.tb1;
-    // tile t from buf (landed), the next one's loads into nbuf
-    auto run = [&](const uint4* buf, uint4* nbuf, int t, Scales& sc, Pages& p) __attribute__((always_inline)) {
-        publish_lds_loads();                      // tile t landed; tile t - 1 read
-        const Scales now = sc;
-        if (t + 1 < end) {
-            stage(nbuf, p.ld);
-            sc = scales(p.sc);
-            p = pages(t + 2);
-        }
+    auto tile = [&](int t, auto form) __attribute__((always_inline)) {
+        constexpr bool edge = decltype(form)::value;
+        const int cur = (t - w.k.tb0) & 1;
+        publish_lds_loads();                      // tile t is whole, tile t - 1 read, t + 1's quants landed
+        convert(f_s[cur ^ 1]);
+        __builtin_amdgcn_sched_barrier(0);
+        load(pl_);
+        pl_ = page_ld(t + 3);
+        const float ksn = ks, vsn = vs;
+        const int64_t sb = block(ps_);
+        ks = a.ks[sb];
+        vs = a.vs[sb];
+        ps_ = page_sc(t + 2);
+        __builtin_amdgcn_sched_barrier(0);
         const int t0 = t * LGX_A8_TILE, pt = t0 + 16 * kg;
-        if (t0 >= wend || t0 + LGX_A8_TILE <= wbeg) return;   // uniform per wave
-        lds_c4* fr = (lds_c4*)buf + lane;
-        // a page outside the tokens seen may hold anything
-        const bool live = pt < wend && pt + LGX_PAGE > wbeg;
-        float vdown;
-        const float r = a8_vscale(live ? now.v : 0.0f, vref, vdown);
+        if (!any || (edge && (t0 >= wend || t0 + LGX_A8_TILE <= wbeg))) return;   // uniform per wave
+        const uint4* fr = f_s[cur] + lane;
+        float S[NT][16], down[NT];
+        {
+            // fragments PF ahead of their products: an LDS read takes as long as
+            // two fragments' products
+            constexpr int PF = 3;
+            v8h kf[4 * NH];
+            v4f acc[4][NT];
+#pragma unroll
+            for (int i = 0; i < PF; ++i) kf[i] = as_v8h(fr[i * 64]);
+#pragma unroll
+            for (int i = 0; i < 4 * NH; ++i) {
+                const int u = i / NH, h = i % NH;
+                if (i + PF < 4 * NH) kf[i + PF] = as_v8h(fr[(i + PF) * 64]);
+#pragma unroll
+                for (int part = 1; part >= 0; --part)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        acc[u][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            kf[i], qh[n][part][h], h == 0 && part == 1 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : acc[u][n], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, PF, 0);
+#pragma unroll
+            for (int i = 0; i < 4 * NH; ++i) {
+                if (i + PF < 4 * NH) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 2 * NT, 0);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) S[n][e] = acc[e >> 2][n][e & 3];
+        }
         v8h ph[NT][2], pl[NT][2];
+        a8_weights<X, edge, NT>(a, S, k, ksn, vsn, pt, ph, pl, down);
+        bool moved = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float S[16];
-            a8_scores<NS>([&](int u, int s) -> uint4 { return fr[(u * NS + s) * 64]; }, qd[n], S);
-            const float down = a8_weights<X>(a, S, k[n], now.k, r, t0, pt, ph[n], pl[n]) * vdown;
-            if (__builtin_amdgcn_ballot_w64(down != 1.0f)) {
+        for (int n = 0; n < NT; ++n) moved = moved || down[n] != 1.0f;
+        if (__builtin_amdgcn_ballot_w64(moved)) {
 #pragma unroll
-                for (int i = 0; i < ND; ++i) o[n][i] *= down;
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < ND; ++i) o[n][i] *= down[n];
+        }
+        {
+            constexpr int PF = 3;
+            const uint4* vr = fr + 2 * 4 * NS * 64;
+            v8h vf[2 * ND];
+#pragma unroll
+            for (int i = 0; i < PF; ++i) vf[i] = as_v8h(vr[i * 64]);
+#pragma unroll
+            for (int i = 0; i < 2 * ND; ++i) {
+                if (i + PF < 2 * ND) vf[i + PF] = as_v8h(vr[(i + PF) * 64]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    o[n][i / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], ph[n][i & 1], o[n][i / 2], 0, 0, 0);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    o[n][i / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], pl[n][i & 1], o[n][i / 2], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, PF, 1);
+#pragma unroll
+            for (int i = 0; i < 2 * ND; ++i) {
+                if (i + PF < 2 * ND) __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+                __builtin_amdgcn_sched_group_barrier(0x008, 2 * NT, 1);
             }
         }
-        a8_pv<ND, NT>([&](int i) -> uint4 { return fr[(4 * NS + i) * 64]; }, ph, pl, o);
     };
-    if (w.k.tb0 < end) {
-        Pages p = pages(w.k.tb0);
-        stage(b0_s, p.ld);
-        Scales sc = scales(p.sc);
-        p = pages(w.k.tb0 + 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    convert(f_s[0]);
+    load(pl_);
+    pl_ = page_ld(w.k.tb0 + 2);
+    // the tiles that every column of the workgroup sees whole, then the others
+    int t = w.k.tb0;
+    if constexpr (!X) {
 #pragma unroll 1
-        for (int t = w.k.tb0; t < end; t += 2) {
-            run(b0_s, b1_s, t, sc, p);
-            if (t + 1 < end) run(b1_s, b0_s, t + 1, sc, p);
-        }
+        for (const int whole = min(end, w.last(w.k.c0) / LGX_A8_TILE); t < whole; ++t) tile(t, A8Whole());
     }
+#pragma unroll 1
+    for (; t < end; ++t) tile(t, A8Edge());
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the wave
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+        const int c = wcol + 16 * n + col;
         k[n].l = col_sum(k[n].l);
-        if (wcol + 16 * n + col < w.k.ncols) a8_store<ND>(a, orow[n], w.k.sp, k[n], vref, kg, o[n]);
+        if (c < w.k.ncols) a8_store<ND>(a, orow(c), w.k.sp, k[n], kg, o[n]);
     }
 }
 
