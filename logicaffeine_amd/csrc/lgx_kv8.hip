@@ -463,7 +463,9 @@ __device__ __forceinline__ void i8_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi
     hi = __builtin_bit_cast(uint32_t, h);
 }
 
-// w minus the low (hi = 0) or high half of a pair of binary16 numbers, exact.
+// w minus the low or high half of a pair of binary16 numbers, exact.  (Neither
+// operand may come from a matrix instruction or a v_exp: the compiler puts no wait
+// states ahead of assembly.)
 template <int HI>
 __device__ __forceinline__ float minus_half(float w, uint32_t pair) {
     float r;
@@ -620,11 +622,12 @@ __device__ __forceinline__ void a8_scores(const KF& kf, const v4i (&qd)[3][NS], 
     }
 }
 
-// One column's running softmax.  L, lo: the tokens it sees; m, l: maximum and sum;
-// e: V scales are taken in units of 2^e, that of the largest one seen so far
-// rounded down, and weights carry 2^13 (they stay below 2^14, and their second
-// binary16 part is not subnormal where it matters).
-#define A8_UP 13
+// One column's running softmax.  L, lo: the tokens it sees; m: its reference, within
+// 4 below the largest score (base 2) so far; l: the sum of 2^(score - m); e: V scales
+// are taken in units of 2^e, that of the largest one seen so far rounded down, and
+// weights carry 2^9 (they stay below 2^14, and their second binary16 part is not
+// subnormal where it matters).
+#define A8_UP 9
 struct A8Col {
     float f, slope, m, l;
     int L, lo, e;
@@ -679,7 +682,10 @@ __device__ __forceinline__ void a8_weights(const lgx_attn8_args& a, float (&S)[N
 #pragma unroll
         for (int e = 3; e < 15; e += 2) mt = fmaxf(fmaxf(mt, S[n][e]), S[n][e + 1]);
         mt = fmaxf(mt, S[n][15]);
-        const float mn = fmaxf(c[n].m, col_max(EDGE ? mt : mt * fk[n]));   // scales are not negative
+        mt = col_max(EDGE ? mt : mt * fk[n]);     // scales are not negative
+        // the reference moves when the maximum passes it by more than 2^4: most
+        // tiles then leave what was summed as it is
+        const float mn = mt > c[n].m + 4.0f ? mt : c[n].m;
         const bool none = mn == -inf;             // nothing seen yet
         const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(c[n].m - mn);
         const int en = max(c[n].e, top);
