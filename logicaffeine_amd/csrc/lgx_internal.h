@@ -177,9 +177,9 @@ enum Kern {
     K_KV8_READ_D128,
     K_ATTN8_D64,     // 16 columns; + 1: with caps, distances or a window; + 2: 128 columns
     K_ATTN8_D128 = K_ATTN8_D64 + 4,
-    K_ATTN8_MERGE_D64 = K_ATTN8_D128 + 4,
-    K_ATTN8_MERGE_D128,
-    K_COUNT
+    K_ATTN8_JOIN_D64 = K_ATTN8_D128 + 4,   // + 1: a wave per (row, head)
+    K_ATTN8_JOIN_D128 = K_ATTN8_JOIN_D64 + 2,
+    K_COUNT = K_ATTN8_JOIN_D128 + 2
 };
 inline const char* const kKernelNames[] = {
     "lgx_k_repack_t16", "lgx_k_quantize_q8_0", "lgx_k_q8q8_gemv",
@@ -231,7 +231,7 @@ inline const char* const kKernelNames[] = {
     "lgx_k_kv8_append1_d64", "lgx_k_kv8_append1_d128", "lgx_k_kv8_read_d64", "lgx_k_kv8_read_d128",
     "lgx_k_attn8_d64_c16", "lgx_k_attn8x_d64_c16", "lgx_k_attn8_d64_c128", "lgx_k_attn8x_d64_c128",
     "lgx_k_attn8_d128_c16", "lgx_k_attn8x_d128_c16", "lgx_k_attn8_d128_c128", "lgx_k_attn8x_d128_c128",
-    "lgx_k_attn8_merge_d64", "lgx_k_attn8_merge_d128",
+    "lgx_k_attn8_join_d64", "lgx_k_attn8_joinw_d64", "lgx_k_attn8_join_d128", "lgx_k_attn8_joinw_d128",
 };
 
 static_assert(sizeof(kKernelNames) / sizeof(kKernelNames[0]) == K_COUNT,

@@ -469,13 +469,20 @@ typedef struct {
     const int32_t* n_new;      // [B], nullable: P
     const float* slopes;       // [hq], nullable
     float* out;                // [B*P][hq][d]
-    float* part;               // nsplit > 1: [B*P*hq][nsplit][d], then (m, l) pairs [B*P*hq][nsplit]
+    // per > 0: the tiles of every (sequence, column block) are split on the device so
+    // that `per` workgroups per KV head share all of them (see A8::place)
+    float* part;               // [per][hkv][columns][d]: results of splits
+    float* ml;                 // [per][hkv][columns][2]: their maxima and sums
+    int32_t* plan;             // [B * ncb][2]: first split, number of splits
     int32_t P, hq, hkv, maxp, num_pages, maxlen;
     int32_t len_add;           // row j sees seq_len + j + len_add tokens
     int32_t window;            // 0: all
-    int32_t nsplit, cps, ncb;  // splits of the tiles, tiles per split, column blocks
+    int32_t per, units, ncb;   // units: B * ncb; ncb: column blocks of a sequence
+    int32_t cps;               // one unit: tiles per split, chosen by the host; else 0
+    int32_t cols;              // columns of a block (the join)
     int32_t rows;              // B*P
     float scale, softcap;
 } lgx_attn8_args;
 #define LGX_A8_TILE 64         // tokens of a tile: four pages
-#define LGX_A8_SPLITS 512      // splits at most
+#define LGX_A8_UNITS 256       // (sequence, column block) pairs whose tiles are split at most
+#define LGX_A8_MIN 4           // tiles of a split at least

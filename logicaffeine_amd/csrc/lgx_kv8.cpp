@@ -28,30 +28,46 @@ int pages_touched(int n) { return (int)(((int64_t)n + LGX_PAGE - 2) / LGX_PAGE +
 // (row, head) pairs of a workgroup.
 int attn8_cols(const lgx_ctx* c, int64_t cols) { return cols <= c->attn8_narrow ? 16 : 128; }
 
-// Splits of the visible tiles: two workgroups per compute unit, a tile per wave
-// at least.
+// Launch over B sequences.  Where one workgroup per (sequence, KV head, column block)
+// would not fill the device several times over, their tiles are split among
+// workgroups (the splitting itself is done on the device, by the lengths).
 lgx_status run_attn8(lgx_ctx* c, lgx_attn8_args& a, int B, int d, bool x, void* stream) {
     const int64_t cols = (int64_t)a.P * (a.hq / a.hkv);
-    const int nc = attn8_cols(c, cols), wt = nc == 16 ? 4 : 1;
-    const int64_t ncb = (cols + nc - 1) / nc, blocks = (int64_t)B * a.hkv * ncb;
-    // a block's rows are at most nc apart
+    const int nc = attn8_cols(c, cols);
+    const int64_t ncb = (cols + nc - 1) / nc, units = B * ncb, blocks = units * a.hkv;
+    a.ncb = (int)ncb;
+    a.cols = nc;
+    // the most tiles that a block can see (its rows are at most nc apart)
     int64_t tiles = cdiv(a.maxlen, LGX_A8_TILE);
     if (a.window) tiles = std::min<int64_t>(tiles, ((int64_t)a.window + nc) / LGX_A8_TILE + 2);
-    const int64_t want = std::min<int64_t>(std::max<int64_t>(1, (int64_t)c->attn8_wgs * c->ncu / blocks), LGX_A8_SPLITS);
-    const int64_t cps = ((tiles + want - 1) / want + wt - 1) / wt * wt;
-    a.ncb = (int)ncb;
-    a.cps = (int)cps;
-    a.nsplit = (int)((tiles + cps - 1) / cps);
-    const int64_t grid = blocks * a.nsplit;
-    if (grid > UINT32_MAX / 256) return fail(LGX_OUT_OF_BOUNDS, "attention of %lld workgroups", (long long)grid);
+    const int64_t want = (int64_t)c->attn8_wgs * c->ncu;
+    const bool split = tiles > LGX_A8_MIN && units <= LGX_A8_UNITS && blocks < (nc == 16 ? 4 * want : want) && !(units == 1 && 2 * blocks > want);
     lgx_status st;
-    const int64_t rh = (int64_t)a.rows * a.hq;
-    if (a.nsplit > 1 &&
-        (st = ensure_ws(c, (size_t)rh * a.nsplit * (d + 2) * sizeof(float), &a.part)) != LGX_OK)
-        return st;
+    if (split) {
+        int64_t per = std::max<int64_t>(units, want / a.hkv);
+        if (units == 1 && !a.window) {
+            a.cps = (int)std::max<int64_t>(LGX_A8_MIN, ((tiles + per - 1) / per + 3) / 4 * 4);
+            per = (tiles + a.cps - 1) / a.cps;
+        }
+        const int64_t slots = per * a.hkv * nc;
+        float* ws = nullptr;
+        if ((st = ensure_ws(c, (size_t)(slots * (d + 2) + 2 * units) * sizeof(float), &ws)) != LGX_OK) return st;
+        a.per = (int)per;
+        a.units = (int)units;
+        a.part = ws;
+        a.ml = ws + slots * d;
+        a.plan = (int32_t*)(a.ml + 2 * slots);
+    }
+    const int64_t grid = split ? (int64_t)a.per * a.hkv : blocks;
+    if (grid > UINT32_MAX / 256) return fail(LGX_OUT_OF_BOUNDS, "attention of %lld workgroups", (long long)grid);
     const int k = (d == 64 ? K_ATTN8_D64 : K_ATTN8_D128) + (nc == 16 ? 0 : 2) + (x ? 1 : 0);
-    if ((st = launch(c, (Kern)k, dim3((unsigned)grid), dim3(256), a, stream)) != LGX_OK || a.nsplit == 1) return st;
-    return launch(c, d == 64 ? K_ATTN8_MERGE_D64 : K_ATTN8_MERGE_D128, dim3((unsigned)rh), dim3(256), a, stream);
+    if ((st = launch(c, (Kern)k, dim3((unsigned)grid), dim3(256), a, stream)) != LGX_OK || !split) return st;
+    // a wave joins a row's head where there are many; a workgroup, whose threads
+    // read more splits at a time, where there are few
+    const int64_t rh = (int64_t)a.rows * a.hq;
+    const int w = rh >= 8 * (int64_t)c->ncu ? 1 : 0;
+    return launch(c, (Kern)((d == 64 ? K_ATTN8_JOIN_D64 : K_ATTN8_JOIN_D128) + w), dim3(w ? cdiv(rh, 4) : (unsigned)rh),
+                  dim3(256), a, stream);
 }
 
 lgx_status attn8(lgx_ctx* c, const float* q, const lgx_kv_i8* kv, const int32_t* page_table,

@@ -518,46 +518,136 @@ __device__ __forceinline__ float col_sum(float v) {
     return v + w;
 }
 
-// What a workgroup of NC columns sees: its sequence, rows, tiles.
+// Inclusive sums over the wave's lanes (VALU moves within rows of 16, then of row
+// 0 and 2's last lane into the next row, then of the lower half's into the upper).
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
+// What a workgroup of NC columns works on: a sequence, a KV head, a block of
+// columns, and a run of tiles.
 struct A8Block {
-    int b, g, G, sp, c0, ncols, sl;
-    int tb0, tb1;      // tiles of the split
+    int b, g, G, c0, ncols, sl;
+    int tb0, tb1;      // tiles
+    int unit;          // b * ncb + column block
+    int pos, ns;       // place among all splits, and splits of the unit
 };
-template <int NC, bool X>
+template <int NC, int WT, bool X>
 struct A8 {
     const lgx_attn8_args& a;
     A8Block k;
-    // tokens that the row of column c sees: [first(c), last(c))
-    __device__ __forceinline__ int last(int c) const {
-        return (int)min((int64_t)k.sl + c / k.G + a.len_add, (int64_t)a.maxlen);
+    // tokens that the row of column c of a sequence of sl tokens sees: [first, last)
+    __device__ __forceinline__ int last(int sl, int c) const {
+        const int j = a.P == 1 ? 0 : c / k.G;
+        return (int)min((int64_t)sl + j + a.len_add, (int64_t)a.maxlen);
     }
-    __device__ __forceinline__ int first(int c) const { return X && a.window ? max(last(c) - a.window, 0) : 0; }
-    // false: no column
+    __device__ __forceinline__ int first(int sl, int c) const { return X && a.window ? max(last(sl, c) - a.window, 0) : 0; }
+    __device__ __forceinline__ int last(int c) const { return last(k.sl, c); }
+    __device__ __forceinline__ int first(int c) const { return first(k.sl, c); }
+    __device__ __forceinline__ int rows(int b) const { return a.n_new ? min(max(a.n_new[b], 0), a.P) : a.P; }
+    __device__ __forceinline__ int2 tiles(int sl, int c0, int ncols) const {
+        return make_int2(first(sl, c0) / LGX_A8_TILE,
+                         (last(sl, min(c0 + NC, ncols) - 1) + LGX_A8_TILE - 1) / LGX_A8_TILE);
+    }
+    // false: nothing to do.  With a.per alone, all units' tiles go in equal runs to the
+    // workgroups (ragged batches: 64 sequences of 256 to 4096 tokens, 28/4 heads of
+    // 128, where runs of the longest length take xx us, equal ones yy): every wave
+    // computes the run length from all lengths (four units per lane), the least
+    // multiple of WT tiles with which all runs fit into a.per per KV head, then
+    // finds the unit and the run of this workgroup in the sums over the units.
     __device__ __forceinline__ bool place() {
-        const int cb = blockIdx.x % a.ncb, rest = blockIdx.x / a.ncb;
-        k.sp = rest % a.nsplit;
-        const int bg = __builtin_amdgcn_readfirstlane(rest / a.nsplit);
-        k.b = __builtin_amdgcn_readfirstlane(bg / a.hkv);
-        k.g = bg - k.b * a.hkv;
         k.G = a.hq / a.hkv;
-        const int nn = a.n_new ? min(max(a.n_new[k.b], 0), a.P) : a.P;
-        k.ncols = nn * k.G;
-        k.c0 = cb * NC;
+        int s = 0, cps = a.cps;
+        if (a.cps) {
+            // one unit without a window: runs of a fixed length, which nothing has
+            // to be read for
+            s = k.pos = __builtin_amdgcn_readfirstlane(blockIdx.x / a.hkv);
+            k.g = blockIdx.x - s * a.hkv;
+            k.unit = 0;
+            k.ns = a.per;
+            if (blockIdx.x == 0 && threadIdx.x == 0) {
+                a.plan[0] = 0;
+                a.plan[1] = a.per;
+            }
+        } else if (a.per) {
+            const int lane = threadIdx.x & 63;
+            k.pos = __builtin_amdgcn_readfirstlane(blockIdx.x / a.hkv);
+            k.g = blockIdx.x - k.pos * a.hkv;
+            int n[4], all = 0;                    // tiles of the lane's units; -1: no such columns
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int u = 4 * lane + i, uc = min(u, a.units - 1), b = a.ncb == 1 ? uc : uc / a.ncb;
+                const int c0 = (uc - b * a.ncb) * NC, ncols = rows(b) * k.G;
+                const int2 t = tiles(max(a.seq_len[b], 0), c0, ncols);
+                n[i] = u < a.units && c0 < ncols ? t.y - t.x : -1;
+                all += max(n[i], 0);
+            }
+            const int total = __builtin_amdgcn_readlane(wave_scan(all), 63);
+            constexpr int least = LGX_A8_MIN;
+            static_assert(least % WT == 0, "the waves of a run have equal shares");
+            cps = max(least, (int)((total + a.per - 1) / a.per + WT - 1) / WT * WT);
+            int m[4], upto;
+            for (;;) {
+                int c = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    m[i] = n[i] < 0 ? 0 : max((int)((unsigned)(n[i] + cps - 1) / (unsigned)cps), 1);
+                    c += m[i];
+                }
+                upto = wave_scan(c);
+                if (__builtin_amdgcn_readlane(upto, 63) <= a.per) break;
+                cps += max(WT, cps / (8 * WT) * WT);   // ends: a.per >= a.units
+            }
+            const uint64_t past = __builtin_amdgcn_ballot_w64(upto > k.pos);
+            if (!past) return false;
+            const int at = __builtin_ctzll(past);
+            s = k.pos - __builtin_amdgcn_readlane(upto - (m[0] + m[1] + m[2] + m[3]), at);
+            int i = 0;
+#pragma unroll
+            for (int q = 0; q < 3; ++q) {
+                const int mq = __builtin_amdgcn_readlane(m[q], at);
+                const bool next = i == q && s >= mq;
+                s -= next ? mq : 0;
+                i += next ? 1 : 0;
+            }
+            const int m0 = __builtin_amdgcn_readlane(m[0], at), m1 = __builtin_amdgcn_readlane(m[1], at);
+            const int m2 = __builtin_amdgcn_readlane(m[2], at), m3 = __builtin_amdgcn_readlane(m[3], at);
+            k.ns = i == 0 ? m0 : i == 1 ? m1 : i == 2 ? m2 : m3;
+            k.unit = 4 * at + i;
+            if (s == 0 && k.g == 0 && threadIdx.x == 0) {
+                a.plan[2 * k.unit] = k.pos;
+                a.plan[2 * k.unit + 1] = k.ns;
+            }
+        } else {
+            // column blocks side by side: they share K and V
+            const int bg = blockIdx.x / a.ncb, cb = blockIdx.x - bg * a.ncb;
+            const int b = bg / a.hkv;
+            k.g = __builtin_amdgcn_readfirstlane(bg - b * a.hkv);
+            k.unit = __builtin_amdgcn_readfirstlane(b * a.ncb + cb);
+            k.ns = 1;
+        }
+        k.b = __builtin_amdgcn_readfirstlane(k.unit / a.ncb);
+        k.c0 = (k.unit - k.b * a.ncb) * NC;
+        k.ncols = rows(k.b) * k.G;
         if (k.c0 >= k.ncols) return false;
         k.sl = max(a.seq_len[k.b], 0);
-        k.tb0 = first(k.c0) / LGX_A8_TILE + k.sp * a.cps;
-        k.tb1 = min((last(min(k.c0 + NC, k.ncols) - 1) + LGX_A8_TILE - 1) / LGX_A8_TILE, k.tb0 + a.cps);
+        const int2 t = tiles(k.sl, k.c0, k.ncols);
+        k.tb0 = t.x + s * cps;
+        k.tb1 = a.per ? min(t.y, k.tb0 + cps) : t.y;
         return true;
     }
 };
 
 // The query of a lane's column: its digits as B operands, the factor that turns
 // an integer score (times the page's K scale) into a score (in base 2 unless X).
-template <int D, bool X>
-__device__ __forceinline__ float a8_query(const lgx_attn8_args& a, const float* qr, v4i (&qd)[3][D / 64]) {
-    constexpr int NS = D / 64;
-    float x[NS][16], am = 0.0f;
-    bool bad = false;
+template <int NS>
+__device__ __forceinline__ void a8_query_load(const float* qr, float (&x)[NS][16]) {
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
@@ -568,6 +658,11 @@ __device__ __forceinline__ float a8_query(const lgx_attn8_args& a, const float* 
             x[s][e + 2] = v.z;
             x[s][e + 3] = v.w;
         }
+}
+template <int NS, bool X>
+__device__ __forceinline__ float a8_query(const lgx_attn8_args& a, const float (&x)[NS][16], v4i (&qd)[3][NS]) {
+    float am = 0.0f;
+    bool bad = false;
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
@@ -751,22 +846,21 @@ __device__ __forceinline__ void a8_pv(const VF& vf, const v8h (&ph)[N][2], const
     }
 }
 
-// A column's result, or its split's.
-template <int ND>
-__device__ __forceinline__ void a8_store(const lgx_attn8_args& a, int64_t orow, int sp, const A8Col& c, int kg,
+// A column's result, or its split's; c: the column, NC columns per block.
+template <int NC, int ND>
+__device__ __forceinline__ void a8_store(const lgx_attn8_args& a, const A8Block& k, int64_t orow, int c, const A8Col& x, int kg,
                                          const v4f (&o)[ND]) {
     constexpr int D = 16 * ND;
-    const float unit = a8_unit(c);
+    const bool part = k.ns > 1;
+    const int64_t at = part ? ((int64_t)k.pos * a.hkv + k.g) * NC + c - k.c0 : orow;
+    const float unit = a8_unit(x);
     // NaN sums stay NaN; nothing seen gives zeros
-    const float s = a.nsplit > 1 ? unit : c.l == 0.0f ? 0.0f : unit / c.l;
-    float* dst = a.nsplit > 1 ? a.part + (orow * a.nsplit + sp) * D : a.out + orow * D;
+    const float s = part ? unit : x.l == 0.0f ? 0.0f : unit / x.l;
+    float* dst = (part ? a.part : a.out) + at * D;
 #pragma unroll
     for (int i = 0; i < ND; ++i)
         *(float4*)(dst + 16 * i + 4 * kg) = make_float4(o[i][0] * s, o[i][1] * s, o[i][2] * s, o[i][3] * s);
-    if (a.nsplit > 1 && kg == 0) {
-        float2* ml = (float2*)(a.part + (int64_t)a.rows * a.hq * a.nsplit * D) + orow * a.nsplit + sp;
-        *ml = make_float2(c.m, c.l);
-    }
+    if (part && kg == 0) *(float2*)(a.ml + 2 * at) = make_float2(x.m, x.l);
 }
 
 // Few columns (a decode row's heads): 16 per workgroup, its four waves take the
@@ -780,7 +874,7 @@ __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
     __shared__ float ml_s[WT / 2 * 3 * 64];
     const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
     const int wt = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    A8<16, X> w{a, {}};
+    A8<16, WT, X> w{a, {}};
     if (!w.place()) return;                       // uniform
     const int b = w.k.b, g = w.k.g, G = w.k.G;
     const int c = w.k.c0 + col, cc = min(c, w.k.ncols - 1);
@@ -816,11 +910,17 @@ __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
     // again, from the cache): a conditional load's registers would be copied, and so
     // waited for, where the branches meet.
     const int mine = end - 1 - t >= 0 ? t + (end - 1 - t) / WT * WT : t;   // the wave's last tile
+    // the query and the first pages in one memory round; its digits while K and V
+    // are on their way
+    float x[NS][16];
     Pages p = pages(t);
+    a8_query_load<NS>(a.q + orow * D + 16 * kg, x);
+    __builtin_amdgcn_sched_barrier(0);
     load_k(p);
     float ks = a.ks[block(p.v)], vs = a.vs[block(p.v)];
     load_v(p);
     p = pages(min(t + WT, mine));
+    __builtin_amdgcn_sched_barrier(0);
     v4f o[1][ND];
 #pragma unroll
     for (int i = 0; i < ND; ++i) o[0][i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
@@ -830,7 +930,7 @@ __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
     k[0].lo = w.first(cc);
     k[0].slope = X && a.slopes ? a.slopes[g * G + cc % G] : 0.0f;
     v4i qd[3][NS];
-    k[0].f = a8_query<D, X>(a, a.q + orow * D + 16 * kg, qd);
+    k[0].f = a8_query<NS, X>(a, x, qd);
     auto tile = [&](auto form) __attribute__((always_inline)) {
         constexpr bool edge = decltype(form)::value;
         const int pt = t * LGX_A8_TILE + 16 * kg;
@@ -886,7 +986,7 @@ __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
         }
         __syncthreads();
     }
-    if (wt == 0 && ok) a8_store<ND>(a, orow, w.k.sp, k[0], kg, o[0]);
+    if (wt == 0 && ok) a8_store<16, ND>(a, w.k, orow, c, k[0], kg, o[0]);
 }
 
 // The query of a lane's column as two binary16 parts per operand (22 bits under the
@@ -941,7 +1041,7 @@ __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
     __shared__ __align__(16) uint4 f_s[2][2 * NF * 64], raw_s[NF * 64];
     const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    A8<64 * NT, X> w{a, {}};
+    A8<64 * NT, 1, X> w{a, {}};
     if (!w.place()) return;                       // uniform
     const int b = w.k.b, g = w.k.g, G = w.k.G;
     const int wcol = w.k.c0 + wave * 16 * NT;     // the wave's first column
@@ -1103,60 +1203,77 @@ __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
     for (int n = 0; n < NT; ++n) {
         const int c = wcol + 16 * n + col;
         k[n].l = col_sum(k[n].l);
-        if (c < w.k.ncols) a8_store<ND>(a, orow(c), w.k.sp, k[n], kg, o[n]);
+        if (c < w.k.ncols) a8_store<64 * NT, ND>(a, w.k, orow(c), c, k[n], kg, o[n]);
     }
 }
 
-// Joins the splits of one (row, head): the splits' weights into LDS, then D / 4
-// threads per split, 1024 / D splits at a time.
-template <int D>
-__device__ __forceinline__ void attn8_merge_body(const lgx_attn8_args& a) {
-    constexpr int Q = D / 4, NG = 256 / Q;
-    __shared__ float w_s[LGX_A8_SPLITS], red_s[4];
-    __shared__ v4f o_s[256];
-    const int tid = threadIdx.x;
-    const int64_t rh = blockIdx.x;
-    const int row = (int)(rh / a.hq), b = row / a.P, j = row - b * a.P;
+// Joins the splits of one (row, head): D / 4 threads per split, TH / (D / 4) splits at
+// a time.  TH: 256 threads, or a wave where there are many rows and so few splits
+// each.
+template <int D, int TH>
+__device__ __forceinline__ void attn8_join_body(const lgx_attn8_args& a) {
+    constexpr int Q = D / 4, NG = TH / Q, NW = TH / 64;
+    __shared__ v4f o_s[NW > 1 ? NG * Q : 1];
+    __shared__ float ml_s[2 * NW];
+    const int tid = threadIdx.x % TH;
+    const int64_t rh = (int64_t)blockIdx.x * (256 / TH) + threadIdx.x / TH;
+    if (rh >= (int64_t)a.rows * a.hq) return;     // uniform per wave
+    const int row = (int)(rh / a.hq), h = (int)(rh - (int64_t)row * a.hq), b = row / a.P, j = row - b * a.P;
     if (a.n_new && j >= a.n_new[b]) return;
-    const float2* ml = (const float2*)(a.part + (int64_t)a.rows * a.hq * a.nsplit * D) + rh * a.nsplit;
-    static_assert(LGX_A8_SPLITS == 512, "two splits per thread");
-    float2 x[2];
+    const int G = a.hq / a.hkv, g = h / G, c = j * G + h - g * G, cb = c / a.cols;
+    const int u = b * a.ncb + cb, pos = a.plan[2 * u], ns = a.plan[2 * u + 1];
+    if (ns < 2) return;
+    auto at = [&](int s) { return ((int64_t)(pos + s) * a.hkv + g) * a.cols + c - cb * a.cols; };
+    float m = -__builtin_inff(), l = 0.0f;
+    for (int s = tid; s < ns; s += TH) m = fmaxf(m, a.ml[2 * at(s)]);
+    m = wave_max(m);
+    if (NW > 1) {
+        if ((tid & 63) == 0) ml_s[tid >> 6] = m;
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        x[i] = tid + 256 * i < a.nsplit ? ml[tid + 256 * i] : make_float2(-__builtin_inff(), 0.0f);
-    float m = wave_max(fmaxf(x[0].x, x[1].x));
-    if ((tid & 63) == 0) red_s[tid >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red_s[0], red_s[1]), fmaxf(red_s[2], red_s[3]));
-    __syncthreads();
-    float l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        // an empty split's maximum is -inf
-        const float w = x[i].x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x[i].x - m);
-        w_s[tid + 256 * i] = w;
-        l = fmaf(w, x[i].y, l);
+        for (int i = 0; i < NW; ++i) m = fmaxf(m, ml_s[i]);
+    }
+    // an empty split's maximum is -inf
+    auto weight = [&](float x) { return x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x - m); };
+    for (int s = tid; s < ns; s += TH) {
+        const float2 x = *(const float2*)(a.ml + 2 * at(s));
+        l = fmaf(weight(x.x), x.y, l);
     }
 #pragma unroll
-    for (int s = 32; s; s >>= 1) l += __shfl_xor(l, s, 64);
-    if ((tid & 63) == 0) red_s[tid >> 6] = l;
-    __syncthreads();
-    l = (red_s[0] + red_s[1]) + (red_s[2] + red_s[3]);
+    for (int s = 32; s; s >>= 1) l += shfl_xor_f(l, s);
+    if (NW > 1) {
+        if ((tid & 63) == 0) ml_s[NW + (tid >> 6)] = l;
+        __syncthreads();
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) l += ml_s[NW + i];
+    }
     const int q = tid % Q, sg = tid / Q;
-    const v4f* p = (const v4f*)(a.part + rh * a.nsplit * D) + q;
     v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (int s = sg; s < a.nsplit; s += NG) o += p[(int64_t)s * Q] * w_s[s];
-    o_s[tid] = o;
-    __syncthreads();
-    if (tid >= Q) return;
+    for (int s = sg; s < ns; s += NG) {
+        const int64_t i = at(s);
+        o += *((const v4f*)(a.part + i * D) + q) * weight(a.ml[2 * i]);
+    }
+    if (NW > 1) {
+        o_s[tid] = o;
+        __syncthreads();
+        if (tid >= Q) return;
 #pragma unroll
-    for (int i = 1; i < NG; ++i) o += o_s[tid + i * Q];
-    const float s = l == 0.0f ? 0.0f : 1.0f / l;
-    *((v4f*)(a.out + rh * D) + q) = o * s;
+        for (int i = 1; i < NG; ++i) o += o_s[tid + i * Q];
+    } else {
+#pragma unroll
+        for (int s = Q; s < 64; s <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += shfl_xor_f(o[e], s);
+        if (tid >= Q) return;
+    }
+    *((v4f*)(a.out + rh * D) + q) = o * (l == 0.0f ? 0.0f : 1.0f / l);
 }
-extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_merge_d64(const lgx_attn8_args a) { attn8_merge_body<64>(a); }
-extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_merge_d128(const lgx_attn8_args a) { attn8_merge_body<128>(a); }
+extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_join_d64(const lgx_attn8_args a) { attn8_join_body<64, 256>(a); }
+extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_join_d128(const lgx_attn8_args a) { attn8_join_body<128, 256>(a); }
+extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_joinw_d64(const lgx_attn8_args a) { attn8_join_body<64, 64>(a); }
+extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_joinw_d128(const lgx_attn8_args a) { attn8_join_body<128, 64>(a); }
 
 #define LGX_A8_KERNELS(D)                                                                                              \
     extern "C" __global__ __launch_bounds__(256, 2) void lgx_k_attn8_d##D##_c16(const lgx_attn8_args a) {              \

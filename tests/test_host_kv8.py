@@ -133,8 +133,8 @@ def test_append_and_read_cover_every_page_that_rows_can_touch(host, rows):
     (1, 28, 4, 128, 8000, 5, 0), (8, 28, 4, 128, 4000, 512, 0), (2, 14, 2, 64, 30000, 3, 700), (1, 14, 2, 64, 30000, 1, 1),
     (1, 28, 4, 128, 100000, 2047, 100), (1, 1, 1, 64, 64, 2047, 0), (300, 8, 8, 64, 2000, 100, 0)])
 def test_attention_reaches_every_tile_of_every_column(host, B, hq, hkv, d, top, rows, window):
-    """The workgroups' splits cover the tiles of 64 tokens that any block of columns
-    sees, and the workspace holds their partial results."""
+    """A workgroup for every block of columns of every KV head at least, and where
+    their tiles are split among more, room for every workgroup's partial results."""
     opts = ["opts", [0.0, 0.0, window, None]] if window else None
     cache = kv(pages=1000, hkv=hkv, d=d)
     call = prefill(B, rows, hq, -(-top // 16), top, cache, opts) if rows > 1 else decode(B, hq, -(-top // 16), top, cache, opts)
@@ -143,15 +143,15 @@ def test_attention_reaches_every_tile_of_every_column(host, B, hq, hkv, d, top, 
     name, gx, gy, gz, block = launches[0]
     assert name.startswith("lgx_k_attn8x_d" if window else "lgx_k_attn8_d") and gy == gz == 1
     cols = int(name.split("_c")[1])
-    ncb = -(-rows * (hq // hkv) // cols)
-    nsplit, rest = divmod(gx, B * hkv * ncb)
-    assert rest == 0 and nsplit >= 1
-    assert len(launches) == (1 if nsplit == 1 else 2)
-    if nsplit > 1:
-        assert launches[1][0] == f"lgx_k_attn8_merge_d{d}"
-        assert alloc >= B * rows * hq * nsplit * (d + 2) * 4
+    units = B * -(-rows * (hq // hkv) // cols)
+    if len(launches) == 1:
+        assert gx == units * hkv and alloc == 0
     else:
-        assert alloc == 0
+        assert gx % hkv == 0 and gx >= units * hkv and units <= 256
+        assert launches[1][0] in (f"lgx_k_attn8_join_d{d}", f"lgx_k_attn8_joinw_d{d}")
+        per = 4 if "joinw" in launches[1][0] else 1
+        assert launches[1][1] * per >= B * rows * hq > (launches[1][1] - 1) * per
+        assert alloc >= gx * cols * (d + 2) * 4 + units * 8
 
 
 def angles(max_pos, rot, theta):
