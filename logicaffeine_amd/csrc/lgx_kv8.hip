@@ -538,7 +538,7 @@ struct A8Block {
     int unit;          // b * ncb + column block
     int pos, ns;       // place among all splits, and splits of the unit
 };
-template <int NC, int WT, bool X>
+template <int NC, bool X>
 struct A8 {
     const lgx_attn8_args& a;
     A8Block k;
@@ -558,8 +558,8 @@ struct A8 {
     // false: nothing to do.  With a.per alone, all units' tiles go in equal runs to the
     // workgroups (ragged batches: 64 sequences of 256 to 4096 tokens, 28/4 heads of
     // 128, where runs of the longest length take xx us, equal ones yy): every wave
-    // computes the run length from all lengths (four units per lane), the least
-    // multiple of WT tiles with which all runs fit into a.per per KV head, then
+    // computes the run length from all lengths (four units per lane), about the least
+    // with which all runs fit into a.per per KV head, then
     // finds the unit and the run of this workgroup in the sums over the units.
     __device__ __forceinline__ bool place() {
         k.G = a.hq / a.hkv;
@@ -579,19 +579,19 @@ struct A8 {
             const int lane = threadIdx.x & 63;
             k.pos = __builtin_amdgcn_readfirstlane(blockIdx.x / a.hkv);
             k.g = blockIdx.x - k.pos * a.hkv;
-            int n[4], all = 0;                    // tiles of the lane's units; -1: no such columns
+            int n[4], len[4], cnt[4], all = 0;    // tiles of the lane's units; -1: no such columns
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int u = 4 * lane + i, uc = min(u, a.units - 1), b = a.ncb == 1 ? uc : uc / a.ncb;
-                const int c0 = (uc - b * a.ncb) * NC, ncols = rows(b) * k.G;
-                const int2 t = tiles(max(a.seq_len[b], 0), c0, ncols);
-                n[i] = u < a.units && c0 < ncols ? t.y - t.x : -1;
+                const int c0 = (uc - b * a.ncb) * NC;
+                cnt[i] = rows(b) * k.G;
+                len[i] = max(a.seq_len[b], 0);
+                const int2 t = tiles(len[i], c0, cnt[i]);
+                n[i] = u < a.units && c0 < cnt[i] ? t.y - t.x : -1;
                 all += max(n[i], 0);
             }
             const int total = __builtin_amdgcn_readlane(wave_scan(all), 63);
-            constexpr int least = LGX_A8_MIN;
-            static_assert(least % WT == 0, "the waves of a run have equal shares");
-            cps = max(least, (int)((total + a.per - 1) / a.per + WT - 1) / WT * WT);
+            cps = max(LGX_A8_MIN, (int)((unsigned)(total + a.per - 1) / (unsigned)a.per));
             int m[4], upto;
             for (;;) {
                 int c = 0;
@@ -602,7 +602,7 @@ struct A8 {
                 }
                 upto = wave_scan(c);
                 if (__builtin_amdgcn_readlane(upto, 63) <= a.per) break;
-                cps += max(WT, cps / (8 * WT) * WT);   // ends: a.per >= a.units
+                cps += max(1, cps >> 4);          // ends: a.per >= a.units
             }
             const uint64_t past = __builtin_amdgcn_ballot_w64(upto > k.pos);
             if (!past) return false;
@@ -616,9 +616,14 @@ struct A8 {
                 s -= next ? mq : 0;
                 i += next ? 1 : 0;
             }
-            const int m0 = __builtin_amdgcn_readlane(m[0], at), m1 = __builtin_amdgcn_readlane(m[1], at);
-            const int m2 = __builtin_amdgcn_readlane(m[2], at), m3 = __builtin_amdgcn_readlane(m[3], at);
-            k.ns = i == 0 ? m0 : i == 1 ? m1 : i == 2 ? m2 : m3;
+            auto pick = [&](const int (&v)[4]) {
+                const int v0 = __builtin_amdgcn_readlane(v[0], at), v1 = __builtin_amdgcn_readlane(v[1], at);
+                const int v2 = __builtin_amdgcn_readlane(v[2], at), v3 = __builtin_amdgcn_readlane(v[3], at);
+                return i == 0 ? v0 : i == 1 ? v1 : i == 2 ? v2 : v3;
+            };
+            k.ns = pick(m);
+            k.sl = pick(len);
+            k.ncols = pick(cnt);
             k.unit = 4 * at + i;
             if (s == 0 && k.g == 0 && threadIdx.x == 0) {
                 a.plan[2 * k.unit] = k.pos;
@@ -634,9 +639,11 @@ struct A8 {
         }
         k.b = __builtin_amdgcn_readfirstlane(k.unit / a.ncb);
         k.c0 = (k.unit - k.b * a.ncb) * NC;
-        k.ncols = rows(k.b) * k.G;
+        if (!a.per || a.cps) {
+            k.ncols = rows(k.b) * k.G;
+            k.sl = max(a.seq_len[k.b], 0);
+        }
         if (k.c0 >= k.ncols) return false;
-        k.sl = max(a.seq_len[k.b], 0);
         const int2 t = tiles(k.sl, k.c0, k.ncols);
         k.tb0 = t.x + s * cps;
         k.tb1 = a.per ? min(t.y, k.tb0 + cps) : t.y;
@@ -874,7 +881,7 @@ __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
     __shared__ float ml_s[WT / 2 * 3 * 64];
     const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
     const int wt = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    A8<16, WT, X> w{a, {}};
+    A8<16, X> w{a, {}};
     if (!w.place()) return;                       // uniform
     const int b = w.k.b, g = w.k.g, G = w.k.G;
     const int c = w.k.c0 + col, cc = min(c, w.k.ncols - 1);
@@ -1041,7 +1048,7 @@ __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
     __shared__ __align__(16) uint4 f_s[2][2 * NF * 64], raw_s[NF * 64];
     const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    A8<64 * NT, 1, X> w{a, {}};
+    A8<64 * NT, X> w{a, {}};
     if (!w.place()) return;                       // uniform
     const int b = w.k.b, g = w.k.g, G = w.k.G;
     const int wcol = w.k.c0 + wave * 16 * NT;     // the wave's first column
