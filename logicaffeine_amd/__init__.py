@@ -299,12 +299,12 @@ class Q8Matrix:
         return self.qs.numel() + 2 * self.d.numel()
 
 
-def _tensor(name, x, dtype: str, shape):
-    """x, refused unless it is a contiguous device tensor of that type and shape
-    (None: any extent)."""
-    if str(x.dtype) != "torch." + dtype or not x.is_contiguous() or not x.is_cuda:
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor on the device")
-    if len(x.shape) != len(shape) or any(w is not None and w != n for w, n in zip(shape, x.shape)):
+def _tensor(name, x, dtype, shape, dev):
+    """x, refused unless it is a contiguous tensor of that type and shape (None: any
+    extent) on dev."""
+    if x.dtype is not dtype or x.device != dev or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor on {dev}, not {x.dtype} on {x.device}")
+    if x.shape != shape and (len(x.shape) != len(shape) or any(w is not None and w != n for w, n in zip(shape, x.shape))):
         raise ValueError(f"{name} has shape {tuple(x.shape)}, expected {tuple(shape)}")
     return x
 
@@ -314,11 +314,15 @@ class KvCacheI8:
     pages [pages][hkv][d][16], float32 scales [pages][hkv] for each."""
 
     def __init__(self, k, v, k_scale, v_scale):
+        import torch as t
+
+        if k.dim() != 4:
+            raise ValueError(f"k has shape {tuple(k.shape)}, expected [pages][hkv][16][d]")
         n, hkv, _, d = k.shape
-        _tensor("k", k, "int8", (n, hkv, 16, d))
-        _tensor("v", v, "int8", (n, hkv, d, 16))
-        _tensor("k_scale", k_scale, "float32", (n, hkv))
-        _tensor("v_scale", v_scale, "float32", (n, hkv))
+        _tensor("k", k, t.int8, (n, hkv, 16, d), k.device)
+        _tensor("v", v, t.int8, (n, hkv, d, 16), k.device)
+        _tensor("k_scale", k_scale, t.float32, (n, hkv), k.device)
+        _tensor("v_scale", v_scale, t.float32, (n, hkv), k.device)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.hkv, self.d, self.device = n, hkv, d, k.device
         self._c = KvI8C(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, hkv, d)
@@ -340,10 +344,12 @@ class Rope:
     pairs (i, i + rot / 2), or (2i, 2i + 1) when interleaved."""
 
     def __init__(self, cos, sin, interleaved: bool = False):
+        import torch as t
+
         n, half = cos.shape
-        _tensor("cos", cos, "float32", (n, half))
-        _tensor("sin", sin, "float32", (n, half))
-        self.cos, self.sin = cos, sin
+        _tensor("cos", cos, t.float32, (n, half), cos.device)
+        _tensor("sin", sin, t.float32, (n, half), cos.device)
+        self.cos, self.sin, self.device = cos, sin, cos.device
         self._c = RopeC(cos.data_ptr(), sin.data_ptr(), 2 * half, int(interleaved), n)
         self.cstruct = C.byref(self._c)
 
@@ -370,7 +376,9 @@ class AttnOpts:
 
     def __init__(self, scale: float = 0.0, softcap: float = 0.0, window: int = 0, slopes=None):
         if slopes is not None:
-            _tensor("slopes", slopes, "float32", (None,))
+            import torch as t
+
+            _tensor("slopes", slopes, t.float32, (None,), slopes.device)
         self.slopes = slopes
         self._c = AttnOptsC(scale, softcap, window, _ptr_or_none(slopes))
         self.cstruct = C.byref(self._c)
@@ -606,12 +614,14 @@ class Context:
         hq = width // d - 2 * hkv
         if rows != B * P or hq < 1 or width % d:
             raise ValueError(f"qkv {tuple(qkv.shape)} is not [{B * P}][(hq + {2 * hkv}) * {d}]")
-        _tensor("qkv", qkv, "float32", (rows, width))
+        _tensor("qkv", qkv, t.float32, qkv.shape, self.dev)
         if bias is not None:
-            _tensor("bias", bias, "float32", (width,))
+            _tensor("bias", bias, t.float32, (width,), self.dev)
+        if rope.device != self.dev:
+            raise ValueError(f"the rotation's tables are on {rope.device}, the context on {self.dev}")
         self._lengths(seq_len, n_new, page_table, kv, B)
         q_out = t.empty((rows, hq, d), dtype=t.float32, device=self.dev) if q_out is None else \
-            _tensor("q_out", q_out, "float32", (rows, hq, d))
+            _tensor("q_out", q_out, t.float32, (rows, hq, d), self.dev)
         _check(lib().lgx_rope_kv_append_i8(
             self.handle, qkv.data_ptr(), _ptr_or_none(bias), rope.cstruct, seq_len.data_ptr(),
             _ptr_or_none(n_new), page_table.data_ptr(), kv.cstruct, q_out.data_ptr(), B, P, hq, maxp, self._s()))
@@ -624,9 +634,9 @@ class Context:
         self._lengths(start, None, page_table, kv, B)
         shape = (B, n, kv.hkv, kv.d)
         k_out = t.empty(shape, dtype=t.float32, device=self.dev) if k_out is None else \
-            _tensor("k_out", k_out, "float32", shape)
+            _tensor("k_out", k_out, t.float32, shape, self.dev)
         v_out = t.empty(shape, dtype=t.float32, device=self.dev) if v_out is None else \
-            _tensor("v_out", v_out, "float32", shape)
+            _tensor("v_out", v_out, t.float32, shape, self.dev)
         _check(lib().lgx_kv_read_i8(self.handle, kv.cstruct, page_table.data_ptr(), start.data_ptr(), B, n, maxp,
                                     k_out.data_ptr(), v_out.data_ptr(), self._s()))
         return k_out, v_out
@@ -634,16 +644,18 @@ class Context:
     def _lengths(self, seq_len, n_new, page_table, kv, B):
         if kv.device != self.dev:
             raise ValueError(f"the cache is on {kv.device}, the context on {self.dev}")
-        _tensor("page_table", page_table, "int32", (B, None))
-        _tensor("lengths", seq_len, "int32", (B,))
+        i32 = self.torch.int32
+        _tensor("page_table", page_table, i32, page_table.shape, self.dev)
+        _tensor("lengths", seq_len, i32, (B,), self.dev)
         if n_new is not None:
-            _tensor("n_new", n_new, "int32", (B,))
+            _tensor("n_new", n_new, i32, (B,), self.dev)
 
     def gqa_decode_attn_i8(self, q, kv: KvCacheI8, page_table, seq_len, max_seq_len: int, opts: AttnOpts = None,
                            out=None):
         """q [B][hq][d] over the first seq_len[b] tokens of the 8-bit cache."""
-        B, hq = q.shape[0], q.shape[1]
-        _tensor("q", q, "float32", (B, None, kv.d))
+        B, hq, d = q.shape
+        if d != kv.d or page_table.shape[0] != B:
+            raise ValueError(f"q {tuple(q.shape)} for heads of {kv.d} and a table of {page_table.shape[0]} sequences")
         self._lengths(seq_len, None, page_table, kv, B)
         out = self._attn_out(q, opts, out)
         _check(lib().lgx_gqa_decode_attn_i8(
@@ -655,8 +667,9 @@ class Context:
                             opts: AttnOpts = None, out=None):
         """q [B*P][hq][d]: row b*P + j (j < n_new[b]) is the query at position
         seq_len[b] + j, causal over the 8-bit cache."""
-        B, hq = page_table.shape[0], q.shape[1]
-        _tensor("q", q, "float32", (B * P, None, kv.d))
+        B, (rows, hq, d) = page_table.shape[0], q.shape
+        if rows != B * P or d != kv.d:
+            raise ValueError(f"q {tuple(q.shape)} is not [{B * P}][hq][{kv.d}]")
         self._lengths(seq_len, n_new, page_table, kv, B)
         out = self._attn_out(q, opts, out)
         _check(lib().lgx_gqa_prefill_attn_i8(
@@ -666,11 +679,13 @@ class Context:
         return out
 
     def _attn_out(self, q, opts, out):
-        if opts is not None and opts.slopes is not None and opts.slopes.numel() != q.shape[1]:
-            raise ValueError(f"{opts.slopes.numel()} slopes for {q.shape[1]} query heads")
+        f32 = self.torch.float32
+        _tensor("q", q, f32, q.shape, self.dev)
+        if opts is not None and opts.slopes is not None:
+            _tensor("slopes", opts.slopes, f32, (q.shape[1],), self.dev)
         if out is None:
             return self.torch.empty_like(q)
-        return _tensor("out", out, "float32", q.shape)
+        return _tensor("out", out, f32, q.shape, self.dev)
 
     def q8_gemm(self, W: Q8Matrix, xq, xd, y=None):
         t = self.torch
