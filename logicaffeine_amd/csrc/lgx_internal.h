@@ -175,9 +175,9 @@ enum Kern {
     K_KV8_APPEND1_D128,
     K_KV8_READ_D64,
     K_KV8_READ_D128,
-    K_ATTN8_D64,     // 16 columns; + 1: with caps, distances or a window; + 2: 128 columns
-    K_ATTN8_D128 = K_ATTN8_D64 + 4,
-    K_ATTN8_JOIN_D64 = K_ATTN8_D128 + 4,   // + 1: a wave per (row, head)
+    K_ATTN8_D64,     // 16 columns; + 1: with caps, distances or a window; + 2, + 4: 32, 128 columns
+    K_ATTN8_D128 = K_ATTN8_D64 + 6,
+    K_ATTN8_JOIN_D64 = K_ATTN8_D128 + 6,   // + 1: a wave per (row, head)
     K_ATTN8_JOIN_D128 = K_ATTN8_JOIN_D64 + 2,
     K_COUNT = K_ATTN8_JOIN_D128 + 2
 };
@@ -229,8 +229,10 @@ inline const char* const kKernelNames[] = {
     "lgx_k_q8_gemm_grpm16",
     "lgx_k_kv8_append_d64", "lgx_k_kv8_append_d128",
     "lgx_k_kv8_append1_d64", "lgx_k_kv8_append1_d128", "lgx_k_kv8_read_d64", "lgx_k_kv8_read_d128",
-    "lgx_k_attn8_d64_c16", "lgx_k_attn8x_d64_c16", "lgx_k_attn8_d64_c128", "lgx_k_attn8x_d64_c128",
-    "lgx_k_attn8_d128_c16", "lgx_k_attn8x_d128_c16", "lgx_k_attn8_d128_c128", "lgx_k_attn8x_d128_c128",
+    "lgx_k_attn8_d64_c16", "lgx_k_attn8x_d64_c16", "lgx_k_attn8_d64_c32",
+    "lgx_k_attn8x_d64_c32", "lgx_k_attn8_d64_c128", "lgx_k_attn8x_d64_c128",
+    "lgx_k_attn8_d128_c16", "lgx_k_attn8x_d128_c16", "lgx_k_attn8_d128_c32",
+    "lgx_k_attn8x_d128_c32", "lgx_k_attn8_d128_c128", "lgx_k_attn8x_d128_c128",
     "lgx_k_attn8_join_d64", "lgx_k_attn8_joinw_d64", "lgx_k_attn8_join_d128", "lgx_k_attn8_joinw_d128",
 };
 
@@ -302,7 +304,8 @@ struct lgx_ctx {
     bool tiled_s4 = true;         // LGX_TILED_S4=0: tiled products always in stages of 2 pairs
     int pfa_rows = 0;             // LGX_PFA_ROWS: force 32 / 16 (query row, head) pairs per prefill attention workgroup
     int attn8_wgs = 2;            // LGX_A8_WGS: workgroups per compute unit the 8-bit cache's attention splits for
-    int attn8_narrow = 48;        // LGX_A8_NARROW: most (row, head) pairs per sequence and KV head through 16-column workgroups
+    int attn8_cols = 0;           // LGX_A8_COLS: force 16 / 32 / 128 (row, head) pairs per workgroup of it (0: by size)
+    int attn8_min = 4;
     bool prefill_serial = false;  // LGX_PREFILL=serial: prefill as P decode passes
     int prefill_chunk = 0;        // LGX_PREFILL_CHUNK: positions per prefill chunk (0: by batch)
     int ncu = 256;                // compute units of the device

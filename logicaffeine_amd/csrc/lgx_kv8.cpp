@@ -26,14 +26,17 @@ lgx_status check_kv(const lgx_kv_i8* kv, int32_t maxp) {
 int pages_touched(int n) { return (int)(((int64_t)n + LGX_PAGE - 2) / LGX_PAGE + 1); }
 
 // (row, head) pairs of a workgroup.
-int attn8_cols(const lgx_ctx* c, int64_t cols) { return cols <= c->attn8_narrow ? 16 : 128; }
+int attn8_cols(const lgx_ctx* c, int64_t cols, int64_t heads) {
+    if (c->attn8_cols == 16 || c->attn8_cols == 32 || c->attn8_cols == 128) return c->attn8_cols;
+    return cols <= 48 ? 16 : 128;
+}
 
 // Launch over B sequences.  Where one workgroup per (sequence, KV head, column block)
 // would not fill the device several times over, their tiles are split among
 // workgroups (the splitting itself is done on the device, by the lengths).
 lgx_status run_attn8(lgx_ctx* c, lgx_attn8_args& a, int B, int d, bool x, void* stream) {
     const int64_t cols = (int64_t)a.P * (a.hq / a.hkv);
-    const int nc = attn8_cols(c, cols);
+    const int nc = attn8_cols(c, cols, (int64_t)B * a.hkv);
     const int64_t ncb = (cols + nc - 1) / nc, units = B * ncb, blocks = units * a.hkv;
     a.ncb = (int)ncb;
     a.cols = nc;
@@ -41,18 +44,19 @@ lgx_status run_attn8(lgx_ctx* c, lgx_attn8_args& a, int B, int d, bool x, void* 
     int64_t tiles = cdiv(a.maxlen, LGX_A8_TILE);
     if (a.window) tiles = std::min<int64_t>(tiles, ((int64_t)a.window + nc) / LGX_A8_TILE + 2);
     const int64_t want = (int64_t)c->attn8_wgs * c->ncu;
-    const bool split = tiles > LGX_A8_MIN && units <= LGX_A8_UNITS && blocks < (nc == 16 ? 4 * want : want) && !(units == 1 && 2 * blocks > want);
+    const bool split = tiles > c->attn8_min && units <= LGX_A8_UNITS && blocks < (nc == 16 ? 4 * want : want) && !(units == 1 && 2 * blocks > want);
     lgx_status st;
     if (split) {
         int64_t per = std::max<int64_t>(units, want / a.hkv);
         if (units == 1 && !a.window) {
-            a.cps = (int)std::max<int64_t>(LGX_A8_MIN, ((tiles + per - 1) / per + 3) / 4 * 4);
+            a.cps = (int)std::max<int64_t>(c->attn8_min, ((tiles + per - 1) / per + 3) / 4 * 4);
             per = (tiles + a.cps - 1) / a.cps;
         }
         const int64_t slots = per * a.hkv * nc;
         float* ws = nullptr;
         if ((st = ensure_ws(c, (size_t)(slots * (d + 2) + 2 * units) * sizeof(float), &ws)) != LGX_OK) return st;
         a.per = (int)per;
+        a.least = c->attn8_min;
         a.units = (int)units;
         a.part = ws;
         a.ml = ws + slots * d;
@@ -60,7 +64,7 @@ lgx_status run_attn8(lgx_ctx* c, lgx_attn8_args& a, int B, int d, bool x, void* 
     }
     const int64_t grid = split ? (int64_t)a.per * a.hkv : blocks;
     if (grid > UINT32_MAX / 256) return fail(LGX_OUT_OF_BOUNDS, "attention of %lld workgroups", (long long)grid);
-    const int k = (d == 64 ? K_ATTN8_D64 : K_ATTN8_D128) + (nc == 16 ? 0 : 2) + (x ? 1 : 0);
+    const int k = (d == 64 ? K_ATTN8_D64 : K_ATTN8_D128) + (nc == 16 ? 0 : nc == 32 ? 2 : 4) + (x ? 1 : 0);
     if ((st = launch(c, (Kern)k, dim3((unsigned)grid), dim3(256), a, stream)) != LGX_OK || !split) return st;
     // a wave joins a row's head where there are many; a workgroup, whose threads
     // read more splits at a time, where there are few

@@ -591,7 +591,7 @@ struct A8 {
                 all += max(n[i], 0);
             }
             const int total = __builtin_amdgcn_readlane(wave_scan(all), 63);
-            cps = max(LGX_A8_MIN, (int)((unsigned)(total + a.per - 1) / (unsigned)a.per));
+            cps = max(a.least, (int)((unsigned)(total + a.per - 1) / (unsigned)a.per));
             int m[4], upto;
             for (;;) {
                 int c = 0;
@@ -742,86 +742,73 @@ __device__ __forceinline__ void a8_reset(A8Col& c) {
 __device__ __forceinline__ int a8_exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 127; }
 __device__ __forceinline__ float a8_unit(const A8Col& c) { return ldexpf(1.0f, c.e - A8_UP); }
 
-// From integer scores to the tile's weights, each times its page's V scale, as two
-// binary16 parts, for N column tiles.  EDGE: some column does not see the whole
-// tile, or the scores are capped, biased or windowed (X).  ks, vs: the scales of
-// the lane's page; pt: its first token.  down[n]: the factor of what was summed
-// before.
-template <bool X, bool EDGE, int N>
-__device__ __forceinline__ void a8_weights(const lgx_attn8_args& a, float (&S)[N][16], A8Col (&c)[N], float ks, float vs, int pt,
-                                           v8h (&ph)[N][2], v8h (&pl)[N][2], float (&down)[N]) {
+// From a column tile's scores (integers, times c.f and the K scale) to its weights,
+// each times its page's V scale, as two binary16 parts.  EDGE: some column does not
+// see the whole tile, or the scores are capped, biased or windowed (X).  ks, vs: the
+// scales of the lane's page; pt: its first token.  down: the factor of what was
+// summed before.
+template <bool X, bool EDGE>
+__device__ __forceinline__ void a8_weights(const lgx_attn8_args& a, float (&S)[16], A8Col& c, float ks, float vs, int pt, v8h (&ph)[2],
+                                           v8h (&pl)[2], float& down) {
     static_assert(EDGE || !X, "other scores are formed ahead of the maximum");
     constexpr float kLog2e = 1.44269504088896341f;
-    const float inf = __builtin_inff();
-    float off[N], fk[N], r[N];
-    int top = 0;
-    if (!EDGE) top = a8_exponent(col_max(vs < inf ? vs : 0.0f));
+    const float inf = __builtin_inff(), fk = c.f * ks;
+    bool page = true;
+    if (EDGE) {
+        const int hi = c.L - pt, lo = c.lo - pt;  // what the column sees of the page
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-        fk[n] = c[n].f * ks;
-        bool page = true;
-        if (EDGE) {
-            const int hi = c[n].L - pt, lo = c[n].lo - pt;       // what the column sees of the page
+        for (int e = 0; e < 16; ++e) S[e] *= fk;
+        if constexpr (X) {
+            if (a.softcap > 0.0f) {
+                const float inv = 1.0f / a.softcap;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) S[n][e] *= fk[n];
-            if constexpr (X) {
-                if (a.softcap > 0.0f) {
-                    const float inv = 1.0f / a.softcap;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) S[n][e] = a.softcap * a8_tanh(S[n][e] * inv);
-                }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) S[n][e] = (S[n][e] - c[n].slope * (float)(hi - 1 - e)) * kLog2e;
+                for (int e = 0; e < 16; ++e) S[e] = a.softcap * a8_tanh(S[e] * inv);
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (e >= hi || e < lo) S[n][e] = -inf;
-            // a page that the column does not see may hold anything
-            page = hi > 0 && lo < LGX_PAGE;
-            top = a8_exponent(col_max(page && vs < inf ? vs : 0.0f));
+            for (int e = 0; e < 16; ++e) S[e] = (S[e] - c.slope * (float)(hi - 1 - e)) * kLog2e;
         }
-        float mt = fmaxf(fmaxf(S[n][0], S[n][1]), S[n][2]);
 #pragma unroll
-        for (int e = 3; e < 15; e += 2) mt = fmaxf(fmaxf(mt, S[n][e]), S[n][e + 1]);
-        mt = fmaxf(mt, S[n][15]);
-        mt = col_max(EDGE ? mt : mt * fk[n]);     // scales are not negative
-        // the reference moves when the maximum passes it by more than 2^4: most
-        // tiles then leave what was summed as it is
-        const float mn = mt > c[n].m + 4.0f ? mt : c[n].m;
-        const bool none = mn == -inf;             // nothing seen yet
-        const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(c[n].m - mn);
-        const int en = max(c[n].e, top);
-        down[n] = ldexpf(alpha, c[n].e - en);
-        c[n].l *= alpha;
-        c[n].m = mn;
-        c[n].e = en;
-        off[n] = none ? 0.0f : -mn;
-        r[n] = page ? ldexpf(vs, A8_UP - en) : 0.0f;
+        for (int e = 0; e < 16; ++e)
+            if (e >= hi || e < lo) S[e] = -inf;
+        // a page that the column does not see may hold anything
+        page = hi > 0 && lo < LGX_PAGE;
+    }
+    const int top = a8_exponent(col_max(page && vs < inf ? vs : 0.0f));
+    float mt = fmaxf(fmaxf(S[0], S[1]), S[2]);
+#pragma unroll
+    for (int e = 3; e < 15; e += 2) mt = fmaxf(fmaxf(mt, S[e]), S[e + 1]);
+    mt = fmaxf(mt, S[15]);
+    mt = col_max(EDGE ? mt : mt * fk);            // scales are not negative
+    // the reference moves when the maximum passes it by more than 2^4: most tiles
+    // then leave what was summed as it is
+    const float mn = mt > c.m + 4.0f ? mt : c.m;
+    const bool none = mn == -inf;                 // nothing seen yet
+    const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(c.m - mn), off = none ? 0.0f : -mn;
+    const int en = max(c.e, top);
+    down = ldexpf(alpha, c.e - en);
+    c.m = mn;
+    c.e = en;
+    const float r = page ? ldexpf(vs, A8_UP - en) : 0.0f;
+    float ps = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        S[e] = __builtin_amdgcn_exp2f(EDGE ? S[e] + off : fmaf(S[e], fk, off));
+        ps += S[e];
+        S[e] *= r;
+    }
+    c.l = fmaf(c.l, alpha, ps);
+    uint32_t hw[8], lw[8];
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+        // the first part rounded toward zero, the second holds the rest
+        const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(S[e], S[e + 1]));
+        hw[e >> 1] = h;
+        lw[e >> 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(minus_half<0>(S[e], h), minus_half<1>(S[e + 1], h)));
     }
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-        float ps = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            S[n][e] = __builtin_amdgcn_exp2f(EDGE ? S[n][e] + off[n] : fmaf(S[n][e], fk[n], off[n]));
-            ps += S[n][e];
-            S[n][e] *= r[n];
-        }
-        c[n].l += ps;
-        uint32_t hw[8], lw[8];
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-            // the first part rounded toward zero, the second holds the rest
-            const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(S[n][e], S[n][e + 1]));
-            hw[e >> 1] = h;
-            lw[e >> 1] =
-                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(minus_half<0>(S[n][e], h), minus_half<1>(S[n][e + 1], h)));
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            ph[n][i] = as_v8h(make_uint4(hw[4 * i], hw[4 * i + 1], hw[4 * i + 2], hw[4 * i + 3]));
-            pl[n][i] = as_v8h(make_uint4(lw[4 * i], lw[4 * i + 1], lw[4 * i + 2], lw[4 * i + 3]));
-        }
+    for (int i = 0; i < 2; ++i) {
+        ph[i] = as_v8h(make_uint4(hw[4 * i], hw[4 * i + 1], hw[4 * i + 2], hw[4 * i + 3]));
+        pl[i] = as_v8h(make_uint4(lw[4 * i], lw[4 * i + 1], lw[4 * i + 2], lw[4 * i + 3]));
     }
 }
 struct A8Edge { static constexpr bool value = true; };
@@ -870,23 +857,21 @@ __device__ __forceinline__ void a8_store(const lgx_attn8_args& a, const A8Block&
     if (part && kg == 0) *(float2*)(a.ml + 2 * at) = make_float2(x.m, x.l);
 }
 
-// Few columns (a decode row's heads): 16 per workgroup, its four waves take the
-// tiles in turn, K and V straight into registers: the next tile's K is in flight
+// 16 NT columns per workgroup (a decode row's heads): its four waves take the tiles in
+// turn, K and V straight into registers: the next tile's K is in flight
 // from the end of the scores on, its V from the end of the PV product; at the end
 // the waves' results are joined in LDS.
-template <int D, bool X>
+template <int D, int NT, bool X>
 __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
     constexpr int WT = 4, NS = D / 64, ND = D / 16;
-    __shared__ v4f o_s[WT / 2 * ND * 64];
-    __shared__ float ml_s[WT / 2 * 3 * 64];
+    __shared__ v4f o_s[WT / 2 * NT * ND * 64];
+    __shared__ float ml_s[WT / 2 * NT * 3 * 64];
     const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
     const int wt = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    A8<16, X> w{a, {}};
+    A8<16 * NT, X> w{a, {}};
     if (!w.place()) return;                       // uniform
     const int b = w.k.b, g = w.k.g, G = w.k.G;
-    const int c = w.k.c0 + col, cc = min(c, w.k.ncols - 1);
-    const bool ok = c < w.k.ncols;
-    const int64_t orow = ((int64_t)b * a.P + cc / G) * a.hq + g * G + cc % G;
+    auto orow = [&](int c) { return ((int64_t)b * a.P + c / G) * a.hq + g * G + c % G; };
     const int32_t* ptab = a.page_table + (int64_t)b * a.maxp;
     struct Pages {
         int k, v;
@@ -919,43 +904,73 @@ __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
     const int mine = end - 1 - t >= 0 ? t + (end - 1 - t) / WT * WT : t;   // the wave's last tile
     // the query and the first pages in one memory round; its digits while K and V
     // are on their way
-    float x[NS][16];
+    float x[NT][NS][16];
     Pages p = pages(t);
-    a8_query_load<NS>(a.q + orow * D + 16 * kg, x);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) a8_query_load<NS>(a.q + orow(min(w.k.c0 + 16 * n + col, w.k.ncols - 1)) * D + 16 * kg, x[n]);
     __builtin_amdgcn_sched_barrier(0);
     load_k(p);
     float ks = a.ks[block(p.v)], vs = a.vs[block(p.v)];
     load_v(p);
     p = pages(min(t + WT, mine));
     __builtin_amdgcn_sched_barrier(0);
-    v4f o[1][ND];
-#pragma unroll
-    for (int i = 0; i < ND; ++i) o[0][i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-    A8Col k[1];
-    a8_reset(k[0]);
-    k[0].L = w.last(cc);                          // columns past the last repeat it
-    k[0].lo = w.first(cc);
-    k[0].slope = X && a.slopes ? a.slopes[g * G + cc % G] : 0.0f;
+    v4f o[NT][ND];
+    A8Col k[NT];
+    // two column tiles' digits do not fit beside the rest: they stay in LDS, the
+    // same for all waves, and pass through registers one column tile at a time
     v4i qd[3][NS];
-    k[0].f = a8_query<NS, X>(a, x, qd);
+    __shared__ v4i q_s[NT > 1 ? NT * 3 * NS * 64 : 1];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[n][i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+        const int cc = min(w.k.c0 + 16 * n + col, w.k.ncols - 1);   // columns past the last repeat it
+        a8_reset(k[n]);
+        k[n].L = w.last(cc);
+        k[n].lo = w.first(cc);
+        k[n].slope = X && a.slopes ? a.slopes[g * G + cc % G] : 0.0f;
+        k[n].f = a8_query<NS, X>(a, x[n], qd);
+        if (NT > 1 && wt == n) {
+#pragma unroll
+            for (int i = 0; i < 3 * NS; ++i) q_s[(n * 3 * NS + i) * 64 + lane] = qd[i / NS][i % NS];
+        }
+    }
+    if (NT > 1) __syncthreads();
     auto tile = [&](auto form) __attribute__((always_inline)) {
         constexpr bool edge = decltype(form)::value;
         const int pt = t * LGX_A8_TILE + 16 * kg;
         const float ksn = ks, vsn = vs;
-        float S[1][16], down[1];
-        a8_scores<NS>([&](int u, int s) { return kw[u][s]; }, qd, S[0]);
         const Pages pn = p;
-        load_k(pn);
-        ks = a.ks[block(pn.v)];
-        vs = a.vs[block(pn.v)];
-        p = pages(min(t + 2 * WT, mine));
-        v8h ph[1][2], pl[1][2];
-        a8_weights<X, edge, 1>(a, S, k, ksn, vsn, pt, ph, pl, down);
-        if (__builtin_amdgcn_ballot_w64(down[0] != 1.0f)) {
+        v8h ph[NT][2], pl[NT][2];
+        float down[NT];
 #pragma unroll
-            for (int i = 0; i < ND; ++i) o[0][i] *= down[0];
+        for (int n = 0; n < NT; ++n) {
+            float S[16];
+            if (NT > 1) {
+                int at = lane;
+                asm volatile("" : "+v"(at));      // read here, not once ahead of the loop
+#pragma unroll
+                for (int i = 0; i < 3 * NS; ++i) qd[i / NS][i % NS] = q_s[(n * 3 * NS + i) * 64 + at];
+            }
+            a8_scores<NS>([&](int u, int s) { return kw[u][s]; }, qd, S);
+            if (n == NT - 1) {
+                load_k(pn);
+                ks = a.ks[block(pn.v)];
+                vs = a.vs[block(pn.v)];
+                p = pages(min(t + 2 * WT, mine));
+            }
+            a8_weights<X, edge>(a, S, k[n], ksn, vsn, pt, ph[n], pl[n], down[n]);
         }
-        a8_pv<ND, 1>([&](int i, uint4& h0, uint4& h1) { i8_to_v8h(vw[i], h0, h1); }, ph, pl, o);
+        bool moved = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) moved = moved || down[n] != 1.0f;
+        if (__builtin_amdgcn_ballot_w64(moved)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < ND; ++i) o[n][i] *= down[n];
+        }
+        a8_pv<ND, NT>([&](int i, uint4& h0, uint4& h1) { i8_to_v8h(vw[i], h0, h1); }, ph, pl, o);
         load_v(pn);
     };
     // the tiles that every column sees whole, then the others
@@ -965,35 +980,47 @@ __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
     }
 #pragma unroll 1
     for (; t < end; t += WT) tile(A8Edge());
-    k[0].l = col_sum(k[0].l);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) k[n].l = col_sum(k[n].l);
     // join the waves, halving their number
 #pragma unroll
     for (int h = WT / 2; h; h >>= 1) {
-        const int at = wt % h;
+        const int at = wt % h * NT;
         if (wt >= h && wt < 2 * h) {
-            ml_s[(at * 3 + 0) * 64 + lane] = k[0].m;
-            ml_s[(at * 3 + 1) * 64 + lane] = k[0].l;
-            ml_s[(at * 3 + 2) * 64 + lane] = (float)k[0].e;
 #pragma unroll
-            for (int i = 0; i < ND; ++i) o_s[(at * ND + i) * 64 + lane] = o[0][i];
+            for (int n = 0; n < NT; ++n) {
+                ml_s[((at + n) * 3 + 0) * 64 + lane] = k[n].m;
+                ml_s[((at + n) * 3 + 1) * 64 + lane] = k[n].l;
+                ml_s[((at + n) * 3 + 2) * 64 + lane] = (float)k[n].e;
+#pragma unroll
+                for (int i = 0; i < ND; ++i) o_s[((at + n) * ND + i) * 64 + lane] = o[n][i];
+            }
         }
         __syncthreads();
         if (wt < h) {
-            const float mo = ml_s[(at * 3 + 0) * 64 + lane], lo = ml_s[(at * 3 + 1) * 64 + lane];
-            const int eo = (int)ml_s[(at * 3 + 2) * 64 + lane], en = max(k[0].e, eo);
-            const float mn = fmaxf(k[0].m, mo);
-            const float w0 = k[0].m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(k[0].m - mn);
-            const float w1 = mo == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mo - mn);
-            const float u0 = ldexpf(w0, k[0].e - en), u1 = ldexpf(w1, eo - en);
-            k[0].l = k[0].l * w0 + lo * w1;
-            k[0].m = mn;
-            k[0].e = en;
 #pragma unroll
-            for (int i = 0; i < ND; ++i) o[0][i] = o[0][i] * u0 + o_s[(at * ND + i) * 64 + lane] * u1;
+            for (int n = 0; n < NT; ++n) {
+                const float mo = ml_s[((at + n) * 3 + 0) * 64 + lane], lo = ml_s[((at + n) * 3 + 1) * 64 + lane];
+                const int eo = (int)ml_s[((at + n) * 3 + 2) * 64 + lane], en = max(k[n].e, eo);
+                const float mn = fmaxf(k[n].m, mo);
+                const float w0 = k[n].m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(k[n].m - mn);
+                const float w1 = mo == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mo - mn);
+                const float u0 = ldexpf(w0, k[n].e - en), u1 = ldexpf(w1, eo - en);
+                k[n].l = k[n].l * w0 + lo * w1;
+                k[n].m = mn;
+                k[n].e = en;
+#pragma unroll
+                for (int i = 0; i < ND; ++i) o[n][i] = o[n][i] * u0 + o_s[((at + n) * ND + i) * 64 + lane] * u1;
+            }
         }
         __syncthreads();
     }
-    if (wt == 0 && ok) a8_store<16, ND>(a, w.k, orow, c, k[0], kg, o[0]);
+    if (wt) return;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int c = w.k.c0 + 16 * n + col;
+        if (c < w.k.ncols) a8_store<16 * NT, ND>(a, w.k, orow(c), c, k[n], kg, o[n]);
+    }
 }
 
 // The query of a lane's column as two binary16 parts per operand (22 bits under the
@@ -1035,15 +1062,15 @@ __device__ __forceinline__ float a8_query16(const lgx_attn8_args& a, const float
     return isbad ? __builtin_nanf("") : a.scale / up * (X ? 1.0f : 1.44269504088896341f);
 }
 
-// Many columns (prefill): 128 per workgroup, 32 per wave.  Every tile is converted to
+// Many columns (prefill): 64 NT per workgroup, 16 NT per wave.  Every tile is converted to
 // binary16 once for all of them: each wave brings a quarter of its quants into LDS
 // (two waves K, two V; a direct load brings one 1 KiB fragment in the order of the
 // lanes), a tile ahead, and then turns them into operands in one of two LDS buffers
 // while the other's tile is in use.  With K in binary16 the scores need no joining of digits: two products,
 // one accumulator.
-template <int D, bool X>
+template <int D, int NT, bool X>
 __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
-    constexpr int NT = 2, NS = D / 64, NH = D / 32, ND = D / 16, NF = 4 * NS + ND, FW = NF / 4;
+    constexpr int NS = D / 64, NH = D / 32, ND = D / 16, NF = 4 * NS + ND, FW = NF / 4;
     static_assert(4 * NS == ND, "waves 0 and 1 bring K, 2 and 3 bring V");
     __shared__ __align__(16) uint4 f_s[2][2 * NF * 64], raw_s[NF * 64];
     const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
@@ -1159,7 +1186,8 @@ __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
                 for (int e = 0; e < 16; ++e) S[n][e] = acc[e >> 2][n][e & 3];
         }
         v8h ph[NT][2], pl[NT][2];
-        a8_weights<X, edge, NT>(a, S, k, ksn, vsn, pt, ph, pl, down);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) a8_weights<X, edge>(a, S[n], k[n], ksn, vsn, pt, ph[n], pl[n], down[n]);
         bool moved = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) moved = moved || down[n] != 1.0f;
@@ -1282,18 +1310,16 @@ extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_join_d128(const lg
 extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_joinw_d64(const lgx_attn8_args a) { attn8_join_body<64, 64>(a); }
 extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_joinw_d128(const lgx_attn8_args a) { attn8_join_body<128, 64>(a); }
 
-#define LGX_A8_KERNELS(D)                                                                                              \
-    extern "C" __global__ __launch_bounds__(256, 2) void lgx_k_attn8_d##D##_c16(const lgx_attn8_args a) {              \
-        attn8_narrow_body<D, false>(a);                                                                                \
+#define LGX_A8_KERNELS(D, C, BODY, NT)                                                                                 \
+    extern "C" __global__ __launch_bounds__(256, 2) void lgx_k_attn8_d##D##_c##C(const lgx_attn8_args a) {             \
+        BODY<D, NT, false>(a);                                                                                         \
     }                                                                                                                  \
-    extern "C" __global__ __launch_bounds__(256, 2) void lgx_k_attn8x_d##D##_c16(const lgx_attn8_args a) {             \
-        attn8_narrow_body<D, true>(a);                                                                                 \
-    }                                                                                                                  \
-    extern "C" __global__ __launch_bounds__(256, 2) void lgx_k_attn8_d##D##_c128(const lgx_attn8_args a) {             \
-        attn8_wide_body<D, false>(a);                                                                                  \
-    }                                                                                                                  \
-    extern "C" __global__ __launch_bounds__(256, 2) void lgx_k_attn8x_d##D##_c128(const lgx_attn8_args a) {            \
-        attn8_wide_body<D, true>(a);                                                                                   \
+    extern "C" __global__ __launch_bounds__(256, 2) void lgx_k_attn8x_d##D##_c##C(const lgx_attn8_args a) {            \
+        BODY<D, NT, true>(a);                                                                                          \
     }
-LGX_A8_KERNELS(64)
-LGX_A8_KERNELS(128)
+LGX_A8_KERNELS(64, 16, attn8_narrow_body, 1)
+LGX_A8_KERNELS(64, 32, attn8_narrow_body, 2)
+LGX_A8_KERNELS(64, 128, attn8_wide_body, 2)
+LGX_A8_KERNELS(128, 16, attn8_narrow_body, 1)
+LGX_A8_KERNELS(128, 32, attn8_narrow_body, 2)
+LGX_A8_KERNELS(128, 128, attn8_wide_body, 2)
