@@ -303,9 +303,8 @@ struct lgx_ctx {
     bool lm_cert = true;          // LGX_LM_CERT=0: greedy tied lm_head through the full logits
     bool tiled_s4 = true;         // LGX_TILED_S4=0: tiled products always in stages of 2 pairs
     int pfa_rows = 0;             // LGX_PFA_ROWS: force 32 / 16 (query row, head) pairs per prefill attention workgroup
-    int attn8_wgs = 2;            // LGX_A8_WGS: workgroups per compute unit the 8-bit cache's attention splits for
+    int attn8_wgs = 1;            // LGX_A8_WGS: workgroups per compute unit the 8-bit cache's attention splits for
     int attn8_cols = 0;           // LGX_A8_COLS: force 16 / 32 / 128 (row, head) pairs per workgroup of it (0: by size)
-    int attn8_min = 4;
     bool prefill_serial = false;  // LGX_PREFILL=serial: prefill as P decode passes
     int prefill_chunk = 0;        // LGX_PREFILL_CHUNK: positions per prefill chunk (0: by batch)
     int ncu = 256;                // compute units of the device

@@ -479,7 +479,6 @@ typedef struct {
     int32_t window;            // 0: all
     int32_t per, units, ncb;   // units: B * ncb; ncb: column blocks of a sequence
     int32_t cps;               // one unit: tiles per split, chosen by the host; else 0
-    int32_t least;             // tiles of a split at least
     int32_t cols;              // columns of a block (the join)
     int32_t rows;              // B*P
     float scale, softcap;

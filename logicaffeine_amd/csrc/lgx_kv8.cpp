@@ -25,44 +25,58 @@ lgx_status check_kv(const lgx_kv_i8* kv, int32_t maxp) {
 // Pages that n tokens from any slot on can touch.
 int pages_touched(int n) { return (int)(((int64_t)n + LGX_PAGE - 2) / LGX_PAGE + 1); }
 
-// (row, head) pairs of a workgroup.
-int attn8_cols(const lgx_ctx* c, int64_t cols, int64_t heads) {
+// (row, head) pairs of a workgroup, for `heads` (sequence, KV head) pairs of `cols`
+// each over up to `tiles` tiles of 64 tokens.  16 and 32 go over a tile's tokens with
+// all four waves, 128 over its columns.  Measured on the 0.5B-, 1.5B- and 7B-shaped
+// heads (us with 16 / 32 / 128):
+//  - 128 from 512 workgroups on, two per compute unit: 8 x 512 rows at 4000 tokens
+//    (7B-shaped, 896 workgroups) 672 / 529 / 498, 8 x 1024 at 1100 (1792) 391 / 306 /
+//    209; below 8 x 256 at 4000 (448) 348 / 265 / 265, 16 x 256 at 2000
+//    (1.5B-shaped, 384) 177 / 136 / 153;
+//  - 32, which read K and V half as often and convert V for twice the columns, from
+//    about 12000 tiles of 16 columns on at head dimension 128: 16 x 64 at 500 (14300)
+//    44.1 / 38.5, 1 x 256 at 4000 (28200) 57.6 / 54.3; below 16 x 64 at 700
+//    (1.5B-shaped, 8400) 25.3 / 30.7, 2 x 64 at 2000 (7200) 28.3 / 30.5; at 64, where a
+//    tile's work is half as long, from about 65000: 8 x 512 at 2000 (0.5B-shaped, 115000)
+//    101 / 95, 8 x 128 at 4000 (56000) 56.2 / 57.4, 4 x 256 at 1000 (14000) 21.5 / 26.2.
+int attn8_cols(const lgx_ctx* c, int64_t heads, int64_t cols, int64_t tiles, int d) {
     if (c->attn8_cols == 16 || c->attn8_cols == 32 || c->attn8_cols == 128) return c->attn8_cols;
-    return cols <= 48 ? 16 : 128;
+    if (cols <= 16) return 16;
+    if (heads * ((cols + 127) / 128) >= 2 * (int64_t)c->ncu) return 128;
+    return heads * ((cols + 15) / 16) * tiles >= (d == 64 ? 65536 : 12288) ? 32 : 16;
 }
 
 // Launch over B sequences.  Where one workgroup per (sequence, KV head, column block)
-// would not fill the device several times over, their tiles are split among
-// workgroups (the splitting itself is done on the device, by the lengths).
+// does not fill the device, their tiles are split among workgroups (the splitting
+// itself is done on the device, by the lengths), two per compute unit.
 lgx_status run_attn8(lgx_ctx* c, lgx_attn8_args& a, int B, int d, bool x, void* stream) {
-    const int64_t cols = (int64_t)a.P * (a.hq / a.hkv);
-    const int nc = attn8_cols(c, cols, (int64_t)B * a.hkv);
-    const int64_t ncb = (cols + nc - 1) / nc, units = B * ncb, blocks = units * a.hkv;
+    const int64_t cols = (int64_t)a.P * (a.hq / a.hkv), heads = (int64_t)B * a.hkv;
+    // the most tiles that a block can see (its rows are at most 128 apart)
+    int64_t tiles = cdiv(a.maxlen, LGX_A8_TILE);
+    if (a.window) tiles = std::min<int64_t>(tiles, ((int64_t)a.window + 128) / LGX_A8_TILE + 2);
+    const int nc = attn8_cols(c, heads, cols, tiles, d);
+    const int64_t ncb = (cols + nc - 1) / nc, units = B * ncb, blocks = heads * ncb;
     a.ncb = (int)ncb;
     a.cols = nc;
-    // the most tiles that a block can see (its rows are at most nc apart)
-    int64_t tiles = cdiv(a.maxlen, LGX_A8_TILE);
-    if (a.window) tiles = std::min<int64_t>(tiles, ((int64_t)a.window + nc) / LGX_A8_TILE + 2);
-    const int64_t want = (int64_t)c->attn8_wgs * c->ncu;
-    const bool split = tiles > c->attn8_min && units <= LGX_A8_UNITS && blocks < (nc == 16 ? 4 * want : want) && !(units == 1 && 2 * blocks > want);
+    int64_t per = (int64_t)c->attn8_wgs * c->ncu / a.hkv;
+    bool split = tiles > LGX_A8_MIN && units <= LGX_A8_UNITS && units < per;
+    if (split && units == 1 && !a.window) {
+        a.cps = (int)std::max<int64_t>(LGX_A8_MIN, ((tiles + per - 1) / per + 3) / 4 * 4);
+        per = (tiles + a.cps - 1) / a.cps;
+        if (per == 1) split = false, a.cps = 0;
+    }
     lgx_status st;
     if (split) {
-        int64_t per = std::max<int64_t>(units, want / a.hkv);
-        if (units == 1 && !a.window) {
-            a.cps = (int)std::max<int64_t>(c->attn8_min, ((tiles + per - 1) / per + 3) / 4 * 4);
-            per = (tiles + a.cps - 1) / a.cps;
-        }
         const int64_t slots = per * a.hkv * nc;
         float* ws = nullptr;
         if ((st = ensure_ws(c, (size_t)(slots * (d + 2) + 2 * units) * sizeof(float), &ws)) != LGX_OK) return st;
         a.per = (int)per;
-        a.least = c->attn8_min;
         a.units = (int)units;
         a.part = ws;
         a.ml = ws + slots * d;
         a.plan = (int32_t*)(a.ml + 2 * slots);
     }
-    const int64_t grid = split ? (int64_t)a.per * a.hkv : blocks;
+    const int64_t grid = split ? per * a.hkv : blocks;
     if (grid > UINT32_MAX / 256) return fail(LGX_OUT_OF_BOUNDS, "attention of %lld workgroups", (long long)grid);
     const int k = (d == 64 ? K_ATTN8_D64 : K_ATTN8_D128) + (nc == 16 ? 0 : nc == 32 ? 2 : 4) + (x ? 1 : 0);
     if ((st = launch(c, (Kern)k, dim3((unsigned)grid), dim3(256), a, stream)) != LGX_OK || !split) return st;

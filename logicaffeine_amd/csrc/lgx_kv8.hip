@@ -591,7 +591,7 @@ struct A8 {
                 all += max(n[i], 0);
             }
             const int total = __builtin_amdgcn_readlane(wave_scan(all), 63);
-            cps = max(a.least, (int)((unsigned)(total + a.per - 1) / (unsigned)a.per));
+            cps = max(LGX_A8_MIN, (int)((unsigned)(total + a.per - 1) / (unsigned)a.per));
             int m[4], upto;
             for (;;) {
                 int c = 0;
@@ -857,8 +857,8 @@ __device__ __forceinline__ void a8_store(const lgx_attn8_args& a, const A8Block&
     if (part && kg == 0) *(float2*)(a.ml + 2 * at) = make_float2(x.m, x.l);
 }
 
-// 16 NT columns per workgroup (a decode row's heads): its four waves take the tiles in
-// turn, K and V straight into registers: the next tile's K is in flight
+// 16 NT columns per workgroup (a decode row's heads): its four waves take the tiles
+// in turn, K and V straight into registers: the next tile's K is in flight
 // from the end of the scores on, its V from the end of the PV product; at the end
 // the waves' results are joined in LDS.
 template <int D, int NT, bool X>
