@@ -233,8 +233,9 @@ lgx_status lgx_gqa_prefill_attn_fast(lgx_ctx* ctx, const float* q, const uint16_
  * tokens (a page) and KV head: value = scale * quant.  K pages are
  * [num_pages][hkv][16][d] (token by token), V pages [num_pages][hkv][d][16]
  * (dimension by dimension: the order in which the attention reads them), both
- * 16-byte aligned; the scales are [num_pages][hkv].  d is 64 or 128.  Half the
- * memory and half the traffic of the binary16 cache.  No counterpart in the
+ * 16-byte aligned; the scales are [num_pages][hkv], not negative.  d is 64 or 128, a
+ * sequence has up to 2^26 pages.  Half the memory and half the traffic of the
+ * binary16 cache.  q, q_out and out of the calls below are 16-byte aligned.  No counterpart in the
  * reference, which has no attention. */
 typedef struct lgx_kv_i8 {
     int8_t* k;
@@ -292,8 +293,9 @@ lgx_status lgx_rope_tables(int32_t max_pos, int32_t rot, double theta, const lgx
  * An old value is therefore never off by more than one step of its block's scale.
  * Slots not appended to keep their quants.  seq_len is not advanced; lengths are
  * clamped to [0, 16 maxp]; tokens past 16 maxp and pages outside [0, num_pages)
- * are not written.  A page may belong to several sequences while none of them
- * appends to it; two sequences that append to one page in a call race. */
+ * are not written.  A page may stand in several entries of the table while none of
+ * them is appended to; a page that a call appends to through two entries gets
+ * either's tokens. */
 lgx_status lgx_rope_kv_append_i8(lgx_ctx* ctx, const float* qkv, const float* bias, const lgx_rope* rope,
                                  const int32_t* seq_len, const int32_t* n_new, const int32_t* page_table,
                                  const lgx_kv_i8* kv, float* q_out, int32_t B, int32_t P, int32_t hq,
@@ -307,7 +309,8 @@ lgx_status lgx_kv_read_i8(lgx_ctx* ctx, const lgx_kv_i8* kv, const int32_t* page
 /* Options of the attention calls below (NULL: none).  The score of a query at
  * position p and a key at t is
  *   s = scale * q.k (scale 0: 1/sqrt(d));  s = softcap * tanh(s / softcap) if
- *   softcap > 0;  s -= slopes[h] * (p - t) if slopes (device binary32 [hq]);
+ *   softcap > 0 (2^-100 at least);  s -= slopes[h] * (p - t) if slopes (device
+ *   binary32 [hq]);
  * with window > 0 only the last `window` tokens up to and with p are seen. */
 typedef struct lgx_attn_opts {
     float scale, softcap;

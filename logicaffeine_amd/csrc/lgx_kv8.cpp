@@ -14,7 +14,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 lgx_status check_kv(const lgx_kv_i8* kv, int32_t maxp) {
     if (!kv) return fail(LGX_NULL_POINTER, "kv is NULL");
     if (!kv->k || !kv->v || !kv->k_scale || !kv->v_scale) return fail(LGX_NULL_POINTER, "NULL cache pointer");
-    if (kv->num_pages <= 0 || kv->hkv <= 0 || maxp <= 0 || maxp > INT32_MAX / LGX_PAGE)
+    if (kv->num_pages <= 0 || kv->hkv <= 0 || maxp <= 0 || maxp > 1 << 26)
         return fail(LGX_INVALID_ARGUMENT, "num_pages=%d hkv=%d maxp=%d", kv->num_pages, kv->hkv, maxp);
     if (kv->d != 64 && kv->d != 128) return fail(LGX_UNSUPPORTED, "head_dim %d (64 or 128)", kv->d);
     if (!aligned16(kv->k) || !aligned16(kv->v))
@@ -105,7 +105,8 @@ lgx_status attn8(lgx_ctx* c, const float* q, const lgx_kv_i8* kv, const int32_t*
     lgx_attn8_args a{};
     a.scale = (float)(1.0 / std::sqrt((double)kv->d));
     if (opts) {
-        if (!std::isfinite(opts->scale) || !std::isfinite(opts->softcap) || opts->softcap < 0.0f || opts->window < 0)
+        if (!std::isfinite(opts->scale) || !std::isfinite(opts->softcap) ||
+            (opts->softcap != 0.0f && !(opts->softcap >= 0x1p-100f)) || opts->window < 0)
             return fail(LGX_INVALID_ARGUMENT, "scale %g, softcap %g, window %d", (double)opts->scale,
                         (double)opts->softcap, opts->window);
         if (opts->scale != 0.0f) a.scale = opts->scale;

@@ -69,6 +69,48 @@ def test_append_is_the_definition(ctx, hq, hkv, d, rot, inter, P, lens, new):
     assert np.array_equal(host(q).reshape(B, P, hq, d), want)
 
 
+@pytest.mark.parametrize("hq,hkv,d,rot,inter,P", [(4, 2, 128, 64, False, 21), (3, 1, 64, 64, True, 5), (2, 2, 128, 128, False, 1)])
+def test_append_from_rows_that_are_only_4_byte_aligned(ctx, hq, hkv, d, rot, inter, P):
+    """The same quants whether rows and tables come in wide loads or number by number."""
+    t, rng = ctx.torch, np.random.default_rng(d + P)
+    lens, width = [7, 16], (hq + 2 * hkv) * d
+    cache, table = ref.Cache(8, hkv, d, rng), table_of(rng, 2, 4)
+    cos, sin = ref.tables(64, rot)
+    x, bias = rng.standard_normal((2, P, width)).astype(np.float32), rng.standard_normal(width).astype(np.float32)
+    kv = upload(ctx, cache)
+
+    def odd(a):
+        buf = t.zeros(a.size + 1, device=ctx.dev)[1:].view(a.shape)
+        buf.copy_(ctx.to_device(a))
+        assert buf.data_ptr() % 16 == 4
+        return buf
+
+    rope = lgx.Rope(odd(cos), odd(sin), inter)
+    q = ctx.rope_kv_append_i8(odd(x.reshape(2 * P, width)), odd(bias), rope, i32(ctx, lens), i32(ctx, table), kv, P)
+    want = cache.append(x, bias, cos, sin, inter, lens, None, table, hq)
+    assert np.array_equal(host(q).reshape(want.shape), want)
+    same_cache(kv, cache)
+
+
+@pytest.mark.parametrize("P,new", [(1, [0, 1, 1, 0, 5, -2]), (3, [0, 0, -1, 0, 0, 0]), (20, [0, 20, 1, 16, 99, -7])])
+def test_append_of_few_or_no_rows(ctx, P, new):
+    """Row counts of zero, negative ones (zero) and too many (P)."""
+    rng = np.random.default_rng(P)
+    hq, hkv, d, B = 3, 1, 64, 6
+    lens = [0, 15, 16, 31, 3, 8]
+    cache, table = ref.Cache(B * 4, hkv, d, rng), table_of(rng, B, 4)
+    cos, sin = ref.tables(64, d)
+    x = rng.standard_normal((B, P, (hq + 2 * hkv) * d)).astype(np.float32)
+    kv = upload(ctx, cache)
+    q = ctx.torch.full((B * P, hq, d), 7.0, device=ctx.dev)
+    ctx.rope_kv_append_i8(ctx.to_device(x.reshape(B * P, -1)), None, rope_of(ctx, cos, sin), i32(ctx, lens), i32(ctx, table), kv, P,
+                          n_new=i32(ctx, new), q_out=q)
+    want = cache.append(x, None, cos, sin, False, lens, new, table, hq)
+    want[np.arange(P) >= np.clip(new, 0, P)[:, None]] = 7.0
+    assert np.array_equal(host(q).reshape(want.shape), want)
+    same_cache(kv, cache)
+
+
 def test_append_token_by_token_keeps_old_values_within_a_step(ctx):
     """Tokens that keep growing, one call each: the device follows the definition, and
     no value is ever off by more than one step of its block's scale, nor is the scale
@@ -249,6 +291,72 @@ def test_prefill(ctx, hq, hkv, d, lens, P, new, opts):
     assert np.all(got[pad] == 7.0)
     want[pad] = 7.0
     check(got, want, bound)
+
+
+@pytest.mark.parametrize("cols", [16, 32, 128])
+@pytest.mark.parametrize("hq,hkv,d,lens,P,new", [PREFILL[i] for i in (0, 2, 4, 7)] + [(28, 4, 128, [700, 3], 33, [33, 20])])
+@pytest.mark.parametrize("opts", [OPTIONS[0], OPTIONS[6]], ids=str)
+def test_prefill_by_every_number_of_columns(monkeypatch, hq, hkv, d, lens, P, new, opts, cols):
+    """16, 32 and 128 (row, head) pairs per workgroup, few and many workgroups."""
+    monkeypatch.setenv("LGX_A8_COLS", str(cols))
+    monkeypatch.setenv("LGX_A8_WGS", "1" if cols == 32 else "5")
+    c = lgx.Context(0)
+    try:
+        before = c.launch_count
+        test_prefill(c, hq, hkv, d, lens, P, new, opts)
+        assert c.launch_count - before in (1, 2)
+    finally:
+        c.close()
+
+
+def test_a_cache_beyond_4_gib(ctx):
+    """Pages whose bytes lie past 2^32: append, read-back, decode and prefill attention
+    give what they give near the start of a small cache."""
+    t, rng = ctx.torch, np.random.default_rng(9)
+    hq, hkv, d, B, P, maxp, big = 16, 8, 128, 2, 20, 40, 290000
+    assert (big - 100) * hkv * 16 * d > 2**32
+    small = ref.Cache(B * maxp, hkv, d, rng)
+    table = table_of(rng, B, maxp)
+    far = table + (big - B * maxp)
+    kv = lgx.KvCacheI8.empty(ctx, big, hkv, d)
+    near = upload(ctx, small)
+    for a, b in ((kv.k, near.k), (kv.v, near.v), (kv.k_scale, near.k_scale), (kv.v_scale, near.v_scale)):
+        a[big - B * maxp:] = b
+    rope = rope_of(ctx, *ref.tables(700, d))
+    x = ctx.to_device(rng.standard_normal((B * P, (hq + 2 * hkv) * d)).astype(np.float32))
+    lens, got = i32(ctx, [601, 300]), []
+    for cache, tab in ((near, i32(ctx, table)), (kv, i32(ctx, far))):
+        q = ctx.rope_kv_append_i8(x, None, rope, lens, tab, cache, P)
+        out = ctx.gqa_prefill_attn_i8(q, cache, tab, lens, P, maxp * 16)
+        one = ctx.gqa_decode_attn_i8(q[:B].contiguous(), cache, tab, lens, maxp * 16)
+        got.append((q, out, one) + ctx.kv_read_i8(cache, tab, lens, P))
+    for a, b in zip(*got):
+        assert t.equal(a, b)
+    assert bool((kv.k[:big - B * maxp] == 0).all()) and bool((kv.v_scale[:big - B * maxp] == 0).all())
+
+
+def test_two_contexts_on_two_streams(ctx):
+    """Split attention of two contexts at once: each has its own workspace."""
+    t, rng = ctx.torch, np.random.default_rng(12)
+    hq, hkv, d, B, L = 8, 2, 128, 2, 9000
+    maxp = -(-L // 16)
+    cache, table = ref.Cache(B * maxp, hkv, d, rng), table_of(rng, B, maxp)
+    kv, tab, lens = upload(ctx, cache), i32(ctx, table), i32(ctx, [L, L - 77])
+    qs = [ctx.to_device(rng.standard_normal((B, hq, d)).astype(np.float32)) for _ in range(2)]
+    want = [ctx.gqa_decode_attn_i8(q, kv, tab, lens, L) for q in qs]
+    other = lgx.Context(0)
+    try:
+        t.cuda.synchronize()
+        streams, outs = [t.cuda.Stream(), t.cuda.Stream()], [[], []]
+        for _ in range(20):
+            for i, c in enumerate((ctx, other)):
+                with t.cuda.stream(streams[i]):
+                    outs[i].append(c.gqa_decode_attn_i8(qs[i], kv, tab, lens, L))
+        t.cuda.synchronize()
+        for i in range(2):
+            assert all(t.equal(o, want[i]) for o in outs[i])
+    finally:
+        other.close()
 
 
 def test_lengths_are_clamped(ctx):

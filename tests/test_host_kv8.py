@@ -88,6 +88,7 @@ REFUSED = [
     (decode(maxp=1 << 27, top=1), "LGX_INVALID_ARGUMENT"), (decode(maxp=0), "LGX_INVALID_ARGUMENT"),
     (decode(opts=["opts", [0.0, -1.0, 0, None]]), "LGX_INVALID_ARGUMENT"),
     (decode(opts=["opts", [0.0, float("inf"), 0, None]]), "LGX_INVALID_ARGUMENT"),
+    (decode(opts=["opts", [0.0, 1e-38, 0, None]]), "LGX_INVALID_ARGUMENT"),
     (decode(opts=["opts", [float("nan"), 0.0, 0, None]]), "LGX_INVALID_ARGUMENT"),
     (decode(opts=["opts", [0.0, 0.0, -1, None]]), "LGX_INVALID_ARGUMENT"),
     (prefill(rows=0), "LGX_INVALID_ARGUMENT"), (prefill(B=1 << 16, rows=1 << 15), "LGX_OUT_OF_BOUNDS"),
@@ -113,6 +114,18 @@ def test_refusals_launch_nothing(host):
 def test_no_rotation_needs_no_tables(host):
     (st, launches, _), = host([append(rope=["rope", [None, None, 0, 0, 1]])])
     assert st == "LGX_OK" and len(launches) == 1
+
+
+@pytest.mark.parametrize("B,rows,hq,hkv,d,top,cols", [
+    (64, 1, 28, 4, 128, 4096, 16), (1, 9, 28, 4, 128, 1000, 16), (8, 16, 28, 4, 128, 2000, 16), (8, 64, 28, 4, 128, 2000, 32),
+    (16, 64, 12, 2, 128, 700, 16), (16, 64, 28, 4, 128, 500, 32), (4, 256, 14, 2, 64, 1000, 16), (8, 512, 14, 2, 64, 2000, 32),
+    (8, 512, 28, 4, 128, 4000, 128), (8, 1024, 28, 4, 128, 1100, 128), (16, 1024, 14, 2, 64, 2000, 128), (1, 1, 16, 1, 64, 10**6, 16)])
+def test_columns_per_workgroup(host, B, rows, hq, hkv, d, top, cols):
+    """The sizes measured on both sides of each rule."""
+    cache = kv(pages=1000, hkv=hkv, d=d)
+    call = prefill(B, rows, hq, -(-top // 16), top, cache) if rows > 1 else decode(B, hq, -(-top // 16), top, cache)
+    (st, launches, _), = host([call])
+    assert st == "LGX_OK" and launches[0][0] == f"lgx_k_attn8_d{d}_c{cols}"
 
 
 @pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 18, 33, 2047])
