@@ -178,7 +178,9 @@ __device__ __forceinline__ int halve8(int v, int grow) {
 
 // Workgroup (block of 16 token slots of sequence b; QH query heads, or a K or V
 // head): thread (slot, c) holds D / 32 pairs of the slot's row.  Query heads share
-// the thread's cosines and sines.
+// the thread's cosines and sines.  Bound by memory: 8 x 2047 rows of 28/4 heads of
+// 128, 575 MB, in 130 us (4.4 TB/s; a copy reaches 5.2); 643 us with every element's
+// row, partner and tables loaded number by number.
 #define KV8_QH LGX_KV8_QH
 template <int D>
 __device__ __forceinline__ void kv8_append_body(const lgx_kv8_append_args& a) {
@@ -329,7 +331,9 @@ extern "C" __global__ __launch_bounds__(256) void lgx_k_kv8_append_d128(const lg
 // One new row per sequence (a decode step): a wave per head, a pair per lane (with
 // D = 64 the upper half of the wave idles).  The row does not depend on the
 // length, so its loads are in flight together with the length's, and the cosines
-// with the page's.
+// with the page's.  Bound by those two memory rounds and the launch: 64 sequences of
+// 28/4 heads of 128 in 4.1 us (8.7 with the form above, 16 of its 256 threads at
+// work).
 template <int D>
 __device__ __forceinline__ void kv8_append1_body(const lgx_kv8_append_args& a) {
     const int p = threadIdx.x & 63, b = blockIdx.x;
@@ -392,7 +396,9 @@ extern "C" __global__ __launch_bounds__(256) void lgx_k_kv8_append1_d128(const l
 // Read-back: tokens start[b] .. + n of every sequence as binary32.  Workgroup
 // (block of 16 token slots of sequence b, KV head).  K: thread (slot, c) has d / 16
 // neighbouring values.  V: a thread has a run of tokens of one dimension, so that
-// neighbouring threads write neighbouring dimensions of a row.
+// neighbouring threads write neighbouring dimensions of a row.  Bound by memory: 8 x
+// 2064 rows of 4 heads of 128, 85 MB, in 17.5 us (4.8 TB/s; V through LDS, written by
+// the row's threads: 38 us, the byte reads of 16 dimensions met in one bank).
 // ---------------------------------------------------------------------------
 template <int D>
 __device__ __forceinline__ void kv8_read_body(const lgx_kv8_read_args& a) {
@@ -862,7 +868,13 @@ __device__ __forceinline__ void a8_store(const lgx_attn8_args& a, const A8Block&
 // 16 NT columns per workgroup (a decode row's heads): its four waves take the tiles
 // in turn, K and V straight into registers: the next tile's K is in flight
 // from the end of the scores on, its V from the end of the PV product; at the end
-// the waves' results are joined in LDS.
+// the waves' results are joined in LDS.  One column tile is bound by memory: 16
+// sequences of 32768 tokens, 12/2 heads of 128, 268 MB, in 52 us (5.2 TB/s), 51 with
+// the loads alone; 64 of 256 to 4096 tokens, 28/4 heads, 145 MB, in 40, 39 with the
+// loads alone (the longest one's workgroup takes what one compute unit can load).
+// Eight waves per workgroup load no faster there (41 us) and wait longer elsewhere (14.7
+// against 12.0 us for one sequence of 8191).  Two column tiles are bound by the VALU
+// and the matrix units in turn: 8 x 64 rows at 2000 tokens 54 us.
 template <int D, int NT, bool X>
 __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
     constexpr int WT = 4, NS = D / 64, ND = D / 16;
@@ -1068,8 +1080,15 @@ __device__ __forceinline__ float a8_query16(const lgx_attn8_args& a, const float
 // binary16 once for all of them: each wave brings a quarter of its quants into LDS
 // (two waves K, two V; a direct load brings one 1 KiB fragment in the order of the
 // lanes), a tile ahead, and then turns them into operands in one of two LDS buffers
-// while the other's tile is in use.  With K in binary16 the scores need no joining of digits: two products,
-// one accumulator.
+// while the other's tile is in use.  With K in binary16 the scores need no joining of
+// digits: two products, one accumulator.  Bound by the matrix units and the VALU in
+// turn: 8 x 512 rows at 4000 tokens, 28/4 heads of 128, in 430 to 480 us by inputs and
+// clock, 0.46 to 0.51 PFLOP/s of the formula's work, twice that executed (q and the
+// weights in two parts; a large binary16 product reaches 1.1 to 1.2 here); matrix units
+// busy for 0.43 of the cycles, the VALU for 0.49.  What got it there, of 783 us: K and
+// V through LDS (565), no masks where all rows see a tile, operands converted once
+// and no load waited for where branches meet (520), a softmax reference that seldom
+// moves (480).  64 columns per workgroup (16 per wave) took as long as 16 or longer.
 template <int D, int NT, bool X>
 __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
     constexpr int NS = D / 64, NH = D / 32, ND = D / 16, NF = 4 * NS + ND, FW = NF / 4;
@@ -1246,7 +1265,8 @@ __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
 
 // Joins the splits of one (row, head): D / 4 threads per split, TH / (D / 4) splits at
 // a time.  TH: 256 threads, or a wave where there are many rows and so few splits
-// each.
+// each.  Three memory rounds behind a launch: 4 us; a thread per dimension, one split
+// after the other, took 10 us for 32 splits and 36 for 125.
 template <int D, int TH>
 __device__ __forceinline__ void attn8_join_body(const lgx_attn8_args& a) {
     constexpr int Q = D / 4, NG = TH / Q, NW = TH / 64;
