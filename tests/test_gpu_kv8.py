@@ -1,5 +1,5 @@
 """The 8-bit KV cache on the device against tests/kv8_ref.py (numpy float64): the
-append's scales and quants to the bit, the attention within the reference's bound."""
+append's scales and quants to the bit, the attention within the bound derived there."""
 import numpy as np
 import pytest
 
@@ -264,6 +264,31 @@ def test_decode_long_contexts(ctx, B, L, window):
     got = decode(ctx, cache, q, table, lens, L, **(dict(window=window) if window else {}))
     want, bound = ref.attend(cache, q[:, None], table, lens, L, prefill=False, window=window)
     check(got, want[:, 0], bound[:, 0])
+
+
+@pytest.mark.parametrize("B,window", [(70, 0), (255, 0), (255, 90), (300, 0)])
+def test_decode_many_ragged_sequences(ctx, B, window):
+    """Batches whose tiles are split by all their lengths (up to 256 sequences and KV
+    heads together) and one that is not, empty sequences among them."""
+    rng = np.random.default_rng(B + window)
+    hq, hkv, d, top = 2, 1, 64, 900
+    lens = rng.integers(0, top + 1, B)
+    lens[::7] = rng.integers(0, 3, len(lens[::7]))
+    lens[B // 2] = top
+    maxp = -(-top // 16)
+    cache, table = ref.Cache(B * maxp, hkv, d, rng), table_of(rng, B, maxp)
+    q = rng.standard_normal((B, hq, d)).astype(np.float32)
+    got = decode(ctx, cache, q, table, lens, top, **(dict(window=window) if window else {}))
+    want, bound = ref.attend(cache, q[:, None], table, lens, top, prefill=False, window=window)
+    check(got, want[:, 0], bound[:, 0])
+    assert np.all(got[lens == 0] == 0.0)
+
+
+def test_decode_when_every_length_is_zero(ctx):
+    cache = ref.Cache(200, 2, 128)
+    cache.ks[:] = cache.vs[:] = np.nan
+    got = decode(ctx, cache, np.ones((2, 4, 128), np.float32), np.arange(200).reshape(2, 100), [0, 0], 1600)
+    assert np.all(got == 0.0)
 
 
 PREFILL = [(14, 2, 64, [0, 37, 500], 40, None), (28, 4, 128, [0, 200], 72, None), (12, 2, 128, [500, 0, 255], 9, [9, 4, 0]),
