@@ -689,7 +689,7 @@ __device__ __forceinline__ float a8_query(const lgx_attn8_args& a, const float (
     const bool isbad = col_max(bad ? 1.0f : 0.0f) != 0.0f;
     // the largest power of two that keeps every |q| within 127 * 65536, the
     // range of three balanced digits
-    const float up = __uint_as_float(__float_as_uint(fminf(8323072.0f / am, 0x1p100f)) & 0x7f800000u);
+    const float up = __uint_as_float(__float_as_uint(fminf(127.0f * 65536.0f / am, 0x1p100f)) & 0x7f800000u);
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
@@ -1244,6 +1244,7 @@ __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
     };
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     convert(f_s[0]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the quants are read before the next overwrite them
     load(pl_);
     pl_ = page_ld(w.k.tb0 + 2);
     // the tiles that every column of the workgroup sees whole, then the others

@@ -130,7 +130,7 @@ def attend(cache, q, table, seq_len, max_len, n_new=None, prefill=True, scale=No
                 w = np.exp(s - s.max())
                 w /= w.sum()
                 out[b, j, h] = w @ vv
-                e = np.abs(qq).max() / 8323072 * abs(scale) * np.abs(kk).sum(1) + eps * (
+                e = np.abs(qq).max() / (127 * 65536) * abs(scale) * np.abs(kk).sum(1) + eps * (
                     8 * np.abs(raw) + (8 * softcap if softcap else 0.0) + 4 * np.abs(far) + 4 * np.abs(s - s.max()))
                 # each weight's share of the error; far tokens with no weight have none
                 mean = (w * e).sum()
