@@ -30,7 +30,9 @@
  * asynchronous on `stream` (a hipStream_t; NULL = the null stream); argument
  * errors are reported synchronously, kernel faults at the caller's next
  * synchronisation.  Calls that share one ctx must be ordered on one stream
- * (they share the workspace); use one ctx per concurrent stream.
+ * (they share the workspace), replays of graphs recorded with it among them; use
+ * one ctx per concurrent stream.  A workspace that a recorded call uses is kept
+ * until lgx_ctx_destroy, also when later calls need a larger one.
  *
  * Q8_0 matrices.  W is [n][k] with k % 32 == 0: int8 quants and one binary16
  * scale per 32-block (raw IEEE half bits).  The device kernels read the quants

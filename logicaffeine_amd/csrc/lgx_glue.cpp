@@ -157,7 +157,7 @@ lgx_status lgx_lm_head_f16(lgx_ctx* c, const float* x, const uint16_t* emb, int3
             const int mm = std::min(kLmMaxM, m - r0);
             float* out = logits + (int64_t)r0 * vocab;
             float* part = out;
-            if (nr > 1 && (st = ensure_ws(c, (size_t)nr * mm * vocab * sizeof(float), &part)) != LGX_OK)
+            if (nr > 1 && (st = ensure_ws(c, (size_t)nr * mm * vocab * sizeof(float), stream, &part)) != LGX_OK)
                 return st;
             lgx_lmhead_args a{x + (int64_t)r0 * h, emb, part, mm, h, vocab};
             if ((st = launch(c, K_LM_HEAD_F16, dim3(cdiv(vocab, 256), nr), dim3(256), a, stream)) !=
@@ -206,7 +206,7 @@ lgx_status lgx_lm_head_f16_t64(lgx_ctx* c, const float* x, const uint16_t* emb_t
         const int mc = (m + 15) / 16, nr = (h + 1023) / 1024;
         const size_t nxt = (size_t)mc * 16 * h;
         float* xt = nullptr;
-        if ((st = ensure_ws(c, (nxt + (nr > 1 ? (size_t)nr * m * vocab : 0)) * sizeof(float), &xt)) !=
+        if ((st = ensure_ws(c, (nxt + (nr > 1 ? (size_t)nr * m * vocab : 0)) * sizeof(float), stream, &xt)) !=
             LGX_OK)
             return st;
         lgx_t64_args ta{x, xt, m, h};
@@ -231,7 +231,7 @@ lgx_status lgx_argmax(lgx_ctx* c, const float* logits, int32_t m, int32_t vocab,
         if (!logits || !out) return fail(LGX_NULL_POINTER, "NULL tensor");
         if (m <= 0 || vocab <= 0) return fail(LGX_INVALID_ARGUMENT, "m %d, vocab %d", m, vocab);
         float* cand = nullptr;
-        if ((st = ensure_ws(c, (size_t)m * argmax_slices(vocab) * 8, &cand)) != LGX_OK) return st;
+        if ((st = ensure_ws(c, (size_t)m * argmax_slices(vocab) * 8, stream, &cand)) != LGX_OK) return st;
         return launch_argmax(c, logits, 1, m, vocab, out, nullptr, 0, cand, stream);
     });
 }
@@ -261,7 +261,7 @@ lgx_status lgx_lm_head_argmax_f16(lgx_ctx* c, const float* x, const uint16_t* em
             return fail(LGX_UNSUPPORTED, "m %d (<= %d), vocab %d (<= 655360), h %d (h %% 64 == 0, h <= %d)",
                         m, LGX_LMC_MAXB, vocab, h, LGX_LMC_MAXH);
         float* ws = nullptr;
-        if ((st = ensure_ws(c, (size_t)m * lm_cert_slices(vocab) * sizeof(lgx_lmc_summary), &ws)) !=
+        if ((st = ensure_ws(c, (size_t)m * lm_cert_slices(vocab) * sizeof(lgx_lmc_summary), stream, &ws)) !=
             LGX_OK)
             return st;
         return launch_lm_cert(c, x, emb, emb_t64, rowc, m, h, vocab, (lgx_lmc_summary*)ws, bounds,
@@ -281,7 +281,7 @@ lgx_status lgx_sample(lgx_ctx* c, const float* logits, int32_t m, int32_t vocab,
         if ((st = sample_check(top_k, top_p, temperature, vocab, &sp)) != LGX_OK) return st;
         sp.seed = seed;
         float* cand = nullptr;
-        if ((st = ensure_ws(c, sample_cand_bytes(m, vocab), &cand)) != LGX_OK) return st;
+        if ((st = ensure_ws(c, sample_cand_bytes(m, vocab), stream, &cand)) != LGX_OK) return st;
         return launch_sample(c, sp, logits, 1, m, vocab, positions, out, nullptr, 0, cand, stream);
     });
 }

@@ -136,6 +136,7 @@ lgx_status lgx_ctx_destroy(lgx_ctx* c) {
         }
         for (auto ev : c->event_pool) (void)hipEventDestroy(ev);
         if (c->ws) (void)hipFree(c->ws);
+        for (void* p : c->ws_kept) (void)hipFree(p);
         if (c->module) (void)hipModuleUnload(c->module);
         c->magic = 0;
         delete c;
@@ -400,7 +401,7 @@ lgx_status lgx_gqa_decode_attn(lgx_ctx* c, const float* q, const uint16_t* kpage
         a.maxlen = max_seq_len;
         a.nchunk = (max_seq_len + LGX_ATTN_CHUNK - 1) / LGX_ATTN_CHUNK;
         a.scale = (float)(1.0 / std::sqrt((double)d));
-        st = ensure_ws(c, (size_t)B * hq * a.nchunk * (d + 2) * sizeof(float), &a.part);
+        st = ensure_ws(c, (size_t)B * hq * a.nchunk * (d + 2) * sizeof(float), stream, &a.part);
         if (st != LGX_OK) return st;
         a.rot = attn_rot(a.nchunk);
         st = launch(c, (Kern)k, dim3(a.nchunk, B * hkv), dim3(256), a, stream);
@@ -447,7 +448,7 @@ lgx_status lgx_gqa_prefill_attn(lgx_ctx* c, const float* q, const uint16_t* kpag
         a.len_add = 1;
         a.qpr = P;
         a.scale = (float)(1.0 / std::sqrt((double)d));
-        st = ensure_ws(c, (size_t)B * P * hq * a.nchunk * (d + 2) * sizeof(float), &a.part);
+        st = ensure_ws(c, (size_t)B * P * hq * a.nchunk * (d + 2) * sizeof(float), stream, &a.part);
         if (st != LGX_OK) return st;
         if ((st = launch_prefill_attn(c, a, d, stream)) != LGX_OK) return st;
         return launch(c, d == 64 ? K_ATTN_COMBINE_D64 : K_ATTN_COMBINE_D128, dim3(B * P * hq), dim3(d),
@@ -510,7 +511,7 @@ static lgx_status q8_gemm_impl(lgx_ctx* c, const lgx_q8_matrix* W, const int8_t*
         return run_gemv_group(c, &g, 1, stream);
     }
     auto room = [&](size_t bytes, float** out) -> lgx_status {
-        if (!scratch) return ensure_ws(c, bytes, out);
+        if (!scratch) return ensure_ws(c, bytes, stream, out);
         if (bytes > cap)
             return fail(LGX_OUT_OF_BOUNDS,
                         "[%d x %d] product over m = %d needs %zu scratch bytes (limit %zu)", W->n,
@@ -656,7 +657,7 @@ lgx_status lgx_q8_gemm_quantize_group(lgx_ctx* c, int32_t count, const lgx_q8_ma
             total += xq_b[i] + xd_b[i] + pt_b[i];
         }
         float* ws = nullptr;
-        if ((st = ensure_ws(c, total, &ws)) != LGX_OK) return st;
+        if ((st = ensure_ws(c, total, stream, &ws)) != LGX_OK) return st;
         char* wp = (char*)ws;
         int8_t* xq[LGX_MGROUP_MAX];
         uint16_t* xd[LGX_MGROUP_MAX];

@@ -313,6 +313,8 @@ struct lgx_ctx {
     std::atomic<int> live_models{0};  // lgx_model handles built on this ctx and not destroyed
     void* ws = nullptr;       // range partials
     size_t ws_bytes = 0;
+    bool ws_recorded = false;         // a launch recorded into a graph may use ws
+    std::vector<void*> ws_kept;       // outgrown workspaces that graphs may use
     void* scratch = nullptr;  // this device's LGX_NOALLOC_SCRATCH_BYTES array (lgx_scratch.hip)
     std::mutex ws_mu;
     // per-kernel device timing (lgx_ctx_set_kernel_timing): launches go
@@ -408,18 +410,28 @@ inline lgx_status enter(lgx_ctx* c) {
 }
 
 // Scratch for range partials, grown on demand.  hipFree of the old buffer
-// waits for the device, so work still using it has finished.
-inline lgx_status ensure_ws(lgx_ctx* c, size_t bytes, float** out) {
+// waits for the device, so work still using it has finished; one that was
+// handed out to a stream under capture is kept for the graph's replays until
+// the ctx ends (sizes grow by half at least: all kept ones are below twice the
+// newest).
+inline lgx_status ensure_ws(lgx_ctx* c, size_t bytes, void* stream, float** out) {
     std::lock_guard<std::mutex> lk(c->ws_mu);
     if (bytes > c->ws_bytes) {
         size_t nb = bytes < (size_t)1 << 20 ? (size_t)1 << 20 : bytes + bytes / 2;
-        if (c->ws) LGX_HIP(hipFree(c->ws));
+        if (c->ws && c->ws_recorded) c->ws_kept.push_back(c->ws);
+        else if (c->ws) LGX_HIP(hipFree(c->ws));
         c->ws = nullptr;
         c->ws_bytes = 0;
+        c->ws_recorded = false;
         hipError_t e = hipMalloc(&c->ws, nb);
         if (e != hipSuccess)
             return fail(LGX_OUT_OF_MEMORY, "workspace of %zu bytes: %s", nb, hipGetErrorString(e));
         c->ws_bytes = nb;
+    }
+    if (stream && !c->ws_recorded) {   // the null stream cannot be captured
+        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+        (void)hipStreamIsCapturing((hipStream_t)stream, &cs);
+        c->ws_recorded = cs == hipStreamCaptureStatusActive;
     }
     *out = (float*)c->ws;
     return LGX_OK;
@@ -590,7 +602,7 @@ inline lgx_status run_q8(lgx_ctx* c, Kern kern, const lgx_q8_matrix* W, const fl
     } else if (a.nranges > 1 && part_ws) {
         a.part = part_ws;   // caller-provided room for nranges * m * n partials
     } else if (a.nranges > 1) {
-        lgx_status st = ensure_ws(c, (size_t)a.nranges * m * W->n * sizeof(float), &a.part);
+        lgx_status st = ensure_ws(c, (size_t)a.nranges * m * W->n * sizeof(float), stream, &a.part);
         if (st != LGX_OK) return st;
     }
     const bool streaming =

@@ -69,7 +69,7 @@ lgx_status run_attn8(lgx_ctx* c, lgx_attn8_args& a, int B, int d, bool x, void* 
     if (split) {
         const int64_t slots = per * a.hkv * nc;
         float* ws = nullptr;
-        if ((st = ensure_ws(c, (size_t)(slots * (d + 2) + 2 * units) * sizeof(float), &ws)) != LGX_OK) return st;
+        if ((st = ensure_ws(c, (size_t)(slots * (d + 2) + 2 * units) * sizeof(float), stream, &ws)) != LGX_OK) return st;
         a.per = (int)per;
         a.units = (int)units;
         a.part = ws;
