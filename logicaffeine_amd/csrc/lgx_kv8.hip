@@ -194,7 +194,7 @@ __device__ __forceinline__ void kv8_append_body(const lgx_kv8_append_args& a) {
     const int sl = min(max(a.seq_len[b], 0), a.maxp * LGX_PAGE);
     const int nn = a.n_new ? min(max(a.n_new[b], 0), a.P) : a.P;
     const int pb = sl / LGX_PAGE + (blockIdx.x - b * a.nblk), t0 = pb * LGX_PAGE;
-    if (t0 >= sl + nn) return;                    // uniform: no new row in this block
+    if (nn == 0 || t0 >= sl + nn) return;         // uniform: no new row in this block
     const int j = t0 + slot - sl;                 // row of this slot
     const bool is_new = j >= 0 && j < nn;
     const int rot = isv ? 0 : a.rot;

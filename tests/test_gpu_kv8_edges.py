@@ -20,6 +20,34 @@ def i32(ctx, x):
     return ctx.to_device(np.asarray(x, np.int32))
 
 
+def no_rope(ctx):
+    t = ctx.torch
+    return lgx.Rope(t.empty((1, 0), device=ctx.dev), t.empty((1, 0), device=ctx.dev))
+
+
+# ---- append ---------------------------------------------------------------
+
+@pytest.mark.parametrize("P", [1, 2, 20])
+def test_a_sequence_without_new_rows_touches_nothing(ctx, P):
+    """Row counts of zero and below: the page that the length points into keeps its
+    scale's bits, whatever they are, and its quants."""
+    rng, hq, hkv, d = np.random.default_rng(P), 2, 2, 64
+    lens, new = [5, 15, 16, 20, 3], [0, -3, 0, 0, 1]
+    B, maxp = len(lens), 4
+    cache, table = ref.Cache(B * maxp, hkv, d, rng), rng.permutation(B * maxp).astype(np.int32).reshape(B, maxp)
+    for b, v in enumerate((np.inf, -1.0, np.nan, -np.inf)):
+        cache.ks[table[b]] = cache.vs[table[b]] = np.float32(v)
+    # a number of its own payload, so that a NaN written back in another form would show
+    cache.ks.view(np.uint32)[table[2]] = cache.vs.view(np.uint32)[table[2]] = 0x7fc01234
+    kv = upload(ctx, cache)
+    x = rng.standard_normal((B, P, (hq + 2 * hkv) * d)).astype(np.float32)
+    ctx.rope_kv_append_i8(ctx.to_device(x.reshape(B * P, -1)), None, no_rope(ctx), i32(ctx, lens), i32(ctx, table), kv, P,
+                          n_new=i32(ctx, new))
+    cache.append(x, None, *ref.tables(64, 0), False, lens, new, table, hq)
+    for got, want in ((kv.k, cache.k), (kv.v, cache.v), (kv.k_scale, cache.ks), (kv.v_scale, cache.vs)):
+        assert host(got).tobytes() == want.tobytes()
+
+
 # ---- recorded steps -------------------------------------------------------
 
 def test_a_recorded_step_outlives_a_larger_call():
