@@ -167,9 +167,15 @@ __device__ __forceinline__ float block_scale(double am, bool bad, float old, int
     }
     return scale;
 }
-__device__ __forceinline__ int quant8(double y, double inv) {
-    const int m = (int)fmin(floor(fabs(y) * inv + 0.5), 127.0);
-    return y < 0.0 ? -m : m;
+// The integer nearest to y / scale, halves away from zero; inv: 1 / scale rounded (0
+// for a scale of 0 or NaN, whose quants are 0).  |y| inv, rounded too, may say one
+// integer less or more than the quotient's whole part; what is left of |y| after
+// that many scales is a multiple of the smaller of their units and no larger than |y|,
+// so a binary64 number, and its comparison with half a scale is exact.
+__device__ __forceinline__ int quant8(double y, double scale, double inv) {
+    const double a = fabs(y), m = floor(a * inv);
+    const int q = min((int)m + (inv > 0.0 && fma(-m, scale, a) >= 0.5 * scale), 127);
+    return y < 0.0 ? -q : q;
 }
 __device__ __forceinline__ int halve8(int v, int grow) {
     const int m = grow > 8 ? 0 : ((v < 0 ? -v : v) + (1 << (grow - 1))) >> grow;
@@ -275,7 +281,7 @@ __device__ __forceinline__ void kv8_append_body(const lgx_kv8_append_args& a) {
     const double inv = scale > 0.0f ? 1.0 / (double)scale : 0.0;
     int q[2 * H];
 #pragma unroll
-    for (int e = 0; e < 2 * H; ++e) q[e] = bad ? 0 : quant8(y[e], inv);
+    for (int e = 0; e < 2 * H; ++e) q[e] = bad ? 0 : quant8(y[e], scale, inv);
     const bool again = slot < s0 && grow > 0;     // an old token whose quants shrink
     if (!isv) {
         int8_t* kr = a.k + (blk * LGX_PAGE + slot) * D;
@@ -376,7 +382,7 @@ __device__ __forceinline__ void kv8_append1_body(const lgx_kv8_append_args& a) {
     if (p == 0) *sp = scale;
     if (!on) return;
     const double inv = scale > 0.0f ? 1.0 / (double)scale : 0.0;
-    const int q0 = bad ? 0 : quant8(x[0], inv), q1 = bad ? 0 : quant8(z[0], inv);
+    const int q0 = bad ? 0 : quant8(x[0], scale, inv), q1 = bad ? 0 : quant8(z[0], scale, inv);
     // K: slot s0 of 16 rows; V: column s0
     int8_t* base = (isv ? a.v : a.k) + blk * LGX_PAGE * D;
     const int ds = isv ? LGX_PAGE : 1, ts = isv ? 1 : D;

@@ -1,4 +1,6 @@
 """The 8-bit KV cache at the edges of what its calls take, against the definition."""
+from fractions import Fraction
+
 import numpy as np
 import pytest
 
@@ -26,6 +28,83 @@ def no_rope(ctx):
 
 
 # ---- append ---------------------------------------------------------------
+
+def nearest(y, scale):
+    """The whole number nearest to y / scale, halves away from zero, exactly."""
+    r = abs(Fraction(float(y))) / Fraction(float(scale))
+    m = (r + Fraction(1, 2)).__floor__()
+    return -m if y < 0 else m
+
+
+def tie_rows(n, d, scale, rng):
+    """n rows of d numbers whose quotients by `scale` are halves and their neighbours,
+    the first number 127 scale."""
+    k = rng.integers(0, 127, (n, d))
+    y = ((k + 0.5) * scale).astype(np.float32)
+    assert (y.astype(np.float64) == (k + 0.5) * scale).all()
+    y[1::3] = np.nextafter(y[1::3], np.float32(0))
+    y[2::3] = np.nextafter(y[2::3], np.float32(np.inf))
+    y *= rng.choice(np.float32([-1, 1]), y.shape)
+    y[0, 0] = 127 * scale
+    return y
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("P", [1, 9, 16])
+def test_quants_at_exact_ties(ctx, P, d):
+    """quant = the nearest integer to value / scale, halves away from zero: also where
+    value * (1 / scale) would round to the other side of the half."""
+    rng, hkv, hq = np.random.default_rng(P + d), 1, 1
+    scales = np.arange(3, 3 + 2 * 200, 2)            # odd numbers: their reciprocals are rounded
+    B = len(scales)
+    x = np.zeros((B, P, 3, d), np.float32)
+    for b, s in enumerate(scales):
+        x[b, :, 1], x[b, :, 2] = tie_rows(P, d, s, rng), tie_rows(P, d, s, rng)
+    kv = lgx.KvCacheI8.empty(ctx, B, hkv, d)
+    ctx.rope_kv_append_i8(ctx.to_device(x.reshape(B * P, 3 * d)), None, no_rope(ctx), i32(ctx, [0] * B),
+                          i32(ctx, np.arange(B).reshape(B, 1)), kv, P)
+    assert np.array_equal(host(kv.k_scale)[:, 0], scales) and np.array_equal(host(kv.v_scale)[:, 0], scales)
+    want = np.array([[[nearest(y, s) for y in row] for row in x[b, :, 1:].reshape(-1, d)] for b, s in enumerate(scales)])
+    want = want.reshape(B, P, 2, d)
+    assert np.array_equal(host(kv.k)[:, 0, :P], want[:, :, 0])
+    assert np.array_equal(host(kv.v)[:, 0, :, :P].transpose(0, 2, 1), want[:, :, 1])
+
+
+@pytest.mark.parametrize("P", [1, 5])
+def test_quants_next_to_a_tie_in_64_bits(ctx, P):
+    """bias + row is a binary64 number: 1/2 - 2^-54 is nearer to 0 than to 1."""
+    d, hkv = 64, 1
+    x = np.zeros((P, 3, d), np.float32)
+    x[:, 1:] = np.float32(-2.0 ** -54)
+    x[0, 1:, 0] = 126.5
+    bias = np.full(3 * d, 0.5, np.float32)
+    kv = lgx.KvCacheI8.empty(ctx, 1, hkv, d)
+    ctx.rope_kv_append_i8(ctx.to_device(x.reshape(P, 3 * d)), ctx.to_device(bias), no_rope(ctx), i32(ctx, [0]), i32(ctx, [[0]]), kv, P)
+    want = np.zeros((P, d), np.int8)
+    want[0, 0] = 127
+    assert host(kv.k_scale)[0, 0] == 1.0 and host(kv.v_scale)[0, 0] == 1.0
+    assert np.array_equal(host(kv.k)[0, 0, :P], want) and np.array_equal(host(kv.v)[0, 0, :, :P].T, want)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_growth_at_every_fill_of_a_page(ctx, d):
+    """One row per sequence into pages that hold 1 .. 15 tokens, blocks that double 0 to
+    12 times, scales of zero among them."""
+    rng, hq, hkv, B = np.random.default_rng(d), 2, 2, 15 * 14
+    cache, table = ref.Cache(B, hkv, d, rng), rng.permutation(B).astype(np.int32).reshape(B, 1)
+    lens, grow = np.repeat(np.arange(1, 16), 14), np.tile(np.arange(14), 15)
+    x = rng.standard_normal((B, 1, (hq + 2 * hkv) * d)).astype(np.float32)
+    for b in range(B):
+        top = np.abs(x[b]).max() / 127
+        cache.ks[table[b, 0]] = cache.vs[table[b, 0]] = 0.0 if grow[b] == 13 else np.float32(top * 1.5 / 2.0 ** grow[b])
+    kv = upload(ctx, cache)
+    ctx.rope_kv_append_i8(ctx.to_device(x[:, 0]), None, no_rope(ctx), i32(ctx, lens), i32(ctx, table), kv)
+    before = [cache.k.copy(), cache.v.copy()]
+    cache.append(x, None, *ref.tables(16, 0), False, lens, None, table, hq)
+    for got, want in ((kv.k, cache.k), (kv.v, cache.v), (kv.k_scale, cache.ks), (kv.v_scale, cache.vs)):
+        assert np.array_equal(host(got), want)
+    assert all((a != b).any((1, 2, 3)).all() for a, b in zip(before, (cache.k, cache.v)))
+
 
 @pytest.mark.parametrize("P", [1, 2, 20])
 def test_a_sequence_without_new_rows_touches_nothing(ctx, P):
