@@ -739,90 +739,115 @@ __device__ __forceinline__ void a8_scores(const KF& kf, const v4i (&qd)[3][NS], 
 }
 
 // One column's running softmax.  L, lo: the tokens it sees; m: its reference, within
-// 4 below the largest score (base 2) so far; l: the sum of 2^(score - m); e: V scales
-// are taken in units of 2^e, that of the largest one seen so far rounded down, and
-// weights carry 2^9 (they stay below 2^14, and their second binary16 part is not
-// subnormal where it matters).
-#define A8_UP 9
+// 4 below the largest score (base 2) so far; l: the sum of 2^(score - m).  e: the PV
+// operand of a token is 2^(score - m) vs 2^(A8_UP - e), vs its page's V scale, e a whole
+// number that keeps the largest such operand between 2^10 and 2^15, at binary16's upper
+// end.  What a page contributes decides, not its V scale alone: a large scale that meets
+// no weight, or a heavy page of small values, takes no bits from the others.
+#define A8_UP 137              // 10, and the 127 by which a8_exponent is biased
 struct A8Col {
-    float f, slope, m, l;
-    int L, lo, e;
+    float f, slope, m, l, e;
+    int L, lo;
 };
 __device__ __forceinline__ void a8_reset(A8Col& c) {
     c.m = -__builtin_inff();
     c.l = 0.0f;
-    c.e = -126;
+    c.e = -400.0f;
 }
-__device__ __forceinline__ int a8_exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 127; }
-__device__ __forceinline__ float a8_unit(const A8Col& c) { return ldexpf(1.0f, c.e - A8_UP); }
+__device__ __forceinline__ int a8_exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 255); }
 
-// From a column tile's scores (integers, times c.f and the K scale) to its weights,
-// each times its page's V scale, as two binary16 parts.  EDGE: some column does not
+// From the scores of N column tiles (integers, times k.f and the K scale) to their
+// weights, each times its page's V scale, as two binary16 parts; o, what was summed
+// before, is brought to the new references where they move.  EDGE: some column does not
 // see the whole tile, or the scores are capped, biased or windowed (X).  ks, vs: the
-// scales of the lane's page; pt: its first token.  down: the factor of what was
-// summed before.
-template <bool X, bool EDGE>
-__device__ __forceinline__ void a8_weights(const lgx_attn8_args& a, float (&S)[16], A8Col& c, float ks, float vs, int pt, v8h (&ph)[2],
-                                           v8h (&pl)[2], float& down) {
+// scales of the lane's page; pt: its first token.
+template <bool X, bool EDGE, int N, int ND>
+__device__ __forceinline__ void a8_weights(const lgx_attn8_args& a, float (*S)[16], A8Col* k, float ks, float vs, int pt, v8h (*ph)[2],
+                                           v8h (*pl)[2], v4f (*o)[ND]) {
     static_assert(EDGE || !X, "other scores are formed ahead of the maximum");
     constexpr float kLog2e = 1.44269504088896341f;
-    const float inf = __builtin_inff(), fk = c.f * ks;
-    bool page = true;
-    if (EDGE) {
-        const int hi = c.L - pt, lo = c.lo - pt;  // what the column sees of the page
+    const float inf = __builtin_inff();
+    const int ve = a8_exponent(vs);
+    float fk[N], mt[N], top[N];
+    bool page[N], moves = false;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) S[e] *= fk;
-        if constexpr (X) {
-            if (a.softcap > 0.0f) {
-                const float inv = 1.0f / a.softcap;
+    for (int n = 0; n < N; ++n) {
+        fk[n] = k[n].f * ks;
+        page[n] = true;
+        if (EDGE) {
+            const int hi = k[n].L - pt, lo = k[n].lo - pt;   // what the column sees of the page
 #pragma unroll
-                for (int e = 0; e < 16; ++e) S[e] = a.softcap * a8_tanh(S[e] * inv);
+            for (int e = 0; e < 16; ++e) S[n][e] *= fk[n];
+            if constexpr (X) {
+                if (a.softcap > 0.0f) {
+                    const float inv = 1.0f / a.softcap;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) S[n][e] = a.softcap * a8_tanh(S[n][e] * inv);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) S[n][e] = (S[n][e] - k[n].slope * (float)(hi - 1 - e)) * kLog2e;
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) S[e] = (S[e] - c.slope * (float)(hi - 1 - e)) * kLog2e;
+            for (int e = 0; e < 16; ++e)
+                if (e >= hi || e < lo) S[n][e] = -inf;
+            // a page that the column does not see may hold anything
+            page[n] = hi > 0 && lo < LGX_PAGE;
+        }
+        float m = fmaxf(fmaxf(S[n][0], S[n][1]), S[n][2]);
+#pragma unroll
+        for (int e = 3; e < 15; e += 2) m = fmaxf(fmaxf(m, S[n][e]), S[n][e + 1]);
+        m = fmaxf(m, S[n][15]);
+        if (!EDGE) m *= fk[n];                    // scales are not negative
+        // the page's largest contribution, -inf where the column sees nothing of it
+        top[n] = col_max(m + (float)ve);
+        mt[n] = col_max(m);
+        // the references move when a maximum passes theirs by more than 2^4: most
+        // tiles leave what was summed as it is
+        moves = moves || mt[n] > k[n].m + 4.0f || top[n] > k[n].m + k[n].e + 4.0f;
+    }
+    if (__builtin_amdgcn_ballot_w64(moves)) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const float mn = mt[n] > k[n].m + 4.0f ? mt[n] : k[n].m;
+            const bool none = mn == -inf;         // nothing seen yet
+            const float d = none ? 0.0f : k[n].m - mn;
+            const float rel = fmaxf(none ? -inf : top[n] - mn, -400.0f);   // a NaN falls away
+            const float en = mn != k[n].m || rel > k[n].e + 4.0f ? floorf(fmaxf(rel, k[n].e + d)) : k[n].e;
+            const float down = __builtin_amdgcn_exp2f(d + (k[n].e - en));
+#pragma unroll
+            for (int i = 0; i < ND; ++i) o[n][i] *= down;
+            k[n].l *= __builtin_amdgcn_exp2f(d);
+            k[n].m = mn;
+            k[n].e = en;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const float off = k[n].m == -inf ? 0.0f : -k[n].m;
+        // below 2^128: a larger factor's weights are under 2^-113 of the row's largest
+        const float r = page[n] ? ldexpf(vs, min(A8_UP - (int)k[n].e, 2 * 127 - ve)) : 0.0f;
+        float ps = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            S[n][e] = __builtin_amdgcn_exp2f(EDGE ? S[n][e] + off : fmaf(S[n][e], fk[n], off));
+            ps += S[n][e];
+            S[n][e] *= r;
+        }
+        k[n].l += ps;
+        uint32_t hw[8], lw[8];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+            // the first part rounded toward zero, the second holds the rest
+            const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(S[n][e], S[n][e + 1]));
+            hw[e >> 1] = h;
+            lw[e >> 1] = __builtin_bit_cast(
+                uint32_t, __builtin_amdgcn_cvt_pkrtz(minus_half<0>(S[n][e], h), minus_half<1>(S[n][e + 1], h)));
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-            if (e >= hi || e < lo) S[e] = -inf;
-        // a page that the column does not see may hold anything
-        page = hi > 0 && lo < LGX_PAGE;
-    }
-    const int top = a8_exponent(col_max(page && vs < inf ? vs : 0.0f));
-    float mt = fmaxf(fmaxf(S[0], S[1]), S[2]);
-#pragma unroll
-    for (int e = 3; e < 15; e += 2) mt = fmaxf(fmaxf(mt, S[e]), S[e + 1]);
-    mt = fmaxf(mt, S[15]);
-    mt = col_max(EDGE ? mt : mt * fk);            // scales are not negative
-    // the reference moves when the maximum passes it by more than 2^4: most tiles
-    // then leave what was summed as it is
-    const float mn = mt > c.m + 4.0f ? mt : c.m;
-    const bool none = mn == -inf;                 // nothing seen yet
-    const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(c.m - mn), off = none ? 0.0f : -mn;
-    const int en = max(c.e, top);
-    down = ldexpf(alpha, c.e - en);
-    c.m = mn;
-    c.e = en;
-    const float r = page ? ldexpf(vs, A8_UP - en) : 0.0f;
-    float ps = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        S[e] = __builtin_amdgcn_exp2f(EDGE ? S[e] + off : fmaf(S[e], fk, off));
-        ps += S[e];
-        S[e] *= r;
-    }
-    c.l = fmaf(c.l, alpha, ps);
-    uint32_t hw[8], lw[8];
-#pragma unroll
-    for (int e = 0; e < 16; e += 2) {
-        // the first part rounded toward zero, the second holds the rest
-        const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(S[e], S[e + 1]));
-        hw[e >> 1] = h;
-        lw[e >> 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(minus_half<0>(S[e], h), minus_half<1>(S[e + 1], h)));
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        ph[i] = as_v8h(make_uint4(hw[4 * i], hw[4 * i + 1], hw[4 * i + 2], hw[4 * i + 3]));
-        pl[i] = as_v8h(make_uint4(lw[4 * i], lw[4 * i + 1], lw[4 * i + 2], lw[4 * i + 3]));
+        for (int i = 0; i < 2; ++i) {
+            ph[n][i] = as_v8h(make_uint4(hw[4 * i], hw[4 * i + 1], hw[4 * i + 2], hw[4 * i + 3]));
+            pl[n][i] = as_v8h(make_uint4(lw[4 * i], lw[4 * i + 1], lw[4 * i + 2], lw[4 * i + 3]));
+        }
     }
 }
 struct A8Edge { static constexpr bool value = true; };
@@ -861,13 +886,14 @@ __device__ __forceinline__ void a8_store(const lgx_attn8_args& a, const A8Block&
     constexpr int D = 16 * ND;
     const bool part = k.ns > 1;
     const int64_t at = part ? ((int64_t)k.pos * a.hkv + k.g) * NC + c - k.c0 : orow;
-    const float unit = a8_unit(x);
+    const int unit = (int)x.e - A8_UP;
     // NaN sums stay NaN; nothing seen gives zeros
-    const float s = part ? unit : x.l == 0.0f ? 0.0f : unit / x.l;
+    const float s = part ? 1.0f : x.l == 0.0f ? 0.0f : 1.0f / x.l;
     float* dst = (part ? a.part : a.out) + at * D;
 #pragma unroll
     for (int i = 0; i < ND; ++i)
-        *(float4*)(dst + 16 * i + 4 * kg) = make_float4(o[i][0] * s, o[i][1] * s, o[i][2] * s, o[i][3] * s);
+        *(float4*)(dst + 16 * i + 4 * kg) =
+            make_float4(ldexpf(o[i][0] * s, unit), ldexpf(o[i][1] * s, unit), ldexpf(o[i][2] * s, unit), ldexpf(o[i][3] * s, unit));
     if (part && kg == 0) *(float2*)(a.ml + 2 * at) = make_float2(x.m, x.l);
 }
 
@@ -962,33 +988,23 @@ __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
         const float ksn = ks, vsn = vs;
         const Pages pn = p;
         v8h ph[NT][2], pl[NT][2];
-        float down[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float S[16];
+            float S[1][16];
             if (NT > 1) {
                 int at = lane;
                 asm volatile("" : "+v"(at));      // read here, not once ahead of the loop
 #pragma unroll
                 for (int i = 0; i < 3 * NS; ++i) qd[i / NS][i % NS] = q_s[(n * 3 * NS + i) * 64 + at];
             }
-            a8_scores<NS>([&](int u, int s) { return kw[u][s]; }, qd, S);
+            a8_scores<NS>([&](int u, int s) { return kw[u][s]; }, qd, S[0]);
             if (n == NT - 1) {
                 load_k(pn);
                 ks = a.ks[block(pn.v)];
                 vs = a.vs[block(pn.v)];
                 p = pages(min(t + 2 * WT, mine));
             }
-            a8_weights<X, edge>(a, S, k[n], ksn, vsn, pt, ph[n], pl[n], down[n]);
-        }
-        bool moved = false;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) moved = moved || down[n] != 1.0f;
-        if (__builtin_amdgcn_ballot_w64(moved)) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < ND; ++i) o[n][i] *= down[n];
+            a8_weights<X, edge, 1, ND>(a, S, k + n, ksn, vsn, pt, ph + n, pl + n, o + n);
         }
         a8_pv<ND, NT>([&](int i, uint4& h0, uint4& h1) { i8_to_v8h(vw[i], h0, h1); }, ph, pl, o);
         load_v(pn);
@@ -1011,7 +1027,7 @@ __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
             for (int n = 0; n < NT; ++n) {
                 ml_s[((at + n) * 3 + 0) * 64 + lane] = k[n].m;
                 ml_s[((at + n) * 3 + 1) * 64 + lane] = k[n].l;
-                ml_s[((at + n) * 3 + 2) * 64 + lane] = (float)k[n].e;
+                ml_s[((at + n) * 3 + 2) * 64 + lane] = k[n].e;
 #pragma unroll
                 for (int i = 0; i < ND; ++i) o_s[((at + n) * ND + i) * 64 + lane] = o[n][i];
             }
@@ -1021,11 +1037,13 @@ __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float mo = ml_s[((at + n) * 3 + 0) * 64 + lane], lo = ml_s[((at + n) * 3 + 1) * 64 + lane];
-                const int eo = (int)ml_s[((at + n) * 3 + 2) * 64 + lane], en = max(k[n].e, eo);
+                const float eo = ml_s[((at + n) * 3 + 2) * 64 + lane];
                 const float mn = fmaxf(k[n].m, mo);
-                const float w0 = k[n].m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(k[n].m - mn);
-                const float w1 = mo == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mo - mn);
-                const float u0 = ldexpf(w0, k[n].e - en), u1 = ldexpf(w1, eo - en);
+                // a wave that has seen nothing: -inf, so weights of 0
+                const float d0 = k[n].m == -__builtin_inff() ? k[n].m : k[n].m - mn, d1 = mo == -__builtin_inff() ? mo : mo - mn;
+                const float en = fmaxf(floorf(fmaxf(k[n].e + d0, eo + d1)), -400.0f);
+                const float w0 = __builtin_amdgcn_exp2f(d0), w1 = __builtin_amdgcn_exp2f(d1);
+                const float u0 = __builtin_amdgcn_exp2f(d0 + (k[n].e - en)), u1 = __builtin_amdgcn_exp2f(d1 + (eo - en));
                 k[n].l = k[n].l * w0 + lo * w1;
                 k[n].m = mn;
                 k[n].e = en;
@@ -1181,7 +1199,7 @@ __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
         const int t0 = t * LGX_A8_TILE, pt = t0 + 16 * kg;
         if (!any || (edge && (t0 >= wend || t0 + LGX_A8_TILE <= wbeg))) return;   // uniform per wave
         const uint4* fr = f_s[cur] + lane;
-        float S[NT][16], down[NT];
+        float S[NT][16];
         {
             // fragments PF ahead of their products: an LDS read takes as long as
             // two fragments' products
@@ -1213,17 +1231,7 @@ __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
                 for (int e = 0; e < 16; ++e) S[n][e] = acc[e >> 2][n][e & 3];
         }
         v8h ph[NT][2], pl[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) a8_weights<X, edge>(a, S[n], k[n], ksn, vsn, pt, ph[n], pl[n], down[n]);
-        bool moved = false;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) moved = moved || down[n] != 1.0f;
-        if (__builtin_amdgcn_ballot_w64(moved)) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < ND; ++i) o[n][i] *= down[n];
-        }
+        a8_weights<X, edge, NT, ND>(a, S, k, ksn, vsn, pt, ph, pl, o);
         {
             constexpr int PF = 3;
             const uint4* vr = fr + 2 * 4 * NS * 64;

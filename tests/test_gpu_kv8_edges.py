@@ -9,6 +9,8 @@ import logicaffeine_amd as lgx
 
 pytestmark = pytest.mark.gpu
 
+EPS = 2.0 ** -24                                     # half a step of binary32
+
 
 def host(t):
     return t.cpu().numpy()
@@ -125,6 +127,116 @@ def test_a_sequence_without_new_rows_touches_nothing(ctx, P):
     cache.append(x, None, *ref.tables(64, 0), False, lens, new, table, hq)
     for got, want in ((kv.k, cache.k), (kv.v, cache.v), (kv.k_scale, cache.ks), (kv.v_scale, cache.vs)):
         assert host(got).tobytes() == want.tobytes()
+
+
+# ---- attention ------------------------------------------------------------
+
+def attend(cache, q, table, seq_len, prefill, scale=None, slopes=None):
+    """q [B][P][hq][d] -> (float64 results, bound element by element).
+
+    The bound counts nothing that its weight takes away.  A score that is off by e changes
+    the result by at most sum(w e |v|) + sum(w e) sum(w |v|).  e: q to half a step of
+    max|q| / 4161536 per product; eight binary32 roundings of the score, four of the
+    distance term and of the difference to the maximum.  A weight with its V scale, w vs:
+    22 bits, and no better than 2^-34 of the row's largest w vs (the subnormal end of
+    binary16); exp2 to one unit; n / 32 + 64 partial sums twice over in binary32."""
+    B, P, hq, d = q.shape
+    G = hq // cache.hkv
+    scale = 1.0 / np.sqrt(d) if scale is None else scale
+    out, bound = np.zeros(q.shape), np.zeros(q.shape)
+    for b in range(B):
+        for j in range(P):
+            L = int(seq_len[b]) + j + (1 if prefill else 0)
+            k, v = cache.rows(table[b], L)
+            pages = np.arange(L) // 16
+            back = (L - 1 - np.arange(L)).astype(np.float64)
+            for h in range(hq):
+                kk, vv, qq = k[:, h // G], v[:, h // G], q[b, j, h].astype(np.float64)
+                vs = cache.vs[table[b][pages], h // G].astype(np.float64)
+                raw = kk @ qq * scale
+                far = slopes[h].astype(np.float64) * back if slopes is not None else 0.0 * back
+                s = raw - far
+                w = np.exp(s - s.max())
+                w /= w.sum()
+                out[b, j, h] = w @ vv
+                e = np.abs(qq).max() / (127 * 65536) * abs(scale) * np.abs(kk).sum(1) + EPS * (
+                    8 * np.abs(raw) + 4 * np.abs(far) + 4 * np.abs(s - s.max()))
+                size = w @ np.abs(vv)
+                step = 2.0 ** -34 * (w * vs).max() * np.abs(np.divide(vv, vs[:, None], out=np.zeros_like(vv), where=vs[:, None] > 0)).sum(0)
+                bound[b, j, h] = (w * e) @ np.abs(vv) + (w @ e) * size + EPS * (8 + 2 * (L / 32 + 64)) * size + step
+    return out, bound
+
+
+def check(got, want, bound, tight):
+    """Within the bound, which itself is a small part of each row's largest result."""
+    assert (bound.max(-1) <= tight * np.abs(want).max(-1)).all(), (bound.max(-1) / np.abs(want).max(-1)).max()
+    worst = np.abs(got - want) - bound
+    assert (worst <= 0).all(), (worst.max(), np.unravel_index(worst.argmax(), worst.shape))
+
+
+def far_scales(rng, d, hkv, pages, kind, ratio):
+    """A cache whose heavy pages (weights next to one) and whose large pages are others.
+    "faint": the large pages weigh e^-300; "hollow": the heavy pages' V is `ratio`
+    times the others' (0: all zero), which weigh about e^-15."""
+    cache = ref.Cache(pages, hkv, d, rng)
+    heavy = rng.random(pages) < 0.5
+    heavy[0], heavy[1] = True, False
+    # q is about 1 in every dimension: a score is 8 (or 11.3) times scale and mean quant
+    cache.ks[:] = np.float32(0.5)
+    gap = {"faint": 300.0, "hollow": 15.0}[kind]
+    drop = int(round(gap / (np.sqrt(d) * 0.5)))
+    cache.k[:] = rng.integers(18, 23, cache.k.shape)
+    cache.k[~heavy] -= np.int8(drop)
+    cache.vs[:] = np.float32(0.01)
+    cache.vs[~heavy if kind == "faint" else heavy] *= np.float32(ratio)
+    return cache
+
+
+FAR = [("faint", 1e6), ("faint", 1e9), ("faint", 1e15), ("faint", 1e30), ("hollow", 0.0), ("hollow", 1e-20), ("hollow", 1e-6)]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("cols", [16, 32, 128])
+@pytest.mark.parametrize("kind,ratio", FAR)
+def test_v_scales_do_not_cost_the_pages_that_matter(monkeypatch, d, cols, kind, ratio):
+    """V scales count by the weight that meets them, in every kernel, in any order of the
+    pages, split among workgroups or not."""
+    monkeypatch.setenv("LGX_A8_COLS", str(cols))
+    c = lgx.Context(0)
+    try:
+        rng = np.random.default_rng(d + cols)
+        hq, hkv, P, maxp = 4, 2, 40, 30
+        cache = far_scales(rng, d, hkv, 2 * maxp, kind, ratio)
+        table = np.stack([rng.permutation(2 * maxp)[:maxp] for _ in range(2)]).astype(np.int32)
+        q = (1 + 0.02 * rng.standard_normal((2, P, hq, d))).astype(np.float32)
+        lens = [maxp * 16 - P, 150]
+        kv, tab = upload(c, cache), i32(c, table)
+        got = host(c.gqa_prefill_attn_i8(c.to_device(q.reshape(2 * P, hq, d)), kv, tab, i32(c, lens), P, maxp * 16))
+        check(got.reshape(q.shape), *attend(cache, q, table, lens, True), tight=1e-3)
+        got = host(c.gqa_decode_attn_i8(c.to_device(q[:, 0].copy()), kv, tab, i32(c, lens), maxp * 16))
+        want, bound = attend(cache, q[:, :1], table, lens, False)
+        check(got, want[:, 0], bound[:, 0], tight=1e-3)
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("ratio", [1e6, 1e9, 1e20])
+@pytest.mark.parametrize("P", [1, 70])
+def test_distance_bias_hides_far_pages_of_large_values(ctx, P, ratio):
+    """Pages whose distance leaves them no weight, with values far above the near ones'."""
+    rng, hq, hkv, d, maxp = np.random.default_rng(P), 4, 2, 64, 40
+    cache = ref.Cache(maxp, hkv, d, rng)
+    cache.vs[: maxp // 2] *= np.float32(ratio)
+    table = np.arange(maxp, dtype=np.int32)[None]
+    q = rng.standard_normal((1, P, hq, d)).astype(np.float32)
+    lens, slopes = [maxp * 16 - P + (P == 1)], np.float32([2.0, 3.0, 1.5, 2.5])
+    opts = lgx.AttnOpts(slopes=ctx.to_device(slopes))
+    want, bound = attend(cache, q, table, lens, P > 1, slopes=slopes)
+    if P == 1:
+        got = ctx.gqa_decode_attn_i8(ctx.to_device(q[:, 0]), upload(ctx, cache), i32(ctx, table), i32(ctx, lens), maxp * 16, opts)
+    else:
+        got = ctx.gqa_prefill_attn_i8(ctx.to_device(q[0]), upload(ctx, cache), i32(ctx, table), i32(ctx, lens), P, maxp * 16, opts=opts)
+    check(host(got).reshape(want.shape), want, bound, tight=1e-3)
 
 
 # ---- recorded steps -------------------------------------------------------
