@@ -475,6 +475,13 @@ __device__ __forceinline__ void i8_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi
     hi = __builtin_bit_cast(uint32_t, h);
 }
 
+// Two numbers rounded to binary16 (v_cvt_pk_f16_f32).
+__device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){lo, hi}, v2h));
+}
+
 // w minus the low or high half of a pair of binary16 numbers, exact.  (Neither
 // operand may come from a matrix instruction or a v_exp: the compiler puts no wait
 // states ahead of assembly.)
@@ -837,11 +844,13 @@ __device__ __forceinline__ void a8_weights(const lgx_attn8_args& a, float (*S)[1
         uint32_t hw[8], lw[8];
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
-            // the first part rounded toward zero, the second holds the rest
-            const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(S[n][e], S[n][e + 1]));
+            // both parts rounded to nearest: the sum of the weights and that of their
+            // roundings then differ to either side, also where the second part is
+            // subnormal (cut, the results were 7.5e-8 low, and by 2^-17 of the weights
+            // of 131072 tokens behind one that weighs as much as they together)
+            const uint32_t h = f16_pair(S[n][e], S[n][e + 1]);
             hw[e >> 1] = h;
-            lw[e >> 1] = __builtin_bit_cast(
-                uint32_t, __builtin_amdgcn_cvt_pkrtz(minus_half<0>(S[n][e], h), minus_half<1>(S[n][e + 1], h)));
+            lw[e >> 1] = f16_pair(minus_half<0>(S[n][e], h), minus_half<1>(S[n][e + 1], h));
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
