@@ -871,20 +871,29 @@ __device__ __forceinline__ void i8_to_v8h(const uint4& v, uint4& h0, uint4& h1) 
     i8_to_f16(v.w, h1.z, h1.w);
 }
 // o += V^T . P^T for N column tiles; vf(i, h0, h1): V operands of dimensions 16 i ..
+// A tile's products are summed from zero and joined to o on the VALU.  The matrix unit
+// adds them in groups of eight and rounds its sum after each: added to o itself, the
+// second parts of the weights fall below half a step of it as o grows (equal weights of
+// 65536 tokens: 3.2e-5 off; a sink among 131072: 2.5e-5, now 1.2e-5 of repeated pages'
+// own roundings).  It costs 3 % of prompts (8 x 512 rows at 4000 tokens 445 against 434
+// us) and nothing where memory bounds.
 template <int ND, int N, class VF>
 __device__ __forceinline__ void a8_pv(const VF& vf, const v8h (&ph)[N][2], const v8h (&pl)[N][2], v4f (&o)[N][ND]) {
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
         uint4 h0, h1;
         vf(i, h0, h1);
+        v4f t[N];
 #pragma unroll
-        for (int n = 0; n < N; ++n) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h0), ph[n][0], o[n][i], 0, 0, 0);
+        for (int n = 0; n < N; ++n) t[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h0), pl[n][0], (v4f){0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
-        for (int n = 0; n < N; ++n) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h1), ph[n][1], o[n][i], 0, 0, 0);
+        for (int n = 0; n < N; ++n) t[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h0), ph[n][0], t[n], 0, 0, 0);
 #pragma unroll
-        for (int n = 0; n < N; ++n) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h0), pl[n][0], o[n][i], 0, 0, 0);
+        for (int n = 0; n < N; ++n) t[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h1), pl[n][1], t[n], 0, 0, 0);
 #pragma unroll
-        for (int n = 0; n < N; ++n) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h1), pl[n][1], o[n][i], 0, 0, 0);
+        for (int n = 0; n < N; ++n) t[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(h1), ph[n][1], t[n], 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < N; ++n) o[n][i] += t[n];
     }
 }
 
@@ -1245,6 +1254,7 @@ __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
             constexpr int PF = 3;
             const uint4* vr = fr + 2 * 4 * NS * 64;
             v8h vf[2 * ND];
+            v4f t[ND][NT];
 #pragma unroll
             for (int i = 0; i < PF; ++i) vf[i] = as_v8h(vr[i * 64]);
 #pragma unroll
@@ -1252,17 +1262,19 @@ __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
                 if (i + PF < 2 * ND) vf[i + PF] = as_v8h(vr[(i + PF) * 64]);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    o[n][i / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], ph[n][i & 1], o[n][i / 2], 0, 0, 0);
+                    t[i / 2][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], pl[n][i & 1],
+                                                                         i & 1 ? t[i / 2][n] : (v4f){0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    o[n][i / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], pl[n][i & 1], o[n][i / 2], 0, 0, 0);
-            }
-            __builtin_amdgcn_sched_group_barrier(0x100, PF, 1);
+                    t[i / 2][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], ph[n][i & 1], t[i / 2][n], 0, 0, 0);
+                // a tile's sum from zero (a8_pv), of dimensions whose products have ended
+                if (i >= 3 && i & 1) {
 #pragma unroll
-            for (int i = 0; i < 2 * ND; ++i) {
-                if (i + PF < 2 * ND) __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
-                __builtin_amdgcn_sched_group_barrier(0x008, 2 * NT, 1);
+                    for (int n = 0; n < NT; ++n) o[n][i / 2 - 1] += t[i / 2 - 1][n];
+                }
             }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[n][ND - 1] += t[ND - 1][n];
         }
     };
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

@@ -287,6 +287,88 @@ def test_weights_are_rounded_without_a_bias(monkeypatch, cols):
         c.close()
 
 
+def test_a_sink_among_many_tokens(monkeypatch):
+    """One token with half of the weight before 131072 others, all in one wave: their
+    weights' second parts are subnormal, and rounded, not cut.
+
+    In units in which the sink's weight is 2^10 at least theirs are 2^-7 and off by 2^-25
+    at most, to either side: 1008 distinct weights of a head that come again and again put
+    2^-18 / sqrt(3 * 1008) / 2 on the result, 3.5e-8.  The sums: 63 pages come again 32.5
+    times in each of the column's four lanes and in the tiles, and a sum that stays in its
+    binade rounds them alike each time, by 2^-24 at most.  The weights' sum: the lane that
+    holds the sink 32.5 sqrt(63 / 3) 2^-24 = 8.9e-6, the three others, a quarter of it high,
+    2.2e-6 each, of a total of 2: 4.8e-6 on all of a head.  A dimension's sum, up to twice as
+    high, 8.9e-6, over a head's 64 dimensions 1.1e-6.  Together 4.9e-6 for a head, 3.1e-7 for
+    the mean over 256 of them, where cut weights lack 2^-17 of the others' half, 3.8e-6, and
+    sums whose second parts fall below half a step of the first ones' lack 2^-13 of it,
+    1.2e-4.  Five deviations are allowed."""
+    monkeypatch.setenv("LGX_A8_COLS", "128")
+    monkeypatch.setenv("LGX_A8_WGS", "1")
+    c = lgx.Context(0)
+    try:
+        rng, hkv, d, pages, P = np.random.default_rng(3), 256, 64, 64, 2
+        n = 131072 // 16
+        cache = ref.Cache(pages, hkv, d, rng)
+        cache.v[:] = np.abs(cache.v.astype(np.int16)).clip(1, 127)
+        cache.vs[:] = np.float32(0.01)
+        cache.ks[:] = np.float32(2.0 ** -6)
+        cache.k[:] = rng.integers(-20, 21, cache.k.shape)
+        # page 0 is the sink's: its token 0 scores ln(131072) more than the others, q = 1
+        cache.k[0, :, 0] = int(round(np.log(131072.0) / (2.0 ** -6 * 8)))
+        table = np.concatenate([[0], 1 + np.arange(n - 1) % (pages - 1)]).astype(np.int32)[None]
+        q = np.ones((1, P, hkv, d), np.float32)
+        L = n * 16 - P
+        got = host(c.gqa_prefill_attn_i8(c.to_device(q[0]), upload(c, cache), i32(c, table), i32(c, [L]), P, n * 16))
+        full = np.bincount(table[0, :-1], minlength=pages).astype(np.float64)
+        errs = []
+        for j in range(P):
+            count = np.repeat(full[:, None], 16, 1)
+            count[table[0, -1], :16 - P + j + 1] += 1
+            for g in range(hkv):
+                s = cache.k[:, g].astype(np.float64).sum(-1) * 2.0 ** -6 / 8
+                w = count * np.exp(s - s.max())
+                v = cache.v[:, g].astype(np.float64) * float(np.float32(0.01))
+                want = np.einsum("pt,pdt->d", w, v) / w.sum()
+                errs.append(((got[j, g] - want) / want).mean())
+        assert 0.3 < w[0, 0] / w.sum() < 0.7
+        assert np.abs(np.mean(errs)) <= 5 * 3.1e-7 and np.abs(errs).max() <= 5 * 4.9e-6, (np.mean(errs), np.abs(errs).max())
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("P", [1, 2])
+def test_equal_weights_over_a_long_context(monkeypatch, P):
+    """q = 0: the mean of 65536 values of one sign, by one workgroup.  The sum of the
+    weights is exact.  A dimension's sum is rounded once for each of up to 1024 tiles, to
+    either side, by at most 2^-24 of what it has reached: sqrt(1024 / 3 / 3) 2^-24 = 6.4e-7
+    at the end; within the tiles roundings are 1024 times smaller; the weight itself, the V
+    scale, is held to 2^-23.  Six deviations (of 64 dimensions the largest) and that: 4.0e-6.
+    (Second parts added one by one to sums of 2^15 of the first are lost: 5e-5 to 1e-4.)"""
+    monkeypatch.setenv("LGX_A8_COLS", "16" if P == 1 else "128")
+    c = lgx.Context(0)
+    try:
+        rng, B, d, n = np.random.default_rng(P), 256, 64, 4096
+        cache = ref.Cache(n, 1, d, rng)
+        cache.v[:] = np.abs(cache.v.astype(np.int16)).clip(1, 127)
+        cache.vs[:] = np.float32(0.01)
+        table = np.broadcast_to(rng.permutation(n).astype(np.int32), (B, n))
+        kv, tab, L = upload(c, cache), i32(c, np.ascontiguousarray(table)), n * 16 - (P > 1) * P
+        q = c.torch.zeros((B * P, 1, d), device=c.dev)
+        before = c.launch_count
+        if P == 1:
+            got = host(c.gqa_decode_attn_i8(q, kv, tab, i32(c, [L] * B), n * 16))
+        else:
+            got = host(c.gqa_prefill_attn_i8(q, kv, tab, i32(c, [L] * B), P, n * 16))
+        assert c.launch_count - before == 1          # nothing is split
+        _, v = cache.rows(table[0], n * 16)
+        for j in range(P):
+            want = v[:L + j + (P > 1), 0].mean(0)
+            err = np.abs(got.reshape(B, P, d)[:, j] - want) / want
+            assert err.max() <= 4.0e-6, (j, err.max())
+    finally:
+        c.close()
+
+
 # ---- recorded steps -------------------------------------------------------
 
 def test_a_recorded_step_outlives_a_larger_call():
