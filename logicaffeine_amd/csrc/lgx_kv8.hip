@@ -700,9 +700,10 @@ __device__ __forceinline__ float a8_query(const lgx_attn8_args& a, const float (
         }
     am = col_max(am);
     const bool isbad = col_max(bad ? 1.0f : 0.0f) != 0.0f;
-    // the largest power of two that keeps every |q| within 127 * 65536, the
-    // range of three balanced digits
-    const float up = __uint_as_float(__float_as_uint(fminf(127.0f * 65536.0f / am, 0x1p100f)) & 0x7f800000u);
+    // the largest power of two that keeps every |q| within 127 * 65536, the range of
+    // three balanced digits; up to 2^122, where scale / up is still a normal number (rows
+    // below 2^-99 in magnitude have fewer bits)
+    const float up = __uint_as_float(__float_as_uint(fminf(127.0f * 65536.0f / am, 0x1p122f)) & 0x7f800000u);
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
@@ -1106,7 +1107,7 @@ __device__ __forceinline__ float a8_query16(const lgx_attn8_args& a, const float
         }
     am = col_max(am);
     const bool isbad = col_max(bad ? 1.0f : 0.0f) != 0.0f;
-    const float up = __uint_as_float(__float_as_uint(fminf(32768.0f / am, 0x1p100f)) & 0x7f800000u);
+    const float up = __uint_as_float(__float_as_uint(fminf(32768.0f / am, 0x1p122f)) & 0x7f800000u);
 #pragma unroll
     for (int h = 0; h < NH; ++h)
 #pragma unroll

@@ -369,6 +369,23 @@ def test_equal_weights_over_a_long_context(monkeypatch, P):
         c.close()
 
 
+@pytest.mark.parametrize("P", [1, 70])
+@pytest.mark.parametrize("small", [1e-20, 1e-25, 1e-28])
+def test_tiny_queries_under_large_k_scales(ctx, P, small):
+    """Queries down to 2^-93 with keys as large: the scores are ordinary numbers."""
+    rng, hq, hkv, d, maxp = np.random.default_rng(P), 4, 2, 64, 10
+    cache = ref.Cache(maxp, hkv, d, rng)
+    cache.ks = (cache.ks * np.float32(1 / small)).astype(np.float32)
+    q = (rng.standard_normal((1, P, hq, d)) * small).astype(np.float32)
+    table, lens = np.arange(maxp, dtype=np.int32)[None], [maxp * 16 - P]
+    want, bound = attend(cache, q, table, lens, P > 1)
+    if P == 1:
+        got = ctx.gqa_decode_attn_i8(ctx.to_device(q[:, 0]), upload(ctx, cache), i32(ctx, table), i32(ctx, lens), maxp * 16)
+    else:
+        got = ctx.gqa_prefill_attn_i8(ctx.to_device(q[0]), upload(ctx, cache), i32(ctx, table), i32(ctx, lens), P, maxp * 16)
+    check(host(got).reshape(want.shape), want, bound, tight=1e-3)
+
+
 # ---- recorded steps -------------------------------------------------------
 
 def test_a_recorded_step_outlives_a_larger_call():
