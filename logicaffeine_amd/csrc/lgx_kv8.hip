@@ -898,7 +898,8 @@ __device__ __forceinline__ void a8_pv(const VF& vf, const v8h (&ph)[N][2], const
     }
 }
 
-// A column's result, or its split's; c: the column, NC columns per block.
+// A column's result, or its split's (divided by the split's own sum of weights, so that
+// it is no larger than V's values); c: the column, NC columns per block.
 template <int NC, int ND>
 __device__ __forceinline__ void a8_store(const lgx_attn8_args& a, const A8Block& k, int64_t orow, int c, const A8Col& x, int kg,
                                          const v4f (&o)[ND]) {
@@ -907,7 +908,7 @@ __device__ __forceinline__ void a8_store(const lgx_attn8_args& a, const A8Block&
     const int64_t at = part ? ((int64_t)k.pos * a.hkv + k.g) * NC + c - k.c0 : orow;
     const int unit = (int)x.e - A8_UP;
     // NaN sums stay NaN; nothing seen gives zeros
-    const float s = part ? 1.0f : x.l == 0.0f ? 0.0f : 1.0f / x.l;
+    const float s = x.l == 0.0f ? 0.0f : 1.0f / x.l;
     float* dst = (part ? a.part : a.out) + at * D;
 #pragma unroll
     for (int i = 0; i < ND; ++i)
@@ -1327,12 +1328,12 @@ __device__ __forceinline__ void attn8_join_body(const lgx_attn8_args& a) {
 #pragma unroll
         for (int i = 0; i < NW; ++i) m = fmaxf(m, ml_s[i]);
     }
-    // an empty split's maximum is -inf
-    auto weight = [&](float x) { return x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x - m); };
-    for (int s = tid; s < ns; s += TH) {
-        const float2 x = *(const float2*)(a.ml + 2 * at(s));
-        l = fmaf(weight(x.x), x.y, l);
-    }
+    // a split's sum of weights by the common maximum; an empty one's own is -inf
+    auto weight = [&](int64_t i) {
+        const float2 x = *(const float2*)(a.ml + 2 * i);
+        return (x.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x.x - m)) * x.y;
+    };
+    for (int s = tid; s < ns; s += TH) l += weight(at(s));
 #pragma unroll
     for (int s = 32; s; s >>= 1) l += shfl_xor_f(l, s);
     if (NW > 1) {
@@ -1342,12 +1343,13 @@ __device__ __forceinline__ void attn8_join_body(const lgx_attn8_args& a) {
 #pragma unroll
         for (int i = 0; i < NW; ++i) l += ml_s[NW + i];
     }
+    const float r = l == 0.0f ? 0.0f : 1.0f / l;  // ahead of the sum, which then stays within V's values
     const int q = tid % Q, sg = tid / Q;
     v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
     for (int s = sg; s < ns; s += NG) {
         const int64_t i = at(s);
-        o += *((const v4f*)(a.part + i * D) + q) * weight(a.ml[2 * i]);
+        o += *((const v4f*)(a.part + i * D) + q) * (weight(i) * r);
     }
     if (NW > 1) {
         o_s[tid] = o;
@@ -1362,7 +1364,7 @@ __device__ __forceinline__ void attn8_join_body(const lgx_attn8_args& a) {
             for (int e = 0; e < 4; ++e) o[e] += shfl_xor_f(o[e], s);
         if (tid >= Q) return;
     }
-    *((v4f*)(a.out + rh * D) + q) = o * (l == 0.0f ? 0.0f : 1.0f / l);
+    *((v4f*)(a.out + rh * D) + q) = o;
 }
 extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_join_d64(const lgx_attn8_args a) { attn8_join_body<64, 256>(a); }
 extern "C" __global__ __launch_bounds__(256) void lgx_k_attn8_join_d128(const lgx_attn8_args a) { attn8_join_body<128, 256>(a); }

@@ -386,6 +386,26 @@ def test_tiny_queries_under_large_k_scales(ctx, P, small):
     check(host(got).reshape(want.shape), want, bound, tight=1e-3)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("B,P", [(1, 1), (3, 1), (2, 5), (40, 1)])
+def test_values_near_the_largest_numbers(ctx, B, P, d):
+    """A result lies within its values, also where those are 1e38 and their sum over a
+    split's tokens is not a number any more, or 1e-36."""
+    rng, hq, hkv, maxp = np.random.default_rng(B + P + d), 4, 2, 320
+    cache, table = ref.Cache(maxp, hkv, d, rng), rng.integers(0, maxp, (B, maxp)).astype(np.int32)
+    cache.ks[:] = np.float32(0.002)
+    cache.vs[:, 0], cache.vs[:, 1] = np.float32(1e38 / 127), np.float32(2e-38)
+    lens = rng.integers(3000, maxp * 16 - P, B)
+    q = rng.standard_normal((B, P, hq, d)).astype(np.float32)
+    want, bound = attend(cache, q, table, lens, P > 1)
+    if P == 1:
+        got = ctx.gqa_decode_attn_i8(ctx.to_device(q[:, 0]), upload(ctx, cache), i32(ctx, table), i32(ctx, lens), maxp * 16)
+    else:
+        got = ctx.gqa_prefill_attn_i8(ctx.to_device(q.reshape(B * P, hq, d)), upload(ctx, cache), i32(ctx, table), i32(ctx, lens), P,
+                                      maxp * 16)
+    check(host(got).reshape(want.shape), want, bound + 2.0 ** -149, tight=1e-3)
+
+
 # ---- recorded steps -------------------------------------------------------
 
 def test_a_recorded_step_outlives_a_larger_call():
