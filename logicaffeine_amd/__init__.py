@@ -309,7 +309,21 @@ def _tensor(name, x, dtype, shape, dev):
     return x
 
 
-class KvCacheI8:
+class _Held:
+    """What a C struct points to.  Attributes are given by the constructor and stay:
+    the struct would go on naming the memory of a tensor that was put aside."""
+
+    def _hold(self, **attributes):
+        self.__dict__.update(attributes)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{type(self).__name__}.{name} cannot be set: make a new {type(self).__name__}")
+
+    def __delattr__(self, name):
+        raise AttributeError(f"{type(self).__name__}.{name} cannot be deleted")
+
+
+class KvCacheI8(_Held):
     """An 8-bit paged KV cache (lgx_kv_i8): int8 K pages [pages][hkv][16][d] and V
     pages [pages][hkv][d][16], float32 scales [pages][hkv] for each."""
 
@@ -323,10 +337,8 @@ class KvCacheI8:
         _tensor("v", v, t.int8, (n, hkv, d, 16), k.device)
         _tensor("k_scale", k_scale, t.float32, (n, hkv), k.device)
         _tensor("v_scale", v_scale, t.float32, (n, hkv), k.device)
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.num_pages, self.hkv, self.d, self.device = n, hkv, d, k.device
-        self._c = KvI8C(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, hkv, d)
-        self.cstruct = C.byref(self._c)
+        self._hold(k=k, v=v, k_scale=k_scale, v_scale=v_scale, num_pages=n, hkv=hkv, d=d, device=k.device,
+                   cstruct=C.byref(KvI8C(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, hkv, d)))
 
     @classmethod
     def empty(cls, ctx: "Context", num_pages: int, hkv: int, d: int) -> "KvCacheI8":
@@ -338,7 +350,7 @@ class KvCacheI8:
                    t.zeros((num_pages, hkv), dtype=t.float32, device=ctx.dev))
 
 
-class Rope:
+class Rope(_Held):
     """Rotation of query and key heads (lgx_rope): cos / sin are float32 device
     tensors [positions][rot / 2], the first rot dimensions of a head are turned in
     pairs (i, i + rot / 2), or (2i, 2i + 1) when interleaved."""
@@ -349,9 +361,8 @@ class Rope:
         n, half = cos.shape
         _tensor("cos", cos, t.float32, (n, half), cos.device)
         _tensor("sin", sin, t.float32, (n, half), cos.device)
-        self.cos, self.sin, self.device = cos, sin, cos.device
-        self._c = RopeC(cos.data_ptr(), sin.data_ptr(), 2 * half, int(interleaved), n)
-        self.cstruct = C.byref(self._c)
+        self._hold(cos=cos, sin=sin, device=cos.device,
+                   cstruct=C.byref(RopeC(cos.data_ptr(), sin.data_ptr(), 2 * half, int(interleaved), n)))
 
     @classmethod
     def tables(cls, ctx: "Context", max_pos: int, rot: int, theta: float = 1e6, interleaved: bool = False,
@@ -370,7 +381,7 @@ class Rope:
         return cls(cos.to(ctx.dev), sin.to(ctx.dev), interleaved)
 
 
-class AttnOpts:
+class AttnOpts(_Held):
     """Options of the 8-bit cache's attention (lgx_attn_opts): scale 0 is
     1 / sqrt(d); softcap 0 and window 0 are none; slopes: float32 [hq]."""
 
@@ -379,9 +390,7 @@ class AttnOpts:
             import torch as t
 
             _tensor("slopes", slopes, t.float32, (None,), slopes.device)
-        self.slopes = slopes
-        self._c = AttnOptsC(scale, softcap, window, _ptr_or_none(slopes))
-        self.cstruct = C.byref(self._c)
+        self._hold(slopes=slopes, cstruct=C.byref(AttnOptsC(scale, softcap, window, _ptr_or_none(slopes))))
 
 
 class Context:
