@@ -654,7 +654,7 @@ class Context:
         if kv.device != self.dev:
             raise ValueError(f"the cache is on {kv.device}, the context on {self.dev}")
         i32 = self.torch.int32
-        _tensor("page_table", page_table, i32, page_table.shape, self.dev)
+        _tensor("page_table", page_table, i32, (B, page_table.shape[-1]), self.dev)
         _tensor("lengths", seq_len, i32, (B,), self.dev)
         if n_new is not None:
             _tensor("n_new", n_new, i32, (B,), self.dev)
@@ -663,8 +663,8 @@ class Context:
                            out=None):
         """q [B][hq][d] over the first seq_len[b] tokens of the 8-bit cache."""
         B, hq, d = q.shape
-        if d != kv.d or page_table.shape[0] != B:
-            raise ValueError(f"q {tuple(q.shape)} for heads of {kv.d} and a table of {page_table.shape[0]} sequences")
+        if d != kv.d or page_table.shape[:1] != (B,):
+            raise ValueError(f"q {tuple(q.shape)} for heads of {kv.d} and a page table {tuple(page_table.shape)}")
         self._lengths(seq_len, None, page_table, kv, B)
         out = self._attn_out(q, opts, out)
         _check(lib().lgx_gqa_decode_attn_i8(
@@ -676,7 +676,7 @@ class Context:
                             opts: AttnOpts = None, out=None):
         """q [B*P][hq][d]: row b*P + j (j < n_new[b]) is the query at position
         seq_len[b] + j, causal over the 8-bit cache."""
-        B, (rows, hq, d) = page_table.shape[0], q.shape
+        (B, _), (rows, hq, d) = page_table.shape, q.shape
         if rows != B * P or d != kv.d:
             raise ValueError(f"q {tuple(q.shape)} is not [{B * P}][hq][{kv.d}]")
         self._lengths(seq_len, n_new, page_table, kv, B)

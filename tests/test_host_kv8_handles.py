@@ -11,6 +11,13 @@ def cache(pages=4, hkv=2, d=64):
                          torch.zeros((pages, hkv)), torch.zeros((pages, hkv)))
 
 
+def context():
+    """The binding's checks run ahead of the library's, which would refuse this handle."""
+    c = lgx.Context.__new__(lgx.Context)
+    c.torch, c.dev, c.handle = torch, torch.device("cpu"), None
+    return c
+
+
 @pytest.mark.parametrize("make,name", [
     (cache, "k"), (cache, "v"), (cache, "k_scale"), (cache, "v_scale"), (cache, "num_pages"), (cache, "hkv"), (cache, "d"),
     (lambda: lgx.Rope(torch.ones((9, 32)), torch.zeros((9, 32))), "cos"),
@@ -30,3 +37,15 @@ def test_a_handle_refuses_what_it_could_not_take_over(make, name):
     if isinstance(before, torch.Tensor):
         before.fill_(1)                              # the contents stay the caller's
         assert bool((getattr(x, name) == 1).all())
+
+
+@pytest.mark.parametrize("shape", [(2,), (2, 4, 1), (2, 4, 0), (2, 4, 3)])
+def test_a_page_table_is_a_matrix(shape):
+    c, kv = context(), cache()
+    q, lens, table = torch.zeros((2, 4, 64)), torch.ones(2, dtype=torch.int32), torch.zeros(shape, dtype=torch.int32)
+    for call in (lambda: c.gqa_decode_attn_i8(q, kv, table, lens, 64), lambda: c.gqa_prefill_attn_i8(q, kv, table, lens, 1, 64),
+                 lambda: c.rope_kv_append_i8(torch.zeros((2, 512)), None, lgx.Rope(torch.ones((9, 32)), torch.zeros((9, 32))), lens,
+                                             table, kv),
+                 lambda: c.kv_read_i8(kv, table, lens, 3)):
+        with pytest.raises(ValueError):
+            call()
