@@ -129,6 +129,28 @@ def test_a_sequence_without_new_rows_touches_nothing(ctx, P):
         assert host(got).tobytes() == want.tobytes()
 
 
+@pytest.mark.parametrize("P", [1, 20])
+def test_an_idle_row_names_pages_that_others_append_to(ctx, P):
+    """Slots of a padded batch that have no sequence any more: their table rows still name
+    pages that other sequences of the same call append to, and whose blocks grow."""
+    rng, hq, hkv, d, B = np.random.default_rng(P), 2, 2, 64, 32
+    maxp = 3
+    lens, new = rng.integers(1, 16, B), np.where(np.arange(B) % 2, 0, P)
+    cache, table = ref.Cache(B * maxp, hkv, d, rng), rng.permutation(B * maxp).astype(np.int32).reshape(B, maxp)
+    table[1::2] = table[0::2]                        # an idle row for each live one, inside the same page
+    lens[1::2] = lens[0::2]
+    x = (rng.standard_normal((B, P, (hq + 2 * hkv) * d)) * 1e3).astype(np.float32)
+    want = ref.Cache(B * maxp, hkv, d)
+    want.k, want.v, want.ks, want.vs = (a.copy() for a in (cache.k, cache.v, cache.ks, cache.vs))
+    want.append(x, None, *ref.tables(64, 0), False, lens, new, table, hq)
+    for _ in range(5):
+        kv = upload(ctx, cache)
+        ctx.rope_kv_append_i8(ctx.to_device(x.reshape(B * P, -1)), None, no_rope(ctx), i32(ctx, lens), i32(ctx, table), kv, P,
+                              n_new=i32(ctx, new))
+        for got, w in ((kv.k, want.k), (kv.v, want.v), (kv.k_scale, want.ks), (kv.v_scale, want.vs)):
+            assert np.array_equal(host(got), w)
+
+
 # ---- attention ------------------------------------------------------------
 
 def attend(cache, q, table, seq_len, prefill, scale=None, slopes=None):
