@@ -323,9 +323,12 @@ typedef struct lgx_attn_opts {
  * tokens of sequence b (the query is at position seq_len[b] - 1), lengths clamped
  * to [0, max_seq_len], page ids to [0, num_pages); seq_len 0 gives zeros.
  * hq/hkv in 1..16.  Not the canonical schedule: scores from int8 products with q
- * in 24 bits, weights in 22 bits, binary32 sums (about 1e-6 of the 64-bit result
- * over the cache's values); the same inputs give the same bits.  Partial results
- * of long contexts live in the ctx workspace. */
+ * in 24 bits (22 in calls of many rows; fewer where a whole query head is below
+ * 2^-99), each weight times its V scale in 22 bits, or to 2^-35 of the row's largest
+ * such product where it is smaller (weights below 2^-113 of the largest may count as
+ * 0), binary32 sums: 1e-7 to 3e-7 of the 64-bit result over the cache's values for
+ * random inputs; the same inputs give the same bits.  Partial results of long
+ * contexts live in the ctx workspace. */
 lgx_status lgx_gqa_decode_attn_i8(lgx_ctx* ctx, const float* q, const lgx_kv_i8* kv, const int32_t* page_table,
                                   const int32_t* seq_len, int32_t B, int32_t hq, int32_t maxp,
                                   int32_t max_seq_len, const lgx_attn_opts* opts, float* out, void* stream);

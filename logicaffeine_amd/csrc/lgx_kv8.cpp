@@ -26,19 +26,20 @@ lgx_status check_kv(const lgx_kv_i8* kv, int32_t maxp) {
 int pages_touched(int n) { return (int)(((int64_t)n + LGX_PAGE - 2) / LGX_PAGE + 1); }
 
 // (row, head) pairs of a workgroup, for `heads` (sequence, KV head) pairs of `cols`
-// each over up to `tiles` tiles of 64 tokens.  16 and 32 go over a tile's tokens with
-// all four waves, 128 over its columns.  Measured on the 0.5B-, 1.5B- and 7B-shaped
-// heads (us with 16 / 32 / 128):
+// each over up to `tiles` tiles of 64 tokens (of max_seq_len: the lengths are on the
+// device).  16 and 32 go over a tile's tokens with all four waves, 128 over its columns.
+// Measured on the 0.5B-, 1.5B- and 7B-shaped heads (us with 16 / 32 / 128):
 //  - 128 from 512 workgroups on, two per compute unit: 8 x 512 rows at 4000 tokens
-//    (7B-shaped, 896 workgroups) 672 / 529 / 498, 8 x 1024 at 1100 (1792) 391 / 306 /
-//    209; below 8 x 256 at 4000 (448) 348 / 265 / 265, 16 x 256 at 2000
-//    (1.5B-shaped, 384) 177 / 136 / 153;
+//    (7B-shaped, 896 workgroups) 581 / 449 / 437, 8 x 1024 at 1100 (1792) 346 / 286 /
+//    196; below 8 x 256 at 4000 (448) 299 / 237 / 231, 16 x 256 at 2000
+//    (1.5B-shaped, 384) 149 / 116 / 121;
 //  - 32, which read K and V half as often and convert V for twice the columns, from
 //    about 12000 tiles of 16 columns on at head dimension 128: 16 x 64 at 500 (14300)
-//    44.1 / 38.5, 1 x 256 at 4000 (28200) 57.6 / 54.3; below 16 x 64 at 700
-//    (1.5B-shaped, 8400) 25.3 / 30.7, 2 x 64 at 2000 (7200) 28.3 / 30.5; at 64, where a
-//    tile's work is half as long, from about 65000: 8 x 512 at 2000 (0.5B-shaped, 115000)
-//    101 / 95, 8 x 128 at 4000 (56000) 56.2 / 57.4, 4 x 256 at 1000 (14000) 21.5 / 26.2.
+//    40.3 / 38.2, 8 x 64 at 2000 (28700) 53.2 / 43.6, 1 x 256 at 4000 (28200) 47.0 / 48.7;
+//    below 16 x 64 at 700 (1.5B-shaped, 8400) 23.4 / 24.2, 2 x 64 at 2000 (7200)
+//    22.4 / 26.7; at 64, where a tile's work is half as long, from about 65000: 8 x 512 at
+//    2000 (0.5B-shaped, 115000) 87.0 / 86.0, 8 x 128 at 4000 (56000) 53.6 / 48.9, 4 x 256
+//    at 1000 (14000) 18.8 / 19.4.
 int attn8_cols(const lgx_ctx* c, int64_t heads, int64_t cols, int64_t tiles, int d) {
     if (c->attn8_cols == 16 || c->attn8_cols == 32 || c->attn8_cols == 128) return c->attn8_cols;
     if (cols <= 16) return 16;
@@ -46,9 +47,10 @@ int attn8_cols(const lgx_ctx* c, int64_t heads, int64_t cols, int64_t tiles, int
     return heads * ((cols + 15) / 16) * tiles >= (d == 64 ? 65536 : 12288) ? 32 : 16;
 }
 
-// Launch over B sequences.  Where one workgroup per (sequence, KV head, column block)
-// does not fill the device, their tiles are split among workgroups (the splitting
-// itself is done on the device, by the lengths), two per compute unit.
+// Launch over B sequences.  Where there are fewer (sequence, KV head, column block)s
+// than compute units (times attn8_wgs), their tiles are split among that many
+// workgroups; the splitting itself is done on the device, by the lengths.  From there
+// on each is one workgroup's, also a sequence far longer than the others.
 lgx_status run_attn8(lgx_ctx* c, lgx_attn8_args& a, int B, int d, bool x, void* stream) {
     const int64_t cols = (int64_t)a.P * (a.hq / a.hkv), heads = (int64_t)B * a.hkv;
     // the most tiles that a block can see (its rows are at most 128 apart)

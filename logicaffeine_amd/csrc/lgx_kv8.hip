@@ -451,16 +451,19 @@ extern "C" __global__ __launch_bounds__(256) void lgx_k_kv8_read_d128(const lgx_
 //   scores   S^T[token][column] = K . Q^T on v_mfma_i32_16x16x64_i8, K quants as
 //            they lie in memory.  q is an integer of 24 bits (its row scaled by a
 //            power of two) in three signed base-256 digits: three exact int32
-//            products, joined in binary32.
+//            products, joined in binary32.  (128 columns: K and two parts of q in
+//            binary16.)
 //   softmax  running maximum and sum per column, in base 2.
 //   PV       O^T[dim][column] += V^T . P^T on v_mfma_f32_16x16x32_f16: V quants are
 //            binary16 numbers, a weight (times its page's V scale) is the sum of
-//            two binary16 numbers, 22 bits.  Accumulation in binary32.
+//            two binary16 numbers, 22 bits.  The matrix unit sums a tile, the VALU
+//            the tiles, both in binary32.
 // Row 4 p + v of score sub-tile u is token 4 u + v of page p, so that lane (column,
 // kg) ends up with all 16 scores of page kg: its scales are one value per lane,
 // and its weights are the PV operand as they stand (V's 16-byte loads give lane
-// (dim, kg) the 16 tokens of page kg).  Nothing passes through LDS or across
-// lanes but the column maximum.
+// (dim, kg) the 16 tokens of page kg).  Scores and weights pass neither through LDS
+// nor across lanes, but for the column's maxima; through LDS go, with 32 columns, the
+// query's digits, and with 128 the tiles of K and V.
 // ---------------------------------------------------------------------------
 
 // Four int8 quants as binary16: the byte of v + 128 under the exponent of 1024
@@ -921,12 +924,12 @@ __device__ __forceinline__ void a8_store(const lgx_attn8_args& a, const A8Block&
 // in turn, K and V straight into registers: the next tile's K is in flight
 // from the end of the scores on, its V from the end of the PV product; at the end
 // the waves' results are joined in LDS.  One column tile is bound by memory: 16
-// sequences of 32768 tokens, 12/2 heads of 128, 268 MB, in 52 us (5.2 TB/s), 51 with
-// the loads alone; 64 of 256 to 4096 tokens, 28/4 heads, 145 MB, in 40, 39 with the
-// loads alone (the longest one's workgroup takes what one compute unit can load).
-// Eight waves per workgroup load no faster there (41 us) and wait longer elsewhere (14.7
-// against 12.0 us for one sequence of 8191).  Two column tiles are bound by the VALU
-// and the matrix units in turn: 8 x 64 rows at 2000 tokens 54 us.
+// sequences of 32768 tokens, 12/2 heads of 128, 268 MB, in 51 us (5.2 TB/s), 51 with
+// the loads alone; 64 of 256 to 4096 tokens, 28/4 heads, 145 MB, in 39, as with the
+// loads alone (the longest one's workgroup takes what one compute unit can load), and 53
+// with capped scores.  Eight waves per workgroup load no faster there and wait a fifth
+// longer for one sequence of 8191.  Two column tiles are bound by the VALU and the matrix
+// units in turn: 8 x 64 rows at 2000 tokens 43 us, the operations alone 13.
 template <int D, int NT, bool X>
 __device__ __forceinline__ void attn8_narrow_body(const lgx_attn8_args& a) {
     constexpr int WT = 4, NS = D / 64, ND = D / 16;
@@ -1126,13 +1129,15 @@ __device__ __forceinline__ float a8_query16(const lgx_attn8_args& a, const float
 // lanes), a tile ahead, and then turns them into operands in one of two LDS buffers
 // while the other's tile is in use.  With K in binary16 the scores need no joining of
 // digits: two products, one accumulator.  Bound by the matrix units and the VALU in
-// turn: 8 x 512 rows at 4000 tokens, 28/4 heads of 128, in 430 to 480 us by inputs and
-// clock, 0.46 to 0.51 PFLOP/s of the formula's work, twice that executed (q and the
-// weights in two parts; a large binary16 product reaches 1.1 to 1.2 here); matrix units
-// busy for 0.43 of the cycles, the VALU for 0.49.  What got it there, of 783 us: K and
-// V through LDS (565), no masks where all rows see a tile, operands converted once
-// and no load waited for where branches meet (520), a softmax reference that seldom
-// moves (480).  64 columns per workgroup (16 per wave) took as long as 16 or longer.
+// turn: 8 x 512 rows at 4000 tokens, 28/4 heads of 128, in 434 to 457 us by the card and
+// its clock (513 in a profiler's few dispatches, at 1.97 GHz), 0.48 to 0.51 PFLOP/s of the
+// formula's work, twice that executed (q and the weights in two parts; a large binary16
+// product reaches 1.1 to 1.2 here); matrix units busy for 0.41 of the cycles, the VALU for
+// 0.53.  What brought it down from 783 us: K and V through LDS
+// (565), no masks where all rows see a tile, operands converted once and no load waited
+// for where branches meet (520), a softmax reference that seldom moves (480).  64 columns
+// per workgroup (16 per wave) took as long as 16 or longer.  The same rows with a cap of
+// 30 take 855 us, with a window of 1000 tokens 170.
 template <int D, int NT, bool X>
 __device__ __forceinline__ void attn8_wide_body(const lgx_attn8_args& a) {
     constexpr int NS = D / 64, NH = D / 32, ND = D / 16, NF = 4 * NS + ND, FW = NF / 4;
