@@ -202,7 +202,7 @@ def _sample_inputs(case, g):
         else:
             # most of the vocabulary far below a few dozen likely tokens
             likely = torch.randint(0, V, (len(x), 40), device="cuda", generator=g)
-            x = (2.0 * x).scatter_add_(1, likely, 6.0 + 3.0 * torch.randn(likely.shape, device="cuda", generator=g))
+            x = (2.0 * x).scatter_add_(1, likely, 12.0 + 3.0 * torch.randn(likely.shape, device="cuda", generator=g))
             logits[lo:lo + 64] = x
     pick = lambda *values: torch.tensor(values, device="cuda")[torch.randint(0, len(values), (m,), device="cuda", generator=g)]  # noqa: E731
     if case["mixed"]:
