@@ -1,6 +1,6 @@
 """Build recipe of liblgx (no cmake, no JIT cache: everything lands in-tree).
 
-    lgx_kernels.hsaco  hipcc --genco --offload-arch=gfx950 (device code only)
+    lgx_kernels.hsaco  hipcc --offload-arch=gfx950 (device code only) per kernel file, linked
     liblgx.so          g++ host launcher over the HIP module API
 
 Run as ``python -m logicaffeine_amd.build``; ``__graft_entry__.build()`` calls
@@ -9,6 +9,7 @@ Run as ``python -m logicaffeine_amd.build``; ``__graft_entry__.build()`` calls
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import subprocess
 import sys
@@ -26,7 +27,7 @@ LIB = os.path.join(HERE, "liblgx.so")
 # instructions disabled (v_pk_*_f32 are never generated).  MFMA destinations
 # in VGPRs.
 HIP_FLAGS = [
-    "--genco", "--no-gpu-bundle-output", f"--offload-arch={ARCH}", "-O3", "-std=c++17",
+    "--offload-device-only", "--no-gpu-bundle-output", f"--offload-arch={ARCH}", "-O3", "-std=c++17",
     "-ffp-contract=off", "-fhip-fp32-correctly-rounded-divide-sqrt",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     # MFMA results in ordinary VGPRs (gfx950 allows it): the epilogues read
@@ -40,17 +41,37 @@ def _run(cmd):
     subprocess.run(cmd, check=True)
 
 
-def build_kernels() -> str:
-    src = os.path.join(CSRC, "lgx_kernels.hip")
+KERNEL_SOURCES = ["lgx_kernels.hip", "lgx_pages.hip"]
+BUILD_DIR = os.path.join(HERE, "_build")
+
+
+def _compile_kernels(source: str) -> str:
+    """One kernel file to an AMDGPU object, by way of its assembly (hipcc itself
+    links whatever it compiles for the device)."""
+    stem = os.path.join(BUILD_DIR, os.path.splitext(source)[0])
+    _run([os.path.join(ROCM, "bin", "hipcc"), *HIP_FLAGS, "-S", "-I", CSRC, "-o", stem + ".s", os.path.join(CSRC, source)])
+    _run([os.path.join(ROCM, "llvm", "bin", "clang"), "--target=amdgcn-amd-amdhsa", f"-mcpu={ARCH}", "-c", "-o", stem + ".o",
+          stem + ".s"])
+    os.remove(stem + ".s")
+    return stem + ".o"
+
+
+def build_kernels(only=None) -> str:
+    """The code object of all kernel files, compiled side by side.  only: compile
+    these again and link them with the others' objects of an earlier build."""
+    os.makedirs(BUILD_DIR, exist_ok=True)
+    todo = [s for s in KERNEL_SOURCES if only is None or s in only]
+    with concurrent.futures.ThreadPoolExecutor(len(todo)) as pool:
+        list(pool.map(_compile_kernels, todo))
+    objects = [os.path.join(BUILD_DIR, os.path.splitext(s)[0] + ".o") for s in KERNEL_SOURCES]
     tmp = HSACO + ".tmp"
-    _run([os.path.join(ROCM, "bin", "hipcc"), *HIP_FLAGS, "-I", CSRC, "-o", tmp, src])
+    _run([os.path.join(ROCM, "llvm", "bin", "ld.lld"), "-shared", "--no-undefined", "-o", tmp, *objects])
     os.replace(tmp, HSACO)
     return HSACO
 
 
 HOST_SOURCES = ["lgx_host.cpp", "lgx_glue.cpp", "lgx_model.cpp", "lgx_gen.cpp", "lgx_gguf.cpp",
-                "lgx_f16gemm.cpp", "lgx_kv8.cpp"]
-BUILD_DIR = os.path.join(HERE, "_build")
+                "lgx_f16gemm.cpp", "lgx_kv8.cpp", "lgx_pages.cpp"]
 
 
 def build_scratch() -> str:

@@ -17,18 +17,8 @@
 // kernel for any of these operations; the path is specified by the block
 // format (GGML Q8_0: 32 int8 + one f16 scale) and the decode step of a
 // Qwen2-style model.
-#include <hip/hip_runtime.h>
-#include <stdint.h>
+#include "lgx_device.h"
 
-#include "lgx_kargs.h"
-
-typedef int v4i __attribute__((ext_vector_type(4)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef float v16f __attribute__((ext_vector_type(16)));
-typedef float v32f __attribute__((ext_vector_type(32)));
-typedef int v16i __attribute__((ext_vector_type(16)));
-typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 // Streaming 128-bit load of weight data (read once per call: non-temporal).
 __device__ __forceinline__ uint4 ld_stream(const uint4* p) {
@@ -54,41 +44,6 @@ __device__ __forceinline__ uint4 ld_buf_cached(__amdgpu_buffer_rsrc_t r, int off
     return make_uint4(v.x, v.y, v.z, v.w);
 }
 
-__device__ __forceinline__ float h2f(uint32_t h) {
-    return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
-}
-
-__device__ __forceinline__ uint16_t f2h(float f) {
-    return __builtin_bit_cast(uint16_t, (_Float16)f);
-}
-
-__device__ __forceinline__ int shfl_xor_i(int v, int m) { return __shfl_xor(v, m, 64); }
-__device__ __forceinline__ float shfl_xor_f(float v, int m) { return __shfl_xor(v, m, 64); }
-
-// DPP lane moves for the wave reductions (VALU operations, where a shuffle
-// is an LDS round trip): quad_perm [1,0,3,2] (0xB1) and [2,3,0,1] (0x4E),
-// row_half_mirror (0x141: lane i <- 7 - i of its 8), row_mirror (0x140:
-// lane i <- 15 - i of its 16), row_shl:S (0x100 + S: lane i <- lane i + S of
-// its 16-lane row).  A lane without a source keeps its own value.
-template <int CTRL>
-__device__ __forceinline__ float dpp_f(float v) {
-    const int x = __builtin_bit_cast(int, v);
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false));
-}
-// Maximum over each aligned group of 8 lanes, in every lane of the group
-// (fmaxf is order-free, so any pairing gives the same value).
-__device__ __forceinline__ float max8(float m) {
-    m = fmaxf(m, dpp_f<0xB1>(m));
-    m = fmaxf(m, dpp_f<0x4E>(m));
-    return fmaxf(m, dpp_f<0x141>(m));
-}
-// Maximum over the wave, in every lane.
-__device__ __forceinline__ float wave_max(float m) {
-    m = max8(m);
-    m = fmaxf(m, dpp_f<0x140>(m));
-    m = fmaxf(m, shfl_xor_f(m, 16));
-    return fmaxf(m, shfl_xor_f(m, 32));
-}
 // The halving tree over the wave's 64 slots, lane i += lane i + s for
 // s = 32, 16, ..., 1 (the same pairs and order as the shuffle form); the
 // sum is lane 0's.
@@ -1579,31 +1534,6 @@ __device__ __forceinline__ void static_for(F&& f) {
 // lgx_k_attn_combine merges the chunks.  LDS: 32 KiB of V + 1088 bytes per
 // head.
 // ---------------------------------------------------------------------------
-typedef __attribute__((address_space(3))) void lds_void;
-typedef short v4s __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) v4s lds_v4s;
-
-// Direct global->LDS loads (a wave instruction's 64 pieces of 16 or 4 bytes
-// land one after the other at l, which is uniform) that the compiler does not
-// count: it makes every LDS read of a loop wait for those it knows, whichever
-// buffer they fill.  They write no register; publish_lds_loads waits for them.
-__device__ __forceinline__ void load_lds_16(const void* g, lds_void* l) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                 : : "s"((uint32_t)(uintptr_t)l), "v"(g) : "memory", "m0");
-}
-__device__ __forceinline__ void load_lds_4(const void* g, lds_void* l) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
-                 : : "s"((uint32_t)(uintptr_t)l), "v"(g) : "memory", "m0");
-}
-// Barrier that publishes this wave's direct global->LDS loads to the
-// workgroup.  The wait is written out: the compiler waits for such a load
-// where its own wave reads the data, which in a loop may be only after the
-// barrier, when the other waves already read.
-__device__ __forceinline__ void publish_lds_loads() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-}
-
 // 16-byte piece slot of piece c of V row t in LDS: at D = 128 the 128-byte
 // halves of odd rows change places, so that the four rows of a transposing
 // load meet no bank twice more than they must.
@@ -3546,8 +3476,6 @@ extern "C" __global__ __launch_bounds__(256) void lgx_k_lm_rowconst(const lgx_lm
     }
 }
 
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ v8h as_v8h(uint4 u) { return __builtin_bit_cast(v8h, u); }
 
 #define LGX_LMC_RING 4                  // k-steps in flight: the one in use and three ahead
 extern "C" __global__ __launch_bounds__(64 * LGX_LMC_GROUPS) void lgx_k_lm_cert(const lgx_lmc_args a) {

@@ -478,80 +478,6 @@ __device__ __forceinline__ void i8_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi
     hi = __builtin_bit_cast(uint32_t, h);
 }
 
-// Two numbers rounded to binary16 (v_cvt_pk_f16_f32).
-__device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {
-    typedef float v2f __attribute__((ext_vector_type(2)));
-    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){lo, hi}, v2h));
-}
-
-// w minus the low or high half of a pair of binary16 numbers, exact.  (Neither
-// operand may come from a matrix instruction or a v_exp: the compiler puts no wait
-// states ahead of assembly.)
-template <int HI>
-__device__ __forceinline__ float minus_half(float w, uint32_t pair) {
-    float r;
-    if (HI) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(pair), "v"(w));
-    else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(pair), "v"(w));
-    return r;
-}
-
-// tanh: below 0.35 the odd series (the term after the last is under 1.3e-8 of
-// the result), else (1 - t) / (1 + t), t = exp(-2 |x|), where 1 - t > 0.5.
-__device__ __forceinline__ float a8_tanh(float x) {
-    const float ax = fabsf(x), t = __builtin_amdgcn_exp2f(-2.8853900817779268f * ax);
-    const float big = copysignf((1.0f - t) / (1.0f + t), x);
-    const float y = x * x;
-    float p = fmaf(y, -1382.0f / 155925.0f, 62.0f / 2835.0f);
-    p = fmaf(y, p, -17.0f / 315.0f);
-    p = fmaf(y, p, 2.0f / 15.0f);
-    p = fmaf(y, p, -1.0f / 3.0f);
-    return ax < 0.35f ? fmaf(x * y, p, x) : big;
-}
-
-// Joins over the four lanes of a column: the swaps leave a row of 16 lanes beside
-// its neighbour's, then half a wave beside the other.
-__device__ __forceinline__ float col_join16(float v, float& other) {
-    typedef unsigned v2u __attribute__((ext_vector_type(2)));
-    const unsigned x = __float_as_uint(v);
-    const v2u r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    other = __uint_as_float(r[1]);
-    return __uint_as_float(r[0]);
-}
-__device__ __forceinline__ float col_join32(float v, float& other) {
-    typedef unsigned v2u __attribute__((ext_vector_type(2)));
-    const unsigned x = __float_as_uint(v);
-    const v2u r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    other = __uint_as_float(r[1]);
-    return __uint_as_float(r[0]);
-}
-__device__ __forceinline__ float col_max(float v) {
-    float w;
-    v = col_join16(v, w);
-    v = fmaxf(v, w);
-    v = col_join32(v, w);
-    return fmaxf(v, w);
-}
-__device__ __forceinline__ float col_sum(float v) {
-    float w;
-    v = col_join16(v, w);
-    v = v + w;
-    v = col_join32(v, w);
-    return v + w;
-}
-
-// Inclusive sums over the wave's lanes (VALU moves within rows of 16, then of row
-// 0 and 2's last lane into the next row, then of the lower half's into the upper).
-__device__ __forceinline__ int wave_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-    return v;
-}
-
 // What a workgroup of NC columns works on: a sequence, a KV head, a block of
 // columns, and a run of tiles.
 struct A8Block {
