@@ -340,6 +340,135 @@ lgx_status lgx_gqa_prefill_attn_i8(lgx_ctx* ctx, const float* q, const lgx_kv_i8
                                    int32_t hq, int32_t maxp, int32_t max_seq_len, const lgx_attn_opts* opts,
                                    float* out, void* stream);
 
+/* ---- drafted tokens ----
+ * A step that checks several drafted tokens of each sequence at once: the drafts are a
+ * tree of N <= 256 nodes per sequence, node 0 the sequence's last token and every
+ * node's parent before it.  Node j of sequence b is row b*N + j of the calls below, cache
+ * slot seq_len[b] + j, and position seq_len[b] + depth: nodes of one depth share a
+ * position, each has a slot.  n_nodes (device int32 [B], nullable: N) says how many of a
+ * sequence's rows are nodes; the others are padding, for which nothing is read and
+ * whose outputs are left as they are.
+ *   lgx_tree_plan             once per tree: depths, and which nodes each one sees
+ *   lgx_rope_kv_append_rows   per layer: queries rotated, keys and values to the cache
+ *   lgx_gqa_tree_attn         per layer: their attention
+ *   lgx_sample_filtered       the token behind each node
+ *   lgx_tree_accept           the path of nodes whose tokens were picked
+ *   lgx_kv_keep               the path's rows moved together in every layer's cache
+ * No counterpart in the reference. */
+/* A paged binary16 cache (that of lgx_gqa_decode_attn): K and V pages
+ * [num_pages][hkv][16][d], 16-byte aligned; d 64 or 128. */
+typedef struct lgx_kv_f16 {
+    uint16_t* k;
+    uint16_t* v;
+    int32_t num_pages, hkv, d;
+} lgx_kv_f16;
+
+/* depth[b][j] = the number of node j's ancestors; mask[b][j] = ceil(N / 64) words of
+ * which bit i % 64 of word i / 64 is set where node i is node j or its ancestor.
+ * parent [B][N]: the parent's number, below j, or -1 for a node that hangs from the
+ * cached tokens (as does one with any other value). */
+lgx_status lgx_tree_plan(lgx_ctx* ctx, const int32_t* parent, const int32_t* n_nodes, int32_t B, int32_t N,
+                         int32_t* depth, uint64_t* mask, void* stream);
+/* lgx_rope_kv_append of N rows per sequence (any number): row b*N + j of qkv
+ * ([B*N][(hq + 2 hkv) d]: q heads | k heads | v heads), plus bias (nullable), is rotated to
+ * position seq_len[b] + depth[b][j] (depth NULL: j, a run of new tokens), q written to
+ * q_out [B*N][hq][d], k and v rounded to binary16 into slot seq_len[b] + j.  With rot = d and
+ * pairs of halves the bits of lgx_rope_kv_append.  rope as in
+ * lgx_rope_kv_append_i8.  Lengths are clamped to [0, 16 maxp]; tokens past 16 maxp and
+ * pages outside [0, num_pages) are not written.  seq_len is not advanced. */
+lgx_status lgx_rope_kv_append_rows(lgx_ctx* ctx, const float* qkv, const float* bias, const lgx_rope* rope,
+                                   const int32_t* seq_len, const int32_t* depth, const int32_t* n_new,
+                                   const int32_t* page_table, const lgx_kv_f16* kv, float* q_out, int32_t B, int32_t N,
+                                   int32_t hq, int32_t maxp, void* stream);
+/* tokens [B][N]: the nodes' tokens; picked [B][N]: the token chosen behind each node.
+ * From node 0 the path goes on to the lowest child whose token is the one picked behind the
+ * node, and ends where there is none: path[b] = its nodes, then -1; count[b] = their
+ * number, 0 for a sequence without nodes; next[b] = the token picked behind the last
+ * (left as it is without nodes); new_len[b] = seq_len[b] + count[b] (both nullable, and
+ * possibly the same). */
+lgx_status lgx_tree_accept(lgx_ctx* ctx, const int32_t* tokens, const int32_t* parent, const int32_t* picked,
+                           const int32_t* n_nodes, const int32_t* seq_len, int32_t B, int32_t N, int32_t* path,
+                           int32_t* count, int32_t* next, int32_t* new_len, void* stream);
+/* Rows start[b] + keep[b][i], i < n_keep[b] (<= N, any number), of every sequence become
+ * rows start[b] + i, in the caches of all layers (host array of `layers` caches of one shape,
+ * read before the call returns).  keep [B][N] ascends strictly, from 0 on; where it does
+ * not, the sequence's rows from start[b] on hold any of their values.  Rows past 16 maxp
+ * and on pages outside [0, num_pages) stay.  Also drops tokens from the middle of a
+ * cache.  The pages of those rows must be the sequence's own. */
+lgx_status lgx_kv_keep(lgx_ctx* ctx, const lgx_kv_f16* kv, int32_t layers, const int32_t* page_table,
+                       const int32_t* start, const int32_t* keep, const int32_t* n_keep, int32_t B, int32_t N,
+                       int32_t maxp, void* stream);
+
+/* A token for each of m rows of binary32 logits (ld >= vocab elements apart), with settings
+ * per row (device arrays [m], nullable) and a given random number u[i] of [0, 1):
+ *   weights  w_j = exp((l_j - l_max) / temperature); NaN and -inf are never taken
+ *   order    larger logits first, of equal ones (-0 = +0) the lower index
+ *   top_k    the first top_k in that order (0, the default, or less: all)
+ *   top_p    of those the shortest run from the first on that weighs top_p or more of their
+ *            sum, one token at least (1, the default, or more, or NaN: all)
+ *   min_p    of those the tokens with w_j >= min_p (0, the default, or less, or NaN: all;
+ *            above 1: 1)
+ *   draw     of those, by index, the first at which the sum of weights passes u times
+ *            their whole weight
+ * A temperature of 0 (or less, or NaN) takes the first in order.  out[i] = the token,
+ * prob[i] (nullable) = its share of the kept weight.  A row without any token gives 0 and
+ * 0.  u below 0 or NaN counts as 0, from 1 on as the last.  Weights are summed in units of
+ * 2^-42 or in binary64, so that equal inputs give equal tokens in any batch, and a choice
+ * differs from the definition's only where two sums are within about 1e-12 of each
+ * other.  vocab <= 2^20, m <= 65535.  Intermediates live in the ctx workspace. */
+lgx_status lgx_sample_filtered(lgx_ctx* ctx, const float* logits, int64_t ld, int32_t m, int32_t vocab,
+                               const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                               const float* u, int32_t* out, float* prob, void* stream);
+
+/* ---- pages of a cache ----
+ * Bookkeeping for the page tables of the caches above, on the device: ref[page] counts
+ * the table entries that name a page (0: the page is free), and an entry without a
+ * page holds -1 (any value outside [0, num_pages) counts as none).  Tables are int32
+ * [S][maxp]; a page holds 16 tokens.  The entries past ceil(seq_len / 16) of a row are
+ * the row's own or -1: pages are shared through lgx_pages_fork alone, and a
+ * sequence that is cut short gives the rest back (lgx_pages_free).  All results
+ * depend on the inputs alone.  No counterpart in the reference. */
+typedef struct lgx_page_pool {
+    int32_t* ref;         /* device [num_pages] */
+    int32_t num_pages;
+} lgx_page_pool;
+/* Sequence dst[i] becomes a copy of sequence src[i] (device int32 [n], rows of the
+ * table, n <= 1024): the pages that row dst[i] held are given back, it names the pages of
+ * src[i]'s tokens, each with one holder more, and seq_len[dst[i]] = seq_len[src[i]].  No
+ * page is copied; lgx_pages_reserve does that where one is written to.  A source may
+ * occur several times.  A pair is left out whose target is a source of the call or the
+ * target of an earlier pair, or of which a row is not among the S. */
+lgx_status lgx_pages_fork(lgx_ctx* ctx, const lgx_page_pool* pool, int32_t* page_table, int32_t* seq_len,
+                          const int32_t* src, const int32_t* dst, int32_t S, int32_t n, int32_t maxp, void* stream);
+/* Room for need[b] more tokens (device int32, <= 0: none; tokens past 16 maxp get
+ * none) behind the seq_len[b] tokens of each of B <= 1024 sequences, as if they were
+ * served one after the other: where need[b] > 0, every entry without a page among those of
+ * the new tokens gets one, and if the first new token falls into a page that other
+ * entries name too, the sequence leaves that page to them for a new one and (old, new) is
+ * added to copies [B][2]; n_copies[0] of them are written.  New pages are the
+ * lowest free ones in the order of (sequence, entry).  If there are too few, nothing
+ * changes, n_copies[0] is 0 and lacking[0], else 0, says how many more it would take.  The
+ * copies have to be made (lgx_pages_copy) before the old pages change hands again. */
+lgx_status lgx_pages_reserve(lgx_ctx* ctx, const lgx_page_pool* pool, int32_t* page_table, const int32_t* seq_len,
+                             const int32_t* need, int32_t B, int32_t maxp, int32_t* copies, int32_t* n_copies,
+                             int32_t* lacking, void* stream);
+/* Copies page copies[i][0] to page copies[i][1] for i < min(n_copies[0], max_copies)
+ * in every plane: an array of num_pages pages of page_bytes each (a layer's K or V
+ * pages, or an 8-bit cache's scales).  planes: host array, read before the call returns.
+ * No page may be both source and target of a call.  Pairs outside [0, num_pages) are
+ * left out. */
+typedef struct lgx_page_plane {
+    void* data;
+    int64_t page_bytes;
+} lgx_page_plane;
+lgx_status lgx_pages_copy(lgx_ctx* ctx, const lgx_page_plane* planes, int32_t n_planes, int32_t num_pages,
+                          const int32_t* copies, const int32_t* n_copies, int32_t max_copies, void* stream);
+/* Gives back the pages of every row's entries from ceil(keep[b] / 16) on (keep: device
+ * int32 [B], <= 0: all): one holder less each, the entries become -1.  keep[b] = 0 ends
+ * a sequence, seq_len[b] returns what it reserved and did not use. */
+lgx_status lgx_pages_free(lgx_ctx* ctx, const lgx_page_pool* pool, int32_t* page_table, const int32_t* keep, int32_t B,
+                          int32_t maxp, void* stream);
+
 /* ---- range partials (for consumers that fuse the range tree) ---- */
 /* Number of canonical 32-block ranges of K = the partial count of a product. */
 int32_t lgx_q8_range_count(int32_t k);

@@ -103,6 +103,15 @@ SIGNATURES = {
     "lgx_kv_read_i8": (C.c_int, [_P, _P, _P, _P, _I32, _I32, _I32, _P, _P, _P]),
     "lgx_gqa_decode_attn_i8": (C.c_int, [_P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _P, _P, _P]),
     "lgx_gqa_prefill_attn_i8": (C.c_int, [_P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _P]),
+    "lgx_tree_plan": (C.c_int, [_P, _P, _P, _I32, _I32, _P, _P, _P]),
+    "lgx_rope_kv_append_rows": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _P]),
+    "lgx_tree_accept": (C.c_int, [_P, _P, _P, _P, _P, _P, _I32, _I32, _P, _P, _P, _P, _P]),
+    "lgx_kv_keep": (C.c_int, [_P, _P, _I32, _P, _P, _P, _P, _I32, _I32, _I32, _P]),
+    "lgx_sample_filtered": (C.c_int, [_P, _P, C.c_int64, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "lgx_pages_fork": (C.c_int, [_P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _P]),
+    "lgx_pages_reserve": (C.c_int, [_P, _P, _P, _P, _P, _I32, _I32, _P, _P, _P, _P]),
+    "lgx_pages_copy": (C.c_int, [_P, _P, _I32, _I32, _P, _P, _I32, _P]),
+    "lgx_pages_free": (C.c_int, [_P, _P, _P, _P, _I32, _I32, _P]),
 }
 
 # Model shapes of the decode benchmarks (random-init Qwen2.5-0.5B / -7B shaped
@@ -246,6 +255,21 @@ class AttnOptsC(C.Structure):
     _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("window", _I32), ("slopes", _P)]
 
 
+class KvF16C(C.Structure):
+    """lgx_kv_f16."""
+    _fields_ = [("k", _P), ("v", _P), ("num_pages", _I32), ("hkv", _I32), ("d", _I32)]
+
+
+class PagePoolC(C.Structure):
+    """lgx_page_pool."""
+    _fields_ = [("ref", _P), ("num_pages", _I32)]
+
+
+class PagePlaneC(C.Structure):
+    """lgx_page_plane."""
+    _fields_ = [("data", _P), ("page_bytes", C.c_int64)]
+
+
 _lib = None
 
 
@@ -350,6 +374,28 @@ class KvCacheI8(_Held):
                    t.zeros((num_pages, hkv), dtype=t.float32, device=ctx.dev))
 
 
+class KvCacheF16(_Held):
+    """A binary16 paged KV cache (lgx_kv_f16): K and V pages [pages][hkv][16][d], both
+    float16, or both int16 with its bits."""
+
+    def __init__(self, k, v):
+        import torch as t
+
+        if k.dim() != 4 or k.dtype not in (t.float16, t.int16):
+            raise ValueError(f"k is {k.dtype} {tuple(k.shape)}, expected float16 or int16 [pages][hkv][16][d]")
+        n, hkv, _, d = k.shape
+        _tensor("k", k, k.dtype, (n, hkv, 16, d), k.device)
+        _tensor("v", v, k.dtype, (n, hkv, 16, d), k.device)
+        c = KvF16C(k.data_ptr(), v.data_ptr(), n, hkv, d)
+        self._hold(k=k, v=v, num_pages=n, hkv=hkv, d=d, device=k.device, c=c, cstruct=C.byref(c))
+
+    @classmethod
+    def empty(cls, ctx: "Context", num_pages: int, hkv: int, d: int) -> "KvCacheF16":
+        """A cache of zeros on ctx's device."""
+        t = ctx.torch
+        return cls(*(t.zeros((num_pages, hkv, 16, d), dtype=t.float16, device=ctx.dev) for _ in range(2)))
+
+
 class Rope(_Held):
     """Rotation of query and key heads (lgx_rope): cos / sin are float32 device
     tensors [positions][rot / 2], the first rot dimensions of a head are turned in
@@ -391,6 +437,36 @@ class AttnOpts(_Held):
 
             _tensor("slopes", slopes, t.float32, (None,), slopes.device)
         self._hold(slopes=slopes, cstruct=C.byref(AttnOptsC(scale, softcap, window, _ptr_or_none(slopes))))
+
+
+class PagePool(_Held):
+    """The holders of a cache's pages (lgx_page_pool): int32 [pages], 0 for a free page."""
+
+    def __init__(self, ref):
+        import torch as t
+
+        _tensor("ref", ref, t.int32, (None,), ref.device)
+        self._hold(ref=ref, num_pages=ref.shape[0], device=ref.device, cstruct=C.byref(PagePoolC(ref.data_ptr(), ref.shape[0])))
+
+    @classmethod
+    def empty(cls, ctx: "Context", num_pages: int) -> "PagePool":
+        """A pool of free pages on ctx's device."""
+        return cls(ctx.torch.zeros(num_pages, dtype=ctx.torch.int32, device=ctx.dev))
+
+
+class PagePlanes(_Held):
+    """The arrays that a page copy goes over: contiguous tensors [pages][...] of one
+    device, such as every layer's K and V pages and an 8-bit cache's scales."""
+
+    def __init__(self, tensors):
+        tensors = tuple(tensors)
+        if not tensors:
+            raise ValueError("no planes")
+        n, device = tensors[0].shape[0], tensors[0].device
+        for x in tensors:
+            _tensor("a plane", x, x.dtype, (n, *x.shape[1:]), device)
+        array = (PagePlaneC * len(tensors))(*[PagePlaneC(x.data_ptr(), x[0].numel() * x.element_size()) for x in tensors])
+        self._hold(tensors=tensors, num_pages=n, device=device, count=len(tensors), carray=array)
 
 
 class Context:
@@ -695,6 +771,159 @@ class Context:
         if out is None:
             return self.torch.empty_like(q)
         return _tensor("out", out, f32, q.shape, self.dev)
+
+    # ---- drafted tokens --------------------------------------------------
+    def tree_plan(self, parent, n_nodes=None):
+        """(depth [B][N] int32, mask [B][N][ceil(N / 64)] int64) of trees of drafts given by
+        every node's parent [B][N] (-1: hangs from the cached tokens)."""
+        t = self.torch
+        _tensor("parent", parent, t.int32, (None, None), self.dev)
+        B, N = parent.shape
+        if n_nodes is not None:
+            _tensor("n_nodes", n_nodes, t.int32, (B,), self.dev)
+        depth = t.zeros((B, N), dtype=t.int32, device=self.dev)
+        mask = t.zeros((B, N, (N + 63) // 64), dtype=t.int64, device=self.dev)
+        _check(lib().lgx_tree_plan(self.handle, parent.data_ptr(), _ptr_or_none(n_nodes), B, N, depth.data_ptr(),
+                                   mask.data_ptr(), self._s()))
+        return depth, mask
+
+    def rope_kv_append_rows(self, qkv, bias, rope: Rope, seq_len, page_table, kv: KvCacheF16, N: int = 1, depth=None,
+                            n_new=None, q_out=None):
+        """Rotates and appends rows [B*N][(hq + 2 hkv) d] (row b*N + j: slot seq_len[b] + j,
+        position seq_len[b] + depth[b][j], or + j) to the binary16 cache; returns the rotated
+        queries [B*N][hq][d]."""
+        t = self.torch
+        B, maxp = page_table.shape
+        d, hkv = kv.d, kv.hkv
+        rows, width = qkv.shape
+        hq = width // d - 2 * hkv
+        if rows != B * N or hq < 1 or width % d:
+            raise ValueError(f"qkv {tuple(qkv.shape)} is not [{B * N}][(hq + {2 * hkv}) * {d}]")
+        _tensor("qkv", qkv, t.float32, qkv.shape, self.dev)
+        if bias is not None:
+            _tensor("bias", bias, t.float32, (width,), self.dev)
+        if rope.device != self.dev:
+            raise ValueError(f"the rotation's tables are on {rope.device}, the context on {self.dev}")
+        self._lengths(seq_len, n_new, page_table, kv, B)
+        if depth is not None:
+            _tensor("depth", depth, t.int32, (B, N), self.dev)
+        q_out = t.empty((rows, hq, d), dtype=t.float32, device=self.dev) if q_out is None else \
+            _tensor("q_out", q_out, t.float32, (rows, hq, d), self.dev)
+        _check(lib().lgx_rope_kv_append_rows(
+            self.handle, qkv.data_ptr(), _ptr_or_none(bias), rope.cstruct, seq_len.data_ptr(), _ptr_or_none(depth),
+            _ptr_or_none(n_new), page_table.data_ptr(), kv.cstruct, q_out.data_ptr(), B, N, hq, maxp, self._s()))
+        return q_out
+
+    def tree_accept(self, tokens, parent, picked, seq_len=None, n_nodes=None, next_tokens=None):
+        """(path [B][N], count [B], next token [B], seq_len + count or None): the nodes from
+        node 0 on whose tokens were picked behind their parents."""
+        t = self.torch
+        _tensor("tokens", tokens, t.int32, (None, None), self.dev)
+        B, N = tokens.shape
+        _tensor("parent", parent, t.int32, (B, N), self.dev)
+        _tensor("picked", picked, t.int32, (B, N), self.dev)
+        for name, x in (("seq_len", seq_len), ("n_nodes", n_nodes), ("next_tokens", next_tokens)):
+            if x is not None:
+                _tensor(name, x, t.int32, (B,), self.dev)
+        path = t.empty((B, N), dtype=t.int32, device=self.dev)
+        count = t.empty(B, dtype=t.int32, device=self.dev)
+        if next_tokens is None:
+            next_tokens = (t.empty if n_nodes is None else t.zeros)(B, dtype=t.int32, device=self.dev)
+        lens = t.empty(B, dtype=t.int32, device=self.dev) if seq_len is not None else None
+        _check(lib().lgx_tree_accept(self.handle, tokens.data_ptr(), parent.data_ptr(), picked.data_ptr(),
+                                     _ptr_or_none(n_nodes), _ptr_or_none(seq_len), B, N, path.data_ptr(), count.data_ptr(),
+                                     next_tokens.data_ptr(), _ptr_or_none(lens), self._s()))
+        return path, count, next_tokens, lens
+
+    def kv_keep(self, caches, page_table, start, keep, n_keep) -> None:
+        """Rows start[b] + keep[b][i], i < n_keep[b], become rows start[b] + i in every cache
+        (a list of KvCacheF16, one per layer)."""
+        t = self.torch
+        caches = list(caches)
+        if not caches:
+            raise ValueError("no caches")
+        _tensor("keep", keep, t.int32, (page_table.shape[0], None), self.dev)
+        B, N = keep.shape
+        for kv in caches:
+            if kv.device != self.dev:
+                raise ValueError(f"a cache is on {kv.device}, the context on {self.dev}")
+        self._lengths(start, n_keep, page_table, caches[0], B)
+        array = (KvF16C * len(caches))(*[kv.c for kv in caches])
+        _check(lib().lgx_kv_keep(self.handle, array, len(caches), page_table.data_ptr(), start.data_ptr(), keep.data_ptr(),
+                                 n_keep.data_ptr(), B, N, page_table.shape[1], self._s()))
+
+    def sample_filtered(self, logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=None, prob=None):
+        """(tokens [m] int32, their probabilities [m]) of rows of logits [m][vocab] (a row
+        may be longer in memory) by given random numbers u [m] of [0, 1) and per-row settings:
+        float32 [m] temperature, top_p, min_p, int32 [m] top_k."""
+        t = self.torch
+        if logits.dim() != 2 or logits.dtype is not t.float32 or logits.device != self.dev or \
+                (logits.shape[1] > 1 and logits.stride(1) != 1):
+            raise ValueError(f"logits must be float32 rows [m][vocab] on {self.dev}, not {logits.dtype} {tuple(logits.shape)} "
+                             f"on {logits.device}")
+        m, vocab = logits.shape
+        for name, x, dtype in (("u", u, t.float32), ("temperature", temperature, t.float32), ("top_k", top_k, t.int32),
+                               ("top_p", top_p, t.float32), ("min_p", min_p, t.float32)):
+            if x is not None or name == "u":
+                _tensor(name, x, dtype, (m,), self.dev)
+        out = t.empty(m, dtype=t.int32, device=self.dev) if out is None else _tensor("out", out, t.int32, (m,), self.dev)
+        prob = t.empty(m, dtype=t.float32, device=self.dev) if prob is None else \
+            _tensor("prob", prob, t.float32, (m,), self.dev)
+        _check(lib().lgx_sample_filtered(
+            self.handle, logits.data_ptr(), logits.stride(0) if m > 1 else vocab, m, vocab, _ptr_or_none(temperature),
+            _ptr_or_none(top_k), _ptr_or_none(top_p), _ptr_or_none(min_p), u.data_ptr(), out.data_ptr(), prob.data_ptr(),
+            self._s()))
+        return out, prob
+
+    # ---- pages of a cache ------------------------------------------------
+    def _pool(self, pool, page_table, **lengths):
+        if pool.device != self.dev:
+            raise ValueError(f"the pool is on {pool.device}, the context on {self.dev}")
+        i32 = self.torch.int32
+        _tensor("page_table", page_table, i32, (None, None), self.dev)
+        for name, x in lengths.items():
+            _tensor(name, x, i32, (page_table.shape[0],), self.dev)
+
+    def pages_fork(self, pool: PagePool, page_table, seq_len, src, dst) -> None:
+        """Sequence dst[i] becomes a copy of sequence src[i], sharing its pages."""
+        self._pool(pool, page_table, seq_len=seq_len)
+        S, maxp = page_table.shape
+        i32 = self.torch.int32
+        _tensor("src", src, i32, (None,), self.dev)
+        _tensor("dst", dst, i32, src.shape, self.dev)
+        _check(lib().lgx_pages_fork(self.handle, pool.cstruct, page_table.data_ptr(), seq_len.data_ptr(), src.data_ptr(),
+                                    dst.data_ptr(), S, src.shape[0], maxp, self._s()))
+
+    def pages_reserve(self, pool: PagePool, page_table, seq_len, need, out=None):
+        """Room for need[b] tokens behind seq_len[b]: (copies [B][2], n_copies [1],
+        lacking [1]); the copies are pages_copy's."""
+        self._pool(pool, page_table, seq_len=seq_len, need=need)
+        t = self.torch
+        B, maxp = page_table.shape
+        shapes = ((B, 2), (1,), (1,))
+        if out is None:
+            out = tuple(t.zeros(s, dtype=t.int32, device=self.dev) for s in shapes)
+        for name, x, s in zip(("copies", "n_copies", "lacking"), out, shapes, strict=True):
+            _tensor(name, x, t.int32, s, self.dev)
+        _check(lib().lgx_pages_reserve(self.handle, pool.cstruct, page_table.data_ptr(), seq_len.data_ptr(), need.data_ptr(),
+                                       B, maxp, *(x.data_ptr() for x in out), self._s()))
+        return out
+
+    def pages_copy(self, planes: PagePlanes, copies, n_copies) -> None:
+        """Copies page copies[i][0] to copies[i][1], i < n_copies[0], in every plane."""
+        if planes.device != self.dev:
+            raise ValueError(f"the planes are on {planes.device}, the context on {self.dev}")
+        i32 = self.torch.int32
+        _tensor("copies", copies, i32, (None, 2), self.dev)
+        _tensor("n_copies", n_copies, i32, (1,), self.dev)
+        _check(lib().lgx_pages_copy(self.handle, planes.carray, planes.count, planes.num_pages, copies.data_ptr(),
+                                    n_copies.data_ptr(), copies.shape[0], self._s()))
+
+    def pages_free(self, pool: PagePool, page_table, keep) -> None:
+        """Gives back the pages past each sequence's first keep[b] tokens."""
+        self._pool(pool, page_table, keep=keep)
+        B, maxp = page_table.shape
+        _check(lib().lgx_pages_free(self.handle, pool.cstruct, page_table.data_ptr(), keep.data_ptr(), B, maxp, self._s()))
 
     def q8_gemm(self, W: Q8Matrix, xq, xd, y=None):
         t = self.torch

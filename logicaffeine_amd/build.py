@@ -41,7 +41,7 @@ def _run(cmd):
     subprocess.run(cmd, check=True)
 
 
-KERNEL_SOURCES = ["lgx_kernels.hip", "lgx_pages.hip"]
+KERNEL_SOURCES = ["lgx_kernels.hip", "lgx_pages.hip", "lgx_tree.hip", "lgx_filter.hip"]
 BUILD_DIR = os.path.join(HERE, "_build")
 
 
@@ -71,7 +71,8 @@ def build_kernels(only=None) -> str:
 
 
 HOST_SOURCES = ["lgx_host.cpp", "lgx_glue.cpp", "lgx_model.cpp", "lgx_gen.cpp", "lgx_gguf.cpp",
-                "lgx_f16gemm.cpp", "lgx_kv8.cpp", "lgx_pages.cpp"]
+                "lgx_f16gemm.cpp", "lgx_kv8.cpp", "lgx_pages.cpp",
+                "lgx_tree.cpp"]
 
 
 def build_scratch() -> str:

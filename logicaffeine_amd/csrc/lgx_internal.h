@@ -179,7 +179,19 @@ enum Kern {
     K_ATTN8_D128 = K_ATTN8_D64 + 6,
     K_ATTN8_JOIN_D64 = K_ATTN8_D128 + 6,   // + 1: a wave per (row, head)
     K_ATTN8_JOIN_D128 = K_ATTN8_JOIN_D64 + 2,
-    K_COUNT = K_ATTN8_JOIN_D128 + 2
+    K_PAGES_FORK = K_ATTN8_JOIN_D128 + 2,
+    K_PAGES_FREE,
+    K_PAGES_RESERVE,
+    K_PAGES_COPY,
+    K_APPEND_ROWS_D64,
+    K_APPEND_ROWS_D128,
+    K_TREE_PLAN,
+    K_TREE_ACCEPT,
+    K_KV_KEEP_D64,
+    K_KV_KEEP_D128,
+    K_FILTER_SCAN,
+    K_FILTER_PICK,
+    K_COUNT
 };
 inline const char* const kKernelNames[] = {
     "lgx_k_repack_t16", "lgx_k_quantize_q8_0", "lgx_k_q8q8_gemv",
@@ -234,6 +246,9 @@ inline const char* const kKernelNames[] = {
     "lgx_k_attn8_d128_c16", "lgx_k_attn8x_d128_c16", "lgx_k_attn8_d128_c32",
     "lgx_k_attn8x_d128_c32", "lgx_k_attn8_d128_c128", "lgx_k_attn8x_d128_c128",
     "lgx_k_attn8_join_d64", "lgx_k_attn8_joinw_d64", "lgx_k_attn8_join_d128", "lgx_k_attn8_joinw_d128",
+    "lgx_k_pages_fork", "lgx_k_pages_free", "lgx_k_pages_reserve", "lgx_k_pages_copy",
+    "lgx_k_append_rows_d64", "lgx_k_append_rows_d128", "lgx_k_tree_plan", "lgx_k_tree_accept",
+    "lgx_k_kv_keep_d64", "lgx_k_kv_keep_d128", "lgx_k_filter_scan", "lgx_k_filter_pick",
 };
 
 static_assert(sizeof(kKernelNames) / sizeof(kKernelNames[0]) == K_COUNT,

@@ -486,3 +486,114 @@ typedef struct {
 #define LGX_A8_TILE 64         // tokens of a tile: four pages
 #define LGX_A8_UNITS 256       // (sequence, column block) pairs whose tiles are split at most
 #define LGX_A8_MIN 4           // tiles of a split at least
+
+// ---- pages of a cache (lgx_pages.hip) ----
+#define LGX_PAGES_SEQS 1024    // sequences of a reservation at most
+#define LGX_PLANES 128         // planes of a page copy's launch
+typedef struct {
+    int32_t* ref;              // [num_pages] holders of each page
+    int32_t* page_table;       // [S][maxp]
+    int32_t* seq_len;          // [S]
+    const int32_t* src;        // [n]
+    const int32_t* dst;        // [n]
+    int32_t num_pages, S, maxp, n;
+} lgx_fork_args;
+
+typedef struct {
+    int32_t* ref;
+    int32_t* page_table;       // [B][maxp]
+    const int32_t* keep;       // [B] tokens whose pages stay
+    int32_t num_pages, maxp;
+} lgx_pages_free_args;
+
+typedef struct {
+    int32_t* ref;
+    int32_t* page_table;       // [B][maxp]
+    const int32_t* seq_len;    // [B]
+    const int32_t* need;       // [B]
+    int32_t* copies;           // [B][2]
+    int32_t* n_copies;         // [1]
+    int32_t* lacking;          // [1]
+    int32_t* found;            // [min(num_pages, B * maxp)] free pages in order
+    int32_t num_pages, B, maxp;
+} lgx_reserve_args;
+
+typedef struct {
+    char* base[LGX_PLANES];
+    int64_t bytes[LGX_PLANES];  // of a page
+    const int32_t* copies;     // [max][2]
+    const int32_t* n_copies;   // [1]
+    int32_t max, num_pages;
+} lgx_pages_copy_args;
+
+// ---- drafted tokens (lgx_tree.hip) ----
+#define LGX_TREE_NODES 256     // nodes of a sequence's draft tree at most
+// Rows of a binary16 cache: K and V pages [num_pages][hkv][16][d].
+typedef struct {
+    const float* x;            // [B*N][(hq + 2 hkv) d]
+    const float* bias;         // [(hq + 2 hkv) d], nullable
+    const float* cos_t;        // [max_pos][rot / 2]
+    const float* sin_t;
+    const int32_t* seq_len;    // [B]
+    const int32_t* depth;      // [B][N], nullable: row j at depth j
+    const int32_t* n_new;      // [B], nullable: N
+    const int32_t* page_table; // [B][maxp]
+    uint16_t* k;
+    uint16_t* v;
+    float* q_out;              // [B*N][hq][d]
+    int64_t items;             // B * N * (hq + 2 hkv)
+    int32_t N, hq, hkv, maxp, num_pages, max_pos, rot, interleaved;
+    int32_t vec;               // runs of 4 pairs are aligned and of one kind
+} lgx_append_rows_args;
+
+typedef struct {
+    const int32_t* parent;     // [B][N]
+    const int32_t* n_nodes;    // [B], nullable: N
+    int32_t* depth;            // [B][N]
+    uint64_t* mask;            // [B][N][words]
+    int32_t N, words;
+} lgx_tree_plan_args;
+
+typedef struct {
+    const int32_t* tokens;     // [B][N]
+    const int32_t* parent;     // [B][N]
+    const int32_t* picked;     // [B][N]
+    const int32_t* n_nodes;    // [B], nullable: N
+    const int32_t* seq_len;    // [B], nullable
+    int32_t* path;             // [B][N]
+    int32_t* count;            // [B]
+    int32_t* next;             // [B]
+    int32_t* new_len;          // [B], nullable
+    int32_t N;
+} lgx_tree_accept_args;
+
+#define LGX_KEEP_PLANES 128    // K or V arrays of a launch
+typedef struct {
+    uint16_t* base[LGX_KEEP_PLANES];
+    const int32_t* page_table; // [B][maxp]
+    const int32_t* start;      // [B]
+    const int32_t* keep;       // [B][N]
+    const int32_t* n_keep;     // [B]
+    int32_t N, hkv, maxp, num_pages;
+} lgx_kv_keep_args;
+
+// ---- sampling with per-row settings (lgx_filter.hip) ----
+#define LGX_SF_CHUNK 64        // logits whose largest is kept
+#define LGX_SF_SLICE 4096      // logits of a workgroup of the scan
+#define LGX_SF_VOCAB (1 << 20)
+typedef struct {
+    const float* logits;       // [m] rows of vocab, ld apart
+    const float* temperature;  // [m], nullable: 1
+    const int32_t* top_k;      // [m], nullable: 0
+    const float* top_p;        // [m], nullable: 1
+    const float* min_p;        // [m], nullable: 0
+    const float* u;            // [m]
+    int32_t* out;              // [m]
+    float* prob;               // [m], nullable
+    double* sum;               // [m][nslices] of exp((l - slice maximum) / T)
+    float* smax;               // [m][nslices]
+    float* cmax;               // [m][nslices * 64]
+    int64_t ld;
+    int32_t m, vocab, nslices;
+    int32_t vec;               // rows are 16-byte aligned
+} lgx_filter_args;
