@@ -50,6 +50,9 @@ def _compile_kernels(source: str) -> str:
     links whatever it compiles for the device)."""
     stem = os.path.join(BUILD_DIR, os.path.splitext(source)[0])
     _run([os.path.join(ROCM, "bin", "hipcc"), *HIP_FLAGS, "-S", "-I", CSRC, "-o", stem + ".s", os.path.join(CSRC, source)])
+    with open(stem + ".s", "a") as f:
+        # up to the next file's first kernel (256-byte aligned) with s_nop, not with zeros
+        f.write("\n\t.text\n\t.p2alignl 8, 0xbf800000\n")
     _run([os.path.join(ROCM, "llvm", "bin", "clang"), "--target=amdgcn-amd-amdhsa", f"-mcpu={ARCH}", "-c", "-o", stem + ".o",
           stem + ".s"])
     os.remove(stem + ".s")
