@@ -308,7 +308,7 @@ lgx_status lgx_rope_kv_append_i8(lgx_ctx* ctx, const float* qkv, const float* bi
 lgx_status lgx_kv_read_i8(lgx_ctx* ctx, const lgx_kv_i8* kv, const int32_t* page_table, const int32_t* start,
                           int32_t B, int32_t n, int32_t maxp, float* k_out, float* v_out, void* stream);
 
-/* Options of the attention calls below (NULL: none).  The score of a query at
+/* Options of the attention calls below and of lgx_gqa_tree_attn (NULL: none).  The score of a query at
  * position p and a key at t is
  *   s = scale * q.k (scale 0: 1/sqrt(d));  s = softcap * tanh(s / softcap) if
  *   softcap > 0 (2^-100 at least);  s -= slopes[h] * (p - t) if slopes (device
@@ -380,6 +380,22 @@ lgx_status lgx_rope_kv_append_rows(lgx_ctx* ctx, const float* qkv, const float* 
                                    const int32_t* seq_len, const int32_t* depth, const int32_t* n_new,
                                    const int32_t* page_table, const lgx_kv_f16* kv, float* q_out, int32_t B, int32_t N,
                                    int32_t hq, int32_t maxp, void* stream);
+/* Attention of the nodes: out[b*N + j][h] over the first seq_len[b] tokens of sequence b
+ * (clamped to [0, max_seq_len], max_seq_len + N <= 16 maxp) and those nodes i < n_nodes[b] whose
+ * bit is set in mask[b][j] (lgx_tree_plan's words, or any others; NULL: nodes 0 .. j), cache
+ * slots seq_len[b] + i.  opts as above, by positions: node j stands at seq_len[b] +
+ * depth[b][j] (NULL: j; below 0: 0).  q and out [B*N][hq][d], 16-byte aligned; hq/hkv in
+ * 1..16; page ids are clamped to [0, num_pages).  A node that sees nothing gives zeros.  With
+ * N = 1 and neither mask nor depth a decode step whose token is already cached.
+ * Not the canonical schedule: products of binary16 keys and values with queries and
+ * weights of 22 bits (or to 2^-25 of a query row's, 2^-35 of a row's weights' largest),
+ * binary32 sums; 1e-7 to 4e-7 of the 64-bit result, and the same inputs give the same
+ * bits.  What a node does not see may hold anything.  Partial results of long
+ * contexts live in the ctx workspace. */
+lgx_status lgx_gqa_tree_attn(lgx_ctx* ctx, const float* q, const lgx_kv_f16* kv, const int32_t* page_table,
+                             const int32_t* seq_len, const int32_t* n_nodes, const int32_t* depth, const uint64_t* mask,
+                             int32_t B, int32_t N, int32_t hq, int32_t maxp, int32_t max_seq_len,
+                             const lgx_attn_opts* opts, float* out, void* stream);
 /* tokens [B][N]: the nodes' tokens; picked [B][N]: the token chosen behind each node.
  * From node 0 the path goes on to the lowest child whose token is the one picked behind the
  * node, and ends where there is none: path[b] = its nodes, then -1; count[b] = their

@@ -105,6 +105,7 @@ SIGNATURES = {
     "lgx_gqa_prefill_attn_i8": (C.c_int, [_P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _P]),
     "lgx_tree_plan": (C.c_int, [_P, _P, _P, _I32, _I32, _P, _P, _P]),
     "lgx_rope_kv_append_rows": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _P]),
+    "lgx_gqa_tree_attn": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _P]),
     "lgx_tree_accept": (C.c_int, [_P, _P, _P, _P, _P, _P, _I32, _I32, _P, _P, _P, _P, _P]),
     "lgx_kv_keep": (C.c_int, [_P, _P, _I32, _P, _P, _P, _P, _I32, _I32, _I32, _P]),
     "lgx_sample_filtered": (C.c_int, [_P, _P, C.c_int64, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P]),
@@ -813,6 +814,27 @@ class Context:
             self.handle, qkv.data_ptr(), _ptr_or_none(bias), rope.cstruct, seq_len.data_ptr(), _ptr_or_none(depth),
             _ptr_or_none(n_new), page_table.data_ptr(), kv.cstruct, q_out.data_ptr(), B, N, hq, maxp, self._s()))
         return q_out
+
+    def gqa_tree_attn(self, q, kv: KvCacheF16, page_table, seq_len, N: int, max_seq_len: int, mask=None, depth=None,
+                      n_nodes=None, opts: AttnOpts = None, out=None):
+        """q [B*N][hq][d]: row b*N + j is node j of sequence b, whose keys and values are
+        in slot seq_len[b] + j of the binary16 cache; it sees the first seq_len[b] tokens
+        and the nodes of mask [B][N][ceil(N / 64)] (int64 words; None: nodes 0 .. j)."""
+        t = self.torch
+        (B, maxp), (rows, hq, d) = page_table.shape, q.shape
+        if rows != B * N or d != kv.d:
+            raise ValueError(f"q {tuple(q.shape)} is not [{B * N}][hq][{kv.d}]")
+        self._lengths(seq_len, n_nodes, page_table, kv, B)
+        if mask is not None:
+            _tensor("mask", mask, t.int64, (B, N, (N + 63) // 64), self.dev)
+        if depth is not None:
+            _tensor("depth", depth, t.int32, (B, N), self.dev)
+        out = self._attn_out(q, opts, out)
+        _check(lib().lgx_gqa_tree_attn(
+            self.handle, q.data_ptr(), kv.cstruct, page_table.data_ptr(), seq_len.data_ptr(), _ptr_or_none(n_nodes),
+            _ptr_or_none(depth), _ptr_or_none(mask), B, N, hq, maxp, max_seq_len,
+            opts.cstruct if opts is not None else None, out.data_ptr(), self._s()))
+        return out
 
     def tree_accept(self, tokens, parent, picked, seq_len=None, n_nodes=None, next_tokens=None):
         """(path [B][N], count [B], next token [B], seq_len + count or None): the nodes from

@@ -41,7 +41,7 @@ def _run(cmd):
     subprocess.run(cmd, check=True)
 
 
-KERNEL_SOURCES = ["lgx_kernels.hip", "lgx_pages.hip", "lgx_tree.hip", "lgx_filter.hip"]
+KERNEL_SOURCES = ["lgx_kernels.hip", "lgx_pages.hip", "lgx_tree.hip", "lgx_tree_attn.hip", "lgx_filter.hip"]
 BUILD_DIR = os.path.join(HERE, "_build")
 
 

@@ -577,6 +577,30 @@ typedef struct {
     int32_t N, hkv, maxp, num_pages;
 } lgx_kv_keep_args;
 
+typedef struct {
+    const float* q;            // [B*N][hq][d]
+    const uint16_t* k;         // pages [num_pages][hkv][16][d]
+    const uint16_t* v;
+    const int32_t* page_table; // [B][maxp]
+    const int32_t* seq_len;    // [B] cached tokens ahead of the nodes
+    const int32_t* n_nodes;    // [B], nullable: N
+    const int32_t* depth;      // [B][N], nullable: node j at depth j
+    const uint64_t* mask;      // [B][N][words], nullable: nodes 0 .. j
+    const float* slopes;       // [hq], nullable
+    float* out;                // [B*N][hq][d]
+    // per > 0: the tiles of every (sequence, column block) are split on the device so
+    // that `per` workgroups per KV head share all of them (see Tree::place); the
+    // partial results are lgx_k_attn8_join_*'s
+    float* part;               // [per][hkv][columns][d]: results of splits
+    float* ml;                 // [per][hkv][columns][2]: their maxima and sums
+    int32_t* plan;             // [B * ncb][2]: first split, number of splits
+    int32_t N, words, hq, hkv, maxp, num_pages;
+    int32_t maxlen;            // cached tokens at most
+    int32_t window;            // 0: all
+    int32_t per, units, ncb;   // units: B * ncb; ncb: column blocks of a sequence
+    float scale, softcap;
+} lgx_tree_attn_args;
+
 // ---- sampling with per-row settings (lgx_filter.hip) ----
 #define LGX_SF_CHUNK 64        // logits whose largest is kept
 #define LGX_SF_SLICE 4096      // logits of a workgroup of the scan

@@ -26,9 +26,105 @@ lgx_status check_tree(int32_t B, int32_t N) {
     return LGX_OK;
 }
 
+// Launch over B sequences.  Where there are fewer (sequence, KV head, column block)s
+// than compute units, their tiles are split among that many workgroups; the splitting
+// itself is done on the device, by the lengths.  The joining of the splits is that of
+// the 8-bit cache's attention.
+lgx_status run_tree(lgx_ctx* c, lgx_tree_attn_args& a, int B, int d, bool x, void* stream) {
+    const int64_t cols = (int64_t)a.N * (a.hq / a.hkv), heads = (int64_t)B * a.hkv;
+    // the most tiles that a sequence's nodes can see
+    int64_t tiles = cdiv((int64_t)a.maxlen + a.N, LGX_A8_TILE);
+    if (a.window) tiles = std::min<int64_t>(tiles, ((int64_t)a.window + a.N) / LGX_A8_TILE + 2);
+    int nc = c->tree_cols ? c->tree_cols : cols <= 16 ? 16 : cols <= 64 ? 64 : 128;
+    nc = x && d == 128 ? std::min(nc, 64) : nc;
+    const int64_t ncb = (cols + nc - 1) / nc, units = B * ncb, blocks = heads * ncb;
+    a.ncb = (int)ncb;
+    const int64_t per = (int64_t)c->attn8_wgs * c->ncu / a.hkv;
+    const bool split = tiles > LGX_A8_MIN && units <= LGX_A8_UNITS && units < per;
+    lgx_status st;
+    if (split) {
+        const int64_t slots = per * a.hkv * nc;
+        float* ws = nullptr;
+        if ((st = ensure_ws(c, (size_t)(slots * (d + 2) + 2 * units) * sizeof(float), stream, &ws)) != LGX_OK) return st;
+        a.per = (int)per;
+        a.units = (int)units;
+        a.part = ws;
+        a.ml = ws + slots * d;
+        a.plan = (int32_t*)(a.ml + 2 * slots);
+    }
+    const int64_t grid = split ? per * a.hkv : blocks;
+    if (grid > UINT32_MAX / 256) return fail(LGX_OUT_OF_BOUNDS, "attention of %lld workgroups", (long long)grid);
+    const int k = (d == 64 ? K_TREE_ATTN_D64 : K_TREE_ATTN_D128) + (nc == 16 ? 0 : nc == 64 ? 2 : 4) + (x ? 1 : 0);
+    if ((st = launch(c, (Kern)k, dim3((unsigned)grid), dim3(256), a, stream)) != LGX_OK || !split) return st;
+    lgx_attn8_args j{};
+    j.part = a.part;
+    j.ml = a.ml;
+    j.plan = a.plan;
+    j.out = a.out;
+    j.n_new = a.n_nodes;
+    j.P = a.N;
+    j.hq = a.hq;
+    j.hkv = a.hkv;
+    j.ncb = a.ncb;
+    j.cols = nc;
+    j.rows = B * a.N;
+    const int64_t rh = (int64_t)j.rows * a.hq;
+    const int w = rh >= 8 * (int64_t)c->ncu ? 1 : 0;
+    return launch(c, (Kern)((d == 64 ? K_ATTN8_JOIN_D64 : K_ATTN8_JOIN_D128) + w), dim3(w ? cdiv(rh, 4) : (unsigned)rh),
+                  dim3(256), j, stream);
+}
+
 }  // namespace
 
 extern "C" {
+
+lgx_status lgx_gqa_tree_attn(lgx_ctx* c, const float* q, const lgx_kv_f16* kv, const int32_t* page_table,
+                             const int32_t* seq_len, const int32_t* n_nodes, const int32_t* depth, const uint64_t* mask,
+                             int32_t B, int32_t N, int32_t hq, int32_t maxp, int32_t max_seq_len, const lgx_attn_opts* opts,
+                             float* out, void* stream) {
+    return guarded(__func__, [&]() -> lgx_status {
+        lgx_status st = enter(c);
+        if (st != LGX_OK) return st;
+        if ((st = check_kv(kv, maxp)) != LGX_OK) return st;
+        if (!q || !page_table || !seq_len || !out) return fail(LGX_NULL_POINTER, "NULL tensor pointer");
+        if ((st = check_tree(B, N)) != LGX_OK) return st;
+        if (hq <= 0 || hq % kv->hkv != 0) return fail(LGX_INVALID_ARGUMENT, "hq=%d hkv=%d", hq, kv->hkv);
+        if (hq / kv->hkv > 16) return fail(LGX_UNSUPPORTED, "%d query heads per KV head (1..16)", hq / kv->hkv);
+        if (max_seq_len < 0 || max_seq_len > maxp * LGX_PAGE - N)
+            return fail(LGX_OUT_OF_BOUNDS, "max_seq_len %d outside [0, %d]", max_seq_len, maxp * LGX_PAGE - N);
+        if ((int64_t)B * N * hq > INT32_MAX / 128) return fail(LGX_OUT_OF_BOUNDS, "B*N*hq too large");
+        if (!aligned16(q) || !aligned16(out)) return fail(LGX_INVALID_ARGUMENT, "q and out must be 16-byte aligned");
+        lgx_tree_attn_args a{};
+        a.scale = (float)(1.0 / std::sqrt((double)kv->d));
+        if (opts) {
+            if (!std::isfinite(opts->scale) || !std::isfinite(opts->softcap) ||
+                (opts->softcap != 0.0f && !(opts->softcap >= 0x1p-100f)) || opts->window < 0)
+                return fail(LGX_INVALID_ARGUMENT, "scale %g, softcap %g, window %d", (double)opts->scale,
+                            (double)opts->softcap, opts->window);
+            if (opts->scale != 0.0f) a.scale = opts->scale;
+            a.softcap = opts->softcap;
+            a.window = opts->window;
+            a.slopes = opts->slopes;
+        }
+        a.q = q;
+        a.k = kv->k;
+        a.v = kv->v;
+        a.page_table = page_table;
+        a.seq_len = seq_len;
+        a.n_nodes = n_nodes;
+        a.depth = depth;
+        a.mask = mask;
+        a.out = out;
+        a.N = N;
+        a.words = (N + 63) / 64;
+        a.hq = hq;
+        a.hkv = kv->hkv;
+        a.maxp = maxp;
+        a.num_pages = kv->num_pages;
+        a.maxlen = max_seq_len;
+        return run_tree(c, a, B, kv->d, a.softcap > 0.0f || a.window > 0 || a.slopes != nullptr || a.scale < 0.0f, stream);
+    });
+}
 
 lgx_status lgx_rope_kv_append_rows(lgx_ctx* c, const float* qkv, const float* bias, const lgx_rope* rope,
                                    const int32_t* seq_len, const int32_t* depth, const int32_t* n_new,

@@ -198,19 +198,21 @@ __device__ __forceinline__ void kv_keep_body(const lgx_kv_keep_args& a) {
     };
     for (int i0 = 0; i0 < n; i0 += RW * U) {
         uint4 v[U];
-        uint4* to[U];
+        bool on[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * RW + lane / CH;
             const int from = i < n ? keep[i] : -1;
-            uint4* src = from >= 0 && from != i ? at(start + from) : nullptr;
-            to[u] = src ? at(start + i) : nullptr;
-            if (to[u]) v[u] = *src;
+            const uint4* src = from >= 0 && from != i ? at(start + from) : nullptr;
+            on[u] = src != nullptr;
+            v[u] = on[u] ? *src : make_uint4(0u, 0u, 0u, 0u);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // every row is read before one is written
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (to[u]) *to[u] = v[u];
+        for (int u = 0; u < U; ++u) {
+            uint4* dst = on[u] ? at(start + i0 + u * RW + lane / CH) : nullptr;
+            if (dst) *dst = v[u];
+        }
     }
 }
 extern "C" __global__ __launch_bounds__(256) void lgx_k_kv_keep_d64(const lgx_kv_keep_args a) { kv_keep_body<64>(a); }

@@ -1,0 +1,669 @@
+// lgx_tree_attn.hip -- attention of a tree of drafted tokens over the paged binary16
+// cache.
+#include "lgx_device.h"
+
+// ---------------------------------------------------------------------------
+// Sequence b has sl cached tokens and n nodes behind them, token sl + i being node i.  Node
+// j stands at position sl + depth[j] and sees the cached tokens (within the window,
+// if there is one) and the nodes of its mask.  The (node, query head) pairs of one
+// KV head are the columns of the products, 16 to a matrix instruction; a tile is 64
+// tokens, four pages.
+//   scores   S^T[token][column] = K . Q^T on v_mfma_f32_16x16x32_f16.  q is scaled by a
+//            power of two that brings its row's largest value to 2^14 .. 2^15 and is
+//            the sum of two binary16 numbers, 22 bits (2^-25 of the row's largest where
+//            it is far below): two products.
+//   softmax  running maximum and sum per column, in base 2, binary32.
+//   PV       O^T[dim][column] += V^T . P^T on the same instruction: a weight times 2^10 is
+//            the sum of two binary16 numbers, 22 bits, or to 2^-35 of the largest where it
+//            is smaller.  The matrix unit sums a tile, the VALU the tiles.
+// So the results are as exact as binary32 products would be, 1e-7 to 4e-7 of the 64-bit
+// result: a draft is accepted by what a decode step would have said, not by its rounding.
+//
+// Lane (column, kg) gets the scores of tokens 16 u + 4 kg + 0..3 of sub-tile u, and V's
+// transposing LDS loads give lane (dimension, kg) the same four tokens of it: two
+// sub-tiles' weights are the 8 values of a PV operand as they stand.
+//
+// A token that a column does not see has weight 0 and may hold anything: K's score is
+// replaced; V rows behind the last node are cleared; and an infinity or a NaN among the
+// others, which 0 would not hide, leaves a result that is not finite, upon which the
+// column is done over token by token (tree_column).
+// ---------------------------------------------------------------------------
+typedef __attribute__((address_space(3))) uint16_t lds_u16;
+typedef __attribute__((address_space(4))) const int32_t const_i32;
+
+#define TREE_TILE 64
+#define TREE_MIN 4             // tiles of a split at least
+#define TREE_UP 10             // weights as operands: times 2^10
+
+// What a workgroup works on: a sequence, a KV head, a block of NC columns, a run of tiles.
+template <int NC>
+struct Tree {
+    const lgx_tree_attn_args& a;
+    int b, g, G, c0, ncols, sl, n;
+    int tb0, tb1;              // tiles
+    int unit;                  // b * ncb + column block
+    int pos, ns;               // place among all splits, and splits of the unit
+
+    __device__ __forceinline__ int nodes(int b) const { return a.n_nodes ? min(max(a.n_nodes[b], 0), a.N) : a.N; }
+    __device__ __forceinline__ int length(int b) const { return min(max(a.seq_len[b], 0), a.maxlen); }
+    // first and last + 1 tile that a sequence's nodes can see (depths are not negative)
+    __device__ __forceinline__ int2 tiles(int sl, int n) const {
+        const int first = a.window ? max((int)max((int64_t)sl - a.window + 1, (int64_t)0), 0) : 0;
+        return make_int2(first / TREE_TILE, (sl + n + TREE_TILE - 1) / TREE_TILE);
+    }
+    // false: nothing to do.  With a.per all units' tiles go in about equal runs to the
+    // workgroups: every wave computes the run length from all lengths (four units per
+    // lane), nearly the least with which all runs fit into a.per per KV head, then
+    // finds the unit and the run of this workgroup in the sums over the units.
+    __device__ __forceinline__ bool place() {
+        G = a.hq / a.hkv;
+        int s = 0, run = 0;
+        if (a.per) {
+            const int lane = threadIdx.x & 63;
+            pos = __builtin_amdgcn_readfirstlane(blockIdx.x / a.hkv);
+            g = blockIdx.x - pos * a.hkv;
+            int t[4], len[4], cnt[4], all = 0;    // tiles of the lane's units; -1: no such columns
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int u = 4 * lane + i, uc = min(u, a.units - 1), bb = uc / a.ncb;
+                cnt[i] = nodes(bb);
+                len[i] = length(bb);
+                const int2 tt = tiles(len[i], cnt[i]);
+                t[i] = u < a.units && (uc - bb * a.ncb) * NC < cnt[i] * G ? tt.y - tt.x : -1;
+                all += max(t[i], 0);
+            }
+            const int total = __builtin_amdgcn_readlane(wave_scan(all), 63);
+            run = max(TREE_MIN, (int)((unsigned)(total + a.per - 1) / (unsigned)a.per));
+            int m[4], upto;
+            for (;;) {
+                int c = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    m[i] = t[i] < 0 ? 0 : max((int)((unsigned)(t[i] + run - 1) / (unsigned)run), 1);
+                    c += m[i];
+                }
+                upto = wave_scan(c);
+                if (__builtin_amdgcn_readlane(upto, 63) <= a.per) break;
+                run += max(1, run >> 4);          // ends: a.per >= a.units
+            }
+            const uint64_t past = __builtin_amdgcn_ballot_w64(upto > pos);
+            if (!past) return false;
+            const int at = __builtin_ctzll(past);
+            s = pos - __builtin_amdgcn_readlane(upto - (m[0] + m[1] + m[2] + m[3]), at);
+            int i = 0;
+#pragma unroll
+            for (int q = 0; q < 3; ++q) {
+                const int mq = __builtin_amdgcn_readlane(m[q], at);
+                const bool next = i == q && s >= mq;
+                s -= next ? mq : 0;
+                i += next ? 1 : 0;
+            }
+            auto pick = [&](const int (&v)[4]) {
+                const int v0 = __builtin_amdgcn_readlane(v[0], at), v1 = __builtin_amdgcn_readlane(v[1], at);
+                const int v2 = __builtin_amdgcn_readlane(v[2], at), v3 = __builtin_amdgcn_readlane(v[3], at);
+                return i == 0 ? v0 : i == 1 ? v1 : i == 2 ? v2 : v3;
+            };
+            ns = pick(m);
+            sl = pick(len);
+            n = pick(cnt);
+            unit = 4 * at + i;
+            if (s == 0 && g == 0 && threadIdx.x == 0) {
+                a.plan[2 * unit] = pos;
+                a.plan[2 * unit + 1] = ns;
+            }
+        } else {
+            // column blocks side by side: they share K and V
+            const int bg = blockIdx.x / a.ncb, cb = blockIdx.x - bg * a.ncb;
+            const int bb = bg / a.hkv;
+            g = __builtin_amdgcn_readfirstlane(bg - bb * a.hkv);
+            unit = __builtin_amdgcn_readfirstlane(bb * a.ncb + cb);
+            pos = 0;
+            ns = 1;
+        }
+        b = __builtin_amdgcn_readfirstlane(unit / a.ncb);
+        c0 = (unit - b * a.ncb) * NC;
+        if (!a.per) {
+            n = __builtin_amdgcn_readfirstlane(nodes(b));
+            sl = __builtin_amdgcn_readfirstlane(length(b));
+        }
+        ncols = n * G;
+        if (c0 >= ncols) return false;
+        const int2 t = tiles(sl, n);
+        tb0 = t.x + s * run;
+        tb1 = a.per ? min(t.y, tb0 + run) : t.y;
+        return true;
+    }
+    __device__ __forceinline__ int64_t row(int c) const { return (int64_t)b * a.N + c / G; }
+    __device__ __forceinline__ int64_t orow(int c) const { return row(c) * a.hq + g * G + c % G; }
+    __device__ __forceinline__ int depth(int i) const { return a.depth ? max(a.depth[(int64_t)b * a.N + i], 0) : i; }
+    // bit i: node j sees token t0 + i (but for a window among the nodes: in_window)
+    __device__ __forceinline__ uint64_t sees(int t0, int j, int dj) const {
+        const int base = t0 - sl;                 // node of bit 0
+        uint64_t m = 0;
+        if (base < 0) {
+            m = base <= -64 ? ~0ull : (1ull << -base) - 1;
+            const int64_t lo = a.window ? (int64_t)sl + dj - a.window + 1 - t0 : 0;
+            if (lo > 0) m = lo >= 64 ? 0 : m & ~0ull << lo;
+        }
+        if (base > -64) {
+            const int end = (a.mask ? n : j + 1) - base;   // bits from here on are no nodes
+            uint64_t d = ~0ull;
+            if (a.mask) {
+                const uint64_t* w = a.mask + row(j * G) * a.words;
+                if (base < 0) {
+                    d = w[0] << -base;
+                } else {
+                    const int i = base >> 6, s = base & 63;
+                    d = i < a.words ? w[i] >> s : 0;
+                    if (s && i + 1 < a.words) d |= w[i + 1] << (64 - s);
+                }
+            } else if (base < 0) {
+                d <<= -base;
+            }
+            m |= end >= 64 ? d : end > 0 ? d & ((1ull << end) - 1) : 0;
+        }
+        return m;
+    }
+    // position of the column's node less that of token t
+    __device__ __forceinline__ int back(int t, int dj) const { return t < sl ? sl + dj - t : dj - depth(min(t - sl, n - 1)); }
+};
+
+// One column: q's scale, the ALiBi slope, its node and depth; running maximum (base 2) and sum.
+struct TreeCol {
+    float f, slope, m, l;
+    int j, dj;
+};
+struct TreeEdge { static constexpr bool value = true; };
+struct TreeWhole { static constexpr bool value = false; };
+
+// The query of a lane's column in two binary16 parts, dimensions 32 s + 8 kg .. in step s;
+// the factor that makes a score (in base 2 unless X) of a product.
+template <int D, bool X>
+__device__ __forceinline__ float tree_query(const lgx_tree_attn_args& a, const float* qr, v8h (&qh)[2][D / 32]) {
+    constexpr int NS = D / 32;
+    float x[NS][8], am = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            const float4 v = *(const float4*)(qr + 32 * s + e);
+            x[s][e] = v.x;
+            x[s][e + 1] = v.y;
+            x[s][e + 2] = v.z;
+            x[s][e + 3] = v.w;
+        }
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            am = fmaxf(am, fabsf(x[s][e]));
+            bad = bad || !(fabsf(x[s][e]) < __builtin_inff());
+        }
+    am = col_max(am);
+    const bool isbad = col_max(bad ? 1.0f : 0.0f) != 0.0f;
+    // a power of two; up to 2^122, where scale / up is still a normal number
+    const float up = __uint_as_float(__float_as_uint(fminf(32768.0f / am, 0x1p122f)) & 0x7f800000u);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        uint32_t hw[4], lw[4];
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const float y0 = isbad ? 0.0f : x[s][e] * up, y1 = isbad ? 0.0f : x[s][e + 1] * up;
+            hw[e / 2] = f16_pair(y0, y1);
+            lw[e / 2] = f16_pair(minus_half<0>(y0, hw[e / 2]), minus_half<1>(y1, hw[e / 2]));
+        }
+        qh[0][s] = as_v8h(make_uint4(hw[0], hw[1], hw[2], hw[3]));
+        qh[1][s] = as_v8h(make_uint4(lw[0], lw[1], lw[2], lw[3]));
+    }
+    return isbad ? __builtin_nanf("") : a.scale / up * (X ? 1.0f : 1.44269504088896341f);
+}
+
+// From the products of a column tile to its weights as operands; o is brought to the new
+// reference where it moves.  EDGE: some column does not see the whole tile, or the scores
+// are capped, biased or windowed (X).  S[4 u + v]: token t0 + 16 u + 4 kg + v.
+template <bool X, bool EDGE, int ND, class W>
+__device__ __forceinline__ void tree_weights(const W& w, float (&S)[16], TreeCol& k, int t0, int kg, v8h (&ph)[2], v8h (&pl)[2],
+                                             v4f (&o)[ND]) {
+    static_assert(EDGE || !X, "other scores are formed ahead of the maximum");
+    constexpr float kLog2e = 1.44269504088896341f;
+    const lgx_tree_attn_args& a = w.a;
+    const float inf = __builtin_inff();
+    if (EDGE) {
+        const uint64_t sees = w.sees(t0, k.j, k.dj) >> (4 * kg);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) S[e] *= k.f;
+        if constexpr (X) {
+            if (a.softcap > 0.0f) {
+                const float inv = 1.0f / a.softcap;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) S[e] = a.softcap * a8_tanh(S[e] * inv);
+            }
+            const bool tree = t0 + TREE_TILE > w.sl;   // uniform: nodes among the tokens
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int t = t0 + 16 * (e >> 2) + 4 * kg + (e & 3);
+                const int back = tree ? w.back(t, k.dj) : w.sl + k.dj - t;
+                S[e] = (S[e] - k.slope * (float)back) * kLog2e;
+                if (tree && a.window && back >= a.window) S[e] = -inf;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (!(sees >> (16 * (e >> 2) + (e & 3)) & 1)) S[e] = -inf;
+    }
+    float m = fmaxf(fmaxf(S[0], S[1]), S[2]);
+#pragma unroll
+    for (int e = 3; e < 15; e += 2) m = fmaxf(fmaxf(m, S[e]), S[e + 1]);
+    m = fmaxf(m, S[15]);
+    if (!EDGE) m *= k.f;                          // > 0 or NaN
+    const float mt = col_max(m);
+    // the reference moves when a maximum passes it by more than 2^4: most tiles leave
+    // what was summed as it is
+    const bool moves = mt > k.m + 4.0f;
+    if (__builtin_amdgcn_ballot_w64(moves)) {
+        const float mn = moves ? mt : k.m;
+        const float down = k.m == -inf ? 0.0f : __builtin_amdgcn_exp2f(k.m - mn);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[i] *= down;
+        k.l *= down;
+        k.m = mn;
+    }
+    const float off = k.m == -inf ? 0.0f : -k.m;  // nothing seen yet: weights of 0
+    float ps = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        S[e] = __builtin_amdgcn_exp2f(EDGE ? S[e] + off : fmaf(S[e], k.f, off));
+        ps += S[e];
+        S[e] *= (float)(1 << TREE_UP);
+    }
+    k.l += ps;
+    uint32_t hw[8], lw[8];
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+        const uint32_t h = f16_pair(S[e], S[e + 1]);
+        hw[e >> 1] = h;
+        lw[e >> 1] = f16_pair(minus_half<0>(S[e], h), minus_half<1>(S[e + 1], h));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        ph[i] = as_v8h(make_uint4(hw[4 * i], hw[4 * i + 1], hw[4 * i + 2], hw[4 * i + 3]));
+        pl[i] = as_v8h(make_uint4(lw[4 * i], lw[4 * i + 1], lw[4 * i + 2], lw[4 * i + 3]));
+    }
+}
+
+// Column c over its run of tiles, token by token, by one wave: only seen tokens are
+// multiplied.  m, l: the column's reference and sum.
+template <int D, bool X, class W>
+__device__ void tree_column(const W& w, int c, float m, float l, float* dst) {
+    constexpr float kLog2e = 1.44269504088896341f;
+    const lgx_tree_attn_args& a = w.a;
+    const int lane = threadIdx.x & 63, j = c / w.G, dj = w.depth(j);
+    const float* q = a.q + w.orow(c) * D;
+    const float slope = X && a.slopes ? a.slopes[w.g * w.G + c % w.G] : 0.0f;
+    float o[D / 64] = {};
+    for (int t0 = w.tb0 * TREE_TILE; t0 < w.tb1 * TREE_TILE; t0 += 64) {
+        const int t = t0 + lane;
+        const int page = min(max(a.page_table[(int64_t)w.b * a.maxp + min(t / LGX_PAGE, a.maxp - 1)], 0), a.num_pages - 1);
+        const int64_t at = (((int64_t)page * a.hkv + w.g) * LGX_PAGE + t % LGX_PAGE) * D;
+        bool on = w.sees(t0, j, dj) >> lane & 1;
+        float s = 0.0f;
+        if (on) {
+            for (int i = 0; i < D; ++i) s = fmaf(q[i], h2f(a.k[at + i]), s);
+            s *= a.scale;
+            if (X) {
+                if (a.softcap > 0.0f) s = a.softcap * a8_tanh(s / a.softcap);
+                const int back = w.back(t, dj);
+                s -= slope * (float)back;
+                on = !a.window || back < a.window;
+            }
+            s = __builtin_amdgcn_exp2f(s * kLog2e - m);
+        }
+        uint64_t todo = __builtin_amdgcn_ballot_w64(on);
+        while (todo) {
+            const int i = __builtin_ctzll(todo);
+            todo &= todo - 1;
+            const float wt = __shfl(s, i, 64);
+            const int64_t vat = __shfl((long long)at, i, 64);
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e) o[e] = fmaf(wt, h2f(a.v[vat + 64 * e + lane]), o[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) dst[64 * e + lane] = o[e] / l;
+}
+
+// A column's result, or its split's (divided by the split's own sum of weights).
+template <int D, int NC, bool X, class W>
+__device__ __forceinline__ void tree_store(const W& w, int c, const TreeCol& k, int kg, const v4f (&o)[D / 16]) {
+    const lgx_tree_attn_args& a = w.a;
+    const bool part = w.ns > 1, on = c < w.ncols;
+    const int64_t at = part ? ((int64_t)w.pos * a.hkv + w.g) * NC + c - w.c0 : w.orow(on ? c : 0);
+    float* dst = (part ? a.part : a.out) + at * D;
+    const float r = k.l == 0.0f ? 0.0f : 1.0f / (k.l * (float)(1 << TREE_UP));   // nothing seen gives zeros
+    bool bad = false;
+    if (on) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            const v4f x = o[i] * r;
+            *(float4*)(dst + 16 * i + 4 * kg) = make_float4(x[0], x[1], x[2], x[3]);
+            bad = bad || !(fabsf(x[0]) + fabsf(x[1]) + fabsf(x[2]) + fabsf(x[3]) < __builtin_inff());
+        }
+        if (part && kg == 0) *(float2*)(a.ml + 2 * at) = make_float2(k.m, k.l);
+    }
+    uint64_t again = __builtin_amdgcn_ballot_w64(bad && k.l == k.l);
+    again = (again | again >> 16 | again >> 32 | again >> 48) & 0xffff;
+    if (again) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the first results are written
+    while (again) {
+        const int i = __builtin_ctzll(again);
+        again &= again - 1;
+        tree_column<D, X>(w, __shfl(c, i, 64), __shfl(k.m, i, 64), __shfl(k.l, i, 64),
+                          (float*)__shfl((unsigned long long)(uintptr_t)dst, i, 64));
+    }
+}
+
+// V operands of dimensions 16 i .. from the LDS rows of a tile: tokens of sub-tiles 2 h and
+// 2 h + 1.  Lane (col, kg) loads token 16 u + 4 kg + col / 4, dimensions 16 i + 4 (col % 4) ..,
+// and receives dimension 16 i + col of tokens 16 u + 4 kg .. + 3.  Pieces of a row change
+// places by the token, so that the rows of a load fall on different banks.
+template <int D>
+struct TreeV {
+    static constexpr int CH = D / 8, SW = CH / 2 - 1;
+    static __device__ __forceinline__ int piece(int t, int c) { return c ^ ((t & SW) << 1); }
+    static __device__ __forceinline__ v8h operand(const lds_u16* v, int i, int h, int col, int kg) {
+        uint2 x[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int t = 16 * (2 * h + u) + 4 * kg + (col >> 2);
+            x[u] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                 (lds_v4s*)(v + t * D + piece(t, 2 * i + ((col >> 1) & 1)) * 8 + (col & 1) * 4)));
+        }
+        return as_v8h(make_uint4(x[0].x, x[0].y, x[1].x, x[1].y));
+    }
+};
+// Its K operands: row (token) 16 u + col, dimensions 32 s + 8 kg ..
+template <int D>
+struct TreeK {
+    static constexpr int CH = D / 8;
+    static __device__ __forceinline__ int piece(int t, int c) { return c ^ (t & (CH - 1)); }
+    static __device__ __forceinline__ v8h operand(const lds_u16* k, int u, int s, int col, int kg) {
+        typedef __attribute__((address_space(3))) const u32x4 lds_u4;
+        const int t = 16 * u + col;
+        return __builtin_bit_cast(v8h, *(lds_u4*)(k + t * D + piece(t, 4 * s + kg) * 8));
+    }
+};
+
+// Page numbers of a tile, through the scalar cache.
+template <class W>
+struct TreePages {
+    int p[4];
+    __device__ __forceinline__ TreePages(const W& w, int t) {
+        const_i32* table = (const_i32*)(w.a.page_table + (int64_t)w.b * w.a.maxp);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) p[u] = table[min(4 * t + u, w.a.maxp - 1)];
+    }
+    __device__ __forceinline__ int64_t block(const W& w, int u, int d) const {
+        return ((int64_t)min(max(p[u], 0), w.a.num_pages - 1) * w.a.hkv + w.g) * (LGX_PAGE * d);
+    }
+};
+
+// 16 columns per workgroup (single tokens and few drafts): its four waves take the
+// tiles in turn, K straight into registers, V into the wave's LDS: the next tile's K is in
+// flight from the end of the scores on, its V from the end of the PV product; at the end
+// the waves' results are joined in LDS.
+template <int D, bool X>
+__device__ __forceinline__ void tree_narrow_body(const lgx_tree_attn_args& a) {
+    constexpr int WT = 4, NS = D / 32, ND = D / 16, CH = D / 8;
+    constexpr int TPI = 64 / CH, NI = TREE_TILE / TPI;   // tokens of a 1 KiB load, loads of a tile
+    __shared__ __align__(16) uint16_t v_s[WT][TREE_TILE * D];
+    static_assert(sizeof(v_s) >= WT / 2 * (ND * 64 * sizeof(v4f) + 2 * 64 * sizeof(float)), "the join's share");
+    const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
+    const int wt = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    typedef Tree<16> W;
+    typedef TreePages<W> Pages;
+    W w{a};
+    if (!w.place()) return;                       // uniform
+    uint4 kw[4][NS];
+    auto load_k = [&](const Pages& p) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint16_t* base = a.k + p.block(w, u, D);
+#pragma unroll
+            for (int s = 0; s < NS; ++s) kw[u][s] = *(const uint4*)(base + (col * D + 8 * kg + 32 * s));
+        }
+    };
+    lds_u16* const vb = (lds_u16*)v_s[wt];
+    auto load_v = [&](const Pages& p) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const uint16_t* base = a.v + p.block(w, i * TPI / LGX_PAGE, D);
+            const int r = i * TPI % LGX_PAGE + lane / CH;
+            __builtin_amdgcn_global_load_lds((const void*)(base + (r * D + TreeV<D>::piece(r, lane % CH) * 8)),
+                                             (lds_void*)(vb + i * 512), 16, 0, 0);
+        }
+    };
+    int t = w.tb0 + wt;
+    const int end = w.tb1, T = w.sl + w.n;
+    // Loads are issued whether or not there is such a tile (the wave's last one's again)
+    const int mine = end - 1 - t >= 0 ? t + (end - 1 - t) / WT * WT : t;
+    Pages p(w, t);
+    load_k(p);
+    load_v(p);
+    p = Pages(w, min(t + WT, mine));
+    __builtin_amdgcn_sched_barrier(0);
+    v4f o[ND];
+#pragma unroll
+    for (int i = 0; i < ND; ++i) o[i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    TreeCol k;
+    v8h qh[2][NS];
+    {
+        const int c = min(w.c0 + col, w.ncols - 1);   // columns past the last repeat it
+        k = {0.0f, X && a.slopes ? a.slopes[w.g * w.G + c % w.G] : 0.0f, -__builtin_inff(), 0.0f, c / w.G, 0};
+        k.dj = w.depth(k.j);
+        k.f = tree_query<D, X>(a, a.q + w.orow(c) * D + 8 * kg, qh);
+    }
+    auto tile = [&](auto form) __attribute__((always_inline)) {
+        constexpr bool edge = decltype(form)::value;
+        const int t0 = t * TREE_TILE;
+        const Pages pn = p;
+        v8h ph[2], pl[2];
+        float S[16];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int part = 1; part >= 0; --part)
+#pragma unroll
+                for (int s = 0; s < NS; ++s) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(kw[u][s]), qh[part][s], acc, 0, 0, 0);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) S[4 * u + v] = acc[v];
+        }
+        load_k(pn);
+        p = Pages(w, min(t + 2 * WT, mine));
+        tree_weights<X, edge, ND>(w, S, k, t0, kg, ph, pl, o);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * NS) : "memory");   // V is there; the next K may be under way
+        if (edge && t0 + TREE_TILE > T) {
+            // rows behind the last node: weight 0 times whatever they hold
+            for (int i = lane; i < TREE_TILE * CH; i += 64)
+                if (t0 + i / CH >= T) *(uint4*)(v_s[wt] + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+            const v8h v0 = TreeV<D>::operand(vb, i, 0, col, kg), v1 = TreeV<D>::operand(vb, i, 1, col, kg);
+            v4f r = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[0], (v4f){0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+            r = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[0], r, 0, 0, 0);
+            r = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[1], r, 0, 0, 0);
+            r = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[1], r, 0, 0, 0);
+            o[i] += r;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // V is read before the next overwrites it
+        load_v(pn);
+    };
+    // the tiles of cached tokens alone, then the others
+    if constexpr (!X) {
+#pragma unroll 1
+        for (const int whole = min(end, w.sl / TREE_TILE); t < whole; t += WT) tile(TreeWhole());
+    }
+#pragma unroll 1
+    for (; t < end; t += WT) tile(TreeEdge());
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the loop
+    __syncthreads();
+    k.l = col_sum(k.l);
+    // join the waves, halving their number
+    v4f* o_s = (v4f*)v_s;
+    float* ml_s = (float*)(o_s + WT / 2 * ND * 64);
+#pragma unroll
+    for (int h = WT / 2; h; h >>= 1) {
+        const int at = wt % h;
+        if (wt >= h && wt < 2 * h) {
+            ml_s[(at * 2 + 0) * 64 + lane] = k.m;
+            ml_s[(at * 2 + 1) * 64 + lane] = k.l;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) o_s[(at * ND + i) * 64 + lane] = o[i];
+        }
+        __syncthreads();
+        if (wt < h) {
+            const float mo = ml_s[(at * 2 + 0) * 64 + lane], lo = ml_s[(at * 2 + 1) * 64 + lane];
+            const float mn = fmaxf(k.m, mo);
+            // a wave that has seen nothing: weights of 0
+            const float u0 = k.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(k.m - mn);
+            const float u1 = mo == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mo - mn);
+            k.l = k.l * u0 + lo * u1;
+            k.m = mn;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) o[i] = o[i] * u0 + o_s[(at * ND + i) * 64 + lane] * u1;
+        }
+        __syncthreads();
+    }
+    if (wt) return;
+    tree_store<D, 16, X>(w, w.c0 + col, k, kg, o);
+}
+
+// 64 NT columns per workgroup, 16 NT per wave: tiles of K and V pass through LDS, the
+// next one in flight from the barrier that publishes this one on.
+template <int D, int NT, bool X>
+__device__ __forceinline__ void tree_wide_body(const lgx_tree_attn_args& a) {
+    constexpr int NS = D / 32, ND = D / 16, CH = D / 8, NC = 64 * NT;
+    constexpr int TPI = 64 / CH, NI = TREE_TILE / TPI;   // tokens of a 1 KiB load, loads of a tile's K or V
+    __shared__ __align__(16) uint16_t kv_s[2][2][TREE_TILE * D];
+    const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    typedef Tree<NC> W;
+    typedef TreePages<W> Pages;
+    W w{a};
+    if (!w.place()) return;                       // uniform
+    // waves 0 and 1 bring K, 2 and 3 V
+    auto load = [&](int buf, const Pages& p) __attribute__((always_inline)) {
+        lds_u16* to = (lds_u16*)kv_s[buf][wave >> 1];
+#pragma unroll
+        for (int j = 0; j < NI / 2; ++j) {
+            const int i = (wave & 1) * (NI / 2) + j;
+            const int u = i * TPI / LGX_PAGE, r = i * TPI % LGX_PAGE + lane / CH;   // page, row
+            const int pg = u == 0 ? p.p[0] : u == 1 ? p.p[1] : u == 2 ? p.p[2] : p.p[3];
+            const int64_t blk = ((int64_t)min(max(pg, 0), a.num_pages - 1) * a.hkv + w.g) * (LGX_PAGE * D);
+            const int c = wave < 2 ? TreeK<D>::piece(r, lane % CH) : TreeV<D>::piece(r, lane % CH);
+            load_lds_16((wave < 2 ? a.k : a.v) + blk + (r * D + c * 8), (lds_void*)(to + i * 512));
+        }
+    };
+    const int end = w.tb1, T = w.sl + w.n;
+    int t = w.tb0;
+    load(0, Pages(w, t));
+    Pages p(w, min(t + 1, end - 1));
+    const int wcol = w.c0 + wave * 16 * NT;
+    const bool any = wcol < w.ncols;              // else the wave only loads
+    v4f o[NT][ND];
+    TreeCol k[NT];
+    v8h qh[NT][2][NS];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[n][i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+        const int c = min(wcol + 16 * n + col, w.ncols - 1);   // columns past the last repeat it
+        k[n] = {0.0f, X && a.slopes ? a.slopes[w.g * w.G + c % w.G] : 0.0f, -__builtin_inff(), 0.0f, c / w.G, 0};
+        k[n].dj = w.depth(k[n].j);
+        k[n].f = tree_query<D, X>(a, a.q + w.orow(c) * D + 8 * kg, qh[n]);
+    }
+    auto tile = [&](auto form) __attribute__((always_inline)) {
+        constexpr bool edge = decltype(form)::value;
+        const int t0 = t * TREE_TILE, cur = (t - w.tb0) & 1;
+        publish_lds_loads();                      // this tile is there, the last one read
+        if (edge && t0 + TREE_TILE > T) {         // uniform
+            // rows behind the last node: weight 0 times whatever they hold
+            for (int i = threadIdx.x; i < TREE_TILE * CH; i += 256)
+                if (t0 + i / CH >= T) *(uint4*)(kv_s[cur][1] + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+            __syncthreads();
+        }
+        if (t + 1 < end) {                        // uniform
+            load(cur ^ 1, p);
+            p = Pages(w, min(t + 2, end - 1));
+        }
+        if (!any) return;
+        const lds_u16* ks = (const lds_u16*)kv_s[cur][0];
+        const lds_u16* vs = (const lds_u16*)kv_s[cur][1];
+        float S[NT][16];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            v4f acc[NT];
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                const v8h kf = TreeK<D>::operand(ks, u, s, col, kg);
+#pragma unroll
+                for (int part = 1; part >= 0; --part)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            kf, qh[n][part][s], s == 0 && part == 1 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : acc[n], 0, 0, 0);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) S[n][4 * u + v] = acc[n][v];
+        }
+        v8h ph[NT][2], pl[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) tree_weights<X, edge, ND>(w, S[n], k[n], t0, kg, ph[n], pl[n], o[n]);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+            const v8h v0 = TreeV<D>::operand(vs, i, 0, col, kg), v1 = TreeV<D>::operand(vs, i, 1, col, kg);
+            v4f r[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) r[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[n][0], (v4f){0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) r[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[n][0], r[n], 0, 0, 0);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) r[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[n][1], r[n], 0, 0, 0);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) r[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[n][1], r[n], 0, 0, 0);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[n][i] += r[n];
+        }
+    };
+    // the tiles of cached tokens alone, then the others
+    if constexpr (!X) {
+#pragma unroll 1
+        for (const int whole = min(end, w.sl / TREE_TILE); t < whole; ++t) tile(TreeWhole());
+    }
+#pragma unroll 1
+    for (; t < end; ++t) tile(TreeEdge());
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the wave
+    if (!any) return;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        k[n].l = col_sum(k[n].l);
+        tree_store<D, NC, X>(w, wcol + 16 * n + col, k[n], kg, o[n]);
+    }
+}
+
+#define LGX_TREE_KERNEL(NAME, BODY) \
+    extern "C" __global__ __launch_bounds__(256, 2) void NAME(const lgx_tree_attn_args a) { BODY(a); }
+LGX_TREE_KERNEL(lgx_k_tree_attn_d64_c16, (tree_narrow_body<64, false>))
+LGX_TREE_KERNEL(lgx_k_tree_attnx_d64_c16, (tree_narrow_body<64, true>))
+LGX_TREE_KERNEL(lgx_k_tree_attn_d64_c64, (tree_wide_body<64, 1, false>))
+LGX_TREE_KERNEL(lgx_k_tree_attnx_d64_c64, (tree_wide_body<64, 1, true>))
+LGX_TREE_KERNEL(lgx_k_tree_attn_d64_c128, (tree_wide_body<64, 2, false>))
+LGX_TREE_KERNEL(lgx_k_tree_attnx_d64_c128, (tree_wide_body<64, 2, true>))
+LGX_TREE_KERNEL(lgx_k_tree_attn_d128_c16, (tree_narrow_body<128, false>))
+LGX_TREE_KERNEL(lgx_k_tree_attnx_d128_c16, (tree_narrow_body<128, true>))
+LGX_TREE_KERNEL(lgx_k_tree_attn_d128_c64, (tree_wide_body<128, 1, false>))
+LGX_TREE_KERNEL(lgx_k_tree_attnx_d128_c64, (tree_wide_body<128, 1, true>))
+LGX_TREE_KERNEL(lgx_k_tree_attn_d128_c128, (tree_wide_body<128, 2, false>))
