@@ -125,76 +125,247 @@ __device__ __forceinline__ uint32_t sf_key(float l) {
 }
 
 #define SF_NT 1024
+#define SF_BINS 1024                              // of a selection's first step
+#define SF_FEW 512                                // elements that one wave chooses among
 struct SfLds {
-    uint64_t bins[2048];                          // of a selection; before it, runs of 64 and the places of their tokens
+    union {
+        uint64_t bins[SF_BINS];
+        uint16_t runs[SF_LIST];                   // runs of 64 logits to read
+    };
     uint64_t wi[SF_LIST];                         // weight << 20 | index
     uint32_t key[SF_LIST];
+    uint64_t few[SF_FEW];                         // measures of a selection's second step
+    uint32_t few_key[SF_FEW];
     uint64_t wave[SF_NT / 64];
     double dwave[SF_NT / 64];
     uint64_t below;
-    int found;
+    uint32_t at;
+    int found, count;
 };
 static_assert(sizeof(SfLds) <= 81920, "two workgroups per compute unit");
-static_assert(LGX_SF_VOCAB <= 1 << 20, "an index has 20 bits beside its weight");
+static_assert(LGX_SF_VOCAB <= 1 << 20 && LGX_SF_VOCAB / LGX_SF_CHUNK <= 65536, "an index has 20 bits, a run 16");
+
+// Inclusive sums over the lanes, as wave_scan.
+__device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {
+    auto step = [&](auto C, auto R) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, decltype(C)::value, decltype(R)::value, 0xf, false);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), decltype(C)::value, decltype(R)::value, 0xf, false);
+        v += (uint64_t)hi << 32 | lo;
+    };
+    struct A { enum { value = 0x111 }; };
+    struct B { enum { value = 0x112 }; };
+    struct C { enum { value = 0x114 }; };
+    struct D { enum { value = 0x118 }; };
+    struct E { enum { value = 0x142 }; };
+    struct F { enum { value = 0x143 }; };
+    struct All { enum { value = 0xf }; };
+    struct Odd { enum { value = 0xa }; };
+    struct Upper { enum { value = 0xc }; };
+    step(A{}, All{});
+    step(B{}, All{});
+    step(C{}, All{});
+    step(D{}, All{});
+    step(E{}, Odd{});
+    step(F{}, Upper{});
+    return v;
+}
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) { return lane_of(wave_scan64(v), 63); }
 
 // Inclusive sums over the workgroup's threads.
 template <class V>
 __device__ __forceinline__ V sf_scan(V v, V* waves, V& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if constexpr (sizeof(V) == 8 && V(0.5) == V(0)) {
+        v = wave_scan64(v);
+    } else {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const V o = __shfl_up(v, d, 64);
-        v += lane >= d ? o : V(0);
+        for (int d = 1; d < 64; d <<= 1) {
+            const V o = __shfl_up(v, d, 64);
+            v += lane >= d ? o : V(0);
+        }
     }
     if (lane == 63) waves[wave] = v;
     __syncthreads();
     V before = 0;
     total = 0;
+#pragma unroll
     for (int w = 0; w < SF_NT / 64; ++w) {
-        before += w < wave ? waves[w] : V(0);
-        total += waves[w];
+        const V o = waves[w];
+        before += w < wave ? o : V(0);
+        total += o;
     }
     __syncthreads();
     return before + v;
 }
+// Their sum alone.
+__device__ __forceinline__ uint64_t sf_sum(uint64_t v, uint64_t* waves) {
+    v = wave_sum64(v);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
+    __syncthreads();
+    uint64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < SF_NT / 64; ++w) total += waves[w];
+    __syncthreads();
+    return total;
+}
 
-// The smallest key whose elements and those of smaller keys measure `need` (> 0) or more,
-// found digit by digit with sums per digit; below: the measure of smaller keys; false
-// if all together measure less.  each(f): f(key, measure function) for the thread's
-// elements.
-template <class E>
-__device__ __forceinline__ bool sf_select(SfLds& s, uint64_t need, uint32_t& key, uint64_t& below, const E& each) {
-    const int tid = threadIdx.x;
-    uint32_t prefix = 0;
+// The smallest key of one wave's E elements per lane such that those up to it measure
+// `need` or more (no more than all); below: the measure of smaller keys.  Bisection
+// of the keys' range; sum(k): the measure of keys <= k.
+template <class F>
+__device__ __forceinline__ uint32_t sf_bisect(uint32_t lo, uint32_t hi, uint64_t need, uint64_t& below, const F& sum) {
     below = 0;
-    int shift = 21;
-#pragma unroll 1
-    for (int round = 0; round < 3; ++round) {
-        const int bits = round < 2 ? 11 : 10;
-        s.bins[tid] = 0;
-        s.bins[tid + SF_NT] = 0;
-        __syncthreads();
-        each([&](uint32_t k, auto measure) {
-            if (round == 0 || k >> (shift + bits) == prefix)
-                __hip_atomic_fetch_add(&s.bins[(k >> shift) & ((1u << bits) - 1)], (uint64_t)measure(), __ATOMIC_RELAXED,
-                                       __HIP_MEMORY_SCOPE_WORKGROUP);
-        });
-        __syncthreads();
-        const uint64_t b0 = s.bins[2 * tid], b1 = s.bins[2 * tid + 1];
-        uint64_t total;
-        const uint64_t upto = below + sf_scan<uint64_t>(b0 + b1, s.wave, total);
-        if (total + below < need) return false;   // uniform; in the first round if ever
-        if (upto >= need && upto - b0 - b1 < need) {
-            const bool first = upto - b1 >= need;
-            s.found = 2 * tid + !first;
-            s.below = upto - b1 - (first ? b0 : 0);
+    while (lo < hi) {                             // uniform
+        const uint32_t mid = lo + (hi - lo) / 2;
+        const uint64_t s = sum(mid);
+        if (s >= need) {
+            hi = mid;
+        } else {
+            lo = mid + 1;
+            below = s;                            // the last such sum is that of keys < lo
+        }
+    }
+    return lo;
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d, 64));
+    return v;
+}
+
+// The row's tokens that can be kept, in LDS or in memory: logit, key, index and weight of
+// element i; valid: not below tau.  Elements ascend by index.
+struct SfInLds {
+    const SfLds& s;
+    int n;
+    __device__ __forceinline__ bool valid(int) const { return true; }
+    __device__ __forceinline__ uint32_t key(int i) const { return s.key[i]; }
+    __device__ __forceinline__ int index(int i) const { return (int)(s.wi[i] & 0xfffff); }
+    __device__ __forceinline__ uint64_t weight(int i) const { return s.wi[i] >> 20; }
+};
+struct SfInRow {
+    const float* x;
+    int n;
+    float tau, M;
+    double inv;
+    __device__ __forceinline__ bool valid(int i) const { return x[i] >= tau; }
+    __device__ __forceinline__ uint32_t key(int i) const { return sf_key(x[i]); }
+    __device__ __forceinline__ int index(int i) const { return i; }
+    __device__ __forceinline__ uint64_t weight(int i) const { return (uint64_t)rint(sf_weight(x[i], M, inv) * SF_ONE); }
+};
+
+// Bin of a key: linear in the logit between the row's maximum and tau, so that keys of
+// one bin follow each other.  A constant for all calls of a row.
+struct SfBins {
+    float M, scale;
+    __device__ __forceinline__ SfBins(float M, float tau) : M(M), scale((float)SF_BINS / (M - tau)) {
+        if (!(scale > 0.0f && scale < 1e30f)) scale = 0.0f;   // one logit, or an infinite range: one bin
+    }
+    __device__ __forceinline__ int operator()(uint32_t key) const {
+        const float l = __uint_as_float(key & 0x80000000u ? key : ~key & 0x7fffffffu);
+        const float b = (M - l) * scale;
+        return b < (float)(SF_BINS - 1) ? (int)b : SF_BINS - 1;   // (NaN: the last)
+    }
+};
+
+// The smallest key such that elements of it and of smaller keys measure `need` (> 0) or
+// more; below: the measure of smaller keys; false if all together measure less.  each(f):
+// f(key, measure function) for the thread's elements.  Sums per bin, then the elements of
+// the bin that passes `need`: by one wave if they are few, else digit by digit.
+template <class E>
+__device__ __forceinline__ bool sf_select(SfLds& s, const SfBins& bin, uint64_t need, uint32_t& key, uint64_t& below, const E& each) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    s.bins[tid] = 0;
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    each([&](uint32_t k, auto measure) {
+        __hip_atomic_fetch_add(&s.bins[bin(k)], (uint64_t)measure(), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    });
+    __syncthreads();
+    const uint64_t mine = s.bins[tid];
+    uint64_t total;
+    const uint64_t upto = sf_scan<uint64_t>(mine, s.wave, total);
+    if (total < need) return false;               // uniform
+    if (upto >= need && upto - mine < need) {
+        s.found = tid;
+        s.below = upto - mine;
+    }
+    __syncthreads();
+    const int at = s.found;
+    const uint64_t base = s.below;
+    each([&](uint32_t k, auto measure) {
+        if (bin(k) != at) return;
+        const int i = __hip_atomic_fetch_add(&s.count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (i < SF_FEW) {
+            s.few_key[i] = k;
+            s.few[i] = (uint64_t)measure();
+        }
+    });
+    __syncthreads();
+    const int n = s.count;
+    if (n <= SF_FEW) {
+        if (tid < 64) {
+            uint32_t k[SF_FEW / 64], lo = 0xffffffffu, hi = 0;
+            uint64_t m[SF_FEW / 64];
+#pragma unroll
+            for (int e = 0; e < SF_FEW / 64; ++e) {
+                const int i = 64 * e + lane;
+                k[e] = i < n ? s.few_key[i] : 0xffffffffu;
+                m[e] = i < n ? s.few[i] : 0;
+                lo = min(lo, k[e]);
+                hi = max(hi, i < n ? k[e] : 0u);
+            }
+            lo = ~wave_max_u32(~lo);
+            hi = wave_max_u32(hi);
+            const int ne = (n + 63) / 64;
+            uint64_t b;
+            const uint32_t t = sf_bisect(lo, hi, need - base, b, [&](uint32_t mid) {
+                uint64_t v = 0;
+#pragma unroll
+                for (int e = 0; e < SF_FEW / 64; ++e)
+                    if (e < ne) v += k[e] <= mid ? m[e] : 0;
+                return wave_sum64(v);
+            });
+            if (lane == 0) {
+                s.at = t;
+                s.below = base + b;
+            }
         }
         __syncthreads();
-        prefix = prefix << bits | (uint32_t)s.found;
+        key = s.at;
         below = s.below;
         __syncthreads();
-        shift -= round == 1 ? 10 : 11;
+        return true;
     }
+    // many in one bin: equal or nearly equal logits
+    uint32_t prefix = 0;
+    below = base;
+    int shift = 24;
+#pragma unroll 1
+    for (int round = 0; round < 4; ++round, shift -= 8) {
+        __syncthreads();
+        if (tid < 256) s.bins[tid] = 0;
+        __syncthreads();
+        each([&](uint32_t k, auto measure) {
+            if (bin(k) == at && (round == 0 || k >> (shift + 8) == prefix))
+                __hip_atomic_fetch_add(&s.bins[k >> shift & 255], (uint64_t)measure(), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        });
+        __syncthreads();
+        const uint64_t b = tid < 256 ? s.bins[tid] : 0;
+        const uint64_t up = below + sf_scan<uint64_t>(b, s.wave, total);
+        if (up >= need && up - b < need) {
+            s.found = tid;
+            s.below = up - b;
+        }
+        __syncthreads();
+        prefix = prefix << 8 | (uint32_t)s.found;
+        below = s.below;
+    }
+    __syncthreads();
     key = prefix;
     return true;
 }
@@ -213,7 +384,7 @@ __device__ __forceinline__ int sf_first(SfLds& s, int n, uint64_t t, const M& me
         uint64_t m = 0;
         for (int i = a + lane; i < e; i += 64) m += measure(i);
         const uint64_t upto = sf_scan<uint64_t>(m, s.wave, total);
-        const uint64_t all = __shfl(upto, 63, 64), before = __shfl(upto - m, 0, 64);
+        const uint64_t all = lane_of(upto, 63), before = lane_of(upto - m, 0);
         if (lane == 0 && all > t && before <= t) {
             s.found = wave;
             s.below = before;
@@ -233,63 +404,40 @@ __device__ __forceinline__ int sf_first(SfLds& s, int n, uint64_t t, const M& me
     return min(max(at, 0), n - 1);                // an element even of rows that change meanwhile
 }
 
-// The row's tokens that can be kept: in LDS, or in memory.  key(i, k): element i's key,
-// false if it is none; index and weight of element i.
-struct SfInLds {
-    const SfLds& s;
-    int n;
-    __device__ __forceinline__ bool key(int i, uint32_t& k) const {
-        k = s.key[i];
-        return true;
-    }
-    __device__ __forceinline__ int index(int i) const { return (int)(s.wi[i] & 0xfffff); }
-    __device__ __forceinline__ uint64_t weight(int i) const { return s.wi[i] >> 20; }
-};
-struct SfInRow {
-    const float* x;
-    int n;
-    float tau, M;
-    double inv;
-    __device__ __forceinline__ bool key(int i, uint32_t& k) const {
-        k = sf_key(x[i]);
-        return x[i] >= tau;
-    }
-    __device__ __forceinline__ int index(int i) const { return i; }
-    __device__ __forceinline__ uint64_t weight(int i) const { return (uint64_t)rint(sf_weight(x[i], M, inv) * SF_ONE); }
-};
+// What remains of u: the sum that the drawn token's has to pass.
+__device__ __forceinline__ uint64_t sf_draw(float u, uint64_t total) {
+    return u > 0.0f ? min((uint64_t)(fmin((double)u, 1.0) * (double)total), total - 1) : 0;
+}
 
-// Selection and draw; all: the weight of every token of the row in units of 2^-42, where
-// no top-k cuts it.  Elements ascend by index.
+// Selection and draw by the workgroup; all: the weight of every token of the row in units
+// of 2^-42, where no top-k cuts it.
 template <class S>
-__device__ __forceinline__ void sf_choose(SfLds& s, const lgx_filter_args& a, const SfRow& r, int row, double all, const S& e) {
+__device__ __forceinline__ void sf_choose(SfLds& s, const lgx_filter_args& a, const SfRow& r, const SfBins& bin, int row, double all,
+                                          const S& e) {
     // kept: key < last, or key == last and place <= most
     uint32_t last = 0xffffffffu;
     int most = 0x7fffffff;
     auto kept = [&](uint32_t key, int i) { return key < last || (key == last && i <= most); };
     auto each = [&](auto f) {
-        uint32_t k;
-        for (int i = threadIdx.x; i < e.n; i += SF_NT)
-            if (e.key(i, k) && kept(k, i)) f(k, i);
+        for (int i = threadIdx.x; i < e.n; i += SF_NT) {
+            const uint32_t k = e.key(i);
+            if (e.valid(i) && kept(k, i)) f(k, i);
+        }
     };
     auto sum = [&](auto f) {
-        uint64_t n = 0, total;
+        uint64_t n = 0;
         each([&](uint32_t k, int i) { n += f(k, i); });
-        sf_scan<uint64_t>(n, s.wave, total);
-        return total;
+        return sf_sum(n, s.wave);
     };
     // of the kept tokens with key `last` only the first n (>= 1)
     auto cut = [&](uint64_t n) {
         if (sum([&](uint32_t k, int) { return k == last; }) <= n) return;
-        const int at = sf_first(s, e.n, n - 1, [&](int i) {
-            uint32_t k;
-            return (uint64_t)(e.key(i, k) && k == last && i <= most);
-        });
-        most = at;
+        most = sf_first(s, e.n, n - 1, [&](int i) { return (uint64_t)(e.valid(i) && e.key(i) == last && i <= most); });
     };
     uint32_t key;
     uint64_t below;
     // fewer tokens than top_k that count: all of them
-    if (r.k && sf_select(s, r.k, key, below, [&](auto f) { each([&](uint32_t k, int) { f(k, [] { return 1; }); }); })) {
+    if (r.k && sf_select(s, bin, r.k, key, below, [&](auto f) { each([&](uint32_t k, int) { f(k, [] { return 1; }); }); })) {
         last = key;
         cut(r.k - below);
     }
@@ -297,7 +445,7 @@ __device__ __forceinline__ void sf_choose(SfLds& s, const lgx_filter_args& a, co
         // of the kept tokens those that reach the share, the first at least
         const double whole = r.k ? (double)sum([&](uint32_t, int i) { return e.weight(i); }) : all;
         const uint64_t need = max((uint64_t)ceil((double)r.p * whole), (uint64_t)1);
-        if (sf_select(s, need, key, below, [&](auto f) { each([&](uint32_t k, int i) { f(k, [&] { return e.weight(i); }); }); })) {
+        if (sf_select(s, bin, need, key, below, [&](auto f) { each([&](uint32_t k, int i) { f(k, [&] { return e.weight(i); }); }); })) {
             if (key != last) most = 0x7fffffff;
             last = key;
             // tokens of one logit weigh the same: what they weigh together, by their number
@@ -312,15 +460,97 @@ __device__ __forceinline__ void sf_choose(SfLds& s, const lgx_filter_args& a, co
         return w >= low ? w : 0;
     };
     const uint64_t total = sum([&](uint32_t, int i) { return weight(i); });
-    const double u = (double)a.u[row];
-    const uint64_t t = u > 0.0 ? min((uint64_t)(fmin(u, 1.0) * (double)total), total - 1) : 0;
-    const int at = sf_first(s, e.n, t, [&](int i) {
-        uint32_t k;
-        return e.key(i, k) && kept(k, i) ? weight(i) : 0;
-    });
+    const int at = sf_first(s, e.n, sf_draw(a.u[row], total), [&](int i) { return e.valid(i) && kept(e.key(i), i) ? weight(i) : 0; });
     if (threadIdx.x == 0) {
         a.out[row] = e.index(at);
         if (a.prob) a.prob[row] = (float)((double)weight(at) / (double)total);
+    }
+}
+
+// The same by one wave, for the n <= 512 elements of the list: lane l holds elements
+// l ne .. , so that sums over lanes go by index; no barriers.
+__device__ __forceinline__ void sf_choose_wave(const SfLds& s, const lgx_filter_args& a, const SfRow& r, int row, double all, int n) {
+    constexpr int E = SF_FEW / 64;
+    const int lane = threadIdx.x & 63, ne = (n + 63) / 64;
+    uint32_t k[E], lo = 0xffffffffu, hi = 0;
+    uint64_t wi[E];
+    bool on[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int i = lane * ne + e;
+        on[e] = e < ne && i < n;
+        k[e] = on[e] ? s.key[i] : 0xffffffffu;
+        wi[e] = on[e] ? s.wi[i] : 0;
+        lo = min(lo, k[e]);
+        hi = max(hi, on[e] ? k[e] : 0u);
+    }
+    lo = ~wave_max_u32(~lo);
+    hi = wave_max_u32(hi);
+    // of the kept elements those of keys below t, and the first m of key t
+    auto cut = [&](uint32_t t, uint64_t m) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) c += on[e] && k[e] == t;
+        uint32_t before = (uint32_t)wave_scan((int)c) - c;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const bool eq = on[e] && k[e] == t;
+            on[e] = on[e] && (k[e] < t || (eq && before < m));
+            before += eq;
+        }
+        hi = t;
+    };
+    uint64_t below;
+    if (r.k && r.k < n) {
+        const uint32_t t = sf_bisect(lo, hi, r.k, below, [&](uint32_t mid) {
+            uint32_t c = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e < ne) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on[e] && k[e] <= mid));
+            return (uint64_t)c;
+        });
+        cut(t, r.k - below);
+    }
+    auto sum = [&](auto f) {
+        uint64_t v = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (e < ne) v += on[e] && f(e) ? wi[e] >> 20 : 0;
+        return wave_sum64(v);
+    };
+    if (r.p < 1.0f) {
+        const uint64_t have = sum([](int) { return true; });
+        const uint64_t need = max((uint64_t)ceil((double)r.p * (r.k ? (double)have : all)), (uint64_t)1);
+        if (need <= have) {
+            const uint32_t t = sf_bisect(lo, hi, need, below, [&](uint32_t mid) { return sum([&](int e) { return k[e] <= mid; }); });
+            uint32_t c = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e < ne) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(on[e] && k[e] == t));
+            const uint64_t w = sum([&](int e) { return k[e] == t; }) / c;   // one weight for one logit
+            cut(t, (need - below + w - 1) / w);
+        }
+    }
+    const uint64_t low = (uint64_t)ceil((double)r.mp * SF_ONE);
+    uint64_t mine = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        on[e] = on[e] && wi[e] >> 20 >= low;
+        mine += on[e] ? wi[e] >> 20 : 0;
+    }
+    const uint64_t upto = wave_scan64(mine), total = lane_of(upto, 63), t = sf_draw(a.u[row], total);
+    if (upto > t && upto - mine <= t) {
+        uint64_t c = upto - mine;
+        bool done = false;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            c += on[e] ? wi[e] >> 20 : 0;
+            if (!done && c > t) {
+                done = true;
+                a.out[row] = (int)(wi[e] & 0xfffff);
+                if (a.prob) a.prob[row] = (float)((double)(wi[e] >> 20) / (double)total);
+            }
+        }
     }
 }
 
@@ -415,74 +645,106 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
     tau -= fmaxf(fabsf(M), fabsf(tau)) * 1e-6f;
     if (!(tau == tau)) tau = M == __builtin_inff() ? M : ninf;
     if (r.k && r.k <= nruns) {
-        uint64_t below;
-        uint32_t key;
-        sf_select(s, r.k, key, below, [&](auto f) {
-            for (int c = tid; c < nruns; c += SF_NT) f(sf_key(cmax[c]), [] { return 1; });
-        });
-        tau = fmaxf(tau, __uint_as_float(key & 0x80000000u ? key : ~key & 0x7fffffffu));
+        // a bin of the runs' maxima by which k of them are reached, and its lowest
+        s.bins[tid] = 0;
+        if (tid == 0) s.at = 0;
+        __syncthreads();
+        const SfBins bin(M, fmaxf(tau, -3e38f));
+        for (int c = tid; c < nruns; c += SF_NT) {
+            const float v = cmax[c];
+            if (v >= tau)
+                __hip_atomic_fetch_add((uint32_t*)&s.bins[bin(sf_key(v))], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+        __syncthreads();
+        const uint64_t mine = (uint32_t)s.bins[tid];
+        uint64_t total;
+        const uint64_t upto = sf_scan<uint64_t>(mine, s.wave, total);
+        if (total >= (uint64_t)r.k) {             // uniform
+            if (upto >= (uint64_t)r.k && upto - mine < (uint64_t)r.k) s.found = tid;
+            __syncthreads();
+            const int at = s.found;
+            uint32_t low = 0;
+            for (int c = tid; c < nruns; c += SF_NT) {
+                const float v = cmax[c];
+                if (v >= tau && bin(sf_key(v)) <= at) low = max(low, sf_key(v));
+            }
+            low = wave_max_u32(low);
+            if (lane == 0) __hip_atomic_fetch_max(&s.at, low, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            __syncthreads();
+            const uint32_t key = s.at;
+            tau = fmaxf(tau, __uint_as_float(key & 0x80000000u ? key : ~key & 0x7fffffffu));
+        }
     }
-    // the runs that reach it, in order
-    uint16_t* runs = (uint16_t*)s.bins;
-    uint16_t* place = runs + SF_LIST;
-    static_assert(2 * SF_LIST * sizeof(uint16_t) <= sizeof(s.bins) && LGX_SF_VOCAB / LGX_SF_CHUNK <= 65536, "runs and places in the bins");
-    int nr = 0;
-    for (int c0 = 0; c0 < nruns; c0 += SF_NT) {
-        const int c = c0 + tid;
+    // the runs that reach it, in order: a sixteenth of them per wave
+    const int rw = (nruns + SF_NT - 1) / SF_NT * 64;
+    int mine = 0;
+    for (int c = wave * rw + lane; c < (wave + 1) * rw; c += 64)
+        mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(c < nruns && cmax[min(c, nruns - 1)] >= tau));
+    if (lane == 0) s.wave[wave] = (uint64_t)mine;
+    __syncthreads();
+    int nr = 0, to = 0;
+#pragma unroll
+    for (int w = 0; w < SF_NT / 64; ++w) {
+        const int c = (int)s.wave[w];
+        to += w < wave ? c : 0;
+        nr += c;
+    }
+    for (int c = wave * rw + lane; c < (wave + 1) * rw; c += 64) {
         const bool on = c < nruns && cmax[min(c, nruns - 1)] >= tau;
-        uint64_t more;
-        const int at = nr + (int)sf_scan<uint64_t>(on, s.wave, more) - 1;
-        if (on && at < SF_LIST) runs[at] = (uint16_t)c;
-        nr += (int)more;
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(on);
+        const int q = to + __builtin_popcountll(hit & ((1ull << lane) - 1));
+        if (on && q < SF_LIST) s.runs[q] = (uint16_t)c;
+        to += __builtin_popcountll(hit);
     }
     __syncthreads();
-    int n = 0;
-    bool fits = nr <= SF_LIST;
-    // f(q, the lane's token of run q, its logit): waves take the runs in turn, four in flight
-    auto tokens = [&](auto f) {
-        for (int q0 = wave; q0 < nr; q0 += SF_NT / 16) {
-            float v[4];
-            int t[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                t[u] = runs[min(q0 + u * (SF_NT / 64), nr - 1)] * LGX_SF_CHUNK + lane;
-                v[u] = t[u] < V ? x[t[u]] : __builtin_nanf("");
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (q0 + u * (SF_NT / 64) < nr) f(q0 + u * (SF_NT / 64), t[u], v[u]);
-        }
-    };
-    if (fits) {
-        tokens([&](int q, int, float v) {
-            const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(v >= tau));
-            if (lane == 0) place[q] = (uint16_t)c;
-        });
-        __syncthreads();
-        for (int q0 = 0; q0 < nr; q0 += SF_NT) {
-            const int q = q0 + tid, c = q < nr ? place[q] : 0;
-            uint64_t more;
-            const int at = n + (int)sf_scan<uint64_t>((uint64_t)c, s.wave, more) - c;
-            if (q < nr) place[q] = (uint16_t)min(at, SF_LIST);
-            n += (int)more;
-        }
-        fits = n <= SF_LIST;
-        __syncthreads();
-    }
     const double all = S * SF_ONE;
-    if (fits) {                                   // uniform
-        tokens([&](int q, int t, float v) {
-            const uint64_t hit = __builtin_amdgcn_ballot_w64(v >= tau);
-            const int to = place[q] + __builtin_popcountll(hit & ((1ull << lane) - 1));
-            if (v >= tau) {
-                s.key[to] = sf_key(v);
-                s.wi[to] = (uint64_t)rint(sf_weight(v, M, r.inv) * SF_ONE) << 20 | (uint64_t)t;
+    const SfBins bin(M, fmaxf(tau, -3e38f));
+    if (nr <= SF_LIST) {
+        // their tokens that reach it, in order: a sixteenth of the runs per wave
+        const int per = (nr + SF_NT / 64 - 1) / (SF_NT / 64), q0 = min(wave * per, nr), q1 = min(q0 + per, nr);
+        auto tokens = [&](auto f) {               // four runs in flight
+            for (int q = q0; q < q1; q += 4) {
+                float v[4];
+                int t[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    t[u] = s.runs[min(q + u, q1 - 1)] * LGX_SF_CHUNK + lane;
+                    v[u] = t[u] < V && q + u < q1 ? x[t[u]] : __builtin_nanf("");
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) f(t[u], v[u]);
             }
-        });
+        };
+        int c = 0;
+        tokens([&](int, float v) { c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v >= tau)); });
+        if (lane == 0) s.dwave[wave] = (double)c;
         __syncthreads();
-        sf_choose(s, a, r, row, all, SfInLds{s, n});
-    } else {
-        // more than LDS holds: the row itself
-        sf_choose(s, a, r, row, all, SfInRow{x, V, tau, M, r.inv});
+        int n = 0, at = 0;
+#pragma unroll
+        for (int w = 0; w < SF_NT / 64; ++w) {
+            const int m = (int)s.dwave[w];
+            at += w < wave ? m : 0;
+            n += m;
+        }
+        if (n <= SF_LIST) {                       // uniform
+            tokens([&](int t, float v) {
+                const uint64_t hit = __builtin_amdgcn_ballot_w64(v >= tau);
+                const int i = at + __builtin_popcountll(hit & ((1ull << lane) - 1));
+                if (v >= tau) {
+                    s.key[i] = sf_key(v);
+                    s.wi[i] = (uint64_t)rint(sf_weight(v, M, r.inv) * SF_ONE) << 20 | (uint64_t)t;
+                }
+                at += __builtin_popcountll(hit);
+            });
+            __syncthreads();
+            if (n <= SF_FEW) {
+                if (wave == 0) sf_choose_wave(s, a, r, row, all, n);
+            } else {
+                sf_choose(s, a, r, bin, row, all, SfInLds{s, n});
+            }
+            return;
+        }
     }
+    // more than LDS holds: the row itself
+    sf_choose(s, a, r, bin, row, all, SfInRow{x, V, tau, M, r.inv});
 }
