@@ -237,26 +237,48 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     return v;
 }
 
-// The row's tokens that can be kept, in LDS or in memory: logit, key, index and weight of
-// element i; valid: not below tau.  Elements ascend by index.
+// The row's tokens that can be kept, in LDS or in memory: load(i) is element i, the others
+// say of it whether it counts (not below tau), its key, index and weight.  Elements
+// ascend by index.  U: loads in flight per thread.
 struct SfInLds {
+    static constexpr int U = 1;
+    struct Raw {
+        uint32_t key;
+        uint64_t wi;
+    };
     const SfLds& s;
     int n;
-    __device__ __forceinline__ bool valid(int) const { return true; }
-    __device__ __forceinline__ uint32_t key(int i) const { return s.key[i]; }
-    __device__ __forceinline__ int index(int i) const { return (int)(s.wi[i] & 0xfffff); }
-    __device__ __forceinline__ uint64_t weight(int i) const { return s.wi[i] >> 20; }
+    __device__ __forceinline__ Raw load(int i) const { return {s.key[i], s.wi[i]}; }
+    __device__ __forceinline__ bool valid(const Raw&) const { return true; }
+    __device__ __forceinline__ uint32_t key(const Raw& x) const { return x.key; }
+    __device__ __forceinline__ int index(const Raw& x, int) const { return (int)(x.wi & 0xfffff); }
+    __device__ __forceinline__ uint64_t weight(const Raw& x) const { return x.wi >> 20; }
 };
 struct SfInRow {
+    static constexpr int U = 8;
+    typedef float Raw;
     const float* x;
     int n;
     float tau, M;
     double inv;
-    __device__ __forceinline__ bool valid(int i) const { return x[i] >= tau; }
-    __device__ __forceinline__ uint32_t key(int i) const { return sf_key(x[i]); }
-    __device__ __forceinline__ int index(int i) const { return i; }
-    __device__ __forceinline__ uint64_t weight(int i) const { return (uint64_t)rint(sf_weight(x[i], M, inv) * SF_ONE); }
+    __device__ __forceinline__ float load(int i) const { return x[i]; }
+    __device__ __forceinline__ bool valid(float v) const { return v >= tau; }
+    __device__ __forceinline__ uint32_t key(float v) const { return sf_key(v); }
+    __device__ __forceinline__ int index(float, int i) const { return i; }
+    __device__ __forceinline__ uint64_t weight(float v) const { return (uint64_t)rint(sf_weight(v, M, inv) * SF_ONE); }
 };
+// f(element, i) for the elements first, first + step, .. below end
+template <class S, class F>
+__device__ __forceinline__ void sf_each(const S& e, int first, int end, int step, const F& f) {
+    for (int i0 = first; i0 < end; i0 += step * S::U) {
+        typename S::Raw x[S::U];
+#pragma unroll
+        for (int u = 0; u < S::U; ++u) x[u] = e.load(min(i0 + u * step, end - 1));
+#pragma unroll
+        for (int u = 0; u < S::U; ++u)
+            if (i0 + u * step < end) f(x[u], i0 + u * step);
+    }
+}
 
 // Bin of a key: linear in the logit between the row's maximum and tau, so that keys of
 // one bin follow each other.  A constant for all calls of a row.
@@ -273,11 +295,17 @@ struct SfBins {
 };
 
 // The smallest key such that elements of it and of smaller keys measure `need` (> 0) or
-// more; below: the measure of smaller keys; false if all together measure less.  each(f):
-// f(key, measure function) for the thread's elements.  Sums per bin, then the elements of
-// the bin that passes `need`: by one wave if they are few, else digit by digit.
+// more.  Elements of one key measure the same.
+struct SfCut {
+    uint32_t key;
+    uint64_t below;                               // the measure of smaller keys
+    uint64_t equal, one;                          // elements of the key, and what each measures
+};
+// false if all together measure less.  each(f): f(key, measure function) for the thread's
+// elements.  Sums per bin, then the elements of the bin that passes `need`: by one wave
+// if they are few, else digit by digit.
 template <class E>
-__device__ __forceinline__ bool sf_select(SfLds& s, const SfBins& bin, uint64_t need, uint32_t& key, uint64_t& below, const E& each) {
+__device__ __forceinline__ bool sf_select(SfLds& s, const SfBins& bin, uint64_t need, SfCut& c, const E& each) {
     const int tid = threadIdx.x, lane = tid & 63;
     s.bins[tid] = 0;
     if (tid == 0) s.count = 0;
@@ -330,20 +358,30 @@ __device__ __forceinline__ bool sf_select(SfLds& s, const SfBins& bin, uint64_t 
                     if (e < ne) v += k[e] <= mid ? m[e] : 0;
                 return wave_sum64(v);
             });
+            uint64_t v = 0;
+            uint32_t q = 0;
+#pragma unroll
+            for (int e = 0; e < SF_FEW / 64; ++e) {
+                const bool eq = 64 * e + lane < n && k[e] == t;
+                v += eq ? m[e] : 0;
+                q += __builtin_popcountll(__builtin_amdgcn_ballot_w64(eq));
+            }
+            v = wave_sum64(v);
             if (lane == 0) {
-                s.at = t;
-                s.below = base + b;
+                s.few_key[0] = t;
+                s.few[0] = base + b;
+                s.few[1] = q;
+                s.few[2] = v / q;
             }
         }
         __syncthreads();
-        key = s.at;
-        below = s.below;
+        c = {s.few_key[0], s.few[0], s.few[1], s.few[2]};
         __syncthreads();
         return true;
     }
     // many in one bin: equal or nearly equal logits
     uint32_t prefix = 0;
-    below = base;
+    uint64_t below = base;
     int shift = 24;
 #pragma unroll 1
     for (int round = 0; round < 4; ++round, shift -= 8) {
@@ -366,23 +404,31 @@ __device__ __forceinline__ bool sf_select(SfLds& s, const SfBins& bin, uint64_t 
         below = s.below;
     }
     __syncthreads();
-    key = prefix;
+    uint64_t equal = 0, sum = 0;
+    each([&](uint32_t k, auto measure) {
+        if (k != prefix) return;
+        ++equal;
+        sum += (uint64_t)measure();
+    });
+    equal = sf_sum(equal, s.wave);
+    sum = sf_sum(sum, s.wave);
+    c = {prefix, below, equal, sum / equal};
     return true;
 }
 
-// The first of n elements at which the sum of measures passes t (t below the sum of
-// all), on every thread: the wave's sixteenth that holds it, then that one's, down to
-// an element per thread.
-template <class M>
-__device__ __forceinline__ int sf_first(SfLds& s, int n, uint64_t t, const M& measure) {
+// The first element at which the sum of measures passes t (t below the sum of all), on
+// every thread: the wave's sixteenth that holds it, then that one's, down to an
+// element per thread.  measure(element, i).
+template <class S, class M>
+__device__ __forceinline__ int sf_first(SfLds& s, const S& e, uint64_t t, const M& measure) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int lo = 0, hi = n;
+    int lo = 0, hi = e.n;
     uint64_t total;
 #pragma unroll 1
     while (hi - lo > SF_NT) {
-        const int part = (hi - lo + SF_NT - 1) / SF_NT * 64, a = lo + wave * part, e = min(a + part, hi);
+        const int part = (hi - lo + SF_NT - 1) / SF_NT * 64, a = lo + wave * part;
         uint64_t m = 0;
-        for (int i = a + lane; i < e; i += 64) m += measure(i);
+        sf_each(e, a + lane, min(a + part, hi), 64, [&](const typename S::Raw& x, int i) { m += measure(x, i); });
         const uint64_t upto = sf_scan<uint64_t>(m, s.wave, total);
         const uint64_t all = lane_of(upto, 63), before = lane_of(upto - m, 0);
         if (lane == 0 && all > t && before <= t) {
@@ -395,13 +441,13 @@ __device__ __forceinline__ int sf_first(SfLds& s, int n, uint64_t t, const M& me
         t -= s.below;
         __syncthreads();
     }
-    const uint64_t m = lo + tid < hi ? measure(lo + tid) : 0;
+    const uint64_t m = lo + tid < hi ? measure(e.load(lo + tid), lo + tid) : 0;
     const uint64_t upto = sf_scan<uint64_t>(m, s.wave, total);
     if (upto > t && upto - m <= t) s.found = lo + tid;
     __syncthreads();
     const int at = s.found;
     __syncthreads();
-    return min(max(at, 0), n - 1);                // an element even of rows that change meanwhile
+    return min(max(at, 0), e.n - 1);              // an element even of rows that change meanwhile
 }
 
 // What remains of u: the sum that the drawn token's has to pass.
@@ -414,63 +460,98 @@ __device__ __forceinline__ uint64_t sf_draw(float u, uint64_t total) {
 template <class S>
 __device__ __forceinline__ void sf_choose(SfLds& s, const lgx_filter_args& a, const SfRow& r, const SfBins& bin, int row, double all,
                                           const S& e) {
+    typedef typename S::Raw Raw;
     // kept: key < last, or key == last and place <= most
     uint32_t last = 0xffffffffu;
     int most = 0x7fffffff;
-    auto kept = [&](uint32_t key, int i) { return key < last || (key == last && i <= most); };
+    auto kept = [&](const Raw& x, int i) {
+        const uint32_t k = e.key(x);
+        return e.valid(x) && (k < last || (k == last && i <= most));
+    };
     auto each = [&](auto f) {
-        for (int i = threadIdx.x; i < e.n; i += SF_NT) {
-            const uint32_t k = e.key(i);
-            if (e.valid(i) && kept(k, i)) f(k, i);
-        }
+        sf_each(e, threadIdx.x, e.n, SF_NT, [&](const Raw& x, int i) {
+            if (kept(x, i)) f(x, i);
+        });
     };
     auto sum = [&](auto f) {
         uint64_t n = 0;
-        each([&](uint32_t k, int i) { n += f(k, i); });
+        each([&](const Raw& x, int) { n += f(x); });
         return sf_sum(n, s.wave);
     };
-    // of the kept tokens with key `last` only the first n (>= 1)
-    auto cut = [&](uint64_t n) {
-        if (sum([&](uint32_t k, int) { return k == last; }) <= n) return;
-        most = sf_first(s, e.n, n - 1, [&](int i) { return (uint64_t)(e.valid(i) && e.key(i) == last && i <= most); });
+    // of the kept tokens those of smaller keys and the first n (>= 1) of the cut's
+    auto keep = [&](const SfCut& c, uint64_t n) {
+        if (c.key != last) most = 0x7fffffff;
+        last = c.key;
+        if (n < c.equal)
+            most = sf_first(s, e, n - 1, [&](const Raw& x, int i) { return (uint64_t)(e.valid(x) && e.key(x) == last && i <= most); });
     };
-    uint32_t key;
-    uint64_t below;
+    SfCut c;
+    uint64_t total = 0;                           // weight of the kept tokens, once known
     // fewer tokens than top_k that count: all of them
-    if (r.k && sf_select(s, bin, r.k, key, below, [&](auto f) { each([&](uint32_t k, int) { f(k, [] { return 1; }); }); })) {
-        last = key;
-        cut(r.k - below);
-    }
+    if (r.k && sf_select(s, bin, r.k, c, [&](auto f) { each([&](const Raw& x, int) { f(e.key(x), [] { return 1; }); }); }))
+        keep(c, r.k - c.below);
     if (r.p < 1.0f) {
         // of the kept tokens those that reach the share, the first at least
-        const double whole = r.k ? (double)sum([&](uint32_t, int i) { return e.weight(i); }) : all;
+        const double whole = r.k ? (double)sum([&](const Raw& x) { return e.weight(x); }) : all;
         const uint64_t need = max((uint64_t)ceil((double)r.p * whole), (uint64_t)1);
-        if (sf_select(s, bin, need, key, below, [&](auto f) { each([&](uint32_t k, int i) { f(k, [&] { return e.weight(i); }); }); })) {
-            if (key != last) most = 0x7fffffff;
-            last = key;
-            // tokens of one logit weigh the same: what they weigh together, by their number
-            const uint64_t w = sum([&](uint32_t k, int i) { return k == last ? e.weight(i) : 0; }) /
-                               sum([&](uint32_t k, int) { return k == last; });
-            cut((need - below + w - 1) / w);
+        if (sf_select(s, bin, need, c, [&](auto f) { each([&](const Raw& x, int) { f(e.key(x), [&] { return e.weight(x); }); }); })) {
+            const uint64_t n = min((need - c.below + c.one - 1) / c.one, c.equal);
+            keep(c, n);
+            total = c.below + n * c.one;
         }
     }
     const uint64_t low = (uint64_t)ceil((double)r.mp * SF_ONE);
-    auto weight = [&](int i) {
-        const uint64_t w = e.weight(i);
+    auto weight = [&](const Raw& x) {
+        const uint64_t w = e.weight(x);
         return w >= low ? w : 0;
     };
-    const uint64_t total = sum([&](uint32_t, int i) { return weight(i); });
-    const int at = sf_first(s, e.n, sf_draw(a.u[row], total), [&](int i) { return e.valid(i) && kept(e.key(i), i) ? weight(i) : 0; });
+    if (total == 0 || low) total = sum([&](const Raw& x) { return weight(x); });
+    const int at = sf_first(s, e, sf_draw(a.u[row], total), [&](const Raw& x, int i) { return kept(x, i) ? weight(x) : 0; });
     if (threadIdx.x == 0) {
-        a.out[row] = e.index(at);
-        if (a.prob) a.prob[row] = (float)((double)weight(at) / (double)total);
+        const Raw x = e.load(at);
+        a.out[row] = e.index(x, at);
+        if (a.prob) a.prob[row] = (float)((double)weight(x) / (double)total);
     }
 }
 
-// The same by one wave, for the n <= 512 elements of the list: lane l holds elements
-// l ne .. , so that sums over lanes go by index; no barriers.
-__device__ __forceinline__ void sf_choose_wave(const SfLds& s, const lgx_filter_args& a, const SfRow& r, int row, double all, int n) {
+// The same by one wave, for n <= 64 elements of the list, one per lane: each lane sums over
+// those that come before its own in the order of (key, index).
+__device__ __forceinline__ void sf_choose_lanes(const SfLds& s, const lgx_filter_args& a, const SfRow& r, int row, double all, int n) {
+    const int lane = threadIdx.x & 63;
+    bool on = lane < n;
+    const uint32_t key = on ? s.key[lane] : 0xffffffffu;
+    const uint64_t wi = on ? s.wi[lane] : 0, w = wi >> 20;
+    if (r.k || r.p < 1.0f) {
+        uint64_t before = 0;                      // weight of the elements ahead, and their number << 52
+        const uint64_t wn = w | 1ull << 52;
+        for (int j = 0; j < n; ++j) {             // 64 weights of 2^42 stay below 2^49
+            const uint32_t kj = (uint32_t)__builtin_amdgcn_readlane((int)key, j);
+            const uint64_t wj = lane_of(wn, j);
+            before += kj < key || (kj == key && j < lane) ? wj : 0;
+        }
+        if (r.k) on = on && (int)(before >> 52) < r.k;
+        if (r.p < 1.0f) {
+            const double whole = r.k ? (double)wave_sum64(on ? w : 0) : all;
+            const uint64_t need = max((uint64_t)ceil((double)r.p * whole), (uint64_t)1);
+            on = on && (before & ((1ull << 52) - 1)) < need;
+        }
+    }
+    on = on && w >= (uint64_t)ceil((double)r.mp * SF_ONE);
+    const uint64_t mine = on ? w : 0, upto = wave_scan64(mine), total = lane_of(upto, 63), t = sf_draw(a.u[row], total);
+    if (upto > t && upto - mine <= t) {
+        a.out[row] = (int)(wi & 0xfffff);
+        if (a.prob) a.prob[row] = (float)((double)w / (double)total);
+    }
+}
+
+// The same for n <= 512: lane l holds elements l ne .. , so that sums over lanes go by index.
+// Where top-k leaves 64 at most, they go on as above.
+__device__ __forceinline__ void sf_choose_wave(SfLds& s, const lgx_filter_args& a, SfRow r, int row, double all, int n) {
     constexpr int E = SF_FEW / 64;
+    if (n <= 64) {                                // uniform
+        sf_choose_lanes(s, a, r, row, all, n);
+        return;
+    }
     const int lane = threadIdx.x & 63, ne = (n + 63) / 64;
     uint32_t k[E], lo = 0xffffffffu, hi = 0;
     uint64_t wi[E];
@@ -510,6 +591,23 @@ __device__ __forceinline__ void sf_choose_wave(const SfLds& s, const lgx_filter_
             return (uint64_t)c;
         });
         cut(t, r.k - below);
+        if (r.k <= 64) {
+            uint32_t c = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) c += on[e];
+            uint32_t to = (uint32_t)wave_scan((int)c) - c;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (on[e]) {
+                    s.key[to] = k[e];
+                    s.wi[to] = wi[e];
+                }
+                to += on[e];
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave reads what its lanes wrote
+            sf_choose_lanes(s, a, r, row, all, r.k);
+            return;
+        }
     }
     auto sum = [&](auto f) {
         uint64_t v = 0;
@@ -644,17 +742,23 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
     if (r.p < 1.0f && !r.k) tau = fmaxf(tau, M + T * (logf((1.0f - r.p) / (float)V) + logf((float)S) - 0.001f));
     tau -= fmaxf(fabsf(M), fabsf(tau)) * 1e-6f;
     if (!(tau == tau)) tau = M == __builtin_inff() ? M : ninf;
+    // the runs' maxima, a sixteenth of them per wave
+    constexpr int CM = LGX_SF_VOCAB / LGX_SF_CHUNK / SF_NT;
+    const int rw = (nruns + SF_NT - 1) / SF_NT;   // per lane
+    const int c0 = wave * 64 * rw + lane;
+    float cm[CM];
+#pragma unroll
+    for (int j = 0; j < CM; ++j) cm[j] = j < rw && c0 + 64 * j < nruns ? cmax[c0 + 64 * j] : __builtin_nanf("");
     if (r.k && r.k <= nruns) {
-        // a bin of the runs' maxima by which k of them are reached, and its lowest
+        // a bin of theirs by which k of them are reached, and its lowest
         s.bins[tid] = 0;
         if (tid == 0) s.at = 0;
         __syncthreads();
         const SfBins bin(M, fmaxf(tau, -3e38f));
-        for (int c = tid; c < nruns; c += SF_NT) {
-            const float v = cmax[c];
-            if (v >= tau)
-                __hip_atomic_fetch_add((uint32_t*)&s.bins[bin(sf_key(v))], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        }
+#pragma unroll
+        for (int j = 0; j < CM; ++j)
+            if (cm[j] >= tau)
+                __hip_atomic_fetch_add((uint32_t*)&s.bins[bin(sf_key(cm[j]))], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         __syncthreads();
         const uint64_t mine = (uint32_t)s.bins[tid];
         uint64_t total;
@@ -664,10 +768,9 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
             __syncthreads();
             const int at = s.found;
             uint32_t low = 0;
-            for (int c = tid; c < nruns; c += SF_NT) {
-                const float v = cmax[c];
-                if (v >= tau && bin(sf_key(v)) <= at) low = max(low, sf_key(v));
-            }
+#pragma unroll
+            for (int j = 0; j < CM; ++j)
+                if (cm[j] >= tau && bin(sf_key(cm[j])) <= at) low = max(low, sf_key(cm[j]));
             low = wave_max_u32(low);
             if (lane == 0) __hip_atomic_fetch_max(&s.at, low, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             __syncthreads();
@@ -675,25 +778,25 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
             tau = fmaxf(tau, __uint_as_float(key & 0x80000000u ? key : ~key & 0x7fffffffu));
         }
     }
-    // the runs that reach it, in order: a sixteenth of them per wave
-    const int rw = (nruns + SF_NT - 1) / SF_NT * 64;
+    // the runs that reach it, in order
     int mine = 0;
-    for (int c = wave * rw + lane; c < (wave + 1) * rw; c += 64)
-        mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(c < nruns && cmax[min(c, nruns - 1)] >= tau));
-    if (lane == 0) s.wave[wave] = (uint64_t)mine;
+#pragma unroll
+    for (int j = 0; j < CM; ++j) mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(cm[j] >= tau));
+    if (lane == 0) s.dwave[wave] = (double)mine;
     __syncthreads();
     int nr = 0, to = 0;
 #pragma unroll
     for (int w = 0; w < SF_NT / 64; ++w) {
-        const int c = (int)s.wave[w];
+        const int c = (int)s.dwave[w];
         to += w < wave ? c : 0;
         nr += c;
     }
-    for (int c = wave * rw + lane; c < (wave + 1) * rw; c += 64) {
-        const bool on = c < nruns && cmax[min(c, nruns - 1)] >= tau;
-        const uint64_t hit = __builtin_amdgcn_ballot_w64(on);
+    __syncthreads();                              // the bins and these counts are read
+#pragma unroll
+    for (int j = 0; j < CM; ++j) {
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(cm[j] >= tau);
         const int q = to + __builtin_popcountll(hit & ((1ull << lane) - 1));
-        if (on && q < SF_LIST) s.runs[q] = (uint16_t)c;
+        if (cm[j] >= tau && q < SF_LIST) s.runs[q] = (uint16_t)(c0 + 64 * j);
         to += __builtin_popcountll(hit);
     }
     __syncthreads();
@@ -702,21 +805,21 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
     if (nr <= SF_LIST) {
         // their tokens that reach it, in order: a sixteenth of the runs per wave
         const int per = (nr + SF_NT / 64 - 1) / (SF_NT / 64), q0 = min(wave * per, nr), q1 = min(q0 + per, nr);
-        auto tokens = [&](auto f) {               // four runs in flight
-            for (int q = q0; q < q1; q += 4) {
-                float v[4];
-                int t[4];
+        float v[4];
+        int t[4];
+        auto load = [&](int q) {                  // four runs in flight
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    t[u] = s.runs[min(q + u, q1 - 1)] * LGX_SF_CHUNK + lane;
-                    v[u] = t[u] < V && q + u < q1 ? x[t[u]] : __builtin_nanf("");
-                }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) f(t[u], v[u]);
+            for (int u = 0; u < 4; ++u) {
+                t[u] = s.runs[min(q + u, q1 - 1)] * LGX_SF_CHUNK + lane;
+                v[u] = t[u] < V && q + u < q1 ? x[t[u]] : __builtin_nanf("");
             }
         };
         int c = 0;
-        tokens([&](int, float v) { c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v >= tau)); });
+        for (int q = q0; q < q1; q += 4) {
+            load(q);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[u] >= tau));
+        }
         if (lane == 0) s.dwave[wave] = (double)c;
         __syncthreads();
         int n = 0, at = 0;
@@ -727,15 +830,19 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
             n += m;
         }
         if (n <= SF_LIST) {                       // uniform
-            tokens([&](int t, float v) {
-                const uint64_t hit = __builtin_amdgcn_ballot_w64(v >= tau);
-                const int i = at + __builtin_popcountll(hit & ((1ull << lane) - 1));
-                if (v >= tau) {
-                    s.key[i] = sf_key(v);
-                    s.wi[i] = (uint64_t)rint(sf_weight(v, M, r.inv) * SF_ONE) << 20 | (uint64_t)t;
+            for (int q = q0; q < q1; q += 4) {
+                if (q1 - q0 > 4) load(q);         // else still there
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const uint64_t hit = __builtin_amdgcn_ballot_w64(v[u] >= tau);
+                    const int i = at + __builtin_popcountll(hit & ((1ull << lane) - 1));
+                    if (v[u] >= tau) {
+                        s.key[i] = sf_key(v[u]);
+                        s.wi[i] = (uint64_t)rint(sf_weight(v[u], M, r.inv) * SF_ONE) << 20 | (uint64_t)t[u];
+                    }
+                    at += __builtin_popcountll(hit);
                 }
-                at += __builtin_popcountll(hit);
-            });
+            }
             __syncthreads();
             if (n <= SF_FEW) {
                 if (wave == 0) sf_choose_wave(s, a, r, row, all, n);
