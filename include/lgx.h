@@ -431,7 +431,7 @@ lgx_status lgx_kv_keep(lgx_ctx* ctx, const lgx_kv_f16* kv, int32_t layers, const
  * 0.  u below 0 or NaN counts as 0, from 1 on as the last.  Weights are summed in units of
  * 2^-42 or in binary64, so that equal inputs give equal tokens in any batch, and a choice
  * differs from the definition's only where two sums are within about 1e-12 of each
- * other.  vocab <= 2^20, m <= 65535.  Intermediates live in the ctx workspace. */
+ * other.  vocab <= 2^19, m <= 65535.  Intermediates live in the ctx workspace. */
 lgx_status lgx_sample_filtered(lgx_ctx* ctx, const float* logits, int64_t ld, int32_t m, int32_t vocab,
                                const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                                const float* u, int32_t* out, float* prob, void* stream);

@@ -8,44 +8,69 @@
 // descending, index ascending) every filter keeps a prefix, and the draw goes over the
 // kept tokens in order of index.
 //
-// Two launches.  The scan reads every logit once: the largest of each 64 (cmax), the
-// largest of each 4096 and the sum of their weights.  The pick, a workgroup per row,
-// derives from them a logit tau below which no token can be kept, reads again only the
-// runs of 64 whose largest reaches it, and selects among those tokens, in LDS; a row
-// with more of them than fit there is gone over in memory.  A row without filters needs
-// the sums and one run of 4096.
+// The scan reads every logit once: the largest of each 64 (cmax), the largest of each 4096
+// and the sum of their weights.  The pick, a workgroup per row, derives from them a
+// logit tau below which no token can be kept, reads again only the runs of 64 whose largest
+// reaches it, and selects among those tokens, in LDS.  A row without filters needs the
+// sums and one run of 4096.  Rows of which top-p or min-p keep more tokens than that list
+// holds (wide) are left to two more launches: bins of the weights, a workgroup per 4096
+// logits, and the choice from them.
 //
 // Sums decide between tokens, so they are exact or nearly: the weights that a
 // selection adds up are whole multiples of 2^-42 in 64-bit integers, whose sums
 // do not depend on any order; the scan's are binary64.  exp is computed in binary64.
 // ---------------------------------------------------------------------------
-#define SF_ONE 0x1p42                             // 2^20 weights stay below 2^63
+#define SF_ONE 0x1p42                             // 2^19 weights stay below 2^62
 #define SF_LIST 4096                              // tokens kept in LDS
 
-// e^x for x <= 0: Cody-Waite reduction by ln 2 in two parts, then the Taylor polynomial
-// of degree 11 on |r| <= 0.347 (the term after it is under 7e-15).
-__device__ __forceinline__ double sf_exp(double x) {
-    const double n = rint(x * 1.4426950408889634074);
-    double r = fma(-n, 0x1.62e42fefap-1, x);
-    r = fma(-n, 0x1.cf79abc9e3b39p-40, r);
-    double p = 1.0 / 39916800.0;
-    p = fma(p, r, 1.0 / 3628800.0);
-    p = fma(p, r, 1.0 / 362880.0);
-    p = fma(p, r, 1.0 / 40320.0);
-    p = fma(p, r, 1.0 / 5040.0);
-    p = fma(p, r, 1.0 / 720.0);
-    p = fma(p, r, 1.0 / 120.0);
-    p = fma(p, r, 1.0 / 24.0);
+// e^x for x <= 0: x = (64 n + j) ln 2 / 64 + r, 2^(j/64) from a table (sf_roots), e^r by its
+// Taylor polynomial of degree 4 (|r| <= 0.0055: the term after it is under 5e-14).
+#define SF_ROOTS 64
+__device__ __forceinline__ double sf_root_exp(double x, const double* roots, int& n) {
+    const double k = rint(x * (SF_ROOTS * 1.4426950408889634074));
+    const double r = fma(-k, 0.69314718055994530942 / SF_ROOTS, x);
+    double p = 1.0 / 24.0;
     p = fma(p, r, 1.0 / 6.0);
     p = fma(p, r, 0.5);
     p = fma(p, r, 1.0);
     p = fma(p, r, 1.0);
-    return x > -700.0 ? ldexp(p, (int)n) : 0.0;
+    const int i = (int)k;
+    n = i >> 6;                                   // floor
+    return roots[i & (SF_ROOTS - 1)] * p;
+}
+__device__ __forceinline__ double sf_exp(double x, const double* roots) {
+    int n;
+    const double p = sf_root_exp(x, roots, n);
+    return x > -700.0 ? __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + ((uint64_t)(int64_t)n << 52)) : 0.0;
+}
+// In units of 2^-42, rounded, for x > -30.5: a shift of the bits (a conversion of binary64
+// to a 64-bit integer takes as long as all of the above).
+__device__ __forceinline__ uint64_t sf_units(double x, const double* roots) {
+    int n;
+    const uint64_t bits = __builtin_bit_cast(uint64_t, sf_root_exp(x, roots, n));
+    const int down = 52 - 42 + 1023 - (int)(bits >> 52) - n;
+    const uint64_t m = (bits & ((1ull << 52) - 1)) | 1ull << 52;
+    return down > 54 ? 0 : (m + (1ull << (down - 1))) >> down;
+}
+// The table, by threads 0 .. 63: e^x of [0, 0.69) by its Taylor polynomial of degree 17
+// (the term after it is under 2e-19).
+__device__ __forceinline__ void sf_roots(double* roots) {
+    if (threadIdx.x >= SF_ROOTS) return;
+    const double x = threadIdx.x * (0.69314718055994530942 / SF_ROOTS);
+    double p = 1.0;
+#pragma unroll
+    for (int i = 17; i; --i) p = fma(p, x / i, 1.0);
+    roots[threadIdx.x] = p;
 }
 // Weight of logit l by the maximum M; 0 for NaN and -inf, 1 for the maximum, whatever it is.
-__device__ __forceinline__ double sf_weight(float l, float M, double inv) {
+__device__ __forceinline__ double sf_weight(float l, float M, double inv, const double* roots) {
     const double x = ((double)l - (double)M) * inv;
-    return l == M ? 1.0 : l > -__builtin_inff() && l < M ? sf_exp(x) : 0.0;
+    return l == M ? 1.0 : l > -__builtin_inff() && l < M ? sf_exp(x, roots) : 0.0;
+}
+
+__device__ __forceinline__ uint64_t sf_weight_units(float l, float M, double inv, const double* roots) {
+    const double x = ((double)l - (double)M) * inv;
+    return l == M ? 1ull << 42 : l > -__builtin_inff() && x > -30.5 ? sf_units(x, roots) : 0;
 }
 
 struct SfRow {
@@ -73,8 +98,10 @@ __device__ __forceinline__ SfRow sf_row(const lgx_filter_args& a, int row) {
 // Workgroup (4096 logits, row): thread t holds 4 (256 i + t) .. + 3 of them.
 extern "C" __global__ __launch_bounds__(256) void lgx_k_filter_scan(const lgx_filter_args a) {
     __shared__ float mx_s[4];
-    __shared__ double sum_s[4];
+    __shared__ double sum_s[4], roots[SF_ROOTS];
     const int tid = threadIdx.x, sl = blockIdx.x, row = blockIdx.y;
+    if (a.slots && sl == 0 && row == 0 && tid == 0) *a.wide_n = 0;
+    sf_roots(roots);
     const SfRow r = sf_row(a, row);
     const float* x = a.logits + (int64_t)row * a.ld;
     const float ninf = -__builtin_inff();
@@ -110,7 +137,7 @@ extern "C" __global__ __launch_bounds__(256) void lgx_k_filter_scan(const lgx_fi
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s += sf_weight(v[i][c], M, r.inv);
+        for (int c = 0; c < 4; ++c) s += sf_weight(v[i][c], M, r.inv, roots);
 #pragma unroll
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
     if ((tid & 63) == 0) sum_s[tid >> 6] = s;
@@ -127,6 +154,7 @@ __device__ __forceinline__ uint32_t sf_key(float l) {
 #define SF_NT 1024
 #define SF_BINS 1024                              // of a selection's first step
 #define SF_FEW 512                                // elements that one wave chooses among
+#define SF_GUESS 256                              // runs whose tokens are tried first for top-p
 struct SfLds {
     union {
         uint64_t bins[SF_BINS];
@@ -138,6 +166,7 @@ struct SfLds {
     uint32_t few_key[SF_FEW];
     uint64_t wave[SF_NT / 64];
     double dwave[SF_NT / 64];
+    double roots[SF_ROOTS];                       // 2^(j / 64)
     uint64_t below;
     uint32_t at;
     int found, count;
@@ -261,11 +290,12 @@ struct SfInRow {
     int n;
     float tau, M;
     double inv;
+    const double* roots;
     __device__ __forceinline__ float load(int i) const { return x[i]; }
     __device__ __forceinline__ bool valid(float v) const { return v >= tau; }
     __device__ __forceinline__ uint32_t key(float v) const { return sf_key(v); }
     __device__ __forceinline__ int index(float, int i) const { return i; }
-    __device__ __forceinline__ uint64_t weight(float v) const { return (uint64_t)rint(sf_weight(v, M, inv) * SF_ONE); }
+    __device__ __forceinline__ uint64_t weight(float v) const { return sf_weight_units(v, M, inv, roots); }
 };
 // f(element, i) for the elements first, first + step, .. below end
 template <class S, class F>
@@ -290,7 +320,7 @@ struct SfBins {
     __device__ __forceinline__ int operator()(uint32_t key) const {
         const float l = __uint_as_float(key & 0x80000000u ? key : ~key & 0x7fffffffu);
         const float b = (M - l) * scale;
-        return b < (float)(SF_BINS - 1) ? (int)b : SF_BINS - 1;   // (NaN: the last)
+        return b < (float)(SF_BINS - 1) ? max((int)b, 0) : SF_BINS - 1;   // (NaN: the last)
     }
 };
 
@@ -662,10 +692,18 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
     const float* cmax = a.cmax + (int64_t)row * a.nslices * 64;
     const int nruns = (V + LGX_SF_CHUNK - 1) / LGX_SF_CHUNK;
     const float ninf = -__builtin_inff();
-    // the row's maximum: at most 256 slices
+    // the runs' maxima, a sixteenth of them per wave
+    constexpr int CM = LGX_SF_VOCAB / LGX_SF_CHUNK / SF_NT;
+    const int rw = (nruns + SF_NT - 1) / SF_NT;   // per lane
+    const int c0 = wave * 64 * rw + lane;
+    float cm[CM];
+#pragma unroll
+    for (int j = 0; j < CM; ++j) cm[j] = j < rw && c0 + 64 * j < nruns ? cmax[c0 + 64 * j] : __builtin_nanf("");
+    // the row's maximum: at most 128 slices
     float M = ninf;
     for (int i = lane; i < a.nslices; i += 64) M = fmaxf(M, smax[i]);
     M = wave_max(M);
+    sf_roots(s.roots);
     if (M == ninf) {                              // uniform: no token at all
         if (tid == 0) {
             a.out[row] = 0;
@@ -676,8 +714,9 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
     if (r.greedy) {
         if (tid == 0) s.found = 0x7fffffff;
         __syncthreads();
-        for (int c = tid; c < nruns; c += SF_NT)
-            if (cmax[c] == M) __hip_atomic_fetch_min(&s.found, c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+#pragma unroll
+        for (int j = 0; j < CM; ++j)
+            if (cm[j] == M) __hip_atomic_fetch_min(&s.found, c0 + 64 * j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         __syncthreads();
         if (wave) return;
         const int i = s.found * LGX_SF_CHUNK + lane;
@@ -688,10 +727,11 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
         }
         return;
     }
+    __syncthreads();                              // the table
     double S = 0.0;                               // of all weights, by M
     if (r.sums()) {
         const double* sums = a.sum + (int64_t)row * a.nslices;
-        const double mine = tid < a.nslices ? sums[tid] * sf_weight(smax[tid], M, r.inv) : 0.0;
+        const double mine = tid < a.nslices ? sums[tid] * sf_weight(smax[tid], M, r.inv, s.roots) : 0.0;
         const double upto = sf_scan<double>(mine, s.dwave, S);
         if (r.plain()) {
             // the slice that the draw falls into: the last with a weight that starts at
@@ -710,7 +750,7 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
             double w[4], c = 0.0, all;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                w[i] = e0 + i < V ? sf_weight(x[min(e0 + i, V - 1)], M, r.inv) : 0.0;
+                w[i] = e0 + i < V ? sf_weight(x[min(e0 + i, V - 1)], M, r.inv, s.roots) : 0.0;
                 c += w[i];
             }
             double at = sf_scan<double>(c, s.dwave, all) - c;
@@ -742,15 +782,14 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
     if (r.p < 1.0f && !r.k) tau = fmaxf(tau, M + T * (logf((1.0f - r.p) / (float)V) + logf((float)S) - 0.001f));
     tau -= fmaxf(fabsf(M), fabsf(tau)) * 1e-6f;
     if (!(tau == tau)) tau = M == __builtin_inff() ? M : ninf;
-    // the runs' maxima, a sixteenth of them per wave
-    constexpr int CM = LGX_SF_VOCAB / LGX_SF_CHUNK / SF_NT;
-    const int rw = (nruns + SF_NT - 1) / SF_NT;   // per lane
-    const int c0 = wave * 64 * rw + lane;
-    float cm[CM];
-#pragma unroll
-    for (int j = 0; j < CM; ++j) cm[j] = j < rw && c0 + 64 * j < nruns ? cmax[c0 + 64 * j] : __builtin_nanf("");
-    if (r.k && r.k <= nruns) {
-        // a bin of theirs by which k of them are reached, and its lowest
+    // Top-p alone: that bound is loose where a few tokens weigh nearly all.  The tokens from
+    // the 256th largest run's maximum on are tried first: if they reach the share, they
+    // are enough.
+    const bool guess = !r.k && r.p < 1.0f && nruns > 2 * SF_GUESS;
+    const int most = r.k ? r.k : SF_GUESS;
+    float high = tau;
+    if (guess || (r.k && r.k <= nruns)) {
+        // a bin of the runs' maxima by which so many of them are reached, and its lowest
         s.bins[tid] = 0;
         if (tid == 0) s.at = 0;
         __syncthreads();
@@ -763,8 +802,8 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
         const uint64_t mine = (uint32_t)s.bins[tid];
         uint64_t total;
         const uint64_t upto = sf_scan<uint64_t>(mine, s.wave, total);
-        if (total >= (uint64_t)r.k) {             // uniform
-            if (upto >= (uint64_t)r.k && upto - mine < (uint64_t)r.k) s.found = tid;
+        if (total >= (uint64_t)most) {            // uniform
+            if (upto >= (uint64_t)most && upto - mine < (uint64_t)most) s.found = tid;
             __syncthreads();
             const int at = s.found;
             uint32_t low = 0;
@@ -775,83 +814,280 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
             if (lane == 0) __hip_atomic_fetch_max(&s.at, low, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             __syncthreads();
             const uint32_t key = s.at;
-            tau = fmaxf(tau, __uint_as_float(key & 0x80000000u ? key : ~key & 0x7fffffffu));
+            high = fmaxf(tau, __uint_as_float(key & 0x80000000u ? key : ~key & 0x7fffffffu));
         }
     }
-    // the runs that reach it, in order
-    int mine = 0;
-#pragma unroll
-    for (int j = 0; j < CM; ++j) mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(cm[j] >= tau));
-    if (lane == 0) s.dwave[wave] = (double)mine;
-    __syncthreads();
-    int nr = 0, to = 0;
-#pragma unroll
-    for (int w = 0; w < SF_NT / 64; ++w) {
-        const int c = (int)s.dwave[w];
-        to += w < wave ? c : 0;
-        nr += c;
-    }
-    __syncthreads();                              // the bins and these counts are read
-#pragma unroll
-    for (int j = 0; j < CM; ++j) {
-        const uint64_t hit = __builtin_amdgcn_ballot_w64(cm[j] >= tau);
-        const int q = to + __builtin_popcountll(hit & ((1ull << lane) - 1));
-        if (cm[j] >= tau && q < SF_LIST) s.runs[q] = (uint16_t)(c0 + 64 * j);
-        to += __builtin_popcountll(hit);
-    }
-    __syncthreads();
     const double all = S * SF_ONE;
-    const SfBins bin(M, fmaxf(tau, -3e38f));
-    if (nr <= SF_LIST) {
-        // their tokens that reach it, in order: a sixteenth of the runs per wave
-        const int per = (nr + SF_NT / 64 - 1) / (SF_NT / 64), q0 = min(wave * per, nr), q1 = min(q0 + per, nr);
-        float v[4];
-        int t[4];
-        auto load = [&](int q) {                  // four runs in flight
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                t[u] = s.runs[min(q + u, q1 - 1)] * LGX_SF_CHUNK + lane;
-                v[u] = t[u] < V && q + u < q1 ? x[t[u]] : __builtin_nanf("");
-            }
-        };
-        int c = 0;
-        for (int q = q0; q < q1; q += 4) {
-            load(q);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[u] >= tau));
+#pragma unroll 1
+    for (bool first = guess && high > tau;; first = false) {   // uniform
+        if (r.k || first) {
+            const float t = tau;
+            tau = high;
+            high = t;
         }
-        if (lane == 0) s.dwave[wave] = (double)c;
+        // the runs that reach tau, in order
+        int mine = 0;
+#pragma unroll
+        for (int j = 0; j < CM; ++j) mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(cm[j] >= tau));
+        __syncthreads();                          // bins and counts are read
+        if (lane == 0) s.dwave[wave] = (double)mine;
         __syncthreads();
-        int n = 0, at = 0;
+        int nr = 0, to = 0;
 #pragma unroll
         for (int w = 0; w < SF_NT / 64; ++w) {
-            const int m = (int)s.dwave[w];
-            at += w < wave ? m : 0;
-            n += m;
+            const int c = (int)s.dwave[w];
+            to += w < wave ? c : 0;
+            nr += c;
         }
-        if (n <= SF_LIST) {                       // uniform
-            for (int q = q0; q < q1; q += 4) {
-                if (q1 - q0 > 4) load(q);         // else still there
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < CM; ++j) {
+            const uint64_t hit = __builtin_amdgcn_ballot_w64(cm[j] >= tau);
+            const int q = to + __builtin_popcountll(hit & ((1ull << lane) - 1));
+            if (cm[j] >= tau && q < SF_LIST) s.runs[q] = (uint16_t)(c0 + 64 * j);
+            to += __builtin_popcountll(hit);
+        }
+        __syncthreads();
+        int n = SF_LIST + 1;
+        uint64_t weighs = 0;
+        if (nr <= SF_LIST) {
+            // their tokens that reach it, in order: a sixteenth of the runs per wave
+            const int per = (nr + SF_NT / 64 - 1) / (SF_NT / 64), q0 = min(wave * per, nr), q1 = min(q0 + per, nr);
+            float v[4];
+            int t[4];
+            auto load = [&](int q) {              // four runs in flight
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const uint64_t hit = __builtin_amdgcn_ballot_w64(v[u] >= tau);
-                    const int i = at + __builtin_popcountll(hit & ((1ull << lane) - 1));
-                    if (v[u] >= tau) {
-                        s.key[i] = sf_key(v[u]);
-                        s.wi[i] = (uint64_t)rint(sf_weight(v[u], M, r.inv) * SF_ONE) << 20 | (uint64_t)t[u];
-                    }
-                    at += __builtin_popcountll(hit);
+                    t[u] = s.runs[min(q + u, q1 - 1)] * LGX_SF_CHUNK + lane;
+                    v[u] = t[u] < V && q + u < q1 ? x[t[u]] : __builtin_nanf("");
                 }
+            };
+            int c = 0;
+            for (int q = q0; q < q1; q += 4) {
+                load(q);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[u] >= tau));
+            }
+            if (lane == 0) s.dwave[wave] = (double)c;
+            __syncthreads();
+            int at = 0;
+            n = 0;
+#pragma unroll
+            for (int w = 0; w < SF_NT / 64; ++w) {
+                const int m = (int)s.dwave[w];
+                at += w < wave ? m : 0;
+                n += m;
+            }
+            if (n <= SF_LIST) {                   // uniform
+                for (int q = q0; q < q1; q += 4) {
+                    if (q1 - q0 > 4) load(q);     // else still there
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const uint64_t hit = __builtin_amdgcn_ballot_w64(v[u] >= tau);
+                        const int i = at + __builtin_popcountll(hit & ((1ull << lane) - 1));
+                        if (v[u] >= tau) {
+                            const uint64_t w = sf_weight_units(v[u], M, r.inv, s.roots);
+                            weighs += w;
+                            s.key[i] = sf_key(v[u]);
+                            s.wi[i] = w << 20 | (uint64_t)t[u];
+                        }
+                        at += __builtin_popcountll(hit);
+                    }
+                }
+                __syncthreads();
+            }
+        }
+        if (first) {                              // uniform
+            if (n > SF_LIST || (double)sf_sum(weighs, s.wave) < ceil((double)r.p * all)) {
+                tau = high;
+                continue;
+            }
+        }
+        const SfBins bin(M, fmaxf(tau, -3e38f));
+        if (n <= SF_FEW) {
+            if (wave == 0) sf_choose_wave(s, a, r, row, all, n);
+        } else if (n <= SF_LIST) {
+            sf_choose(s, a, r, bin, row, all, SfInLds{s, n});
+        } else if (a.slots && !r.k && tau > -3e38f && M < __builtin_inff()) {
+            // more than LDS holds: the row for lgx_k_filter_wide
+            if (tid == 0) {
+                const int i = atomicAdd(a.wide_n, 1);
+                a.wide_row[i] = row;
+                a.wide_tau[i] = tau;
+                a.wide_all[i] = all;
+            }
+        } else {
+            // the row itself
+            sf_choose(s, a, r, bin, row, all, SfInRow{x, V, tau, M, r.inv, s.roots});
+        }
+        return;
+    }
+}
+
+// Bins of the wide rows' weights, slice by slice: workgroup (slice, rows y, y + gridDim.y ..
+// of the list).
+struct SfSliceBins {
+    float M, scale;
+    __device__ __forceinline__ SfSliceBins(float M, float tau) : M(M), scale((float)LGX_SF_BINS / (M - tau)) {
+        if (!(scale > 0.0f && scale < 1e30f)) scale = 0.0f;
+    }
+    __device__ __forceinline__ int operator()(float l) const {
+        const float b = (M - l) * scale;
+        return b < (float)(LGX_SF_BINS - 1) ? (int)b : LGX_SF_BINS - 1;
+    }
+};
+__device__ __forceinline__ float sf_row_max(const lgx_filter_args& a, int row) {
+    float M = -__builtin_inff();
+    for (int i = threadIdx.x & 63; i < a.nslices; i += 64) M = fmaxf(M, a.smax[(int64_t)row * a.nslices + i]);
+    return wave_max(M);
+}
+extern "C" __global__ __launch_bounds__(256) void lgx_k_filter_bins(const lgx_filter_args a) {
+    __shared__ uint64_t bins[LGX_SF_BINS];
+    __shared__ double roots[SF_ROOTS];
+    static_assert(LGX_SF_BINS == 256, "a thread per bin");
+    const int tid = threadIdx.x, sl = blockIdx.x, n = min(*a.wide_n, a.slots);
+    if ((int)blockIdx.y >= n) return;
+    sf_roots(roots);
+    for (int w = blockIdx.y; w < n; w += gridDim.y) {
+        const int row = a.wide_row[w];
+        const float tau = a.wide_tau[w], M = sf_row_max(a, row);
+        const double inv = sf_row(a, row).inv;
+        const float* x = a.logits + (int64_t)row * a.ld;
+        const SfSliceBins bin(M, tau);
+        bins[tid] = 0;
+        __syncthreads();
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int e = sl * LGX_SF_SLICE + 256 * i + tid;
+            v[i] = e < a.vocab ? x[e] : __builtin_nanf("");
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (v[i] >= tau)
+                __hip_atomic_fetch_add(&bins[bin(v[i])], sf_weight_units(v[i], M, inv, roots), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        __syncthreads();
+        a.hist[((int64_t)w * a.nslices + sl) * LGX_SF_BINS + tid] = bins[tid];
+        __syncthreads();
+    }
+}
+
+// The choice in a wide row, from the bins of its slices: the bin in which top-p ends, the
+// tokens in it, then what is kept of each slice, the slice that the draw falls into and
+// the token in it.
+extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_wide(const lgx_filter_args a) {
+    __shared__ SfLds s;
+    const int tid = threadIdx.x, lane = tid & 63, V = a.vocab, all_rows = *a.wide_n;
+    for (int w = blockIdx.x; w < all_rows; w += gridDim.x) {   // uniform
+        const int row = a.wide_row[w];
+        const float tau = a.wide_tau[w], M = sf_row_max(a, row);
+        const double all = a.wide_all[w];
+        const SfRow r = sf_row(a, row);
+        const float* x = a.logits + (int64_t)row * a.ld;
+        const SfInRow e{x, V, tau, M, r.inv, s.roots};
+        __syncthreads();
+        sf_roots(s.roots);
+        const SfSliceBins bin(M, tau);
+        const uint64_t* hist = a.hist + (int64_t)w * a.nslices * LGX_SF_BINS;
+        // weight per bin: four threads a bin, each a quarter of the slices
+        uint64_t mine = 0, total;
+        if (w < a.slots)
+            for (int i = tid >> 8; i < a.nslices; i += SF_NT / LGX_SF_BINS) mine += hist[i * LGX_SF_BINS + (tid & 255)];
+        s.bins[tid] = mine;
+        if (tid == 0) s.count = 0;
+        __syncthreads();
+        mine = tid < LGX_SF_BINS ? s.bins[tid] + s.bins[tid + 256] + s.bins[tid + 512] + s.bins[tid + 768] : 0;
+        const uint64_t upto = sf_scan<uint64_t>(mine, s.wave, total);
+        const uint64_t need = max((uint64_t)ceil((double)r.p * all), (uint64_t)1), low = (uint64_t)ceil((double)r.mp * SF_ONE);
+        // first: the first bin of which not all tokens are known to be kept
+        int first = LGX_SF_BINS;
+        if (r.mp > 0.0f) first = min(first, bin(fminf(M + (float)(1.0 / r.inv) * (logf(r.mp) + 0.001f), M)));
+        uint32_t last = 0xffffffffu;              // kept: key < last, or key == last and index <= most
+        int most = 0x7fffffff;
+        bool few = w < a.slots;
+        if (few && r.p < 1.0f && need <= total) { // uniform
+            if (upto >= need && upto - mine < need) {
+                s.found = tid;
+                s.below = upto - mine;
             }
             __syncthreads();
-            if (n <= SF_FEW) {
-                if (wave == 0) sf_choose_wave(s, a, r, row, all, n);
-            } else {
-                sf_choose(s, a, r, bin, row, all, SfInLds{s, n});
+            const int at = s.found;
+            const uint64_t base = s.below;
+            first = min(first, at);
+            sf_each(e, tid, V, SF_NT, [&](float v, int) {
+                if (!(v >= tau) || bin(v) != at) return;
+                const int i = __hip_atomic_fetch_add(&s.count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                if (i < SF_LIST) {
+                    s.key[i] = sf_key(v);
+                    s.wi[i] = sf_weight_units(v, M, r.inv, s.roots) << 20;
+                }
+            });
+            __syncthreads();
+            const int n = s.count;
+            few = n <= SF_LIST;
+            if (few) {                            // uniform
+                SfCut c;
+                const float wide = bin.scale > 0.0f ? 1.0f / bin.scale : 0.0f;
+                const SfBins sub(fminf(M, M - (float)at * wide + 1e-6f * fabsf(M)), fmaxf(tau, M - (float)(at + 1) * wide));
+                sf_select(s, sub, need - base, c, [&](auto f) {
+                    for (int i = tid; i < n; i += SF_NT) f(s.key[i], [&] { return s.wi[i] >> 20; });
+                });
+                last = c.key;
+                const uint64_t m = (need - base - c.below + c.one - 1) / c.one;
+                if (m < c.equal) most = sf_first(s, e, m - 1, [&](float v, int) { return (uint64_t)(v >= tau && sf_key(v) == last); });
             }
-            return;
+        }
+        if (!few) {                               // equal or nearly equal logits, or no room for bins
+            sf_choose(s, a, r, SfBins(M, tau), row, all, e);
+            continue;
+        }
+        // what is kept of each slice: its bins below `first`, and tokens from there on
+        auto kept = [&](float v, int i) {
+            const uint32_t k = sf_key(v);
+            const uint64_t u = v >= tau && (k < last || (k == last && i <= most)) ? sf_weight_units(v, M, r.inv, s.roots) : 0;
+            return u >= low ? u : 0;
+        };
+        __syncthreads();
+        if (tid < LGX_SF_VOCAB / LGX_SF_SLICE) s.few[tid] = 0;
+        __syncthreads();
+        for (int i = tid >> 6; i < a.nslices; i += SF_NT / 64) {
+            uint64_t m = 0;
+            for (int b = lane; b < first; b += 64) m += hist[i * LGX_SF_BINS + b];
+            m = wave_sum64(m);
+            if (lane == 0) __hip_atomic_fetch_add(&s.few[i], m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+        if (first < LGX_SF_BINS)
+            sf_each(e, tid, V, SF_NT, [&](float v, int i) {
+                if (v >= tau && sf_key(v) <= last && bin(v) >= first)
+                    __hip_atomic_fetch_add(&s.few[i / LGX_SF_SLICE], kept(v, i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            });
+        __syncthreads();
+        mine = tid < a.nslices ? s.few[tid] : 0;
+        const uint64_t to = sf_scan<uint64_t>(mine, s.wave, total), t = sf_draw(a.u[row], total);
+        if (to > t && to - mine <= t) {
+            s.found = tid;
+            s.below = to - mine;
+        }
+        __syncthreads();
+        const int sl = s.found;
+        const uint64_t in = t - s.below;
+        const int i0 = sl * LGX_SF_SLICE + 4 * tid;
+        uint64_t u[4], c = 0, sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            u[i] = i0 + i < V ? kept(x[min(i0 + i, V - 1)], i0 + i) : 0;
+            c += u[i];
+        }
+        uint64_t at = sf_scan<uint64_t>(c, s.wave, sum) - c;
+        bool done = at > in || at + c <= in;      // not this thread's
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            at += u[i];
+            if (!done && at > in) {
+                done = true;
+                a.out[row] = i0 + i;
+                if (a.prob) a.prob[row] = (float)((double)u[i] / (double)total);
+            }
         }
     }
-    // more than LDS holds: the row itself
-    sf_choose(s, a, r, bin, row, all, SfInRow{x, V, tau, M, r.inv});
 }

@@ -191,6 +191,8 @@ enum Kern {
     K_KV_KEEP_D128,
     K_FILTER_SCAN,
     K_FILTER_PICK,
+    K_FILTER_BINS,
+    K_FILTER_WIDE,
     K_TREE_ATTN_D64, // 16 columns; + 1: with caps, distances or a window; + 2, + 4: 64, 128 columns
     K_TREE_ATTN_D128 = K_TREE_ATTN_D64 + 6,
     K_COUNT = K_TREE_ATTN_D128 + 5
@@ -250,7 +252,7 @@ inline const char* const kKernelNames[] = {
     "lgx_k_attn8_join_d64", "lgx_k_attn8_joinw_d64", "lgx_k_attn8_join_d128", "lgx_k_attn8_joinw_d128",
     "lgx_k_pages_fork", "lgx_k_pages_free", "lgx_k_pages_reserve", "lgx_k_pages_copy",
     "lgx_k_append_rows_d64", "lgx_k_append_rows_d128", "lgx_k_tree_plan", "lgx_k_tree_accept",
-    "lgx_k_kv_keep_d64", "lgx_k_kv_keep_d128", "lgx_k_filter_scan", "lgx_k_filter_pick",
+    "lgx_k_kv_keep_d64", "lgx_k_kv_keep_d128", "lgx_k_filter_scan", "lgx_k_filter_pick", "lgx_k_filter_bins", "lgx_k_filter_wide",
     "lgx_k_tree_attn_d64_c16", "lgx_k_tree_attnx_d64_c16", "lgx_k_tree_attn_d64_c64",
     "lgx_k_tree_attnx_d64_c64", "lgx_k_tree_attn_d64_c128", "lgx_k_tree_attnx_d64_c128",
     "lgx_k_tree_attn_d128_c16", "lgx_k_tree_attnx_d128_c16", "lgx_k_tree_attn_d128_c64",

@@ -604,7 +604,8 @@ typedef struct {
 // ---- sampling with per-row settings (lgx_filter.hip) ----
 #define LGX_SF_CHUNK 64        // logits whose largest is kept
 #define LGX_SF_SLICE 4096      // logits of a workgroup of the scan
-#define LGX_SF_VOCAB (1 << 20)
+#define LGX_SF_VOCAB (1 << 19)
+#define LGX_SF_BINS 256        // bins of a wide row's slice
 typedef struct {
     const float* logits;       // [m] rows of vocab, ld apart
     const float* temperature;  // [m], nullable: 1
@@ -617,7 +618,14 @@ typedef struct {
     double* sum;               // [m][nslices] of exp((l - slice maximum) / T)
     float* smax;               // [m][nslices]
     float* cmax;               // [m][nslices * 64]
+    // rows whose kept tokens are too many for one workgroup's list (lgx_k_filter_bins, _wide)
+    int32_t* wide_n;           // [1] their number
+    int32_t* wide_row;         // [m]
+    float* wide_tau;           // [m]
+    double* wide_all;          // [m]
+    uint64_t* hist;            // [slots][nslices][LGX_SF_BINS]
     int64_t ld;
     int32_t m, vocab, nslices;
     int32_t vec;               // rows are 16-byte aligned
+    int32_t slots;             // wide rows with room for their bins; 0: no row can be wide
 } lgx_filter_args;

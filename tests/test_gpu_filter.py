@@ -189,3 +189,32 @@ def test_argument_checks(ctx):
             bad()
     with pytest.raises(lgx.LgxError):
         ctx.sample_filtered(x[:1].expand(2, 10), u)
+
+
+@pytest.mark.parametrize("V", [20000, 151936])
+def test_many_wide_rows_among_others(ctx, V):
+    """Rows whose kept tokens are more than one workgroup lists, by top-p, min-p and both, with
+    ties at the border, beside rows of every other kind."""
+    rng = np.random.default_rng(V)
+    sets = list(itertools.product((1.0, 1.7, 0.0), (0, 40), (1.0, 0.9, 0.5, 0.99), (0.0, 0.3, 0.02)))
+    x = (0.5 * rng.standard_normal((len(sets), V))).astype(np.float32)
+    T, k, p, mp = (np.array(c) for c in zip(*sets))
+    check(ctx, x, rng.random(len(sets), dtype=np.float32), T, k, p, mp)
+    check(ctx, np.round(x, 1), rng.random(len(sets), dtype=np.float32), T, k, p, mp)
+    one = np.where(rng.random(x.shape) < 0.9, np.float32(0.25), x)     # most of a row in one logit
+    check(ctx, one, rng.random(len(sets), dtype=np.float32), T, k, p, mp)
+
+
+def test_more_wide_rows_than_there_is_room_for(ctx):
+    """Bins of 64 MiB hold some 1300 rows of 100000 logits."""
+    m, V = 1500, 100000
+    x = torch.randn(1, V, device=ctx.dev) * 0.2
+    wide = x.expand(m, V).contiguous()
+    p = torch.full((m,), 0.9, device=ctx.dev)
+    u = torch.linspace(0, 0.9999, m, device=ctx.dev)
+    out, prob = ctx.sample_filtered(wide, u, top_p=p)
+    row = x[0].cpu().numpy()
+    for i in (0, 1, 700, 1299, 1300, 1420, 1499):
+        want, share = ref_.choose(row, float(u[i]), p=np.float32(0.9))
+        assert int(out[i]) == want and abs(float(prob[i]) - share) <= 2.0 ** -24 * share + 1e-12
+    assert (out[1:] >= out[:-1]).all()
