@@ -151,6 +151,8 @@ __device__ __forceinline__ uint32_t sf_key(float l) {
     return u & 0x80000000u ? u : ~(u | 0x80000000u);
 }
 
+__device__ __forceinline__ float sf_logit(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key : ~key & 0x7fffffffu); }
+
 #define SF_NT 1024
 #define SF_BINS 1024                              // of a selection's first step
 #define SF_FEW 512                                // elements that one wave chooses among
@@ -310,6 +312,34 @@ __device__ __forceinline__ void sf_each(const S& e, int first, int end, int step
     }
 }
 
+// f(logit, index) for a row's logits, 16 in flight per thread.
+template <class F>
+__device__ __forceinline__ void sf_row_each(const float* x, int V, int vec, const F& f) {
+    const int tid = threadIdx.x, n4 = vec ? V / 4 : 0;
+    for (int i0 = tid; i0 < n4; i0 += 4 * SF_NT) {
+        float4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = ((const float4*)x)[min(i0 + u * SF_NT, n4 - 1)];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = 4 * (i0 + u * SF_NT);
+            if (i >= 4 * n4) break;
+            f(v[u].x, i);
+            f(v[u].y, i + 1);
+            f(v[u].z, i + 2);
+            f(v[u].w, i + 3);
+        }
+    }
+    for (int i0 = 4 * n4 + tid; i0 < V; i0 += 8 * SF_NT) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = x[min(i0 + u * SF_NT, V - 1)];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (i0 + u * SF_NT < V) f(v[u], i0 + u * SF_NT);
+    }
+}
+
 // Bin of a key: linear in the logit between the row's maximum and tau, so that keys of
 // one bin follow each other.  A constant for all calls of a row.
 struct SfBins {
@@ -318,8 +348,7 @@ struct SfBins {
         if (!(scale > 0.0f && scale < 1e30f)) scale = 0.0f;   // one logit, or an infinite range: one bin
     }
     __device__ __forceinline__ int operator()(uint32_t key) const {
-        const float l = __uint_as_float(key & 0x80000000u ? key : ~key & 0x7fffffffu);
-        const float b = (M - l) * scale;
+        const float b = (M - sf_logit(key)) * scale;
         return b < (float)(SF_BINS - 1) ? max((int)b, 0) : SF_BINS - 1;   // (NaN: the last)
     }
 };
@@ -814,7 +843,7 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
             if (lane == 0) __hip_atomic_fetch_max(&s.at, low, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             __syncthreads();
             const uint32_t key = s.at;
-            high = fmaxf(tau, __uint_as_float(key & 0x80000000u ? key : ~key & 0x7fffffffu));
+            high = fmaxf(tau, sf_logit(key));
         }
     }
     const double all = S * SF_ONE;
@@ -984,7 +1013,6 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_wide(const lgx_
         const double all = a.wide_all[w];
         const SfRow r = sf_row(a, row);
         const float* x = a.logits + (int64_t)row * a.ld;
-        const SfInRow e{x, V, tau, M, r.inv, s.roots};
         __syncthreads();
         sf_roots(s.roots);
         const SfSliceBins bin(M, tau);
@@ -999,54 +1027,69 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_wide(const lgx_
         mine = tid < LGX_SF_BINS ? s.bins[tid] + s.bins[tid + 256] + s.bins[tid + 512] + s.bins[tid + 768] : 0;
         const uint64_t upto = sf_scan<uint64_t>(mine, s.wave, total);
         const uint64_t need = max((uint64_t)ceil((double)r.p * all), (uint64_t)1), low = (uint64_t)ceil((double)r.mp * SF_ONE);
-        // first: the first bin of which not all tokens are known to be kept
-        int first = LGX_SF_BINS;
-        if (r.mp > 0.0f) first = min(first, bin(fminf(M + (float)(1.0 / r.inv) * (logf(r.mp) + 0.001f), M)));
-        uint32_t last = 0xffffffffu;              // kept: key < last, or key == last and index <= most
-        int most = 0x7fffffff;
+        // of bins first .. end not all tokens are known to be kept or not: those are listed
+        int first = LGX_SF_BINS, end = LGX_SF_BINS - 1;
+        if (r.mp > 0.0f) first = bin(fminf(M + (float)(1.0 / r.inv) * (logf(r.mp) + 0.001f), M));
+        uint64_t base = 0;                        // weight of the bins below `end`
         bool few = w < a.slots;
-        if (few && r.p < 1.0f && need <= total) { // uniform
+        const bool cut = few && r.p < 1.0f && need <= total;
+        if (cut) {                                // uniform
             if (upto >= need && upto - mine < need) {
                 s.found = tid;
                 s.below = upto - mine;
             }
             __syncthreads();
-            const int at = s.found;
-            const uint64_t base = s.below;
-            first = min(first, at);
-            sf_each(e, tid, V, SF_NT, [&](float v, int) {
-                if (!(v >= tau) || bin(v) != at) return;
-                const int i = __hip_atomic_fetch_add(&s.count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                if (i < SF_LIST) {
-                    s.key[i] = sf_key(v);
-                    s.wi[i] = sf_weight_units(v, M, r.inv, s.roots) << 20;
+            end = s.found;
+            base = s.below;
+            first = min(first, end);
+        }
+        int n = 0;
+        if (few && first < LGX_SF_BINS) {         // uniform
+            sf_row_each(x, V, a.vec, [&](float v, int i) {
+                if (!(v >= tau)) return;
+                const int b = bin(v);
+                if (b < first || b > end) return;
+                const int to = __hip_atomic_fetch_add(&s.count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                if (to < SF_LIST) {
+                    s.key[to] = sf_key(v);
+                    s.wi[to] = sf_weight_units(v, M, r.inv, s.roots) << 20 | (uint64_t)i;
                 }
             });
             __syncthreads();
-            const int n = s.count;
+            n = s.count;
             few = n <= SF_LIST;
-            if (few) {                            // uniform
-                SfCut c;
-                const float wide = bin.scale > 0.0f ? 1.0f / bin.scale : 0.0f;
-                const SfBins sub(fminf(M, M - (float)at * wide + 1e-6f * fabsf(M)), fmaxf(tau, M - (float)(at + 1) * wide));
-                sf_select(s, sub, need - base, c, [&](auto f) {
-                    for (int i = tid; i < n; i += SF_NT) f(s.key[i], [&] { return s.wi[i] >> 20; });
-                });
-                last = c.key;
-                const uint64_t m = (need - base - c.below + c.one - 1) / c.one;
-                if (m < c.equal) most = sf_first(s, e, m - 1, [&](float v, int) { return (uint64_t)(v >= tau && sf_key(v) == last); });
-            }
         }
         if (!few) {                               // equal or nearly equal logits, or no room for bins
-            sf_choose(s, a, r, SfBins(M, tau), row, all, e);
+            sf_choose(s, a, r, SfBins(M, tau), row, all, SfInRow{x, V, tau, M, r.inv, s.roots});
             continue;
         }
-        // what is kept of each slice: its bins below `first`, and tokens from there on
-        auto kept = [&](float v, int i) {
-            const uint32_t k = sf_key(v);
-            const uint64_t u = v >= tau && (k < last || (k == last && i <= most)) ? sf_weight_units(v, M, r.inv, s.roots) : 0;
-            return u >= low ? u : 0;
-        };
+        uint32_t last = 0xffffffffu;              // kept: key < last, or key == last and index <= most
+        int most = 0x7fffffff;
+        if (cut) {
+            auto ends = [&](int i) { return bin(sf_logit(s.key[i])) == end; };
+            SfCut c;
+            const float wide = bin.scale > 0.0f ? 1.0f / bin.scale : 0.0f;
+            const SfBins sub(fminf(M, M - (float)end * wide + 1e-6f * fabsf(M)), fmaxf(tau, M - (float)(end + 1) * wide));
+            sf_select(s, sub, need - base, c, [&](auto f) {
+                for (int i = tid; i < n; i += SF_NT)
+                    if (ends(i)) f(s.key[i], [&] { return s.wi[i] >> 20; });
+            });
+            last = c.key;
+            const uint64_t m = (need - base - c.below + c.one - 1) / c.one;
+            if (m < c.equal) {                    // the m-th lowest index among the equal ones
+                int lo = 0, hi = V - 1;
+                while (lo < hi) {                 // uniform
+                    const int mid = (lo + hi) / 2;
+                    uint64_t q = 0;
+                    for (int i = tid; i < n; i += SF_NT) q += s.key[i] == last && (int)(s.wi[i] & 0xfffff) <= mid;
+                    if (sf_sum(q, s.wave) >= m) hi = mid;
+                    else lo = mid + 1;
+                }
+                most = lo;
+            }
+        }
+        // what is kept of each slice: its bins below `first`, and tokens of the list
+        auto keeps = [&](uint32_t k, int i, uint64_t u) { return (k < last || (k == last && i <= most)) && u >= low ? u : 0; };
         __syncthreads();
         if (tid < LGX_SF_VOCAB / LGX_SF_SLICE) s.few[tid] = 0;
         __syncthreads();
@@ -1056,11 +1099,12 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_wide(const lgx_
             m = wave_sum64(m);
             if (lane == 0) __hip_atomic_fetch_add(&s.few[i], m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         }
-        if (first < LGX_SF_BINS)
-            sf_each(e, tid, V, SF_NT, [&](float v, int i) {
-                if (v >= tau && sf_key(v) <= last && bin(v) >= first)
-                    __hip_atomic_fetch_add(&s.few[i / LGX_SF_SLICE], kept(v, i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            });
+        for (int i = tid; i < n; i += SF_NT) {
+            const uint64_t wi = s.wi[i];
+            const int at = (int)(wi & 0xfffff);
+            __hip_atomic_fetch_add(&s.few[at / LGX_SF_SLICE], keeps(s.key[i], at, wi >> 20), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+        auto kept = [&](float v, int i) { return v >= tau ? keeps(sf_key(v), i, sf_weight_units(v, M, r.inv, s.roots)) : 0; };
         __syncthreads();
         mine = tid < a.nslices ? s.few[tid] : 0;
         const uint64_t to = sf_scan<uint64_t>(mine, s.wave, total), t = sf_draw(a.u[row], total);
