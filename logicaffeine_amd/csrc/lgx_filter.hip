@@ -879,7 +879,8 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
         __syncthreads();
         int n = SF_LIST + 1;
         uint64_t weighs = 0;
-        if (nr <= SF_LIST) {
+        // (runs have a token each at least; one workgroup takes 1 us for 64 of them)
+        if (nr <= (a.slots && !r.k ? SF_LIST / 4 : SF_LIST)) {
             // their tokens that reach it, in order: a sixteenth of the runs per wave
             const int per = (nr + SF_NT / 64 - 1) / (SF_NT / 64), q0 = min(wave * per, nr), q1 = min(q0 + per, nr);
             float v[4];
