@@ -168,7 +168,8 @@ struct Tree {
     __device__ __forceinline__ int back(int t, int dj) const { return t < sl ? sl + dj - t : dj - depth(min(t - sl, n - 1)); }
 };
 
-// One column: q's scale, the ALiBi slope, its node and depth; running maximum (base 2) and sum.
+// One column: q's scale, the distance slope, its node and depth; running maximum (base 2), and
+// sum of weights times 2^10.
 struct TreeCol {
     float f, slope, m, l;
     int j, dj;
@@ -269,15 +270,14 @@ __device__ __forceinline__ void tree_weights(const W& w, float (&S)[16], TreeCol
         k.l *= down;
         k.m = mn;
     }
-    const float off = k.m == -inf ? 0.0f : -k.m;  // nothing seen yet: weights of 0
-    float ps = 0.0f;
+    const float off = TREE_UP - (k.m == -inf ? 0.0f : k.m);   // nothing seen yet: weights of 0
+    float ps[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         S[e] = __builtin_amdgcn_exp2f(EDGE ? S[e] + off : fmaf(S[e], k.f, off));
-        ps += S[e];
-        S[e] *= (float)(1 << TREE_UP);
+        ps[e & 1] += S[e];
     }
-    k.l += ps;
+    k.l += ps[0] + ps[1];
     uint32_t hw[8], lw[8];
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
@@ -340,7 +340,7 @@ __device__ __forceinline__ void tree_store(const W& w, int c, const TreeCol& k, 
     const bool part = w.ns > 1, on = c < w.ncols;
     const int64_t at = part ? ((int64_t)w.pos * a.hkv + w.g) * NC + c - w.c0 : w.orow(on ? c : 0);
     float* dst = (part ? a.part : a.out) + at * D;
-    const float r = k.l == 0.0f ? 0.0f : 1.0f / (k.l * (float)(1 << TREE_UP));   // nothing seen gives zeros
+    const float r = k.l == 0.0f ? 0.0f : 1.0f / k.l, l = k.l * (1.0f / (1 << TREE_UP));   // nothing seen gives zeros
     bool bad = false;
     if (on) {
 #pragma unroll
@@ -349,15 +349,15 @@ __device__ __forceinline__ void tree_store(const W& w, int c, const TreeCol& k, 
             *(float4*)(dst + 16 * i + 4 * kg) = make_float4(x[0], x[1], x[2], x[3]);
             bad = bad || !(fabsf(x[0]) + fabsf(x[1]) + fabsf(x[2]) + fabsf(x[3]) < __builtin_inff());
         }
-        if (part && kg == 0) *(float2*)(a.ml + 2 * at) = make_float2(k.m, k.l);
+        if (part && kg == 0) *(float2*)(a.ml + 2 * at) = make_float2(k.m, l);
     }
-    uint64_t again = __builtin_amdgcn_ballot_w64(bad && k.l == k.l);
+    uint64_t again = __builtin_amdgcn_ballot_w64(bad && l == l);
     again = (again | again >> 16 | again >> 32 | again >> 48) & 0xffff;
     if (again) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the first results are written
     while (again) {
         const int i = __builtin_ctzll(again);
         again &= again - 1;
-        tree_column<D, X>(w, __shfl(c, i, 64), __shfl(k.m, i, 64), __shfl(k.l, i, 64),
+        tree_column<D, X>(w, __shfl(c, i, 64), __shfl(k.m, i, 64), __shfl(l, i, 64),
                           (float*)__shfl((unsigned long long)(uintptr_t)dst, i, 64));
     }
 }
@@ -468,15 +468,18 @@ __device__ __forceinline__ void tree_narrow_body(const lgx_tree_attn_args& a) {
         const Pages pn = p;
         v8h ph[2], pl[2];
         float S[16];
+        {
+            v4f acc[4];                           // the four sub-tiles' chains side by side
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int part = 1; part >= 0; --part)
+                for (int part = 1; part >= 0; --part)
 #pragma unroll
-                for (int s = 0; s < NS; ++s) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_v8h(kw[u][s]), qh[part][s], acc, 0, 0, 0);
+                    for (int u = 0; u < 4; ++u)
+                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            as_v8h(kw[u][s]), qh[part][s], s == 0 && part == 1 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : acc[u], 0, 0, 0);
 #pragma unroll
-            for (int v = 0; v < 4; ++v) S[4 * u + v] = acc[v];
+            for (int e = 0; e < 16; ++e) S[e] = acc[e >> 2][e & 3];
         }
         load_k(pn);
         p = Pages(w, min(t + 2 * WT, mine));
@@ -488,13 +491,22 @@ __device__ __forceinline__ void tree_narrow_body(const lgx_tree_attn_args& a) {
                 if (t0 + i / CH >= T) *(uint4*)(v_s[wt] + i * 8) = make_uint4(0u, 0u, 0u, 0u);
         }
 #pragma unroll
-        for (int i = 0; i < ND; ++i) {
-            const v8h v0 = TreeV<D>::operand(vb, i, 0, col, kg), v1 = TreeV<D>::operand(vb, i, 1, col, kg);
-            v4f r = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[0], (v4f){0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-            r = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[0], r, 0, 0, 0);
-            r = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[1], r, 0, 0, 0);
-            r = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[1], r, 0, 0, 0);
-            o[i] += r;
+        for (int g = 0; g < ND / 4; ++g) {
+            v4f r[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                v8h vf[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vf[i] = TreeV<D>::operand(vb, 4 * g + i, h, col, kg);
+#pragma unroll
+                for (int part = 1; part >= 0; --part)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        r[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            vf[i], part ? pl[h] : ph[h], h == 0 && part == 1 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : r[i], 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[4 * g + i] += r[i];
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // V is read before the next overwrites it
         load_v(pn);
@@ -601,41 +613,62 @@ __device__ __forceinline__ void tree_wide_body(const lgx_tree_attn_args& a) {
         const lds_u16* ks = (const lds_u16*)kv_s[cur][0];
         const lds_u16* vs = (const lds_u16*)kv_s[cur][1];
         float S[NT][16];
+        {
+            // the four sub-tiles' chains side by side, operands a step ahead
+            v4f acc[NT][4];
+            v8h kf[2][4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            v4f acc[NT];
+            for (int u = 0; u < 4; ++u) kf[0][u] = TreeK<D>::operand(ks, u, 0, col, kg);
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
-                const v8h kf = TreeK<D>::operand(ks, u, s, col, kg);
+                if (s + 1 < NS) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) kf[(s + 1) & 1][u] = TreeK<D>::operand(ks, u, s + 1, col, kg);
+                }
 #pragma unroll
                 for (int part = 1; part >= 0; --part)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            kf, qh[n][part][s], s == 0 && part == 1 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : acc[n], 0, 0, 0);
+                    for (int u = 0; u < 4; ++u)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            acc[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                kf[s & 1][u], qh[n][part][s], s == 0 && part == 1 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : acc[n][u], 0, 0, 0);
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int v = 0; v < 4; ++v) S[n][4 * u + v] = acc[n][v];
+                for (int e = 0; e < 16; ++e) S[n][e] = acc[n][e >> 2][e & 3];
         }
         v8h ph[NT][2], pl[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) tree_weights<X, edge, ND>(w, S[n], k[n], t0, kg, ph[n], pl[n], o[n]);
+        // 64 or 32 dimensions at a time, their chains side by side, operands a step ahead
+        constexpr int G = 4 / NT, NG = ND / G;
+        v8h vf[2][G];
 #pragma unroll
-        for (int i = 0; i < ND; ++i) {
-            const v8h v0 = TreeV<D>::operand(vs, i, 0, col, kg), v1 = TreeV<D>::operand(vs, i, 1, col, kg);
-            v4f r[NT];
+        for (int i = 0; i < G; ++i) vf[0][i] = TreeV<D>::operand(vs, i, 0, col, kg);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) r[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[n][0], (v4f){0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+        for (int g = 0; g < NG; ++g) {
+            v4f r[NT][G];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) r[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[n][0], r[n], 0, 0, 0);
+            for (int h = 0; h < 2; ++h) {
+                if (h == 0 || g + 1 < NG) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) r[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[n][1], r[n], 0, 0, 0);
+                    for (int i = 0; i < G; ++i) vf[h ^ 1][i] = TreeV<D>::operand(vs, G * (g + h) + i, h ^ 1, col, kg);
+                }
 #pragma unroll
-            for (int n = 0; n < NT; ++n) r[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[n][1], r[n], 0, 0, 0);
+                for (int part = 1; part >= 0; --part)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) o[n][i] += r[n];
+                    for (int i = 0; i < G; ++i)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            r[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                vf[h][i], part ? pl[n][h] : ph[n][h], h == 0 && part == 1 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : r[n][i], 0, 0, 0);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < G; ++i) o[n][G * g + i] += r[n][i];
         }
     };
     // the tiles of cached tokens alone, then the others
