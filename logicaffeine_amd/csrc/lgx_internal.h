@@ -328,6 +328,7 @@ struct lgx_ctx {
     int pfa_rows = 0;             // LGX_PFA_ROWS: force 32 / 16 (query row, head) pairs per prefill attention workgroup
     int attn8_wgs = 1;            // LGX_A8_WGS: workgroups per compute unit the 8-bit cache's attention splits for
     int attn8_cols = 0;           // LGX_A8_COLS: force 16 / 32 / 128 (row, head) pairs per workgroup of it (0: by size)
+    int tree_wgs = 2;             // LGX_TREE_WGS: workgroups per compute unit the drafts' attention splits for
     int tree_cols = 0;            // LGX_TREE_COLS: force 16 / 64 / 128 (node, head) pairs per workgroup of the drafts' attention (0: by size)
     bool prefill_serial = false;  // LGX_PREFILL=serial: prefill as P decode passes
     int prefill_chunk = 0;        // LGX_PREFILL_CHUNK: positions per prefill chunk (0: by batch)

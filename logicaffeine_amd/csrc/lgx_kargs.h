@@ -588,16 +588,16 @@ typedef struct {
     const uint64_t* mask;      // [B][N][words], nullable: nodes 0 .. j
     const float* slopes;       // [hq], nullable
     float* out;                // [B*N][hq][d]
-    // per > 0: the tiles of every (sequence, column block) are split on the device so
-    // that `per` workgroups per KV head share all of them (see Tree::place); the
-    // partial results are lgx_k_attn8_join_*'s
+    // per > 0: the sequences' tiles are split on the device so that `per` workgroups per
+    // KV head share all of them and their column blocks (see Tree::place); the partial
+    // results are lgx_k_attn8_join_*'s
     float* part;               // [per][hkv][columns][d]: results of splits
     float* ml;                 // [per][hkv][columns][2]: their maxima and sums
     int32_t* plan;             // [B * ncb][2]: first split, number of splits
     int32_t N, words, hq, hkv, maxp, num_pages;
     int32_t maxlen;            // cached tokens at most
     int32_t window;            // 0: all
-    int32_t per, units, ncb;   // units: B * ncb; ncb: column blocks of a sequence
+    int32_t per, units, ncb;   // units: B; ncb: column blocks of a sequence at most
     float scale, softcap;
 } lgx_tree_attn_args;
 

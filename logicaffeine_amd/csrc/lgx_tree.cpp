@@ -39,20 +39,20 @@ lgx_status run_tree(lgx_ctx* c, lgx_tree_attn_args& a, int B, int d, bool x, voi
     nc = x && d == 128 ? std::min(nc, 64) : nc;
     const int64_t ncb = (cols + nc - 1) / nc, units = B * ncb, blocks = heads * ncb;
     a.ncb = (int)ncb;
-    const int64_t per = (int64_t)c->attn8_wgs * c->ncu / a.hkv;
-    const bool split = tiles > LGX_A8_MIN && units <= LGX_A8_UNITS && units < per;
+    a.units = B;
+    const int64_t per = (int64_t)c->tree_wgs * c->ncu / a.hkv;
+    const bool split = tiles > LGX_A8_MIN && B <= LGX_A8_UNITS && units < per;
     lgx_status st;
     if (split) {
         const int64_t slots = per * a.hkv * nc;
         float* ws = nullptr;
         if ((st = ensure_ws(c, (size_t)(slots * (d + 2) + 2 * units) * sizeof(float), stream, &ws)) != LGX_OK) return st;
         a.per = (int)per;
-        a.units = (int)units;
         a.part = ws;
         a.ml = ws + slots * d;
         a.plan = (int32_t*)(a.ml + 2 * slots);
     }
-    const int64_t grid = split ? per * a.hkv : blocks;
+    const int64_t grid = ((split ? per * a.hkv : blocks) + 7) / 8 * 8;   // an eighth per XCD
     if (grid > UINT32_MAX / 256) return fail(LGX_OUT_OF_BOUNDS, "attention of %lld workgroups", (long long)grid);
     const int k = (d == 64 ? K_TREE_ATTN_D64 : K_TREE_ATTN_D128) + (nc == 16 ? 0 : nc == 64 ? 2 : 4) + (x ? 1 : 0);
     if ((st = launch(c, (Kern)k, dim3((unsigned)grid), dim3(256), a, stream)) != LGX_OK || !split) return st;

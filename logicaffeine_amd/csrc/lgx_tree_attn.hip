@@ -42,7 +42,7 @@ struct Tree {
     int b, g, G, c0, ncols, sl, n;
     int tb0, tb1;              // tiles
     int unit;                  // b * ncb + column block
-    int pos, ns;               // place among all splits, and splits of the unit
+    int pos, ns;               // number of the split among all, and splits of the column block
 
     __device__ __forceinline__ int nodes(int b) const { return a.n_nodes ? min(max(a.n_nodes[b], 0), a.N) : a.N; }
     __device__ __forceinline__ int length(int b) const { return min(max(a.seq_len[b], 0), a.maxlen); }
@@ -51,77 +51,102 @@ struct Tree {
         const int first = a.window ? max((int)max((int64_t)sl - a.window + 1, (int64_t)0), 0) : 0;
         return make_int2(first / TREE_TILE, (sl + n + TREE_TILE - 1) / TREE_TILE);
     }
-    // false: nothing to do.  With a.per all units' tiles go in about equal runs to the
-    // workgroups: every wave computes the run length from all lengths (four units per
-    // lane), nearly the least with which all runs fit into a.per per KV head, then
-    // finds the unit and the run of this workgroup in the sums over the units.
+    // Column blocks of n nodes.
+    __device__ __forceinline__ int blocks(int n) const { return (n * G + NC - 1) / NC; }
+    // Workgroup ids go round-robin over the 8 XCDs, each with an L2 of its own: consecutive
+    // places, whose column blocks share K and V, go to one XCD.  -1: none of the `all`.
+    static __device__ __forceinline__ int place_of(int id, int all) {
+        const int each = (all + 7) >> 3, at = (id & 7) * each + (id >> 3);
+        return id >> 3 < each && at < all ? at : -1;
+    }
+    // false: nothing to do.  Places are in order of (sequence, run of tiles, KV head, column
+    // block).  With a.per all sequences' tiles go in about equal runs to the workgroups:
+    // every wave computes the run length from all lengths (four sequences per lane),
+    // nearly the least with which all (run, column block)s fit into a.per, then finds the
+    // sequence and the run of its place in the sums over the sequences.
     __device__ __forceinline__ bool place() {
         G = a.hq / a.hkv;
-        int s = 0, run = 0;
+        int s = 0, run = 0, cb;
+        const int id = __builtin_amdgcn_readfirstlane(blockIdx.x);
         if (a.per) {
             const int lane = threadIdx.x & 63;
-            pos = __builtin_amdgcn_readfirstlane(blockIdx.x / a.hkv);
-            g = blockIdx.x - pos * a.hkv;
-            int t[4], len[4], cnt[4], all = 0;    // tiles of the lane's units; -1: no such columns
+            int t[4], len[4], cnt[4], all = 0;    // tiles of the lane's sequences; 0: no nodes
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int u = 4 * lane + i, uc = min(u, a.units - 1), bb = uc / a.ncb;
-                cnt[i] = nodes(bb);
+                const int u = 4 * lane + i, bb = min(u, a.units - 1);
+                cnt[i] = u < a.units ? nodes(bb) : 0;
                 len[i] = length(bb);
                 const int2 tt = tiles(len[i], cnt[i]);
-                t[i] = u < a.units && (uc - bb * a.ncb) * NC < cnt[i] * G ? tt.y - tt.x : -1;
-                all += max(t[i], 0);
+                t[i] = cnt[i] ? tt.y - tt.x : 0;
+                all += t[i] * blocks(cnt[i]);
             }
             const int total = __builtin_amdgcn_readlane(wave_scan(all), 63);
             run = max(TREE_MIN, (int)((unsigned)(total + a.per - 1) / (unsigned)a.per));
-            int m[4], upto;
+            int m[4], upto, used;
             for (;;) {
                 int c = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    m[i] = t[i] < 0 ? 0 : max((int)((unsigned)(t[i] + run - 1) / (unsigned)run), 1);
-                    c += m[i];
+                    m[i] = (int)((unsigned)(t[i] + run - 1) / (unsigned)run);
+                    c += m[i] * blocks(cnt[i]);
                 }
                 upto = wave_scan(c);
-                if (__builtin_amdgcn_readlane(upto, 63) <= a.per) break;
-                run += max(1, run >> 4);          // ends: a.per >= a.units
+                used = __builtin_amdgcn_readlane(upto, 63);
+                if (used <= a.per) break;
+                run += max(1, run >> 4);          // ends: a.per holds every column block
             }
-            const uint64_t past = __builtin_amdgcn_ballot_w64(upto > pos);
-            if (!past) return false;
-            const int at = __builtin_ctzll(past);
-            s = pos - __builtin_amdgcn_readlane(upto - (m[0] + m[1] + m[2] + m[3]), at);
-            int i = 0;
-#pragma unroll
-            for (int q = 0; q < 3; ++q) {
-                const int mq = __builtin_amdgcn_readlane(m[q], at);
-                const bool next = i == q && s >= mq;
-                s -= next ? mq : 0;
-                i += next ? 1 : 0;
-            }
+            const int at = place_of(id, used * a.hkv);
+            if (at < 0) return false;
+            const int p = (int)((unsigned)at / (unsigned)a.hkv);
+            const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > p));
+            int first = 0, i = 0;                 // of the sequence among the (run, column block)s
             auto pick = [&](const int (&v)[4]) {
-                const int v0 = __builtin_amdgcn_readlane(v[0], at), v1 = __builtin_amdgcn_readlane(v[1], at);
-                const int v2 = __builtin_amdgcn_readlane(v[2], at), v3 = __builtin_amdgcn_readlane(v[3], at);
+                const int v0 = __builtin_amdgcn_readlane(v[0], l), v1 = __builtin_amdgcn_readlane(v[1], l);
+                const int v2 = __builtin_amdgcn_readlane(v[2], l), v3 = __builtin_amdgcn_readlane(v[3], l);
                 return i == 0 ? v0 : i == 1 ? v1 : i == 2 ? v2 : v3;
             };
+            int c[4], sum = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                c[q] = m[q] * blocks(cnt[q]);
+                sum += c[q];
+            }
+            first = __builtin_amdgcn_readlane(upto - sum, l);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) {
+                const int cq = __builtin_amdgcn_readlane(c[q], l);
+                const bool next = i == q && p >= first + cq;
+                first += next ? cq : 0;
+                i += next ? 1 : 0;
+            }
             ns = pick(m);
             sl = pick(len);
             n = pick(cnt);
-            unit = 4 * at + i;
+            b = 4 * l + i;
+            const int ncb = blocks(n), rest = at - first * a.hkv;
+            s = rest / (ncb * a.hkv);
+            const int gc = rest - s * ncb * a.hkv;
+            g = gc / ncb;
+            cb = gc - g * ncb;
+            pos = first + cb * ns + s;            // the column block's splits side by side
+            unit = b * a.ncb + cb;
             if (s == 0 && g == 0 && threadIdx.x == 0) {
                 a.plan[2 * unit] = pos;
                 a.plan[2 * unit + 1] = ns;
             }
         } else {
-            // column blocks side by side: they share K and V
-            const int bg = blockIdx.x / a.ncb, cb = blockIdx.x - bg * a.ncb;
-            const int bb = bg / a.hkv;
-            g = __builtin_amdgcn_readfirstlane(bg - bb * a.hkv);
-            unit = __builtin_amdgcn_readfirstlane(bb * a.ncb + cb);
+            const int at = place_of(id, a.units * a.hkv * a.ncb);
+            if (at < 0) return false;
+            const int bg = at / a.ncb;
+            cb = at - bg * a.ncb;
+            b = bg / a.hkv;
+            g = bg - b * a.hkv;
             pos = 0;
             ns = 1;
         }
-        b = __builtin_amdgcn_readfirstlane(unit / a.ncb);
-        c0 = (unit - b * a.ncb) * NC;
+        b = __builtin_amdgcn_readfirstlane(b);
+        g = __builtin_amdgcn_readfirstlane(g);
+        c0 = __builtin_amdgcn_readfirstlane(cb) * NC;
         if (!a.per) {
             n = __builtin_amdgcn_readfirstlane(nodes(b));
             sl = __builtin_amdgcn_readfirstlane(length(b));
