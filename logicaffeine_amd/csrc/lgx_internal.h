@@ -193,9 +193,9 @@ enum Kern {
     K_FILTER_PICK,
     K_FILTER_BINS,
     K_FILTER_WIDE,
-    K_TREE_ATTN_D64, // 16 columns; + 1: with caps, distances or a window; + 2, + 4: 64, 128 columns
-    K_TREE_ATTN_D128 = K_TREE_ATTN_D64 + 6,
-    K_COUNT = K_TREE_ATTN_D128 + 5
+    K_TREE_ATTN_D64, // + 1: with caps, distances or a window
+    K_TREE_ATTN_D128 = K_TREE_ATTN_D64 + 2,
+    K_COUNT = K_TREE_ATTN_D128 + 2
 };
 inline const char* const kKernelNames[] = {
     "lgx_k_repack_t16", "lgx_k_quantize_q8_0", "lgx_k_q8q8_gemv",
@@ -253,10 +253,7 @@ inline const char* const kKernelNames[] = {
     "lgx_k_pages_fork", "lgx_k_pages_free", "lgx_k_pages_reserve", "lgx_k_pages_copy",
     "lgx_k_append_rows_d64", "lgx_k_append_rows_d128", "lgx_k_tree_plan", "lgx_k_tree_accept",
     "lgx_k_kv_keep_d64", "lgx_k_kv_keep_d128", "lgx_k_filter_scan", "lgx_k_filter_pick", "lgx_k_filter_bins", "lgx_k_filter_wide",
-    "lgx_k_tree_attn_d64_c16", "lgx_k_tree_attnx_d64_c16", "lgx_k_tree_attn_d64_c64",
-    "lgx_k_tree_attnx_d64_c64", "lgx_k_tree_attn_d64_c128", "lgx_k_tree_attnx_d64_c128",
-    "lgx_k_tree_attn_d128_c16", "lgx_k_tree_attnx_d128_c16", "lgx_k_tree_attn_d128_c64",
-    "lgx_k_tree_attnx_d128_c64", "lgx_k_tree_attn_d128_c128",
+    "lgx_k_tree_attn_d64", "lgx_k_tree_attnx_d64", "lgx_k_tree_attn_d128", "lgx_k_tree_attnx_d128",
 };
 
 static_assert(sizeof(kKernelNames) / sizeof(kKernelNames[0]) == K_COUNT,
@@ -329,7 +326,6 @@ struct lgx_ctx {
     int attn8_wgs = 1;            // LGX_A8_WGS: workgroups per compute unit the 8-bit cache's attention splits for
     int attn8_cols = 0;           // LGX_A8_COLS: force 16 / 32 / 128 (row, head) pairs per workgroup of it (0: by size)
     int tree_wgs = 2;             // LGX_TREE_WGS: workgroups per compute unit the drafts' attention splits for
-    int tree_cols = 0;            // LGX_TREE_COLS: force 16 / 64 / 128 (node, head) pairs per workgroup of the drafts' attention (0: by size)
     bool prefill_serial = false;  // LGX_PREFILL=serial: prefill as P decode passes
     int prefill_chunk = 0;        // LGX_PREFILL_CHUNK: positions per prefill chunk (0: by batch)
     int ncu = 256;                // compute units of the device

@@ -600,6 +600,10 @@ typedef struct {
     int32_t per, units, ncb;   // units: B; ncb: column blocks of a sequence at most
     float scale, softcap;
 } lgx_tree_attn_args;
+#define LGX_TREE_TILE 64       // tokens of a tile: four pages
+#define LGX_TREE_COLS 64       // (node, query head) columns of a workgroup
+#define LGX_TREE_UNITS 256     // sequences whose tiles are split at most
+#define LGX_TREE_MIN 4         // tiles of a split at least
 
 // ---- sampling with per-row settings (lgx_filter.hip) ----
 #define LGX_SF_CHUNK 64        // logits whose largest is kept

@@ -27,24 +27,24 @@ lgx_status check_tree(int32_t B, int32_t N) {
 }
 
 // Launch over B sequences.  Where there are fewer (sequence, KV head, column block)s
-// than compute units, their tiles are split among that many workgroups; the splitting
-// itself is done on the device, by the lengths.  The joining of the splits is that of
-// the 8-bit cache's attention.
+// than two to a compute unit, their tiles are split among that many workgroups; the
+// splitting itself is done on the device, by the lengths.  Splits for one to a compute unit
+// against two (28 heads of 4, 128 dimensions): 85 against 69 us for 32 ragged sequences
+// of up to 4096 tokens and 16 nodes, 66 against 56 for 64 of 3000 and 2; but 25.9 against
+// 27.5 for 16 of 2000 and 8.  The joining of the splits is that of the 8-bit cache's attention.
 lgx_status run_tree(lgx_ctx* c, lgx_tree_attn_args& a, int B, int d, bool x, void* stream) {
     const int64_t cols = (int64_t)a.N * (a.hq / a.hkv), heads = (int64_t)B * a.hkv;
     // the most tiles that a sequence's nodes can see
-    int64_t tiles = cdiv((int64_t)a.maxlen + a.N, LGX_A8_TILE);
-    if (a.window) tiles = std::min<int64_t>(tiles, ((int64_t)a.window + a.N) / LGX_A8_TILE + 2);
-    int nc = c->tree_cols ? c->tree_cols : cols <= 16 ? 16 : cols <= 64 ? 64 : 128;
-    nc = x && d == 128 ? std::min(nc, 64) : nc;
-    const int64_t ncb = (cols + nc - 1) / nc, units = B * ncb, blocks = heads * ncb;
+    int64_t tiles = cdiv((int64_t)a.maxlen + a.N, LGX_TREE_TILE);
+    if (a.window) tiles = std::min<int64_t>(tiles, ((int64_t)a.window + a.N) / LGX_TREE_TILE + 2);
+    const int64_t ncb = cdiv(cols, LGX_TREE_COLS), units = B * ncb, blocks = heads * ncb;
     a.ncb = (int)ncb;
     a.units = B;
     const int64_t per = (int64_t)c->tree_wgs * c->ncu / a.hkv;
-    const bool split = tiles > LGX_A8_MIN && B <= LGX_A8_UNITS && units < per;
+    const bool split = tiles > LGX_TREE_MIN && B <= LGX_TREE_UNITS && units < per && units * tiles <= INT32_MAX;
     lgx_status st;
     if (split) {
-        const int64_t slots = per * a.hkv * nc;
+        const int64_t slots = per * a.hkv * LGX_TREE_COLS;
         float* ws = nullptr;
         if ((st = ensure_ws(c, (size_t)(slots * (d + 2) + 2 * units) * sizeof(float), stream, &ws)) != LGX_OK) return st;
         a.per = (int)per;
@@ -54,7 +54,7 @@ lgx_status run_tree(lgx_ctx* c, lgx_tree_attn_args& a, int B, int d, bool x, voi
     }
     const int64_t grid = ((split ? per * a.hkv : blocks) + 7) / 8 * 8;   // an eighth per XCD
     if (grid > UINT32_MAX / 256) return fail(LGX_OUT_OF_BOUNDS, "attention of %lld workgroups", (long long)grid);
-    const int k = (d == 64 ? K_TREE_ATTN_D64 : K_TREE_ATTN_D128) + (nc == 16 ? 0 : nc == 64 ? 2 : 4) + (x ? 1 : 0);
+    const int k = (d == 64 ? K_TREE_ATTN_D64 : K_TREE_ATTN_D128) + (x ? 1 : 0);
     if ((st = launch(c, (Kern)k, dim3((unsigned)grid), dim3(256), a, stream)) != LGX_OK || !split) return st;
     lgx_attn8_args j{};
     j.part = a.part;
@@ -66,7 +66,7 @@ lgx_status run_tree(lgx_ctx* c, lgx_tree_attn_args& a, int B, int d, bool x, voi
     j.hq = a.hq;
     j.hkv = a.hkv;
     j.ncb = a.ncb;
-    j.cols = nc;
+    j.cols = LGX_TREE_COLS;
     j.rows = B * a.N;
     const int64_t rh = (int64_t)j.rows * a.hq;
     const int w = rh >= 8 * (int64_t)c->ncu ? 1 : 0;

@@ -27,16 +27,26 @@
 // replaced; V rows behind the last node are cleared; and an infinity or a NaN among the
 // others, which 0 would not hide, leaves a result that is not finite, upon which the
 // column is done over token by token (tree_column).
+//
+// A workgroup has 64 columns, 16 per wave, and passes tiles of K and V through LDS, where all
+// four waves read them.  Measured against it (128 dimensions, 28 heads of 4):
+//   16 columns per workgroup, the waves sharing the tiles, for up to 16 columns: one token
+//     of 64 sequences of up to 4000 tokens 75 against 70 us, of one of 8000 15.8 against
+//     14.1: a workgroup's waves have more loads in flight where all of them load one tile.
+//   128 columns, 32 per wave, half the LDS reads per product: 64 nodes over 8000 tokens
+//     36.8 against 34.2 us, 100 nodes of 8 sequences of 1000 55 against 44; only 200 nodes
+//     of 2 sequences of 5200 gain (113 against 136), where 22 blocks read the same K and V.
+// What bounds it: few nodes, the cache's bytes (one token of 64 sequences: 4.2 TB/s of
+// the 4.7 that a copy reaches); many, the way of a tile from memory through LDS into the
+// matrix unit, which is busy 32 to 43 % of the time (without the products 53 us become
+// 35 for 100 nodes of 8 sequences); short calls, the launch and the splits' join.
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) uint16_t lds_u16;
 typedef __attribute__((address_space(4))) const int32_t const_i32;
 
-#define TREE_TILE 64
-#define TREE_MIN 4             // tiles of a split at least
 #define TREE_UP 10             // weights as operands: times 2^10
 
-// What a workgroup works on: a sequence, a KV head, a block of NC columns, a run of tiles.
-template <int NC>
+// What a workgroup works on: a sequence, a KV head, a block of columns, a run of tiles.
 struct Tree {
     const lgx_tree_attn_args& a;
     int b, g, G, c0, ncols, sl, n;
@@ -49,10 +59,10 @@ struct Tree {
     // first and last + 1 tile that a sequence's nodes can see (depths are not negative)
     __device__ __forceinline__ int2 tiles(int sl, int n) const {
         const int first = a.window ? max((int)max((int64_t)sl - a.window + 1, (int64_t)0), 0) : 0;
-        return make_int2(first / TREE_TILE, (sl + n + TREE_TILE - 1) / TREE_TILE);
+        return make_int2(first / LGX_TREE_TILE, (sl + n + LGX_TREE_TILE - 1) / LGX_TREE_TILE);
     }
     // Column blocks of n nodes.
-    __device__ __forceinline__ int blocks(int n) const { return (n * G + NC - 1) / NC; }
+    __device__ __forceinline__ int blocks(int n) const { return (n * G + LGX_TREE_COLS - 1) / LGX_TREE_COLS; }
     // Workgroup ids go round-robin over the 8 XCDs, each with an L2 of its own: consecutive
     // places, whose column blocks share K and V, go to one XCD.  -1: none of the `all`.
     static __device__ __forceinline__ int place_of(int id, int all) {
@@ -70,7 +80,7 @@ struct Tree {
         const int id = __builtin_amdgcn_readfirstlane(blockIdx.x);
         if (a.per) {
             const int lane = threadIdx.x & 63;
-            int t[4], len[4], cnt[4], all = 0;    // tiles of the lane's sequences; 0: no nodes
+            int t[4], len[4], cnt[4], all = 0, nb = 0, longest = 0;   // tiles of the lane's sequences; 0: no nodes
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int u = 4 * lane + i, bb = min(u, a.units - 1);
@@ -79,9 +89,17 @@ struct Tree {
                 const int2 tt = tiles(len[i], cnt[i]);
                 t[i] = cnt[i] ? tt.y - tt.x : 0;
                 all += t[i] * blocks(cnt[i]);
+                nb += blocks(cnt[i]);
+                longest = max(longest, t[i]);
             }
             const int total = __builtin_amdgcn_readlane(wave_scan(all), 63);
-            run = max(TREE_MIN, (int)((unsigned)(total + a.per - 1) / (unsigned)a.per));
+            run = max(LGX_TREE_MIN, (int)((unsigned)(total + a.per - 1) / (unsigned)a.per));
+            const int blks = __builtin_amdgcn_readlane(wave_scan(nb), 63);
+            const int top = __builtin_amdgcn_readfirstlane((int)wave_max((float)longest));   // exact: at most 2^24
+            // Whole sequences where they fill the device and are about equally long: then a
+            // split gains less than its results' way through memory costs (b8-n100-l1000
+            // on 28 heads of 4: 51 us whole, 54 split).
+            if (2 * blks >= a.per && (int64_t)4 * top * blks <= (int64_t)5 * total) run = max(run, top);
             int m[4], upto, used;
             for (;;) {
                 int c = 0;
@@ -146,7 +164,7 @@ struct Tree {
         }
         b = __builtin_amdgcn_readfirstlane(b);
         g = __builtin_amdgcn_readfirstlane(g);
-        c0 = __builtin_amdgcn_readfirstlane(cb) * NC;
+        c0 = __builtin_amdgcn_readfirstlane(cb) * LGX_TREE_COLS;
         if (!a.per) {
             n = __builtin_amdgcn_readfirstlane(nodes(b));
             sl = __builtin_amdgcn_readfirstlane(length(b));
@@ -248,8 +266,8 @@ __device__ __forceinline__ float tree_query(const lgx_tree_attn_args& a, const f
 // From the products of a column tile to its weights as operands; o is brought to the new
 // reference where it moves.  EDGE: some column does not see the whole tile, or the scores
 // are capped, biased or windowed (X).  S[4 u + v]: token t0 + 16 u + 4 kg + v.
-template <bool X, bool EDGE, int ND, class W>
-__device__ __forceinline__ void tree_weights(const W& w, float (&S)[16], TreeCol& k, int t0, int kg, v8h (&ph)[2], v8h (&pl)[2],
+template <bool X, bool EDGE, int ND>
+__device__ __forceinline__ void tree_weights(const Tree& w, float (&S)[16], TreeCol& k, int t0, int kg, v8h (&ph)[2], v8h (&pl)[2],
                                              v4f (&o)[ND]) {
     static_assert(EDGE || !X, "other scores are formed ahead of the maximum");
     constexpr float kLog2e = 1.44269504088896341f;
@@ -265,7 +283,7 @@ __device__ __forceinline__ void tree_weights(const W& w, float (&S)[16], TreeCol
 #pragma unroll
                 for (int e = 0; e < 16; ++e) S[e] = a.softcap * a8_tanh(S[e] * inv);
             }
-            const bool tree = t0 + TREE_TILE > w.sl;   // uniform: nodes among the tokens
+            const bool tree = t0 + LGX_TREE_TILE > w.sl;   // uniform: nodes among the tokens
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int t = t0 + 16 * (e >> 2) + 4 * kg + (e & 3);
@@ -319,15 +337,15 @@ __device__ __forceinline__ void tree_weights(const W& w, float (&S)[16], TreeCol
 
 // Column c over its run of tiles, token by token, by one wave: only seen tokens are
 // multiplied.  m, l: the column's reference and sum.
-template <int D, bool X, class W>
-__device__ void tree_column(const W& w, int c, float m, float l, float* dst) {
+template <int D, bool X>
+__device__ void tree_column(const Tree& w, int c, float m, float l, float* dst) {
     constexpr float kLog2e = 1.44269504088896341f;
     const lgx_tree_attn_args& a = w.a;
     const int lane = threadIdx.x & 63, j = c / w.G, dj = w.depth(j);
     const float* q = a.q + w.orow(c) * D;
     const float slope = X && a.slopes ? a.slopes[w.g * w.G + c % w.G] : 0.0f;
     float o[D / 64] = {};
-    for (int t0 = w.tb0 * TREE_TILE; t0 < w.tb1 * TREE_TILE; t0 += 64) {
+    for (int t0 = w.tb0 * LGX_TREE_TILE; t0 < w.tb1 * LGX_TREE_TILE; t0 += 64) {
         const int t = t0 + lane;
         const int page = min(max(a.page_table[(int64_t)w.b * a.maxp + min(t / LGX_PAGE, a.maxp - 1)], 0), a.num_pages - 1);
         const int64_t at = (((int64_t)page * a.hkv + w.g) * LGX_PAGE + t % LGX_PAGE) * D;
@@ -359,11 +377,11 @@ __device__ void tree_column(const W& w, int c, float m, float l, float* dst) {
 }
 
 // A column's result, or its split's (divided by the split's own sum of weights).
-template <int D, int NC, bool X, class W>
-__device__ __forceinline__ void tree_store(const W& w, int c, const TreeCol& k, int kg, const v4f (&o)[D / 16]) {
+template <int D, bool X>
+__device__ __forceinline__ void tree_store(const Tree& w, int c, const TreeCol& k, int kg, const v4f (&o)[D / 16]) {
     const lgx_tree_attn_args& a = w.a;
     const bool part = w.ns > 1, on = c < w.ncols;
-    const int64_t at = part ? ((int64_t)w.pos * a.hkv + w.g) * NC + c - w.c0 : w.orow(on ? c : 0);
+    const int64_t at = part ? ((int64_t)w.pos * a.hkv + w.g) * LGX_TREE_COLS + c - w.c0 : w.orow(on ? c : 0);
     float* dst = (part ? a.part : a.out) + at * D;
     const float r = k.l == 0.0f ? 0.0f : 1.0f / k.l, l = k.l * (1.0f / (1 << TREE_UP));   // nothing seen gives zeros
     bool bad = false;
@@ -418,177 +436,27 @@ struct TreeK {
     }
 };
 
-// Page numbers of a tile, through the scalar cache.
-template <class W>
-struct TreePages {
-    int p[4];
-    __device__ __forceinline__ TreePages(const W& w, int t) {
-        const_i32* table = (const_i32*)(w.a.page_table + (int64_t)w.b * w.a.maxp);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) p[u] = table[min(4 * t + u, w.a.maxp - 1)];
-    }
-    __device__ __forceinline__ int64_t block(const W& w, int u, int d) const {
-        return ((int64_t)min(max(p[u], 0), w.a.num_pages - 1) * w.a.hkv + w.g) * (LGX_PAGE * d);
-    }
-};
-
-// 16 columns per workgroup (single tokens and few drafts): its four waves take the
-// tiles in turn, K straight into registers, V into the wave's LDS: the next tile's K is in
-// flight from the end of the scores on, its V from the end of the PV product; at the end
-// the waves' results are joined in LDS.
+// 16 columns per wave: tiles of K and V pass through LDS, the next one in flight from the
+// barrier that publishes this one on.
 template <int D, bool X>
-__device__ __forceinline__ void tree_narrow_body(const lgx_tree_attn_args& a) {
-    constexpr int WT = 4, NS = D / 32, ND = D / 16, CH = D / 8;
-    constexpr int TPI = 64 / CH, NI = TREE_TILE / TPI;   // tokens of a 1 KiB load, loads of a tile
-    __shared__ __align__(16) uint16_t v_s[WT][TREE_TILE * D];
-    static_assert(sizeof(v_s) >= WT / 2 * (ND * 64 * sizeof(v4f) + 2 * 64 * sizeof(float)), "the join's share");
-    const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
-    const int wt = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    typedef Tree<16> W;
-    typedef TreePages<W> Pages;
-    W w{a};
-    if (!w.place()) return;                       // uniform
-    uint4 kw[4][NS];
-    auto load_k = [&](const Pages& p) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const uint16_t* base = a.k + p.block(w, u, D);
-#pragma unroll
-            for (int s = 0; s < NS; ++s) kw[u][s] = *(const uint4*)(base + (col * D + 8 * kg + 32 * s));
-        }
-    };
-    lds_u16* const vb = (lds_u16*)v_s[wt];
-    auto load_v = [&](const Pages& p) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const uint16_t* base = a.v + p.block(w, i * TPI / LGX_PAGE, D);
-            const int r = i * TPI % LGX_PAGE + lane / CH;
-            __builtin_amdgcn_global_load_lds((const void*)(base + (r * D + TreeV<D>::piece(r, lane % CH) * 8)),
-                                             (lds_void*)(vb + i * 512), 16, 0, 0);
-        }
-    };
-    int t = w.tb0 + wt;
-    const int end = w.tb1, T = w.sl + w.n;
-    // Loads are issued whether or not there is such a tile (the wave's last one's again)
-    const int mine = end - 1 - t >= 0 ? t + (end - 1 - t) / WT * WT : t;
-    Pages p(w, t);
-    load_k(p);
-    load_v(p);
-    p = Pages(w, min(t + WT, mine));
-    __builtin_amdgcn_sched_barrier(0);
-    v4f o[ND];
-#pragma unroll
-    for (int i = 0; i < ND; ++i) o[i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-    TreeCol k;
-    v8h qh[2][NS];
-    {
-        const int c = min(w.c0 + col, w.ncols - 1);   // columns past the last repeat it
-        k = {0.0f, X && a.slopes ? a.slopes[w.g * w.G + c % w.G] : 0.0f, -__builtin_inff(), 0.0f, c / w.G, 0};
-        k.dj = w.depth(k.j);
-        k.f = tree_query<D, X>(a, a.q + w.orow(c) * D + 8 * kg, qh);
-    }
-    auto tile = [&](auto form) __attribute__((always_inline)) {
-        constexpr bool edge = decltype(form)::value;
-        const int t0 = t * TREE_TILE;
-        const Pages pn = p;
-        v8h ph[2], pl[2];
-        float S[16];
-        {
-            v4f acc[4];                           // the four sub-tiles' chains side by side
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-#pragma unroll
-                for (int part = 1; part >= 0; --part)
-#pragma unroll
-                    for (int u = 0; u < 4; ++u)
-                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            as_v8h(kw[u][s]), qh[part][s], s == 0 && part == 1 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : acc[u], 0, 0, 0);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) S[e] = acc[e >> 2][e & 3];
-        }
-        load_k(pn);
-        p = Pages(w, min(t + 2 * WT, mine));
-        tree_weights<X, edge, ND>(w, S, k, t0, kg, ph, pl, o);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * NS) : "memory");   // V is there; the next K may be under way
-        if (edge && t0 + TREE_TILE > T) {
-            // rows behind the last node: weight 0 times whatever they hold
-            for (int i = lane; i < TREE_TILE * CH; i += 64)
-                if (t0 + i / CH >= T) *(uint4*)(v_s[wt] + i * 8) = make_uint4(0u, 0u, 0u, 0u);
-        }
-#pragma unroll
-        for (int g = 0; g < ND / 4; ++g) {
-            v4f r[4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                v8h vf[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) vf[i] = TreeV<D>::operand(vb, 4 * g + i, h, col, kg);
-#pragma unroll
-                for (int part = 1; part >= 0; --part)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        r[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            vf[i], part ? pl[h] : ph[h], h == 0 && part == 1 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : r[i], 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[4 * g + i] += r[i];
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // V is read before the next overwrites it
-        load_v(pn);
-    };
-    // the tiles of cached tokens alone, then the others
-    if constexpr (!X) {
-#pragma unroll 1
-        for (const int whole = min(end, w.sl / TREE_TILE); t < whole; t += WT) tile(TreeWhole());
-    }
-#pragma unroll 1
-    for (; t < end; t += WT) tile(TreeEdge());
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the loop
-    __syncthreads();
-    k.l = col_sum(k.l);
-    // join the waves, halving their number
-    v4f* o_s = (v4f*)v_s;
-    float* ml_s = (float*)(o_s + WT / 2 * ND * 64);
-#pragma unroll
-    for (int h = WT / 2; h; h >>= 1) {
-        const int at = wt % h;
-        if (wt >= h && wt < 2 * h) {
-            ml_s[(at * 2 + 0) * 64 + lane] = k.m;
-            ml_s[(at * 2 + 1) * 64 + lane] = k.l;
-#pragma unroll
-            for (int i = 0; i < ND; ++i) o_s[(at * ND + i) * 64 + lane] = o[i];
-        }
-        __syncthreads();
-        if (wt < h) {
-            const float mo = ml_s[(at * 2 + 0) * 64 + lane], lo = ml_s[(at * 2 + 1) * 64 + lane];
-            const float mn = fmaxf(k.m, mo);
-            // a wave that has seen nothing: weights of 0
-            const float u0 = k.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(k.m - mn);
-            const float u1 = mo == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mo - mn);
-            k.l = k.l * u0 + lo * u1;
-            k.m = mn;
-#pragma unroll
-            for (int i = 0; i < ND; ++i) o[i] = o[i] * u0 + o_s[(at * ND + i) * 64 + lane] * u1;
-        }
-        __syncthreads();
-    }
-    if (wt) return;
-    tree_store<D, 16, X>(w, w.c0 + col, k, kg, o);
-}
-
-// 64 NT columns per workgroup, 16 NT per wave: tiles of K and V pass through LDS, the
-// next one in flight from the barrier that publishes this one on.
-template <int D, int NT, bool X>
-__device__ __forceinline__ void tree_wide_body(const lgx_tree_attn_args& a) {
-    constexpr int NS = D / 32, ND = D / 16, CH = D / 8, NC = 64 * NT;
-    constexpr int TPI = 64 / CH, NI = TREE_TILE / TPI;   // tokens of a 1 KiB load, loads of a tile's K or V
-    __shared__ __align__(16) uint16_t kv_s[2][2][TREE_TILE * D];
+__device__ __forceinline__ void tree_body(const lgx_tree_attn_args& a) {
+    constexpr int NS = D / 32, ND = D / 16, CH = D / 8;
+    constexpr int TPI = 64 / CH, NI = LGX_TREE_TILE / TPI;   // tokens of a 1 KiB load, loads of a tile's K or V
+    __shared__ __align__(16) uint16_t kv_s[2][2][LGX_TREE_TILE * D];
     const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    typedef Tree<NC> W;
-    typedef TreePages<W> Pages;
-    W w{a};
+    Tree w{a};
     if (!w.place()) return;                       // uniform
+    const_i32* table = (const_i32*)(a.page_table + (int64_t)w.b * a.maxp);   // through the scalar cache
+    struct Pages {
+        int p[LGX_TREE_TILE / LGX_PAGE];
+    };
+    auto pages = [&](int t) {
+        Pages r;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) r.p[u] = table[min(4 * t + u, a.maxp - 1)];
+        return r;
+    };
     // waves 0 and 1 bring K, 2 and 3 V
     auto load = [&](int buf, const Pages& p) __attribute__((always_inline)) {
         lds_u16* to = (lds_u16*)kv_s[buf][wave >> 1];
@@ -604,43 +472,42 @@ __device__ __forceinline__ void tree_wide_body(const lgx_tree_attn_args& a) {
     };
     const int end = w.tb1, T = w.sl + w.n;
     int t = w.tb0;
-    load(0, Pages(w, t));
-    Pages p(w, min(t + 1, end - 1));
-    const int wcol = w.c0 + wave * 16 * NT;
+    load(0, pages(t));
+    Pages p = pages(min(t + 1, end - 1));
+    const int wcol = w.c0 + wave * 16;
     const bool any = wcol < w.ncols;              // else the wave only loads
-    v4f o[NT][ND];
-    TreeCol k[NT];
-    v8h qh[NT][2][NS];
+    v4f o[ND];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < ND; ++i) o[n][i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-        const int c = min(wcol + 16 * n + col, w.ncols - 1);   // columns past the last repeat it
-        k[n] = {0.0f, X && a.slopes ? a.slopes[w.g * w.G + c % w.G] : 0.0f, -__builtin_inff(), 0.0f, c / w.G, 0};
-        k[n].dj = w.depth(k[n].j);
-        k[n].f = tree_query<D, X>(a, a.q + w.orow(c) * D + 8 * kg, qh[n]);
+    for (int i = 0; i < ND; ++i) o[i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    TreeCol k;
+    v8h qh[2][NS];
+    {
+        const int c = min(wcol + col, w.ncols - 1);   // columns past the last repeat it
+        k = {0.0f, X && a.slopes ? a.slopes[w.g * w.G + c % w.G] : 0.0f, -__builtin_inff(), 0.0f, c / w.G, 0};
+        k.dj = w.depth(k.j);
+        k.f = tree_query<D, X>(a, a.q + w.orow(c) * D + 8 * kg, qh);
     }
     auto tile = [&](auto form) __attribute__((always_inline)) {
         constexpr bool edge = decltype(form)::value;
-        const int t0 = t * TREE_TILE, cur = (t - w.tb0) & 1;
+        const int t0 = t * LGX_TREE_TILE, cur = (t - w.tb0) & 1;
         publish_lds_loads();                      // this tile is there, the last one read
-        if (edge && t0 + TREE_TILE > T) {         // uniform
+        if (edge && t0 + LGX_TREE_TILE > T) {         // uniform
             // rows behind the last node: weight 0 times whatever they hold
-            for (int i = threadIdx.x; i < TREE_TILE * CH; i += 256)
+            for (int i = threadIdx.x; i < LGX_TREE_TILE * CH; i += 256)
                 if (t0 + i / CH >= T) *(uint4*)(kv_s[cur][1] + i * 8) = make_uint4(0u, 0u, 0u, 0u);
             __syncthreads();
         }
         if (t + 1 < end) {                        // uniform
             load(cur ^ 1, p);
-            p = Pages(w, min(t + 2, end - 1));
+            p = pages(min(t + 2, end - 1));
         }
         if (!any) return;
         const lds_u16* ks = (const lds_u16*)kv_s[cur][0];
         const lds_u16* vs = (const lds_u16*)kv_s[cur][1];
-        float S[NT][16];
+        float S[16];
         {
             // the four sub-tiles' chains side by side, operands a step ahead
-            v4f acc[NT][4];
+            v4f acc[4];
             v8h kf[2][4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) kf[0][u] = TreeK<D>::operand(ks, u, 0, col, kg);
@@ -654,74 +521,54 @@ __device__ __forceinline__ void tree_wide_body(const lgx_tree_attn_args& a) {
                 for (int part = 1; part >= 0; --part)
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-                            acc[n][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                kf[s & 1][u], qh[n][part][s], s == 0 && part == 1 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : acc[n][u], 0, 0, 0);
+                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            kf[s & 1][u], qh[part][s], s == 0 && part == 1 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : acc[u], 0, 0, 0);
             }
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) S[n][e] = acc[n][e >> 2][e & 3];
+            for (int e = 0; e < 16; ++e) S[e] = acc[e >> 2][e & 3];
         }
-        v8h ph[NT][2], pl[NT][2];
+        v8h ph[2], pl[2];
+        tree_weights<X, edge, ND>(w, S, k, t0, kg, ph, pl, o);
+        // 64 dimensions at a time, their chains side by side, operands a step ahead
+        v8h vf[2][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) tree_weights<X, edge, ND>(w, S[n], k[n], t0, kg, ph[n], pl[n], o[n]);
-        // 64 or 32 dimensions at a time, their chains side by side, operands a step ahead
-        constexpr int G = 4 / NT, NG = ND / G;
-        v8h vf[2][G];
+        for (int i = 0; i < 4; ++i) vf[0][i] = TreeV<D>::operand(vs, i, 0, col, kg);
 #pragma unroll
-        for (int i = 0; i < G; ++i) vf[0][i] = TreeV<D>::operand(vs, i, 0, col, kg);
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            v4f r[NT][G];
+        for (int g = 0; g < ND / 4; ++g) {
+            v4f r[4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (h == 0 || g + 1 < NG) {
+                if (h == 0 || g + 1 < ND / 4) {
 #pragma unroll
-                    for (int i = 0; i < G; ++i) vf[h ^ 1][i] = TreeV<D>::operand(vs, G * (g + h) + i, h ^ 1, col, kg);
+                    for (int i = 0; i < 4; ++i) vf[h ^ 1][i] = TreeV<D>::operand(vs, 4 * (g + h) + i, h ^ 1, col, kg);
                 }
 #pragma unroll
                 for (int part = 1; part >= 0; --part)
 #pragma unroll
-                    for (int i = 0; i < G; ++i)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-                            r[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                vf[h][i], part ? pl[n][h] : ph[n][h], h == 0 && part == 1 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : r[n][i], 0, 0, 0);
+                    for (int i = 0; i < 4; ++i)
+                        r[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            vf[h][i], part ? pl[h] : ph[h], h == 0 && part == 1 ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : r[i], 0, 0, 0);
             }
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < G; ++i) o[n][G * g + i] += r[n][i];
+            for (int i = 0; i < 4; ++i) o[4 * g + i] += r[i];
         }
     };
     // the tiles of cached tokens alone, then the others
     if constexpr (!X) {
 #pragma unroll 1
-        for (const int whole = min(end, w.sl / TREE_TILE); t < whole; ++t) tile(TreeWhole());
+        for (const int whole = min(end, w.sl / LGX_TREE_TILE); t < whole; ++t) tile(TreeWhole());
     }
 #pragma unroll 1
     for (; t < end; ++t) tile(TreeEdge());
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the wave
     if (!any) return;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        k[n].l = col_sum(k[n].l);
-        tree_store<D, NC, X>(w, wcol + 16 * n + col, k[n], kg, o[n]);
-    }
+    k.l = col_sum(k.l);
+    tree_store<D, X>(w, wcol + col, k, kg, o);
 }
 
 #define LGX_TREE_KERNEL(NAME, BODY) \
     extern "C" __global__ __launch_bounds__(256, 2) void NAME(const lgx_tree_attn_args a) { BODY(a); }
-LGX_TREE_KERNEL(lgx_k_tree_attn_d64_c16, (tree_narrow_body<64, false>))
-LGX_TREE_KERNEL(lgx_k_tree_attnx_d64_c16, (tree_narrow_body<64, true>))
-LGX_TREE_KERNEL(lgx_k_tree_attn_d64_c64, (tree_wide_body<64, 1, false>))
-LGX_TREE_KERNEL(lgx_k_tree_attnx_d64_c64, (tree_wide_body<64, 1, true>))
-LGX_TREE_KERNEL(lgx_k_tree_attn_d64_c128, (tree_wide_body<64, 2, false>))
-LGX_TREE_KERNEL(lgx_k_tree_attnx_d64_c128, (tree_wide_body<64, 2, true>))
-LGX_TREE_KERNEL(lgx_k_tree_attn_d128_c16, (tree_narrow_body<128, false>))
-LGX_TREE_KERNEL(lgx_k_tree_attnx_d128_c16, (tree_narrow_body<128, true>))
-LGX_TREE_KERNEL(lgx_k_tree_attn_d128_c64, (tree_wide_body<128, 1, false>))
-LGX_TREE_KERNEL(lgx_k_tree_attnx_d128_c64, (tree_wide_body<128, 1, true>))
-LGX_TREE_KERNEL(lgx_k_tree_attn_d128_c128, (tree_wide_body<128, 2, false>))
+LGX_TREE_KERNEL(lgx_k_tree_attn_d64, (tree_body<64, false>))
+LGX_TREE_KERNEL(lgx_k_tree_attnx_d64, (tree_body<64, true>))
+LGX_TREE_KERNEL(lgx_k_tree_attn_d128, (tree_body<128, false>))
+LGX_TREE_KERNEL(lgx_k_tree_attnx_d128, (tree_body<128, true>))

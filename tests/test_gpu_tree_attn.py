@@ -114,19 +114,27 @@ def test_trees_behind_short_contexts(ctx, hq, hkv, d, N):
     check(s, run(ctx, s))
 
 
-@pytest.mark.parametrize("cols", [16, 64, 128])
+@pytest.mark.parametrize("wgs", [1, 5])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("opts", [False, True])
-def test_every_width_of_workgroup(cols, d, opts, monkeypatch):
-    """Forced for sizes that they would not be chosen for, whole and split."""
-    monkeypatch.setenv("LGX_TREE_COLS", str(cols))
+def test_other_splits(wgs, d, opts, monkeypatch):
+    """Runs of tiles for fewer and for more workgroups than there are by default."""
+    monkeypatch.setenv("LGX_TREE_WGS", str(wgs))
     ctx = lgx.Context(0)
-    rng = np.random.default_rng(cols)
+    rng = np.random.default_rng(wgs)
     o, more = (lgx.AttnOpts(softcap=20.0, window=150), dict(cap=20.0, window=150)) if opts else (None, {})
-    for hq, hkv, N, lens in ((4, 2, 1, [300, 5]), (14, 2, 13, [200, 700, 64]), (7, 1, 40, [1000])):
+    for hq, hkv, N, lens in ((4, 2, 1, [300, 5]), (14, 2, 13, [200, 700, 64]), (7, 1, 40, [1000]), (2, 1, 2, [5000, 90])):
         s = make(ctx, rng, len(lens), N, hq, hkv, d, lens, n=[N] + [max(1, N - 3)] * (len(lens) - 1))
         check(s, run(ctx, s, o), **more)
     ctx.close()
+
+
+@pytest.mark.parametrize("lens", [[330] * 140, [330, 290] * 70, [400, 1] * 70, [400] + [30] * 139, [1000] * 100 + [0] * 40])
+def test_batches_that_fill_the_device(ctx, lens):
+    """Sequences of about one length are not split, others are."""
+    rng = np.random.default_rng(sum(lens))
+    s = make(ctx, rng, 140, 2, 4, 2, 64, lens, n=rng.integers(0, 3, 140))
+    check(s, run(ctx, s), only=[0, 1, 2, 57, 99, 100, 138, 139])
 
 
 @pytest.mark.parametrize("hq,hkv,d", SHAPES[:3])
