@@ -1,0 +1,222 @@
+"""Drafts, sampling and a cache's pages together, as a server uses them: sequences of a
+small network go on by trees of drafts, share pages where one forks from another, and
+yield the tokens that they would yield one at a time."""
+import numpy as np
+import pytest
+import torch
+
+import logicaffeine_amd as lgx
+import tree_ref as R
+
+pytestmark = pytest.mark.gpu
+
+LAYERS, HQ, HKV, D, VOCAB, PAGE, MAXP = 2, 6, 2, 64, 300, 16, 12
+H = HQ * D
+
+
+class Net:
+    """Token embedding, LAYERS of attention, logits; in 64 bits on the host for one
+    sequence, by the library for a batch's trees of drafts."""
+
+    def __init__(self, ctx, rng):
+        self.ctx = ctx
+        self.emb = rng.standard_normal((VOCAB, H)).astype(np.float32)
+        self.wqkv = [(rng.standard_normal((H, (HQ + 2 * HKV) * D)) * H ** -0.5).astype(np.float32) for _ in range(LAYERS)]
+        self.out = (rng.standard_normal((H, VOCAB)) * 2 * H ** -0.5).astype(np.float32)
+        self.gpu = {k: [torch.tensor(x, device="cuda") for x in v] if isinstance(v, list) else torch.tensor(v, device="cuda")
+                    for k, v in (("emb", self.emb), ("wqkv", self.wqkv), ("out", self.out))}
+        self.rope = lgx.Rope.tables(ctx, MAXP * PAGE, D, theta=1e4)
+        ang = np.arange(MAXP * PAGE)[:, None] * 1e4 ** (-2.0 * np.arange(D // 2) / D)
+        self.cos, self.sin = np.cos(ang)[:, None], np.sin(ang)[:, None]
+
+    def turn(self, x, first):
+        a, b, n = x[..., :D // 2], x[..., D // 2:], len(x)
+        c, s = self.cos[first:first + n], self.sin[first:first + n]
+        return np.concatenate([a * c - b * s, a * s + b * c], -1)
+
+    def logits(self, tokens):
+        """Behind the last of the tokens."""
+        x = self.emb[tokens].astype(np.float64)
+        for w in self.wqkv:
+            qkv = (x @ w).reshape(len(x), HQ + 2 * HKV, D)
+            q = self.turn(qkv[:, :HQ], 0)
+            k, v = (y.astype(np.float16).astype(np.float64) for y in (self.turn(qkv[:, HQ:HQ + HKV], 0), qkv[:, HQ + HKV:]))
+            s = np.einsum("ighd,jgd->ghij", q.reshape(-1, HKV, HQ // HKV, D), k) / np.sqrt(D)
+            s = np.where(np.tri(len(x), dtype=bool), s, -np.inf)
+            p = np.exp(s - s.max(-1, keepdims=True))
+            x = x + np.einsum("ghij,jgd->ighd", p / p.sum(-1, keepdims=True), v).reshape(len(x), H)
+        return x[-1] @ self.out
+
+    def step(self, tokens, N, lens, table, caches, depth, mask, n, top):
+        """Logits [B*N][VOCAB] behind every node."""
+        x = self.gpu["emb"][tokens.reshape(-1).long()]
+        for w, kv in zip(self.gpu["wqkv"], caches):
+            q = self.ctx.rope_kv_append_rows(x @ w, None, self.rope, lens, table, kv, N, depth, n)
+            o = torch.zeros_like(q)               # rows that are no nodes are left as they are
+            self.ctx.gqa_tree_attn(q, kv, table, lens, N, top, mask, depth, n, out=o)
+            x = x + o.reshape(-1, H)
+        return x @ self.gpu["out"]
+
+
+class Server:
+    """State on the device of S sequences; one round checks a tree of N drafts of each."""
+
+    def __init__(self, net, S, N, pages):
+        ctx = self.ctx = net.ctx
+        self.net, self.S, self.N = net, S, N
+        self.caches = [lgx.KvCacheF16.empty(ctx, pages, HKV, D) for _ in range(LAYERS)]
+        for kv in self.caches:
+            kv.k.fill_(float("nan"))              # what nothing wrote, nothing may read
+            kv.v.fill_(float("nan"))
+        self.pool = lgx.PagePool.empty(ctx, pages)
+        self.planes = lgx.PagePlanes([x for kv in self.caches for x in (kv.k, kv.v)])
+        i32 = dict(dtype=torch.int32, device="cuda")
+        self.table = torch.full((S, MAXP), -1, **i32)
+        self.lens, self.n, self.last = torch.zeros(S, **i32), torch.zeros(S, **i32), torch.zeros(S, **i32)
+        self.tokens, self.parent = torch.zeros((S, N), **i32), torch.full((S, N), -1, **i32)
+        self.room = (torch.zeros((S, 2), **i32), torch.zeros(1, **i32), torch.zeros(1, **i32))
+        self.u = torch.zeros(S * N, device="cuda")
+        self.settings = {}
+
+    def round(self):
+        ctx, N = self.ctx, self.N
+        copies, n_copies, _ = ctx.pages_reserve(self.pool, self.table, self.lens, self.n, out=self.room)
+        ctx.pages_copy(self.planes, copies, n_copies)
+        depth, mask = ctx.tree_plan(self.parent, self.n)
+        logits = self.net.step(self.tokens, N, self.lens, self.table, self.caches, depth, mask, self.n, MAXP * PAGE - N)
+        picked, _ = ctx.sample_filtered(logits, self.u, **self.settings)
+        path, count, _, new = ctx.tree_accept(self.tokens, self.parent, picked.view(self.S, N), self.lens, self.n, self.last)
+        ctx.kv_keep(self.caches, self.table, self.lens, path, count)
+        self.lens.copy_(new)
+        ctx.pages_free(self.pool, self.table, self.lens)
+        self.path, self.count, self.picked = path, count, picked
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = lgx.Context(0)
+    yield c
+    c.close()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("S,N,settings", [
+    (3, 1, {}), (2, 5, dict(temperature=0.0)), (4, 7, dict(temperature=1.0)), (4, 12, dict(temperature=0.8, top_k=20)),
+    (3, 70, dict(temperature=1.0, top_p=0.9, min_p=0.01))])
+def test_drafts_yield_the_tokens_of_single_steps(ctx, S, N, settings, captured):
+    """Every sequence's tokens are those of the 64-bit network and the definition's choice,
+    one at a time.  The random number of a choice belongs to the sequence and the position.
+    Both sides round keys and values to binary16, and a key that 32 and 64 bits round to
+    either side changes a logit by some 1e-4: random numbers are such that logits off by
+    1e-3 give the same choice."""
+    rng = np.random.default_rng(100 * S + N)
+    net, total = Net(ctx, rng), 60
+    u = rng.random((S, total + N + 2)).astype(np.float32)
+    prompt = rng.integers(0, VOCAB, 21)
+    T, k, p, mp = (settings.get(x, y) for x, y in (("temperature", 1.0), ("top_k", 0), ("top_p", 1.0), ("min_p", 0.0)))
+
+    def choice(seq, s):
+        logits = net.logits(seq)
+        for _ in range(100):
+            x = u[s, len(seq) - 1]
+            token = R.choose(logits, x, T, k, p, mp)[0]
+            if all(R.choose(logits + rng.uniform(-1e-3, 1e-3, VOCAB), y, T, k, p, mp)[0] == token
+                   for y in (x, x, max(x - 1e-3, 0), x + 1e-3)):
+                return token
+            u[s, len(seq) - 1] = rng.random()
+        raise AssertionError("no choice is clear")
+
+    want = []
+    for s in range(S):                            # sequence 0's first tokens, then each its own way
+        seq = list(prompt) if s == 0 else want[0][:30]
+        while len(seq) < total:
+            seq.append(choice(seq, s))
+        want.append(seq)
+
+    srv = Server(net, S, N, pages=S * -(-(total + N) // PAGE) + 1)
+    for name, x in settings.items():
+        srv.settings[name] = torch.full((S * N,), x, device="cuda", dtype=torch.int32 if name == "top_k" else torch.float32)
+    graph = None
+
+    def drafts(s, at):
+        """A tree whose node 0 is token `at` of the sequence: the tokens to come among others."""
+        n = int(rng.integers(1, N + 1))
+        tok, par, dep = rng.integers(0, VOCAB, N), np.full(N, -1), np.zeros(N, int)
+        tok[0], right = want[s][at], 0            # `right`: the last node of the true path
+        for j in range(1, n):
+            par[j] = right if rng.random() < 0.7 else rng.integers(0, j)
+            dep[j] = dep[par[j]] + 1
+            nxt = at + dep[j]
+            if par[j] == right and rng.random() < 0.8 and nxt < total:
+                tok[j], right = want[s][nxt], j
+        return tok, par, dep, n
+
+    def fill(live):
+        tokens, parent, n = np.zeros((S, N), np.int32), np.full((S, N), -1, np.int32), np.zeros(S, np.int32)
+        us = np.zeros((S, N), np.float32)
+        for s in live:
+            tokens[s], parent[s], dep, n[s] = drafts(s, len(have[s]) - 1)
+            us[s] = u[s, np.minimum(len(have[s]) - 1 + dep, u.shape[1] - 1)]
+        srv.tokens.copy_(torch.tensor(tokens))
+        srv.parent.copy_(torch.tensor(parent))
+        srv.n.copy_(torch.tensor(n))
+        srv.u.copy_(torch.tensor(us.reshape(-1)))
+
+    def go():
+        nonlocal graph
+        if not captured:
+            return srv.round()
+        if graph is None:
+            saved = [x.clone() for x in (srv.pool.ref, srv.table, srv.lens, srv.last)]
+            planes = [x.clone() for x in srv.planes.tensors]
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):         # libraries set up, workspaces grow
+                srv.round()
+            torch.cuda.current_stream().wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                srv.round()
+            for x, y in zip((srv.pool.ref, srv.table, srv.lens, srv.last, *srv.planes.tensors), saved + planes):
+                x.copy_(y)
+        graph.replay()
+
+    # the prompt but its last token, as a run of new tokens in pieces of N
+    have = {0: list(prompt)}
+    for i in range(0, len(prompt) - 1, N):
+        part = prompt[i:min(i + N, len(prompt) - 1)]
+        one = torch.zeros((S, N), dtype=torch.int32, device="cuda")
+        one[0, :len(part)] = torch.tensor(part, device="cuda")
+        n = torch.tensor([len(part)] + [0] * (S - 1), dtype=torch.int32, device="cuda")
+        ctx.pages_reserve(srv.pool, srv.table, srv.lens, n, out=srv.room)
+        net.step(one, N, srv.lens, srv.table, srv.caches, None, None, n, MAXP * PAGE - N)
+        srv.lens += n
+    rounds = 0
+    while any(len(x) < total for x in have.values()):
+        live = [s for s in have if len(have[s]) < total]
+        fill(live)
+        go()
+        count, path, last = (x.cpu().numpy() for x in (srv.count, srv.path, srv.last))
+        tokens, lens = srv.tokens.cpu().numpy(), srv.lens.cpu().numpy()
+        assert int(srv.room[2]) == 0
+        for s in live:
+            new = [int(tokens[s, j]) for j in path[s, 1:count[s]]] + [int(last[s])]
+            have[s] += new
+            assert count[s] >= 1 and have[s][:total] == want[s][:len(have[s])], (s, rounds)
+            assert lens[s] == len(have[s]) - 1
+        if len(have) == 1 and len(have[0]) >= 32:
+            # the others fork from the first, back to 29 cached tokens, amid a page
+            dst = torch.arange(1, S, dtype=torch.int32, device="cuda")
+            ctx.pages_fork(srv.pool, srv.table, srv.lens, torch.zeros_like(dst), dst)
+            srv.lens[1:] = 29
+            ctx.pages_free(srv.pool, srv.table, srv.lens)
+            assert int(srv.pool.ref.max()) == S
+            have.update({s: want[0][:30] for s in range(1, S)})
+        rounds += 1
+    # every holder accounted for, and all pages come back
+    table = srv.table.cpu().numpy()
+    assert np.array_equal(np.bincount(table[table >= 0], minlength=srv.pool.num_pages), srv.pool.ref.cpu().numpy())
+    ctx.pages_free(srv.pool, srv.table, torch.zeros_like(srv.lens))
+    assert int(srv.pool.ref.abs().sum()) == 0 and bool((srv.table == -1).all())
+    if N > 1:
+        assert rounds < total - len(prompt)       # drafts held
