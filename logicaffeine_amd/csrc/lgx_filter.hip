@@ -23,58 +23,67 @@
 #define SF_ONE 0x1p42                             // 2^19 weights stay below 2^62
 #define SF_LIST 4096                              // tokens kept in LDS
 
-// e^x for x <= 0: x = (64 n + j) ln 2 / 64 + r, 2^(j/64) from a table (sf_roots), e^r by its
-// Taylor polynomial of degree 4 (|r| <= 0.0055: the term after it is under 5e-14).
-#define SF_ROOTS 64
-__device__ __forceinline__ double sf_root_exp(double x, const double* roots, int& n) {
-    const double k = rint(x * (SF_ROOTS * 1.4426950408889634074));
-    const double r = fma(-k, 0.69314718055994530942 / SF_ROOTS, x);
-    double p = 1.0 / 24.0;
-    p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
+// e^x for x <= 0: x = (256 n + j) ln 2 / 256 + r, 2^(j/256) from a table (sf_roots), e^r by its
+// Taylor polynomial of degree 3 (|r| <= 0.00136: the term after it is under 2e-13).  The
+// argument comes in units of ln 2 / 256 (SfScale).
+#define SF_ROOTS 256
+__device__ __forceinline__ double sf_root_exp(double y, const double* roots, int& n) {
+    const double k = rint(y), r = (y - k) * (0.69314718055994530942 / SF_ROOTS);
+    double p = fma(r, 1.0 / 6.0, 0.5);
     p = fma(p, r, 1.0);
     p = fma(p, r, 1.0);
     const int i = (int)k;
-    n = i >> 6;                                   // floor
+    n = i >> 8;                                   // floor
     return roots[i & (SF_ROOTS - 1)] * p;
 }
-__device__ __forceinline__ double sf_exp(double x, const double* roots) {
+#define SF_UNITS_PER (SF_ROOTS * 1.4426950408889634074)   // of an argument's units in 1
+__device__ __forceinline__ double sf_exp(double y, const double* roots) {
     int n;
-    const double p = sf_root_exp(x, roots, n);
-    return x > -700.0 ? __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + ((uint64_t)(int64_t)n << 52)) : 0.0;
+    const double p = sf_root_exp(y, roots, n);
+    return y > -700.0 * SF_UNITS_PER ? __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + ((uint64_t)(int64_t)n << 52)) : 0.0;
 }
 // In units of 2^-42, rounded, for x > -30.5: a shift of the bits (a conversion of binary64
 // to a 64-bit integer takes as long as all of the above).
-__device__ __forceinline__ uint64_t sf_units(double x, const double* roots) {
+__device__ __forceinline__ uint64_t sf_units(double y, const double* roots) {
     int n;
-    const uint64_t bits = __builtin_bit_cast(uint64_t, sf_root_exp(x, roots, n));
+    const uint64_t bits = __builtin_bit_cast(uint64_t, sf_root_exp(y, roots, n));
     const int down = 52 - 42 + 1023 - (int)(bits >> 52) - n;
     const uint64_t m = (bits & ((1ull << 52) - 1)) | 1ull << 52;
     return down > 54 ? 0 : (m + (1ull << (down - 1))) >> down;
 }
-// The table, by threads 0 .. 63: e^x of [0, 0.69) by its Taylor polynomial of degree 17
-// (the term after it is under 2e-19).
+// The table, by threads 0 .. 255: e^x of [0, 0.7) by its Taylor polynomial of degree 15
+// (the term after it is under 2e-16).
 __device__ __forceinline__ void sf_roots(double* roots) {
     if (threadIdx.x >= SF_ROOTS) return;
+    constexpr struct Inverse {                    // 1 / i!
+        double c[16];
+        constexpr Inverse() : c() {
+            double f = 1.0;
+            for (int i = 0; i < 16; ++i) {
+                c[i] = 1.0 / f;
+                f *= i + 1;
+            }
+        }
+    } t;
     const double x = threadIdx.x * (0.69314718055994530942 / SF_ROOTS);
-    double p = 1.0;
+    double p = t.c[15];
 #pragma unroll
-    for (int i = 17; i; --i) p = fma(p, x / i, 1.0);
+    for (int i = 14; i >= 0; --i) p = fma(p, x, t.c[i]);
     roots[threadIdx.x] = p;
 }
 // Weight of logit l by the maximum M; 0 for NaN and -inf, 1 for the maximum, whatever it is.
 __device__ __forceinline__ double sf_weight(float l, float M, double inv, const double* roots) {
-    const double x = ((double)l - (double)M) * inv;
-    return l == M ? 1.0 : l > -__builtin_inff() && l < M ? sf_exp(x, roots) : 0.0;
+    const double y = ((double)l - (double)M) * inv;
+    return l == M ? 1.0 : l > -__builtin_inff() && l < M ? sf_exp(y, roots) : 0.0;
 }
 
 __device__ __forceinline__ uint64_t sf_weight_units(float l, float M, double inv, const double* roots) {
-    const double x = ((double)l - (double)M) * inv;
-    return l == M ? 1ull << 42 : l > -__builtin_inff() && x > -30.5 ? sf_units(x, roots) : 0;
+    const double y = ((double)l - (double)M) * inv;
+    return l == M ? 1ull << 42 : l > -__builtin_inff() && y > -30.5 * SF_UNITS_PER ? sf_units(y, roots) : 0;
 }
 
 struct SfRow {
-    double inv;                                   // 1 / T
+    double inv;                                   // 1 / T in units of ln 2 / 256
     float p, mp;                                  // top_p (1: none), min_p (0: none)
     int k;                                        // top_k (0: none)
     bool greedy;
@@ -82,17 +91,40 @@ struct SfRow {
     // whether the sum of all weights is needed
     __device__ __forceinline__ bool sums() const { return !greedy && !k && (p < 1.0f || mp <= 0.0f); }
 };
+__device__ __forceinline__ float sf_temperature(const lgx_filter_args& a, int row) { return a.temperature ? a.temperature[row] : 1.0f; }
 __device__ __forceinline__ SfRow sf_row(const lgx_filter_args& a, int row) {
     SfRow r;
-    const float T = a.temperature ? a.temperature[row] : 1.0f;
+    const float T = sf_temperature(a, row);
     r.greedy = !(T > 0.0f);
-    r.inv = 1.0 / (double)T;
+    r.inv = SF_UNITS_PER / (double)T;
     const int k = a.top_k ? a.top_k[row] : 0;
     r.k = k > 0 && k < a.vocab ? k : 0;
     const float p = a.top_p ? a.top_p[row] : 1.0f, mp = a.min_p ? a.min_p[row] : 0.0f;
     r.p = p < 1.0f ? fmaxf(p, 0.0f) : 1.0f;       // NaN: none
     r.mp = mp > 0.0f ? fminf(mp, 1.0f) : 0.0f;
     return r;
+}
+
+// Inclusive sums over 16 lanes, and over all lanes, as wave_scan, of 64-bit integers or
+// binary64 numbers.
+template <int C, int R, class V>
+__device__ __forceinline__ V scan64_step(V v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, C, R, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), C, R, 0xf, false);
+    return v + __builtin_bit_cast(V, (uint64_t)hi << 32 | lo);
+}
+template <class V>
+__device__ __forceinline__ V row_scan64(V v) {
+    v = scan64_step<0x111, 0xf>(v);
+    v = scan64_step<0x112, 0xf>(v);
+    v = scan64_step<0x114, 0xf>(v);
+    return scan64_step<0x118, 0xf>(v);
+}
+template <class V>
+__device__ __forceinline__ V wave_scan64(V v) {
+    v = scan64_step<0x142, 0xa>(row_scan64(v));
+    return scan64_step<0x143, 0xc>(v);
 }
 
 // Workgroup (4096 logits, row): thread t holds 4 (256 i + t) .. + 3 of them.
@@ -138,9 +170,8 @@ extern "C" __global__ __launch_bounds__(256) void lgx_k_filter_scan(const lgx_fi
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) s += sf_weight(v[i][c], M, r.inv, roots);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
-    if ((tid & 63) == 0) sum_s[tid >> 6] = s;
+    s = wave_scan64(s);
+    if ((tid & 63) == 63) sum_s[tid >> 6] = s;
     __syncthreads();
     if (tid == 0) a.sum[(int64_t)row * a.nslices + sl] = sum_s[0] + sum_s[1] + (sum_s[2] + sum_s[3]);
 }
@@ -155,7 +186,7 @@ __device__ __forceinline__ float sf_logit(uint32_t key) { return __uint_as_float
 
 #define SF_NT 1024
 #define SF_BINS 1024                              // of a selection's first step
-#define SF_FEW 512                                // elements that one wave chooses among
+#define SF_FEW 448                                // elements that one wave chooses among (64 more: its registers run out)
 #define SF_GUESS 256                              // runs whose tokens are tried first for top-p
 struct SfLds {
     union {
@@ -176,71 +207,39 @@ struct SfLds {
 static_assert(sizeof(SfLds) <= 81920, "two workgroups per compute unit");
 static_assert(LGX_SF_VOCAB <= 1 << 20 && LGX_SF_VOCAB / LGX_SF_CHUNK <= 65536, "an index has 20 bits, a run 16");
 
-// Inclusive sums over the lanes, as wave_scan.
-__device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {
-    auto step = [&](auto C, auto R) {
-        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, decltype(C)::value, decltype(R)::value, 0xf, false);
-        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), decltype(C)::value, decltype(R)::value, 0xf, false);
-        v += (uint64_t)hi << 32 | lo;
-    };
-    struct A { enum { value = 0x111 }; };
-    struct B { enum { value = 0x112 }; };
-    struct C { enum { value = 0x114 }; };
-    struct D { enum { value = 0x118 }; };
-    struct E { enum { value = 0x142 }; };
-    struct F { enum { value = 0x143 }; };
-    struct All { enum { value = 0xf }; };
-    struct Odd { enum { value = 0xa }; };
-    struct Upper { enum { value = 0xc }; };
-    step(A{}, All{});
-    step(B{}, All{});
-    step(C{}, All{});
-    step(D{}, All{});
-    step(E{}, Odd{});
-    step(F{}, Upper{});
-    return v;
-}
-__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 |
-           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+template <class V>
+__device__ __forceinline__ V lane_of(V v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(V, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane) << 32 |
+                                     (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane));
 }
 __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) { return lane_of(wave_scan64(v), 63); }
 
+// What the waves of the workgroup have together and those before this one, from each
+// wave's uniform value.  (Sixteen lanes sum sixteen waves: sixteen waves on four SIMDs
+// make every instruction cost 16 cycles, and a loop over the waves 1 us.)
+template <class V>
+__device__ __forceinline__ V sf_waves(V mine, V* waves, V& total) {
+    static_assert(SF_NT == 1024, "a lane per wave");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (lane == 0) waves[wave] = mine;
+    __syncthreads();
+    const V w = row_scan64(waves[lane & 15]);
+    total = lane_of(w, 15);
+    const V before = wave ? lane_of(w, wave - 1) : V(0);
+    __syncthreads();
+    return before;
+}
 // Inclusive sums over the workgroup's threads.
 template <class V>
 __device__ __forceinline__ V sf_scan(V v, V* waves, V& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if constexpr (sizeof(V) == 8 && V(0.5) == V(0)) {
-        v = wave_scan64(v);
-    } else {
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const V o = __shfl_up(v, d, 64);
-            v += lane >= d ? o : V(0);
-        }
-    }
-    if (lane == 63) waves[wave] = v;
-    __syncthreads();
-    V before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < SF_NT / 64; ++w) {
-        const V o = waves[w];
-        before += w < wave ? o : V(0);
-        total += o;
-    }
-    __syncthreads();
-    return before + v;
+    v = wave_scan64(v);
+    return sf_waves(lane_of(v, 63), waves, total) + v;
 }
 // Their sum alone.
 __device__ __forceinline__ uint64_t sf_sum(uint64_t v, uint64_t* waves) {
-    v = wave_sum64(v);
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
-    __syncthreads();
-    uint64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < SF_NT / 64; ++w) total += waves[w];
-    __syncthreads();
+    uint64_t total;
+    sf_waves(wave_sum64(v), waves, total);
     return total;
 }
 
@@ -263,9 +262,13 @@ __device__ __forceinline__ uint32_t sf_bisect(uint32_t lo, uint32_t hi, uint64_t
     return lo;
 }
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d, 64));
-    return v;
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // The row's tokens that can be kept, in LDS or in memory: load(i) is element i, the others
@@ -603,14 +606,63 @@ __device__ __forceinline__ void sf_choose_lanes(const SfLds& s, const lgx_filter
     }
 }
 
-// The same for n <= 512: lane l holds elements l ne .. , so that sums over lanes go by index.
+// The same by the workgroup, for n <= 128 elements: the weight and the number of those ahead
+// of each, an eighth of them per pair of waves, then two elements per lane of one wave.
+__device__ __forceinline__ void sf_choose_pairs(SfLds& s, const lgx_filter_args& a, const SfRow& r, int row, double all, int n) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (r.k || r.p < 1.0f) {
+        const int i = 64 * (wave & 1) + lane;
+        const uint32_t key = i < n ? s.key[i] : 0u;
+        uint64_t before = 0;                      // number << 52: 128 weights of 2^42 stay below
+#pragma unroll 4
+        for (int j = wave >> 1; j < n; j += SF_NT / 128) {
+            const uint32_t kj = s.key[j];
+            const uint64_t wj = s.wi[j] >> 20 | 1ull << 52;
+            before += kj < key || (kj == key && j < i) ? wj : 0;
+        }
+        s.bins[128 * (wave >> 1) + i] = before;
+        __syncthreads();
+    }
+    if (wave) return;
+    uint64_t w[2], before[2] = {0, 0};
+    bool on[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int i = 2 * lane + e;
+        on[e] = i < n;
+        w[e] = on[e] ? s.wi[i] >> 20 : 0;
+        if (r.k || r.p < 1.0f) {
+#pragma unroll
+            for (int q = 0; q < SF_NT / 128; ++q) before[e] += s.bins[128 * q + i];
+        }
+    }
+    if (r.k) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) on[e] = on[e] && (int)(before[e] >> 52) < r.k;
+    }
+    if (r.p < 1.0f) {
+        const double whole = r.k ? (double)wave_sum64((on[0] ? w[0] : 0) + (on[1] ? w[1] : 0)) : all;
+        const uint64_t need = max((uint64_t)ceil((double)r.p * whole), (uint64_t)1);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) on[e] = on[e] && (before[e] & ((1ull << 52) - 1)) < need;
+    }
+    const uint64_t low = (uint64_t)ceil((double)r.mp * SF_ONE);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (!on[e] || w[e] < low) w[e] = 0;
+    const uint64_t upto = wave_scan64(w[0] + w[1]), total = lane_of(upto, 63), t = sf_draw(a.u[row], total);
+    const uint64_t from = upto - w[0] - w[1];
+    if (upto > t && from <= t) {
+        const int e = from + w[0] > t ? 0 : 1;
+        a.out[row] = (int)(s.wi[2 * lane + e] & 0xfffff);
+        if (a.prob) a.prob[row] = (float)((double)(e ? w[1] : w[0]) / (double)total);
+    }
+}
+
+// The same for n <= SF_FEW: lane l holds elements l ne .. , so that sums over lanes go by index.
 // Where top-k leaves 64 at most, they go on as above.
 __device__ __forceinline__ void sf_choose_wave(SfLds& s, const lgx_filter_args& a, SfRow r, int row, double all, int n) {
     constexpr int E = SF_FEW / 64;
-    if (n <= 64) {                                // uniform
-        sf_choose_lanes(s, a, r, row, all, n);
-        return;
-    }
     const int lane = threadIdx.x & 63, ne = (n + 63) / 64;
     uint32_t k[E], lo = 0xffffffffu, hi = 0;
     uint64_t wi[E];
@@ -728,6 +780,10 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
     float cm[CM];
 #pragma unroll
     for (int j = 0; j < CM; ++j) cm[j] = j < rw && c0 + 64 * j < nruns ? cmax[c0 + 64 * j] : __builtin_nanf("");
+    // (the sums are there only where they are needed)
+    const double part = tid < a.nslices ? a.sum[(int64_t)row * a.nslices + tid] : 0.0;
+    const float part_max = tid < a.nslices ? smax[tid] : ninf;
+    const float u = a.u[row];
     // the row's maximum: at most 128 slices
     float M = ninf;
     for (int i = lane; i < a.nslices; i += 64) M = fmaxf(M, smax[i]);
@@ -759,13 +815,12 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
     __syncthreads();                              // the table
     double S = 0.0;                               // of all weights, by M
     if (r.sums()) {
-        const double* sums = a.sum + (int64_t)row * a.nslices;
-        const double mine = tid < a.nslices ? sums[tid] * sf_weight(smax[tid], M, r.inv, s.roots) : 0.0;
+        const double mine = tid < a.nslices ? part * sf_weight(part_max, M, r.inv, s.roots) : 0.0;
         const double upto = sf_scan<double>(mine, s.dwave, S);
         if (r.plain()) {
             // the slice that the draw falls into: the last with a weight that starts at
             // or before it; then the token in the slice
-            const double t = fmin(fmax((double)a.u[row], 0.0), 1.0) * S;
+            const double t = fmin(fmax((double)u, 0.0), 1.0) * S;
             if (tid == 0) s.found = 0;
             __syncthreads();
             if (mine > 0.0 && upto - mine <= t) __hip_atomic_fetch_max(&s.found, tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
@@ -805,7 +860,7 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
     // the tokens under (1 - p) / V of the whole are less than 1 - p of it together; the k-th
     // largest of the runs' maxima is no larger than the k-th largest token.  The margins
     // are far above the rounding of the logarithms.  (Top-p of the top k weighs all k.)
-    const float T = (float)(1.0 / r.inv);
+    const float T = sf_temperature(a, row);
     float tau = M - 30.0f * T;
     if (r.mp > 0.0f && !(r.k && r.p < 1.0f)) tau = fmaxf(tau, M + T * (logf(r.mp) - 0.001f));
     if (r.p < 1.0f && !r.k) tau = fmaxf(tau, M + T * (logf((1.0f - r.p) / (float)V) + logf((float)S) - 0.001f));
@@ -859,16 +914,9 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
 #pragma unroll
         for (int j = 0; j < CM; ++j) mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(cm[j] >= tau));
         __syncthreads();                          // bins and counts are read
-        if (lane == 0) s.dwave[wave] = (double)mine;
-        __syncthreads();
-        int nr = 0, to = 0;
-#pragma unroll
-        for (int w = 0; w < SF_NT / 64; ++w) {
-            const int c = (int)s.dwave[w];
-            to += w < wave ? c : 0;
-            nr += c;
-        }
-        __syncthreads();
+        uint64_t runs;
+        int to = (int)sf_waves<uint64_t>(mine, s.wave, runs);
+        const int nr = (int)runs;
 #pragma unroll
         for (int j = 0; j < CM; ++j) {
             const uint64_t hit = __builtin_amdgcn_ballot_w64(cm[j] >= tau);
@@ -898,16 +946,9 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
 #pragma unroll
                 for (int u = 0; u < 4; ++u) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[u] >= tau));
             }
-            if (lane == 0) s.dwave[wave] = (double)c;
-            __syncthreads();
-            int at = 0;
-            n = 0;
-#pragma unroll
-            for (int w = 0; w < SF_NT / 64; ++w) {
-                const int m = (int)s.dwave[w];
-                at += w < wave ? m : 0;
-                n += m;
-            }
+            uint64_t tokens;
+            int at = (int)sf_waves<uint64_t>(c, s.wave, tokens);
+            n = (int)tokens;
             if (n <= SF_LIST) {                   // uniform
                 for (int q = q0; q < q1; q += 4) {
                     if (q1 - q0 > 4) load(q);     // else still there
@@ -934,7 +975,9 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
             }
         }
         const SfBins bin(M, fmaxf(tau, -3e38f));
-        if (n <= SF_FEW) {
+        if (n <= 128) {
+            sf_choose_pairs(s, a, r, row, all, n);
+        } else if (n <= SF_FEW) {
             if (wave == 0) sf_choose_wave(s, a, r, row, all, n);
         } else if (n <= SF_LIST) {
             sf_choose(s, a, r, bin, row, all, SfInLds{s, n});
@@ -1030,7 +1073,7 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_wide(const lgx_
         const uint64_t need = max((uint64_t)ceil((double)r.p * all), (uint64_t)1), low = (uint64_t)ceil((double)r.mp * SF_ONE);
         // of bins first .. end not all tokens are known to be kept or not: those are listed
         int first = LGX_SF_BINS, end = LGX_SF_BINS - 1;
-        if (r.mp > 0.0f) first = bin(fminf(M + (float)(1.0 / r.inv) * (logf(r.mp) + 0.001f), M));
+        if (r.mp > 0.0f) first = bin(fminf(M + sf_temperature(a, row) * (logf(r.mp) + 0.001f), M));
         uint64_t base = 0;                        // weight of the bins below `end`
         bool few = w < a.slots;
         const bool cut = few && r.p < 1.0f && need <= total;
