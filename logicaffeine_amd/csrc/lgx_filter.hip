@@ -783,7 +783,6 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
     // (the sums are there only where they are needed)
     const double part = tid < a.nslices ? a.sum[(int64_t)row * a.nslices + tid] : 0.0;
     const float part_max = tid < a.nslices ? smax[tid] : ninf;
-    const float u = a.u[row];
     // the row's maximum: at most 128 slices
     float M = ninf;
     for (int i = lane; i < a.nslices; i += 64) M = fmaxf(M, smax[i]);
@@ -820,7 +819,7 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
         if (r.plain()) {
             // the slice that the draw falls into: the last with a weight that starts at
             // or before it; then the token in the slice
-            const double t = fmin(fmax((double)u, 0.0), 1.0) * S;
+            const double t = fmin(fmax((double)a.u[row], 0.0), 1.0) * S;
             if (tid == 0) s.found = 0;
             __syncthreads();
             if (mine > 0.0 && upto - mine <= t) __hip_atomic_fetch_max(&s.found, tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
@@ -957,13 +956,18 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
                         const uint64_t hit = __builtin_amdgcn_ballot_w64(v[u] >= tau);
                         const int i = at + __builtin_popcountll(hit & ((1ull << lane) - 1));
                         if (v[u] >= tau) {
-                            const uint64_t w = sf_weight_units(v[u], M, r.inv, s.roots);
-                            weighs += w;
                             s.key[i] = sf_key(v[u]);
-                            s.wi[i] = w << 20 | (uint64_t)t[u];
+                            s.wi[i] = (uint64_t)t[u];
                         }
                         at += __builtin_popcountll(hit);
                     }
+                }
+                __syncthreads();
+                // their weights, by as many lanes as there are tokens (a run has few)
+                for (int i = tid; i < n; i += SF_NT) {
+                    const uint64_t w = sf_weight_units(sf_logit(s.key[i]), M, r.inv, s.roots);
+                    weighs += w;
+                    s.wi[i] |= w << 20;
                 }
                 __syncthreads();
             }
