@@ -14,11 +14,14 @@
 template <int D>
 __device__ __forceinline__ void append_rows_body(const lgx_append_rows_args& a) {
     constexpr int TPH = D / 8;                    // threads of a head
-    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / TPH;
-    if (item >= a.items) return;
     const int nh = a.hq + 2 * a.hkv;
-    const int64_t r = item / nh;
-    const int h = (int)(item - r * nh), b = (int)(r / a.N), j = (int)(r - (int64_t)b * a.N);
+    // the workgroup's first head by one division of 64 bits (uniform), the thread's by 32
+    const int64_t item0 = (int64_t)blockIdx.x * (256 / TPH), r0 = item0 / nh;
+    const int of = threadIdx.x / TPH;
+    if (item0 + of >= a.items) return;
+    const unsigned from = (unsigned)(item0 - r0 * nh) + of, down = from / (unsigned)nh;
+    const int64_t r = r0 + down;                  // below 2^31
+    const int h = (int)(from - down * nh), b = (int)((unsigned)r / (unsigned)a.N), j = (int)((unsigned)r - (unsigned)b * a.N);
     if (a.n_new && j >= a.n_new[b]) return;
     const bool isv = h >= a.hq + a.hkv;
     const int rot = isv ? 0 : a.rot, half = rot / 2, p = (threadIdx.x % TPH) * 4;
