@@ -21,7 +21,7 @@
 // do not depend on any order; the scan's are binary64.  exp is computed in binary64.
 // ---------------------------------------------------------------------------
 #define SF_ONE 0x1p42                             // 2^19 weights stay below 2^62
-#define SF_LIST 4096                              // tokens kept in LDS
+#define SF_LIST LGX_SF_LIST                       // tokens kept in LDS
 
 // e^x for x <= 0: x = (256 n + j) ln 2 / 256 + r, 2^(j/256) from a table (sf_roots), e^r by its
 // Taylor polynomial of degree 3 (|r| <= 0.00136: the term after it is under 2e-13).  The
@@ -312,34 +312,6 @@ __device__ __forceinline__ void sf_each(const S& e, int first, int end, int step
 #pragma unroll
         for (int u = 0; u < S::U; ++u)
             if (i0 + u * step < end) f(x[u], i0 + u * step);
-    }
-}
-
-// f(logit, index) for a row's logits, 16 in flight per thread.
-template <class F>
-__device__ __forceinline__ void sf_row_each(const float* x, int V, int vec, const F& f) {
-    const int tid = threadIdx.x, n4 = vec ? V / 4 : 0;
-    for (int i0 = tid; i0 < n4; i0 += 4 * SF_NT) {
-        float4 v[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = ((const float4*)x)[min(i0 + u * SF_NT, n4 - 1)];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int i = 4 * (i0 + u * SF_NT);
-            if (i >= 4 * n4) break;
-            f(v[u].x, i);
-            f(v[u].y, i + 1);
-            f(v[u].z, i + 2);
-            f(v[u].w, i + 3);
-        }
-    }
-    for (int i0 = 4 * n4 + tid; i0 < V; i0 += 8 * SF_NT) {
-        float v[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = x[min(i0 + u * SF_NT, V - 1)];
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (i0 + u * SF_NT < V) f(v[u], i0 + u * SF_NT);
     }
 }
 
@@ -1032,6 +1004,7 @@ extern "C" __global__ __launch_bounds__(256) void lgx_k_filter_bins(const lgx_fi
         const float* x = a.logits + (int64_t)row * a.ld;
         const SfSliceBins bin(M, tau);
         bins[tid] = 0;
+        if (sl == 0 && tid == 0) a.wide_cut[w].count = 0;
         __syncthreads();
         float v[16];
 #pragma unroll
@@ -1049,9 +1022,111 @@ extern "C" __global__ __launch_bounds__(256) void lgx_k_filter_bins(const lgx_fi
     }
 }
 
-// The choice in a wide row, from the bins of its slices: the bin in which top-p ends, the
-// tokens in it, then what is kept of each slice, the slice that the draw falls into and
-// the token in it.
+// From the bins of all slices the one in which top-p ends and the ones that min-p may
+// cut: a slice's tokens in them go to the row's list.  Each workgroup takes a run of the
+// (wide row, slice)s and finds a row's bins for itself, so a run is as long as 1024
+// workgroups leave it (one slice per workgroup read the bins of 256 rows 38 times: 65 us).
+extern "C" __global__ __launch_bounds__(256) void lgx_k_filter_list(const lgx_filter_args a) {
+    __shared__ uint64_t waves[4], below;
+    __shared__ double roots[SF_ROOTS];
+    __shared__ int found, count, start;
+    const int tid = threadIdx.x, lane = tid & 63, n = min(*a.wide_n, a.slots), all_slices = n * a.nslices;
+    const int per = (int)((unsigned)(all_slices + gridDim.x - 1) / gridDim.x), at0 = blockIdx.x * per, at1 = min(at0 + per, all_slices);
+    if (at0 >= at1) return;
+    sf_roots(roots);
+    int w = -1, sl = 0, row = 0, first = 0, end = 0;
+    float tau = 0.0f, M = 0.0f;
+    double inv = 0.0;
+    for (int at = at0; at < at1; ++at, ++sl) {    // uniform
+        if (w < 0 || sl == a.nslices) {           // another row
+            w = at / a.nslices;
+            sl = at - w * a.nslices;
+            row = a.wide_row[w];
+            tau = a.wide_tau[w];
+            M = sf_row_max(a, row);
+            const SfRow r = sf_row(a, row);
+            inv = r.inv;
+            const uint64_t* hist = a.hist + (int64_t)w * a.nslices * LGX_SF_BINS + tid;
+            uint64_t mine = 0;
+#pragma unroll 8
+            for (int i = 0; i < a.nslices; ++i) mine += hist[i * LGX_SF_BINS];
+            uint64_t upto = wave_scan64(mine), total = 0;
+            __syncthreads();
+            if (lane == 63) waves[tid >> 6] = upto;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                upto += i < tid >> 6 ? waves[i] : 0;
+                total += waves[i];
+            }
+            // of bins first .. end not all tokens are known to be kept or not
+            const uint64_t need = max((uint64_t)ceil((double)r.p * a.wide_all[w]), (uint64_t)1);
+            first = LGX_SF_BINS;
+            end = LGX_SF_BINS - 1;
+            uint64_t base = 0;                    // weight of the bins before `end`
+            if (r.mp > 0.0f) first = SfSliceBins(M, tau)(fminf(M + sf_temperature(a, row) * (logf(r.mp) + 0.001f), M));
+            const bool cut = r.p < 1.0f && need <= total;
+            if (cut) {                            // uniform
+                if (upto >= need && upto - mine < need) {
+                    found = tid;
+                    below = upto - mine;
+                }
+                __syncthreads();
+                end = found;
+                base = below;
+                first = min(first, end);
+            }
+            if (sl == 0 && tid == 0) {
+                a.wide_cut[w].first = first;
+                a.wide_cut[w].end = end;
+                a.wide_cut[w].cut = cut;
+                a.wide_cut[w].base = base;
+            }
+        }
+        const float* x = a.logits + (int64_t)row * a.ld;
+        const SfSliceBins bin(M, tau);
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int e = sl * LGX_SF_SLICE + 256 * i + tid;
+            v[i] = e < a.vocab ? x[e] : __builtin_nanf("");
+        }
+        __syncthreads();                          // the last slice's counts are read
+        if (tid == 0) count = 0;
+        __syncthreads();
+        int c = 0;                                // listed of the thread's
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int b = v[i] >= tau ? bin(v[i]) : -1;
+            if (b < first || b > end) v[i] = __builtin_nanf("");
+            else ++c;
+        }
+        int to = wave_scan(c);
+        const int in = __builtin_amdgcn_readlane(to, 63);
+        int from = 0;
+        if (lane == 0) from = __hip_atomic_fetch_add(&count, in, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        to += __builtin_amdgcn_readlane(from, 0) - c;
+        __syncthreads();
+        if (tid == 0) start = atomicAdd(&a.wide_cut[w].count, count);
+        __syncthreads();
+        to += start;
+        uint32_t* keys = a.wide_key + (int64_t)w * LGX_SF_LIST;
+        uint64_t* wis = a.wide_wi + (int64_t)w * LGX_SF_LIST;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (v[i] == v[i]) {
+                if (to < LGX_SF_LIST) {
+                    keys[to] = sf_key(v[i]);
+                    wis[to] = sf_weight_units(v[i], M, inv, roots) << 20 | (uint64_t)(sl * LGX_SF_SLICE + 256 * i + tid);
+                }
+                ++to;
+            }
+    }
+}
+
+// The choice in a wide row, from the bins of its slices and the list: the token with which
+// top-p ends, then what is kept of each slice, the slice that the draw falls into and the
+// token in it.
 extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_wide(const lgx_filter_args a) {
     __shared__ SfLds s;
     const int tid = threadIdx.x, lane = tid & 63, V = a.vocab, all_rows = *a.wide_n;
@@ -1065,47 +1140,19 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_wide(const lgx_
         sf_roots(s.roots);
         const SfSliceBins bin(M, tau);
         const uint64_t* hist = a.hist + (int64_t)w * a.nslices * LGX_SF_BINS;
-        // weight per bin: four threads a bin, each a quarter of the slices
         uint64_t mine = 0, total;
-        if (w < a.slots)
-            for (int i = tid >> 8; i < a.nslices; i += SF_NT / LGX_SF_BINS) mine += hist[i * LGX_SF_BINS + (tid & 255)];
-        s.bins[tid] = mine;
-        if (tid == 0) s.count = 0;
-        __syncthreads();
-        mine = tid < LGX_SF_BINS ? s.bins[tid] + s.bins[tid + 256] + s.bins[tid + 512] + s.bins[tid + 768] : 0;
-        const uint64_t upto = sf_scan<uint64_t>(mine, s.wave, total);
         const uint64_t need = max((uint64_t)ceil((double)r.p * all), (uint64_t)1), low = (uint64_t)ceil((double)r.mp * SF_ONE);
-        // of bins first .. end not all tokens are known to be kept or not: those are listed
-        int first = LGX_SF_BINS, end = LGX_SF_BINS - 1;
-        if (r.mp > 0.0f) first = bin(fminf(M + sf_temperature(a, row) * (logf(r.mp) + 0.001f), M));
-        uint64_t base = 0;                        // weight of the bins below `end`
-        bool few = w < a.slots;
-        const bool cut = few && r.p < 1.0f && need <= total;
-        if (cut) {                                // uniform
-            if (upto >= need && upto - mine < need) {
-                s.found = tid;
-                s.below = upto - mine;
+        const bool room = w < a.slots;
+        const lgx_filter_cut known = a.wide_cut[room ? w : 0];
+        const int first = known.first, end = known.end, n = known.count;
+        const uint64_t base = known.base;         // weight of the bins below `end`
+        const bool cut = known.cut, few = room && n <= SF_LIST;
+        if (few) {                                // uniform
+            for (int i = tid; i < n; i += SF_NT) {
+                s.key[i] = a.wide_key[(int64_t)w * SF_LIST + i];
+                s.wi[i] = a.wide_wi[(int64_t)w * SF_LIST + i];
             }
             __syncthreads();
-            end = s.found;
-            base = s.below;
-            first = min(first, end);
-        }
-        int n = 0;
-        if (few && first < LGX_SF_BINS) {         // uniform
-            sf_row_each(x, V, a.vec, [&](float v, int i) {
-                if (!(v >= tau)) return;
-                const int b = bin(v);
-                if (b < first || b > end) return;
-                const int to = __hip_atomic_fetch_add(&s.count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                if (to < SF_LIST) {
-                    s.key[to] = sf_key(v);
-                    s.wi[to] = sf_weight_units(v, M, r.inv, s.roots) << 20 | (uint64_t)i;
-                }
-            });
-            __syncthreads();
-            n = s.count;
-            few = n <= SF_LIST;
         }
         if (!few) {                               // equal or nearly equal logits, or no room for bins
             sf_choose(s, a, r, SfBins(M, tau), row, all, SfInRow{x, V, tau, M, r.inv, s.roots});
