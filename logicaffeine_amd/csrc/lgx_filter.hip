@@ -13,8 +13,19 @@
 // logit tau below which no token can be kept, reads again only the runs of 64 whose largest
 // reaches it, and selects among those tokens, in LDS.  A row without filters needs the
 // sums and one run of 4096.  Rows of which top-p or min-p keep more tokens than that list
-// holds (wide) are left to two more launches: bins of the weights, a workgroup per 4096
-// logits, and the choice from them.
+// holds (wide) are left to three more launches: bins of the weights by 4096 logits, the
+// tokens of the bins that are neither kept nor cut whole, and the choice among those.
+//
+// What bounds it, at 151936 logits: many rows the scan, which reads at 4.1 to 4.9 TB/s
+// (512 rows of all kinds 60 us of 127; 256 rows without sums 38), and its weights where
+// top-p or no filter needs their sums (another 24 us of 256 rows: binary64 arithmetic).  One
+// row its chain of memory rounds and barriers: scan 3.7 us, pick 6 to 10 us, 1 us each for
+// the launches that find no wide row; 58 us for a row of which 100000 tokens are kept.
+//   One pass over the row by its own workgroup in place of scan and pick: 152064 logits at
+//   one compute unit's rate are 20 us or more a pass, and small batches need all of them.
+//   Tokens read by the runs' maxima: a row with top-k 50 reads 60 to 100 runs of 2374.
+//   Wide rows by their own workgroup: 100 us against 58 for one row, 74 against 50 at
+//   temperature 1.4; but 207 against 237 for 256 of them, which fill the device by themselves.
 //
 // Sums decide between tokens, so they are exact or nearly: the weights that a
 // selection adds up are whole multiples of 2^-42 in 64-bit integers, whose sums
@@ -25,7 +36,7 @@
 
 // e^x for x <= 0: x = (256 n + j) ln 2 / 256 + r, 2^(j/256) from a table (sf_roots), e^r by its
 // Taylor polynomial of degree 3 (|r| <= 0.00136: the term after it is under 2e-13).  The
-// argument comes in units of ln 2 / 256 (SfScale).
+// argument comes in units of ln 2 / 256.
 #define SF_ROOTS 256
 __device__ __forceinline__ double sf_root_exp(double y, const double* roots, int& n) {
     const double k = rint(y), r = (y - k) * (0.69314718055994530942 / SF_ROOTS);

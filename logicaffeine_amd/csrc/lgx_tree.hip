@@ -10,6 +10,10 @@
 //
 // A thread holds 4 pairs of a head: pair p < rot / 2 is (p, p + rot / 2), or (2p, 2p + 1)
 // when interleaved, and turns; the others are (2p, 2p + 1) and do not.
+//
+// Bound by memory: 64 sequences of up to 33 rows of 36 heads of 128 (38 MB where half the
+// rows are padding) take 13.2 to 15.9 us, 2.4 to 2.9 TB/s, after two dependent rounds for a
+// row's number, length and angle.  A small call is those rounds: 3.6 us for 6 rows.
 // ---------------------------------------------------------------------------
 template <int D>
 __device__ __forceinline__ void append_rows_body(const lgx_append_rows_args& a) {
@@ -110,7 +114,8 @@ extern "C" __global__ __launch_bounds__(256) void lgx_k_append_rows_d128(const l
 
 // ---------------------------------------------------------------------------
 // Trees.  parent[j] < j, or -1 where node j hangs from the sequence's last token; any
-// other value counts as -1.
+// other value counts as -1.  A plan or a walk is a few dependent steps of one wave:
+// 2.5 us for the walk of one tree of 6 nodes, 5.0 for 32 of 24.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int tree_parent(int p, int j) { return p >= 0 && p < j ? p : -1; }
 
@@ -180,7 +185,8 @@ extern "C" __global__ __launch_bounds__(64) void lgx_k_tree_accept(const lgx_tre
 // Rows start + keep[i] of a sequence become rows start + i, a wave per (sequence, K or V
 // array of a layer, KV head).  keep ascends, so that a row's new place is never behind
 // its old one, and never a later row's old one: 16 / (D / 64) rows are read before any of
-// them is written, then the next ones.
+// them is written, then the next ones.  A small call is four dependent rounds (3.3 us for 6
+// nodes in 24 layers); 28 layers of 32 sequences, 17 MB, take 6.9 to 7.3 us.
 template <int D>
 __device__ __forceinline__ void kv_keep_body(const lgx_kv_keep_args& a) {
     constexpr int CH = D / 8, RW = 64 / CH, U = 4;   // pieces of a row, rows of a load, loads in flight
