@@ -372,7 +372,7 @@ lgx_status lgx_tree_plan(lgx_ctx* ctx, const int32_t* parent, const int32_t* n_n
 /* lgx_rope_kv_append of N rows per sequence (any number): row b*N + j of qkv
  * ([B*N][(hq + 2 hkv) d]: q heads | k heads | v heads), plus bias (nullable), is rotated to
  * position seq_len[b] + depth[b][j] (depth NULL: j, a run of new tokens), q written to
- * q_out [B*N][hq][d], k and v rounded to binary16 into slot seq_len[b] + j.  With rot = d and
+ * q_out [B*N][hq][d] (apart from qkv), k and v rounded to binary16 into slot seq_len[b] + j.  With rot = d and
  * pairs of halves the bits of lgx_rope_kv_append.  rope as in
  * lgx_rope_kv_append_i8.  Lengths are clamped to [0, 16 maxp]; tokens past 16 maxp and
  * pages outside [0, num_pages) are not written.  seq_len is not advanced. */
@@ -384,8 +384,8 @@ lgx_status lgx_rope_kv_append_rows(lgx_ctx* ctx, const float* qkv, const float* 
  * (clamped to [0, max_seq_len], max_seq_len + N <= 16 maxp) and those nodes i < n_nodes[b] whose
  * bit is set in mask[b][j] (lgx_tree_plan's words, or any others; NULL: nodes 0 .. j), cache
  * slots seq_len[b] + i.  opts as above, by positions: node j stands at seq_len[b] +
- * depth[b][j] (NULL: j; below 0: 0).  q and out [B*N][hq][d], 16-byte aligned; hq/hkv in
- * 1..16; page ids are clamped to [0, num_pages).  A node that sees nothing gives zeros.  With
+ * depth[b][j] (NULL: j; below 0: 0).  q and out [B*N][hq][d], 16-byte aligned, apart from
+ * each other; hq/hkv in 1..16; page ids are clamped to [0, num_pages).  A node that sees nothing gives zeros.  With
  * N = 1 and neither mask nor depth a decode step whose token is already cached.
  * Not the canonical schedule: products of binary16 keys and values with queries and
  * weights of 22 bits (or to 2^-25 of a query row's, 2^-35 of a row's weights' largest),
@@ -464,7 +464,8 @@ lgx_status lgx_pages_fork(lgx_ctx* ctx, const lgx_page_pool* pool, int32_t* page
  * added to copies [B][2]; n_copies[0] of them are written.  New pages are the
  * lowest free ones in the order of (sequence, entry).  If there are too few, nothing
  * changes, n_copies[0] is 0 and lacking[0], else 0, says how many more it would take.  The
- * copies have to be made (lgx_pages_copy) before the old pages change hands again. */
+ * copies have to be made (lgx_pages_copy) before the old pages change hands again.
+ * B (maxp + 1) < 2^31. */
 lgx_status lgx_pages_reserve(lgx_ctx* ctx, const lgx_page_pool* pool, int32_t* page_table, const int32_t* seq_len,
                              const int32_t* need, int32_t B, int32_t maxp, int32_t* copies, int32_t* n_copies,
                              int32_t* lacking, void* stream);

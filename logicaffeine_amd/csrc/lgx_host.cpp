@@ -88,7 +88,7 @@ lgx_status lgx_ctx_create(int32_t device, const char* hsaco_path, lgx_ctx** out)
         c->pfa_rows = env_int("LGX_PFA_ROWS", 0);
         c->attn8_wgs = std::max(1, env_int("LGX_A8_WGS", c->attn8_wgs));
         c->attn8_cols = env_int("LGX_A8_COLS", 0);
-        c->tree_wgs = std::max(1, env_int("LGX_TREE_WGS", c->tree_wgs));
+        c->tree_wgs = std::min(std::max(1, env_int("LGX_TREE_WGS", c->tree_wgs)), 64);
         c->decode_fuse = env_int("LGX_DECODE_FUSE", 1) != 0;
         c->fuse_cols32 = env_int("LGX_FUSE_SWIGLU_COLS", 32) == 64 ? 2 : 1;
         c->merge_o_tiles = std::min(std::max(env_int("LGX_MERGE_O_TILES", 8), 1), 16);

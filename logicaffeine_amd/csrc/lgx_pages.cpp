@@ -54,6 +54,9 @@ lgx_status lgx_pages_reserve(lgx_ctx* c, const lgx_page_pool* pool, int32_t* pag
         if ((st = check_pool(pool, page_table, maxp)) != LGX_OK) return st;
         if (!seq_len || !need || !copies || !n_copies || !lacking) return fail(LGX_NULL_POINTER, "NULL tensor pointer");
         if (B <= 0 || B > LGX_PAGES_SEQS) return fail(LGX_INVALID_ARGUMENT, "B=%d (1..%d)", B, LGX_PAGES_SEQS);
+        // needs are summed in 32 bits
+        if ((int64_t)B * ((int64_t)maxp + 1) > INT32_MAX)
+            return fail(LGX_OUT_OF_BOUNDS, "a table of %d rows of %d entries", B, maxp);
         // a list of the pages found: never more than there are, nor than all entries
         // and one copy per sequence
         const int64_t most = std::min<int64_t>(pool->num_pages, (int64_t)B * ((int64_t)maxp + 1));

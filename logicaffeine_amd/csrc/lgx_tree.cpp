@@ -20,6 +20,9 @@ lgx_status check_kv(const lgx_kv_f16* kv, int32_t maxp) {
     return LGX_OK;
 }
 
+// An output that another row's thread still reads, or that is read again (tree_column).
+bool overlap(const float* a, int64_t na, const float* b, int64_t nb) { return a < b + nb && b < a + na; }
+
 lgx_status check_tree(int32_t B, int32_t N) {
     if (B <= 0 || N <= 0 || N > LGX_TREE_NODES)
         return fail(LGX_INVALID_ARGUMENT, "B=%d, %d nodes (1..%d)", B, N, LGX_TREE_NODES);
@@ -94,6 +97,8 @@ lgx_status lgx_gqa_tree_attn(lgx_ctx* c, const float* q, const lgx_kv_f16* kv, c
             return fail(LGX_OUT_OF_BOUNDS, "max_seq_len %d outside [0, %d]", max_seq_len, maxp * LGX_PAGE - N);
         if ((int64_t)B * N * hq > INT32_MAX / 128) return fail(LGX_OUT_OF_BOUNDS, "B*N*hq too large");
         if (!aligned16(q) || !aligned16(out)) return fail(LGX_INVALID_ARGUMENT, "q and out must be 16-byte aligned");
+        const int64_t n = (int64_t)B * N * hq * kv->d;
+        if (overlap(q, n, out, n)) return fail(LGX_INVALID_ARGUMENT, "q and out overlap");
         lgx_tree_attn_args a{};
         a.scale = (float)(1.0 / std::sqrt((double)kv->d));
         if (opts) {
@@ -145,6 +150,8 @@ lgx_status lgx_rope_kv_append_rows(lgx_ctx* c, const float* qkv, const float* bi
         const int64_t heads = (int64_t)hq + 2 * (int64_t)kv->hkv, rows = (int64_t)B * N;
         if (rows > INT32_MAX || heads > INT32_MAX / kv->d || rows > ((int64_t)1 << 33) / heads)
             return fail(LGX_OUT_OF_BOUNDS, "append of %lld rows of %lld heads", (long long)rows, (long long)heads);
+        if (overlap(qkv, rows * heads * kv->d, q_out, rows * hq * kv->d))
+            return fail(LGX_INVALID_ARGUMENT, "qkv and q_out overlap");
         const int per = 2048 / kv->d;                 // heads of a workgroup
         const int64_t wgs = (rows * heads + per - 1) / per;
         if (wgs > UINT32_MAX / 256) return fail(LGX_OUT_OF_BOUNDS, "append of %lld heads", (long long)(rows * heads));

@@ -30,7 +30,7 @@ for line in sys.stdin:
     st = getattr(L, name)(h, *keep)
     print(json.dumps([lgx.STATUS_NAMES.get(st, st), stub.stub_log().decode().splitlines()]), flush=True)
 """
-P = 1 << 41
+P, Q = 1 << 41, 1 << 42
 NULL, INVALID, UNSUPPORTED, OUT = "LGX_NULL_POINTER", "LGX_INVALID_ARGUMENT", "LGX_UNSUPPORTED", "LGX_OUT_OF_BOUNDS"
 
 
@@ -65,12 +65,12 @@ def kv(**a):
     return ["kv", shape(**a)]
 
 
-def attn(B=2, N=5, hq=14, maxp=10, top=155, cache=0, opts=None, q=P, out=P, table=P, lens=P, n=None, depth=None, mask=None):
+def attn(B=2, N=5, hq=14, maxp=10, top=155, cache=0, opts=None, q=P, out=Q, table=P, lens=P, n=None, depth=None, mask=None):
     return ["lgx_gqa_tree_attn", [q, kv() if cache == 0 else cache, table, lens, n, depth, mask, B, N, hq, maxp, top, opts, out,
                                   None]]
 
 
-def append(B=2, N=5, hq=14, maxp=10, cache=0, rope=0, x=P, q=P, lens=P, table=P):
+def append(B=2, N=5, hq=14, maxp=10, cache=0, rope=0, x=P, q=Q, lens=P, table=P):
     return ["lgx_rope_kv_append_rows", [x, None, ["rope", [P, P, 64, 0, 100]] if rope == 0 else rope, lens, None, None, table,
                                         kv() if cache == 0 else cache, q, B, N, hq, maxp, None]]
 
@@ -121,7 +121,8 @@ REFUSED = [
     (attn(cache=kv(hkv=0)), INVALID), (attn(q=P + 4), INVALID), (attn(out=P + 8), INVALID), (attn(B=0), INVALID),
     (attn(N=0), INVALID), (attn(N=257, top=0, maxp=100), INVALID), (attn(hq=13), INVALID), (attn(hq=0), INVALID),
     (attn(hq=34), UNSUPPORTED), (attn(top=-1), OUT), (attn(top=156), OUT), (attn(maxp=0), INVALID),
-    (attn(maxp=(1 << 26) + 1, top=1), INVALID), (attn(B=1 << 24), OUT),
+    (attn(maxp=(1 << 26) + 1, top=1), INVALID), (attn(B=1 << 24), OUT), (attn(out=P), INVALID),
+    (attn(out=P + 4 * 2 * 5 * 14 * 64 - 16), INVALID), (attn(out=Q, q=Q + 16), INVALID),
     *[(attn(opts=["opts", o]), INVALID) for o in ([0.0, -1.0, 0, None], [0.0, float("inf"), 0, None], [0.0, 1e-38, 0, None],
                                                   [float("nan"), 0.0, 0, None], [0.0, 0.0, -1, None])],
     *[(append(**{a: None}), NULL) for a in ("x", "q", "lens", "table", "cache", "rope")],
@@ -130,7 +131,7 @@ REFUSED = [
     (append(rope=["rope", [P, P, 64, 2, 100]]), INVALID), (append(rope=["rope", [P, P, 64, 0, 0]]), INVALID),
     (append(B=0), INVALID), (append(N=0), INVALID), (append(hq=0), INVALID), (append(hq=15), INVALID),
     (append(cache=kv(d=32)), UNSUPPORTED), (append(cache=kv(k=P + 2)), INVALID), (append(B=1 << 20, N=1 << 12), OUT),
-    (append(B=1 << 15, N=1 << 15), OUT),
+    (append(B=1 << 15, N=1 << 15), OUT), (append(q=P), INVALID), (append(q=P + 4 * 2 * 5 * 18 * 64 - 16), INVALID),
     *[(plan(**{a: None}), NULL) for a in ("parent", "depth", "mask")], (plan(B=0), INVALID), (plan(N=0), INVALID),
     (plan(N=257), INVALID), (plan(B=(1 << 23) + 1), OUT),
     *[(accept(**{a: None}), NULL) for a in ("tokens", "parent", "picked", "path", "count", "nxt", "lens")],
@@ -146,7 +147,8 @@ REFUSED = [
     (fork(pool=["pool", [P, 0]]), INVALID), (fork(S=0), INVALID), (fork(n=0), INVALID), (fork(n=1025), INVALID),
     (fork(maxp=0), INVALID), (fork(maxp=1 << 24), INVALID),
     *[(reserve(**{a: None}), NULL) for a in ("pool", "table", "lens", "need", "copies", "n", "lacking")],
-    (reserve(B=0), INVALID), (reserve(B=1025), INVALID), (reserve(maxp=0), INVALID),
+    (reserve(B=0), INVALID), (reserve(B=1025), INVALID), (reserve(maxp=0), INVALID), (reserve(B=32, maxp=1 << 26), OUT),
+    (reserve(B=1024, maxp=(1 << 21)), OUT),
     *[(copy(**{a: None}), NULL) for a in ("planes", "copies", "n")], (copy(planes=["plane", [P, 64], [None, 64]]), NULL),
     (copy(planes=["plane", [P, 0]]), INVALID), (copy(planes=["plane", [P, 1 << 62]]), INVALID), (copy(n_planes=0), INVALID),
     (copy(pages=0), INVALID), (copy(most=0), INVALID),
