@@ -258,7 +258,8 @@ lgx_status lgx_sample_filtered(lgx_ctx* c, const float* logits, int64_t ld, int3
         // room for the bins and lists of as many wide rows as 64 MiB hold; the others take longer
         const size_t ns = (size_t)m * a.nslices, bins = (size_t)a.nslices * LGX_SF_BINS;
         const size_t slot = 8 * bins + sizeof(lgx_filter_cut) + 12 * LGX_SF_LIST;
-        if (top_p || min_p) a.slots = (int)std::min<size_t>(m, std::max<size_t>(((size_t)64 << 20) / slot, 1));
+        // (a row of no more tokens than a workgroup lists is never wide)
+        if ((top_p || min_p) && vocab > LGX_SF_LIST) a.slots = (int)std::min<size_t>(m, std::max<size_t>(((size_t)64 << 20) / slot, 1));
         const size_t fours = ns * (1 + LGX_SF_SLICE / LGX_SF_CHUNK) + 2 * (size_t)m + 1;
         float* ws = nullptr;
         if ((st = ensure_ws(c, 8 * (ns + m) + a.slots * slot + 4 * fours, stream, &ws)) != LGX_OK) return st;

@@ -220,3 +220,61 @@ def test_drafts_yield_the_tokens_of_single_steps(ctx, S, N, settings, captured):
     assert int(srv.pool.ref.abs().sum()) == 0 and bool((srv.table == -1).all())
     if N > 1:
         assert rounds < total - len(prompt)       # drafts held
+
+
+def test_two_graphs_share_a_workspace_that_grows(ctx):
+    """Split attention, wide rows of logits and a reservation, whose intermediates all lie in
+    the context's workspace, in two graphs replayed in turn; between the replays other inputs and
+    an eager call that needs a larger workspace."""
+    own = lgx.Context(0)
+    rng = np.random.default_rng(8)
+    B, N, hq, hkv, d, L = 2, 5, 4, 2, 64, 900
+    maxp = -(-(L + N) // PAGE)
+    kv = lgx.KvCacheF16(*(torch.tensor(rng.standard_normal((B * maxp, hkv, PAGE, d)), dtype=torch.float16, device="cuda")
+                          for _ in range(2)))
+    table = torch.arange(B * maxp, dtype=torch.int32, device="cuda").view(B, maxp)
+    lens = torch.zeros(B, dtype=torch.int32, device="cuda")
+    q = torch.zeros((B * N, hq, d), device="cuda")
+    logits, u = torch.zeros((3, 30000), device="cuda"), torch.zeros(3, device="cuda")
+    top_p = torch.tensor([0.9, 0.5, 0.99], device="cuda")
+    ref = torch.zeros(50, dtype=torch.int32, device="cuda")
+    rows, held, need = (torch.full(s, v, dtype=torch.int32, device="cuda") for s, v in (((4, 9), -1), ((4,), 0), ((4,), 0)))
+
+    def fill(i):
+        r = np.random.default_rng(100 + i)
+        lens.copy_(torch.tensor(r.integers(0, L + 1, B)))
+        q.copy_(torch.tensor(r.standard_normal(q.shape)))
+        logits.copy_(torch.tensor(0.2 * r.standard_normal(logits.shape)))
+        u.copy_(torch.tensor(r.random(3)))
+        need.copy_(torch.tensor(r.integers(0, 100, 4)))
+        ref.zero_()
+        rows.fill_(-1)
+
+    def work(c):
+        out = c.gqa_tree_attn(q, kv, table, lens, N, L)
+        token, prob = c.sample_filtered(logits, u, top_p=top_p)
+        more = c.pages_reserve(lgx.PagePool(ref), rows, held, need)
+        return [out, token, prob, *more, rows, ref]
+
+    fill(0)
+    work(own)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            result = work(own)
+        graphs.append((g, result))
+    for i in range(8):
+        g, result = graphs[i % 2]
+        fill(i)
+        g.replay()
+        got = [x.clone() for x in result]
+        fill(i)
+        for x, y in zip(got, work(ctx)):
+            assert torch.equal(x, y)
+        if i == 3:                                # outgrows the workspace that the graphs go on using
+            many = torch.randn((400, 40000), device="cuda")
+            own.sample_filtered(many, torch.rand(400, device="cuda"), top_p=torch.full((400,), 0.9, device="cuda"))
+    del graphs, g, result
+    torch.cuda.synchronize()
+    own.close()
