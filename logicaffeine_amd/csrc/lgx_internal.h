@@ -196,7 +196,9 @@ enum Kern {
     K_FILTER_WIDE,
     K_TREE_ATTN_D64, // + 1: with caps, distances or a window
     K_TREE_ATTN_D128 = K_TREE_ATTN_D64 + 2,
-    K_COUNT = K_TREE_ATTN_D128 + 2
+    K_TREE_JOIN_D64 = K_TREE_ATTN_D128 + 2, // + 1: many rows
+    K_TREE_JOIN_D128 = K_TREE_JOIN_D64 + 2,
+    K_COUNT = K_TREE_JOIN_D128 + 2
 };
 inline const char* const kKernelNames[] = {
     "lgx_k_repack_t16", "lgx_k_quantize_q8_0", "lgx_k_q8q8_gemv",
@@ -256,6 +258,7 @@ inline const char* const kKernelNames[] = {
     "lgx_k_kv_keep_d64", "lgx_k_kv_keep_d128", "lgx_k_filter_scan", "lgx_k_filter_pick", "lgx_k_filter_bins",
     "lgx_k_filter_list", "lgx_k_filter_wide",
     "lgx_k_tree_attn_d64", "lgx_k_tree_attnx_d64", "lgx_k_tree_attn_d128", "lgx_k_tree_attnx_d128",
+    "lgx_k_tree_join_d64", "lgx_k_tree_joinr_d64", "lgx_k_tree_join_d128", "lgx_k_tree_joinr_d128",
 };
 
 static_assert(sizeof(kKernelNames) / sizeof(kKernelNames[0]) == K_COUNT,

@@ -590,7 +590,7 @@ typedef struct {
     float* out;                // [B*N][hq][d]
     // per > 0: the sequences' tiles are split on the device so that `per` workgroups per
     // KV head share all of them and their column blocks (see Tree::place); the partial
-    // results are lgx_k_attn8_join_*'s
+    // results are lgx_k_tree_join*'s
     float* part;               // [per][hkv][columns][d]: results of splits
     float* ml;                 // [per][hkv][columns][2]: their maxima and sums
     int32_t* plan;             // [B * ncb][2]: first split, number of splits
@@ -598,6 +598,7 @@ typedef struct {
     int32_t maxlen;            // cached tokens at most
     int32_t window;            // 0: all
     int32_t per, units, ncb;   // units: B; ncb: column blocks of a sequence at most
+    int32_t rows;              // B*N
     float scale, softcap;
 } lgx_tree_attn_args;
 #define LGX_TREE_TILE 64       // tokens of a tile: four pages

@@ -43,6 +43,7 @@ lgx_status run_tree(lgx_ctx* c, lgx_tree_attn_args& a, int B, int d, bool x, voi
     const int64_t ncb = cdiv(cols, LGX_TREE_COLS), units = B * ncb, blocks = heads * ncb;
     a.ncb = (int)ncb;
     a.units = B;
+    a.rows = B * a.N;
     const int64_t per = (int64_t)c->tree_wgs * c->ncu / a.hkv;
     const bool split = tiles > LGX_TREE_MIN && B <= LGX_TREE_UNITS && units < per && units * tiles <= INT32_MAX;
     lgx_status st;
@@ -59,22 +60,13 @@ lgx_status run_tree(lgx_ctx* c, lgx_tree_attn_args& a, int B, int d, bool x, voi
     if (grid > UINT32_MAX / 256) return fail(LGX_OUT_OF_BOUNDS, "attention of %lld workgroups", (long long)grid);
     const int k = (d == 64 ? K_TREE_ATTN_D64 : K_TREE_ATTN_D128) + (x ? 1 : 0);
     if ((st = launch(c, (Kern)k, dim3((unsigned)grid), dim3(256), a, stream)) != LGX_OK || !split) return st;
-    lgx_attn8_args j{};
-    j.part = a.part;
-    j.ml = a.ml;
-    j.plan = a.plan;
-    j.out = a.out;
-    j.n_new = a.n_nodes;
-    j.P = a.N;
-    j.hq = a.hq;
-    j.hkv = a.hkv;
-    j.ncb = a.ncb;
-    j.cols = LGX_TREE_COLS;
-    j.rows = B * a.N;
-    const int64_t rh = (int64_t)j.rows * a.hq;
+    const int64_t rh = (int64_t)B * a.N * a.hq;
+    // one group of lanes for all splits of a (node, query head) from 8 of them to a compute unit
+    // on (14336 of them with 2 or 3 splits: the whole call 66.6 against 75.7 us), several below
+    // (1792 with 18: 33.2 against 34.8)
     const int w = rh >= 8 * (int64_t)c->ncu ? 1 : 0;
-    return launch(c, (Kern)((d == 64 ? K_ATTN8_JOIN_D64 : K_ATTN8_JOIN_D128) + w), dim3(w ? cdiv(rh, 4) : (unsigned)rh),
-                  dim3(256), j, stream);
+    return launch(c, (Kern)((d == 64 ? K_TREE_JOIN_D64 : K_TREE_JOIN_D128) + w), dim3(w ? cdiv(rh * (d / 4), 256) : (unsigned)rh),
+                  dim3(256), a, stream);
 }
 
 }  // namespace

@@ -595,3 +595,70 @@ LGX_TREE_KERNEL(lgx_k_tree_attn_d64, (tree_body<64, false>))
 LGX_TREE_KERNEL(lgx_k_tree_attnx_d64, (tree_body<64, true>))
 LGX_TREE_KERNEL(lgx_k_tree_attn_d128, (tree_body<128, false>))
 LGX_TREE_KERNEL(lgx_k_tree_attnx_d128, (tree_body<128, true>))
+
+// Joins the splits of each (node, query head): D / 4 lanes hold its dimensions, NG such
+// groups take its splits in turn, four in flight, and meet in LDS.  A row is its plan's
+// memory round, then one for each four splits of a group.
+template <int D, int NG>
+__device__ __forceinline__ void tree_join_body(const lgx_tree_attn_args& a) {
+    constexpr int Q = D / 4, IT = 256 / (Q * NG);  // items of a workgroup
+    __shared__ v4f o_s[NG > 1 ? NG * Q : 1];
+    __shared__ float2 ml_s[NG > 1 ? NG : 1];
+    const int q = threadIdx.x % Q, sg = NG > 1 ? threadIdx.x / Q : 0;
+    const unsigned item = blockIdx.x * IT + (NG > 1 ? 0 : threadIdx.x / Q);
+    if (item >= (unsigned)a.rows * (unsigned)a.hq) return;
+    const unsigned row = item / (unsigned)a.hq, b = row / (unsigned)a.N;
+    const int h = (int)(item - row * a.hq), j = (int)(row - b * a.N), G = a.hq / a.hkv;
+    const int g = h / G, c = j * G + h - g * G, u = (int)b * a.ncb + c / LGX_TREE_COLS;
+    const int n = a.n_nodes ? a.n_nodes[b] : a.N;
+    const int2 plan = *(const int2*)(a.plan + 2 * u);
+    if (j >= n || plan.y < 2) return;             // with NG > 1 uniform
+    const float inf = __builtin_inff();
+    const int64_t at0 = ((int64_t)plan.x * a.hkv + g) * LGX_TREE_COLS + c % LGX_TREE_COLS, step = (int64_t)a.hkv * LGX_TREE_COLS;
+    float m = -inf, l = 0.0f;
+    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+    // ls times the mean os, by the maximum ms (an empty split's is -inf; so is a NaN one's, whose ls is NaN)
+    auto join = [&](float ms, float ls, v4f os) {
+        const float mn = fmaxf(m, ms);
+        const float u0 = m == -inf ? 0.0f : __builtin_amdgcn_exp2f(m - mn), u1 = (ms == -inf ? 0.0f : __builtin_amdgcn_exp2f(ms - mn)) * ls;
+        o = o * u0 + os * u1;
+        l = l * u0 + u1;
+        m = mn;
+    };
+    for (int s0 = sg; s0 < plan.y; s0 += 4 * NG) {
+        float2 ml[4];
+        v4f p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t at = at0 + min(s0 + i * NG, plan.y - 1) * step;
+            ml[i] = *(const float2*)(a.ml + 2 * at);
+            p[i] = *((const v4f*)(a.part + at * D) + q);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s0 + i * NG < plan.y) join(ml[i].x, ml[i].y, p[i]);
+    }
+    if constexpr (NG > 1) {
+        o_s[threadIdx.x] = o;                     // not yet divided by l
+        if (q == 0) ml_s[sg] = make_float2(m, l);
+        __syncthreads();
+        if (sg) return;
+        float mx = m;
+#pragma unroll
+        for (int i = 1; i < NG; ++i) mx = fmaxf(mx, ml_s[i].x);
+        l = 0.0f;
+        o = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const float w = ml_s[i].x == -inf ? 0.0f : __builtin_amdgcn_exp2f(ml_s[i].x - mx);
+            l += ml_s[i].y * w;
+            o += o_s[i * Q + q] * w;
+        }
+    }
+    const float r = l == 0.0f ? 0.0f : 1.0f / l;
+    *((v4f*)(a.out + (int64_t)item * D) + q) = o * r;
+}
+extern "C" __global__ __launch_bounds__(256) void lgx_k_tree_join_d64(const lgx_tree_attn_args a) { tree_join_body<64, 16>(a); }
+extern "C" __global__ __launch_bounds__(256) void lgx_k_tree_joinr_d64(const lgx_tree_attn_args a) { tree_join_body<64, 1>(a); }
+extern "C" __global__ __launch_bounds__(256) void lgx_k_tree_join_d128(const lgx_tree_attn_args a) { tree_join_body<128, 8>(a); }
+extern "C" __global__ __launch_bounds__(256) void lgx_k_tree_joinr_d128(const lgx_tree_attn_args a) { tree_join_body<128, 1>(a); }

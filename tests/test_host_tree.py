@@ -179,8 +179,8 @@ def test_attention_covers_every_column(host, B, N, hq, hkv, d, top, opts):
         assert blocks <= gx < blocks + 8 and alloc == 0
     else:
         assert gx >= blocks and B <= 256
-        per = 4 if "joinw" in launches[1][0] else 1
-        assert launches[1][0] in (f"lgx_k_attn8_join_d{d}", f"lgx_k_attn8_joinw_d{d}") and len(launches) == 2
+        per = 1024 // d if "joinr" in launches[1][0] else 1
+        assert launches[1][0] in (f"lgx_k_tree_join_d{d}", f"lgx_k_tree_joinr_d{d}") and len(launches) == 2
         assert launches[1][1] * per >= B * N * hq > (launches[1][1] - 1) * per
         assert alloc >= (gx - 7) // hkv * hkv * 64 * (d + 2) * 4 + blocks // hkv * 8
 
