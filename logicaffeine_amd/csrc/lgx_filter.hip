@@ -326,6 +326,34 @@ __device__ __forceinline__ void sf_each(const S& e, int first, int end, int step
     }
 }
 
+// f(16 logits, their indexes by a function) for a row's logits; NaN past its end.
+template <class F>
+__device__ __forceinline__ void sf_row_each(const float* x, int V, int vec, const F& f) {
+    const int tid = threadIdx.x, n4 = vec ? V / 4 : 0;
+    const float nan = __builtin_nanf("");
+    float v[16];
+    for (int i0 = tid; i0 - tid < n4; i0 += 4 * SF_NT) {   // uniform
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = i0 + u * SF_NT;
+            const float4 w = ((const float4*)x)[min(i, n4 - 1)];
+            v[4 * u] = i < n4 ? w.x : nan;
+            v[4 * u + 1] = i < n4 ? w.y : nan;
+            v[4 * u + 2] = i < n4 ? w.z : nan;
+            v[4 * u + 3] = i < n4 ? w.w : nan;
+        }
+        f(v, [&](int e) { return 4 * (i0 + (e >> 2) * SF_NT) + (e & 3); });
+    }
+    for (int i0 = 4 * n4 + tid; i0 - tid < V; i0 += 16 * SF_NT) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int i = i0 + e * SF_NT;
+            v[e] = i < V ? x[i] : nan;
+        }
+        f(v, [&](int e) { return i0 + e * SF_NT; });
+    }
+}
+
 // Bin of a key: linear in the logit between the row's maximum and tau, so that keys of
 // one bin follow each other.  A constant for all calls of a row.
 struct SfBins {
@@ -975,6 +1003,7 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
                 a.wide_row[i] = row;
                 a.wide_tau[i] = tau;
                 a.wide_all[i] = all;
+                if (i < a.slots) a.wide_done[i] = 0;
             }
         } else {
             // the row itself
@@ -1001,243 +1030,225 @@ __device__ __forceinline__ float sf_row_max(const lgx_filter_args& a, int row) {
     for (int i = threadIdx.x & 63; i < a.nslices; i += 64) M = fmaxf(M, a.smax[(int64_t)row * a.nslices + i]);
     return wave_max(M);
 }
-extern "C" __global__ __launch_bounds__(256) void lgx_k_filter_bins(const lgx_filter_args a) {
-    __shared__ uint64_t bins[LGX_SF_BINS];
-    __shared__ double roots[SF_ROOTS];
-    static_assert(LGX_SF_BINS == 256, "a thread per bin");
-    const int tid = threadIdx.x, sl = blockIdx.x, n = min(*a.wide_n, a.slots);
-    if ((int)blockIdx.y >= n) return;
-    sf_roots(roots);
-    for (int w = blockIdx.y; w < n; w += gridDim.y) {
-        const int row = a.wide_row[w];
-        const float tau = a.wide_tau[w], M = sf_row_max(a, row);
-        const double inv = sf_row(a, row).inv;
-        const float* x = a.logits + (int64_t)row * a.ld;
-        const SfSliceBins bin(M, tau);
-        bins[tid] = 0;
-        if (sl == 0 && tid == 0) a.wide_cut[w].count = 0;
-        __syncthreads();
-        float v[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int e = sl * LGX_SF_SLICE + 256 * i + tid;
-            v[i] = e < a.vocab ? x[e] : __builtin_nanf("");
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (v[i] >= tau)
-                __hip_atomic_fetch_add(&bins[bin(v[i])], sf_weight_units(v[i], M, inv, roots), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        __syncthreads();
-        a.hist[((int64_t)w * a.nslices + sl) * LGX_SF_BINS + tid] = bins[tid];
-        __syncthreads();
-    }
-}
+// What other workgroups of this launch have written, past the caches that are not theirs
+// too: loads and stores of the whole device's scope.  (Fences of that scope in their place
+// would write back and drop whole caches.)
+__device__ __forceinline__ uint64_t sf_shared(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// From the bins of all slices the one in which top-p ends and the ones that min-p may
-// cut: a slice's tokens in them go to the row's list.  Each workgroup takes a run of the
-// (wide row, slice)s and finds a row's bins for itself, so a run is as long as 1024
-// workgroups leave it (one slice per workgroup read the bins of 256 rows 38 times: 65 us).
-extern "C" __global__ __launch_bounds__(256) void lgx_k_filter_list(const lgx_filter_args a) {
-    __shared__ uint64_t waves[4], below;
-    __shared__ double roots[SF_ROOTS];
-    __shared__ int found, count, start;
-    const int tid = threadIdx.x, lane = tid & 63, n = min(*a.wide_n, a.slots), all_slices = n * a.nslices;
-    const int per = (int)((unsigned)(all_slices + gridDim.x - 1) / gridDim.x), at0 = blockIdx.x * per, at1 = min(at0 + per, all_slices);
-    if (at0 >= at1) return;
-    sf_roots(roots);
-    int w = -1, sl = 0, row = 0, first = 0, end = 0;
-    float tau = 0.0f, M = 0.0f;
-    double inv = 0.0;
-    for (int at = at0; at < at1; ++at, ++sl) {    // uniform
-        if (w < 0 || sl == a.nslices) {           // another row
-            w = at / a.nslices;
-            sl = at - w * a.nslices;
-            row = a.wide_row[w];
-            tau = a.wide_tau[w];
-            M = sf_row_max(a, row);
-            const SfRow r = sf_row(a, row);
-            inv = r.inv;
-            const uint64_t* hist = a.hist + (int64_t)w * a.nslices * LGX_SF_BINS + tid;
-            uint64_t mine = 0;
-#pragma unroll 8
-            for (int i = 0; i < a.nslices; ++i) mine += hist[i * LGX_SF_BINS];
-            uint64_t upto = wave_scan64(mine), total = 0;
-            __syncthreads();
-            if (lane == 63) waves[tid >> 6] = upto;
-            __syncthreads();
+// The choice in wide row w, from the bins of its slices: the bin in which top-p ends, the
+// tokens in it, then what is kept of each slice, the slice that the draw falls into and
+// the token in it.
+__device__ __forceinline__ void sf_choose_wide(SfLds& s, const lgx_filter_args& a, const SfRow& r, const SfSliceBins& bin, int w, int row,
+                                               float tau, float M) {
+    const int tid = threadIdx.x, lane = tid & 63, V = a.vocab;
+    const double all = a.wide_all[w];
+    const float* x = a.logits + (int64_t)row * a.ld;
+    const uint64_t* hist = a.hist + (int64_t)w * a.nslices * LGX_SF_BINS;
+    // weight per bin: four threads a bin, each a quarter of the slices
+    uint64_t mine = 0, total;
+    for (int i0 = tid >> 8; i0 < a.nslices; i0 += 12 * (SF_NT / LGX_SF_BINS)) {
+        uint64_t u[12];                       // in flight together
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                upto += i < tid >> 6 ? waves[i] : 0;
-                total += waves[i];
-            }
-            // of bins first .. end not all tokens are known to be kept or not
-            const uint64_t need = max((uint64_t)ceil((double)r.p * a.wide_all[w]), (uint64_t)1);
-            first = LGX_SF_BINS;
-            end = LGX_SF_BINS - 1;
-            uint64_t base = 0;                    // weight of the bins before `end`
-            if (r.mp > 0.0f) first = SfSliceBins(M, tau)(fminf(M + sf_temperature(a, row) * (logf(r.mp) + 0.001f), M));
-            const bool cut = r.p < 1.0f && need <= total;
-            if (cut) {                            // uniform
-                if (upto >= need && upto - mine < need) {
-                    found = tid;
-                    below = upto - mine;
-                }
-                __syncthreads();
-                end = found;
-                base = below;
-                first = min(first, end);
-            }
-            if (sl == 0 && tid == 0) {
-                a.wide_cut[w].first = first;
-                a.wide_cut[w].end = end;
-                a.wide_cut[w].cut = cut;
-                a.wide_cut[w].base = base;
-            }
-        }
-        const float* x = a.logits + (int64_t)row * a.ld;
-        const SfSliceBins bin(M, tau);
-        float v[16];
+        for (int q = 0; q < 12; ++q) u[q] = sf_shared(hist + min(i0 + q * (SF_NT / LGX_SF_BINS), a.nslices - 1) * LGX_SF_BINS + (tid & 255));
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int e = sl * LGX_SF_SLICE + 256 * i + tid;
-            v[i] = e < a.vocab ? x[e] : __builtin_nanf("");
-        }
-        __syncthreads();                          // the last slice's counts are read
-        if (tid == 0) count = 0;
-        __syncthreads();
-        int c = 0;                                // listed of the thread's
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int b = v[i] >= tau ? bin(v[i]) : -1;
-            if (b < first || b > end) v[i] = __builtin_nanf("");
-            else ++c;
-        }
-        int to = wave_scan(c);
-        const int in = __builtin_amdgcn_readlane(to, 63);
-        int from = 0;
-        if (lane == 0) from = __hip_atomic_fetch_add(&count, in, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        to += __builtin_amdgcn_readlane(from, 0) - c;
-        __syncthreads();
-        if (tid == 0) start = atomicAdd(&a.wide_cut[w].count, count);
-        __syncthreads();
-        to += start;
-        uint32_t* keys = a.wide_key + (int64_t)w * LGX_SF_LIST;
-        uint64_t* wis = a.wide_wi + (int64_t)w * LGX_SF_LIST;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (v[i] == v[i]) {
-                if (to < LGX_SF_LIST) {
-                    keys[to] = sf_key(v[i]);
-                    wis[to] = sf_weight_units(v[i], M, inv, roots) << 20 | (uint64_t)(sl * LGX_SF_SLICE + 256 * i + tid);
-                }
-                ++to;
-            }
+        for (int q = 0; q < 12; ++q) mine += i0 + q * (SF_NT / LGX_SF_BINS) < a.nslices ? u[q] : 0;
     }
-}
-
-// The choice in a wide row, from the bins of its slices and the list: the token with which
-// top-p ends, then what is kept of each slice, the slice that the draw falls into and the
-// token in it.
-extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_wide(const lgx_filter_args a) {
-    __shared__ SfLds s;
-    const int tid = threadIdx.x, lane = tid & 63, V = a.vocab, all_rows = *a.wide_n;
-    for (int w = blockIdx.x; w < all_rows; w += gridDim.x) {   // uniform
-        const int row = a.wide_row[w];
-        const float tau = a.wide_tau[w], M = sf_row_max(a, row);
-        const double all = a.wide_all[w];
-        const SfRow r = sf_row(a, row);
-        const float* x = a.logits + (int64_t)row * a.ld;
+    s.bins[tid] = mine;
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    mine = tid < LGX_SF_BINS ? s.bins[tid] + s.bins[tid + 256] + s.bins[tid + 512] + s.bins[tid + 768] : 0;
+    const uint64_t upto = sf_scan<uint64_t>(mine, s.wave, total);
+    const uint64_t need = max((uint64_t)ceil((double)r.p * all), (uint64_t)1), low = (uint64_t)ceil((double)r.mp * SF_ONE);
+    // of bins first .. end not all tokens are known to be kept or not: those are listed
+    int first = LGX_SF_BINS, end = LGX_SF_BINS - 1;
+    if (r.mp > 0.0f) first = bin(fminf(M + sf_temperature(a, row) * (logf(r.mp) + 0.001f), M));
+    uint64_t base = 0;                        // weight of the bins below `end`
+    bool few = true;
+    const bool cut = r.p < 1.0f && need <= total;
+    if (cut) {                                // uniform
+        if (upto >= need && upto - mine < need) {
+            s.found = tid;
+            s.below = upto - mine;
+        }
         __syncthreads();
-        sf_roots(s.roots);
-        const SfSliceBins bin(M, tau);
-        const uint64_t* hist = a.hist + (int64_t)w * a.nslices * LGX_SF_BINS;
-        uint64_t mine = 0, total;
-        const uint64_t need = max((uint64_t)ceil((double)r.p * all), (uint64_t)1), low = (uint64_t)ceil((double)r.mp * SF_ONE);
-        const bool room = w < a.slots;
-        const lgx_filter_cut known = a.wide_cut[room ? w : 0];
-        const int first = known.first, end = known.end, n = known.count;
-        const uint64_t base = known.base;         // weight of the bins below `end`
-        const bool cut = known.cut, few = room && n <= SF_LIST;
-        if (few) {                                // uniform
-            for (int i = tid; i < n; i += SF_NT) {
-                s.key[i] = a.wide_key[(int64_t)w * SF_LIST + i];
-                s.wi[i] = a.wide_wi[(int64_t)w * SF_LIST + i];
+        end = s.found;
+        base = s.below;
+        first = min(first, end);
+    }
+    int n = 0;
+    if (first < LGX_SF_BINS) {                // uniform
+        // counted, then written from one place per wave; weights afterwards, by as many lanes
+        // as there are tokens
+        sf_row_each(x, V, a.vec, [&](float (&v)[16], auto index) __attribute__((always_inline)) {
+            int c = 0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int b = bin(v[e]);
+                const bool on = v[e] >= tau && b >= first && b <= end;
+                v[e] = on ? v[e] : __builtin_nanf("");
+                c += on;
             }
-            __syncthreads();
-        }
-        if (!few) {                               // equal or nearly equal logits, or no room for bins
-            sf_choose(s, a, r, SfBins(M, tau), row, all, SfInRow{x, V, tau, M, r.inv, s.roots});
-            continue;
-        }
-        uint32_t last = 0xffffffffu;              // kept: key < last, or key == last and index <= most
-        int most = 0x7fffffff;
-        if (cut) {
-            auto ends = [&](int i) { return bin(sf_logit(s.key[i])) == end; };
-            SfCut c;
-            const float wide = bin.scale > 0.0f ? 1.0f / bin.scale : 0.0f;
-            const SfBins sub(fminf(M, M - (float)end * wide + 1e-6f * fabsf(M)), fmaxf(tau, M - (float)(end + 1) * wide));
-            sf_select(s, sub, need - base, c, [&](auto f) {
-                for (int i = tid; i < n; i += SF_NT)
-                    if (ends(i)) f(s.key[i], [&] { return s.wi[i] >> 20; });
-            });
-            last = c.key;
-            const uint64_t m = (need - base - c.below + c.one - 1) / c.one;
-            if (m < c.equal) {                    // the m-th lowest index among the equal ones
-                int lo = 0, hi = V - 1;
-                while (lo < hi) {                 // uniform
-                    const int mid = (lo + hi) / 2;
-                    uint64_t q = 0;
-                    for (int i = tid; i < n; i += SF_NT) q += s.key[i] == last && (int)(s.wi[i] & 0xfffff) <= mid;
-                    if (sf_sum(q, s.wave) >= m) hi = mid;
-                    else lo = mid + 1;
+            int to = wave_scan(c);
+            const int all_lanes = __builtin_amdgcn_readlane(to, 63);
+            if (all_lanes == 0) return;           // uniform
+            int from = 0;
+            if (lane == 0) from = __hip_atomic_fetch_add(&s.count, all_lanes, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            to += __builtin_amdgcn_readlane(from, 0) - c;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (v[e] == v[e]) {
+                    if (to < SF_LIST) {
+                        s.key[to] = sf_key(v[e]);
+                        s.wi[to] = (uint64_t)index(e);
+                    }
+                    ++to;
                 }
-                most = lo;
+        });
+        __syncthreads();
+        n = s.count;
+        for (int i = tid; i < min(n, SF_LIST); i += SF_NT)
+            s.wi[i] |= sf_weight_units(sf_logit(s.key[i]), M, r.inv, s.roots) << 20;
+        __syncthreads();
+        few = n <= SF_LIST;
+    }
+    if (!few) {                               // equal or nearly equal logits
+        sf_choose(s, a, r, SfBins(M, tau), row, all, SfInRow{x, V, tau, M, r.inv, s.roots});
+        return;
+    }
+    uint32_t last = 0xffffffffu;              // kept: key < last, or key == last and index <= most
+    int most = 0x7fffffff;
+    if (cut) {
+        auto ends = [&](int i) { return bin(sf_logit(s.key[i])) == end; };
+        SfCut c;
+        const float wide = bin.scale > 0.0f ? 1.0f / bin.scale : 0.0f;
+        const SfBins sub(fminf(M, M - (float)end * wide + 1e-6f * fabsf(M)), fmaxf(tau, M - (float)(end + 1) * wide));
+        sf_select(s, sub, need - base, c, [&](auto f) {
+            for (int i = tid; i < n; i += SF_NT)
+                if (ends(i)) f(s.key[i], [&] { return s.wi[i] >> 20; });
+        });
+        last = c.key;
+        const uint64_t m = (need - base - c.below + c.one - 1) / c.one;
+        if (m < c.equal) {                    // the m-th lowest index among the equal ones
+            int lo = 0, hi = V - 1;
+            while (lo < hi) {                 // uniform
+                const int mid = (lo + hi) / 2;
+                uint64_t q = 0;
+                for (int i = tid; i < n; i += SF_NT) q += s.key[i] == last && (int)(s.wi[i] & 0xfffff) <= mid;
+                if (sf_sum(q, s.wave) >= m) hi = mid;
+                else lo = mid + 1;
             }
+            most = lo;
         }
-        // what is kept of each slice: its bins below `first`, and tokens of the list
-        auto keeps = [&](uint32_t k, int i, uint64_t u) { return (k < last || (k == last && i <= most)) && u >= low ? u : 0; };
-        __syncthreads();
-        if (tid < LGX_SF_VOCAB / LGX_SF_SLICE) s.few[tid] = 0;
-        __syncthreads();
-        for (int i = tid >> 6; i < a.nslices; i += SF_NT / 64) {
+    }
+    // what is kept of each slice: its bins below `first`, and tokens of the list
+    auto keeps = [&](uint32_t k, int i, uint64_t u) { return (k < last || (k == last && i <= most)) && u >= low ? u : 0; };
+    __syncthreads();
+    if (tid < LGX_SF_VOCAB / LGX_SF_SLICE) s.few[tid] = 0;
+    __syncthreads();
+    for (int i0 = tid >> 6; i0 < a.nslices; i0 += 3 * (SF_NT / 64)) {
+        uint64_t u[3][LGX_SF_BINS / 64];
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+#pragma unroll
+            for (int b = 0; b < LGX_SF_BINS / 64; ++b)
+                u[q][b] = sf_shared(hist + min(i0 + q * (SF_NT / 64), a.nslices - 1) * LGX_SF_BINS + 64 * b + lane);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+            const int i = i0 + q * (SF_NT / 64);
+            if (i >= a.nslices) break;        // uniform
             uint64_t m = 0;
-            for (int b = lane; b < first; b += 64) m += hist[i * LGX_SF_BINS + b];
+#pragma unroll
+            for (int b = 0; b < LGX_SF_BINS / 64; ++b) m += 64 * b + lane < first ? u[q][b] : 0;
             m = wave_sum64(m);
             if (lane == 0) __hip_atomic_fetch_add(&s.few[i], m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         }
-        for (int i = tid; i < n; i += SF_NT) {
-            const uint64_t wi = s.wi[i];
-            const int at = (int)(wi & 0xfffff);
-            __hip_atomic_fetch_add(&s.few[at / LGX_SF_SLICE], keeps(s.key[i], at, wi >> 20), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        }
-        auto kept = [&](float v, int i) { return v >= tau ? keeps(sf_key(v), i, sf_weight_units(v, M, r.inv, s.roots)) : 0; };
-        __syncthreads();
-        mine = tid < a.nslices ? s.few[tid] : 0;
-        const uint64_t to = sf_scan<uint64_t>(mine, s.wave, total), t = sf_draw(a.u[row], total);
-        if (to > t && to - mine <= t) {
-            s.found = tid;
-            s.below = to - mine;
-        }
-        __syncthreads();
-        const int sl = s.found;
-        const uint64_t in = t - s.below;
-        const int i0 = sl * LGX_SF_SLICE + 4 * tid;
-        uint64_t u[4], c = 0, sum;
+    }
+    for (int i = tid; i < n; i += SF_NT) {
+        const uint64_t wi = s.wi[i];
+        const int at = (int)(wi & 0xfffff);
+        __hip_atomic_fetch_add(&s.few[at / LGX_SF_SLICE], keeps(s.key[i], at, wi >> 20), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
+    auto kept = [&](float v, int i) { return v >= tau ? keeps(sf_key(v), i, sf_weight_units(v, M, r.inv, s.roots)) : 0; };
+    __syncthreads();
+    mine = tid < a.nslices ? s.few[tid] : 0;
+    const uint64_t to = sf_scan<uint64_t>(mine, s.wave, total), t = sf_draw(a.u[row], total);
+    if (to > t && to - mine <= t) {
+        s.found = tid;
+        s.below = to - mine;
+    }
+    __syncthreads();
+    const int sl = s.found;
+    const uint64_t in = t - s.below;
+    const int i0 = sl * LGX_SF_SLICE + 4 * tid;
+    uint64_t u[4], c = 0, sum;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            u[i] = i0 + i < V ? kept(x[min(i0 + i, V - 1)], i0 + i) : 0;
-            c += u[i];
-        }
-        uint64_t at = sf_scan<uint64_t>(c, s.wave, sum) - c;
-        bool done = at > in || at + c <= in;      // not this thread's
+    for (int i = 0; i < 4; ++i) {
+        u[i] = i0 + i < V ? kept(x[min(i0 + i, V - 1)], i0 + i) : 0;
+        c += u[i];
+    }
+    uint64_t at = sf_scan<uint64_t>(c, s.wave, sum) - c;
+    bool done = at > in || at + c <= in;      // not this thread's
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            at += u[i];
-            if (!done && at > in) {
-                done = true;
-                a.out[row] = i0 + i;
-                if (a.prob) a.prob[row] = (float)((double)u[i] / (double)total);
+    for (int i = 0; i < 4; ++i) {
+        at += u[i];
+        if (!done && at > in) {
+            done = true;
+            a.out[row] = i0 + i;
+            if (a.prob) a.prob[row] = (float)((double)u[i] / (double)total);
+        }
+    }
+}
+
+// The wide rows.  Each workgroup takes a run of their (row, slice)s: bins of the slice's
+// weights, stored; the one that brings a row's last bins goes on with the row.  None waits
+// for another.  Rows without room for bins come after, one per workgroup.
+extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_wide(const lgx_filter_args a) {
+    __shared__ SfLds s;
+    __shared__ int last;
+    const int tid = threadIdx.x, n_all = *a.wide_n, n = min(n_all, a.slots), items = n * a.nslices;
+    const int per = (int)((unsigned)(items + gridDim.x - 1) / gridDim.x), at1 = min((int)blockIdx.x * per + per, items);
+    if (n_all == 0) return;
+    sf_roots(s.roots);
+    for (int at = blockIdx.x * per; at < at1;) {  // uniform
+        const int w = at / a.nslices, sl0 = at - w * a.nslices, sl1 = min(a.nslices, sl0 + at1 - at);
+        const int row = a.wide_row[w];
+        const float tau = a.wide_tau[w], M = sf_row_max(a, row);
+        const SfRow r = sf_row(a, row);
+        const float* x = a.logits + (int64_t)row * a.ld;
+        const SfSliceBins bin(M, tau);
+        for (int sl = sl0; sl < sl1; ++sl) {
+            float v[LGX_SF_SLICE / SF_NT];
+#pragma unroll
+            for (int i = 0; i < LGX_SF_SLICE / SF_NT; ++i) {
+                const int e = sl * LGX_SF_SLICE + SF_NT * i + tid;
+                v[i] = e < a.vocab ? x[e] : __builtin_nanf("");
             }
+            __syncthreads();                      // what was in LDS is read
+            if (tid < LGX_SF_BINS) s.bins[tid] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < LGX_SF_SLICE / SF_NT; ++i)
+                if (v[i] >= tau)
+                    __hip_atomic_fetch_add(&s.bins[bin(v[i])], sf_weight_units(v[i], M, r.inv, s.roots), __ATOMIC_RELAXED,
+                                           __HIP_MEMORY_SCOPE_WORKGROUP);
+            __syncthreads();
+            if (tid < LGX_SF_BINS)
+                __hip_atomic_store(a.hist + ((int64_t)w * a.nslices + sl) * LGX_SF_BINS + tid, s.bins[tid], __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_AGENT);
         }
+        at += sl1 - sl0;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // each wave's bins have reached memory
+        __syncthreads();
+        if (tid == 0)
+            last = __hip_atomic_fetch_add(a.wide_done + w, sl1 - sl0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + sl1 - sl0 == a.nslices;
+        __syncthreads();
+        if (last) sf_choose_wide(s, a, r, bin, w, row, tau, M);   // uniform
+    }
+    for (int w = n + blockIdx.x; w < n_all; w += gridDim.x) {   // uniform
+        const int row = a.wide_row[w];
+        const float tau = a.wide_tau[w], M = sf_row_max(a, row);
+        const SfRow r = sf_row(a, row);
+        __syncthreads();
+        sf_choose(s, a, r, SfBins(M, tau), row, a.wide_all[w], SfInRow{a.logits + (int64_t)row * a.ld, a.vocab, tau, M, r.inv, s.roots});
     }
 }

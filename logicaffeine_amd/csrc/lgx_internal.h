@@ -191,8 +191,6 @@ enum Kern {
     K_KV_KEEP_D128,
     K_FILTER_SCAN,
     K_FILTER_PICK,
-    K_FILTER_BINS,
-    K_FILTER_LIST,
     K_FILTER_WIDE,
     K_TREE_ATTN_D64, // + 1: with caps, distances or a window
     K_TREE_ATTN_D128 = K_TREE_ATTN_D64 + 2,
@@ -255,8 +253,7 @@ inline const char* const kKernelNames[] = {
     "lgx_k_attn8_join_d64", "lgx_k_attn8_joinw_d64", "lgx_k_attn8_join_d128", "lgx_k_attn8_joinw_d128",
     "lgx_k_pages_fork", "lgx_k_pages_free", "lgx_k_pages_reserve", "lgx_k_pages_copy",
     "lgx_k_append_rows_d64", "lgx_k_append_rows_d128", "lgx_k_tree_plan", "lgx_k_tree_accept",
-    "lgx_k_kv_keep_d64", "lgx_k_kv_keep_d128", "lgx_k_filter_scan", "lgx_k_filter_pick", "lgx_k_filter_bins",
-    "lgx_k_filter_list", "lgx_k_filter_wide",
+    "lgx_k_kv_keep_d64", "lgx_k_kv_keep_d128", "lgx_k_filter_scan", "lgx_k_filter_pick", "lgx_k_filter_wide",
     "lgx_k_tree_attn_d64", "lgx_k_tree_attnx_d64", "lgx_k_tree_attn_d128", "lgx_k_tree_attnx_d128",
     "lgx_k_tree_join_d64", "lgx_k_tree_joinr_d64", "lgx_k_tree_join_d128", "lgx_k_tree_joinr_d128",
 };

@@ -612,13 +612,6 @@ typedef struct {
 #define LGX_SF_VOCAB (1 << 19)
 #define LGX_SF_BINS 256        // bins of a wide row's slice
 #define LGX_SF_LIST 4096       // tokens that a workgroup chooses among
-// Of a wide row: of bins first .. end not all tokens are known to be kept or not (listed).
-typedef struct {
-    uint64_t base;             // weight of the bins before `end`
-    int32_t first, end;
-    int32_t cut;               // top-p ends in `end`
-    int32_t count;             // tokens listed, those without room counted too
-} lgx_filter_cut;
 typedef struct {
     const float* logits;       // [m] rows of vocab, ld apart
     const float* temperature;  // [m], nullable: 1
@@ -631,15 +624,13 @@ typedef struct {
     double* sum;               // [m][nslices] of exp((l - slice maximum) / T)
     float* smax;               // [m][nslices]
     float* cmax;               // [m][nslices * 64]
-    // rows whose kept tokens are too many for one workgroup's list (lgx_k_filter_bins, _list, _wide)
+    // rows whose kept tokens are too many for one workgroup's list (lgx_k_filter_wide)
     int32_t* wide_n;           // [1] their number
     int32_t* wide_row;         // [m]
     float* wide_tau;           // [m]
     double* wide_all;          // [m]
     uint64_t* hist;            // [slots][nslices][LGX_SF_BINS]
-    lgx_filter_cut* wide_cut;  // [slots]
-    uint64_t* wide_wi;         // [slots][LGX_SF_LIST] weight << 20 | index
-    uint32_t* wide_key;        // [slots][LGX_SF_LIST]
+    int32_t* wide_done;        // [slots] slices whose bins are there
     int64_t ld;
     int32_t m, vocab, nslices;
     int32_t vec;               // rows are 16-byte aligned

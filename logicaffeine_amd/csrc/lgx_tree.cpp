@@ -247,30 +247,27 @@ lgx_status lgx_sample_filtered(lgx_ctx* c, const float* logits, int64_t ld, int3
         a.vocab = vocab;
         a.nslices = (vocab + LGX_SF_SLICE - 1) / LGX_SF_SLICE;
         a.vec = ld % 4 == 0 && aligned16(logits);
-        // room for the bins and lists of as many wide rows as 64 MiB hold; the others take longer
-        const size_t ns = (size_t)m * a.nslices, bins = (size_t)a.nslices * LGX_SF_BINS;
-        const size_t slot = 8 * bins + sizeof(lgx_filter_cut) + 12 * LGX_SF_LIST;
+        // room for the bins of as many wide rows as 64 MiB hold; the others take longer
+        const size_t ns = (size_t)m * a.nslices, slot = (size_t)a.nslices * LGX_SF_BINS;
         // (a row of no more tokens than a workgroup lists is never wide)
-        if ((top_p || min_p) && vocab > LGX_SF_LIST) a.slots = (int)std::min<size_t>(m, std::max<size_t>(((size_t)64 << 20) / slot, 1));
-        const size_t fours = ns * (1 + LGX_SF_SLICE / LGX_SF_CHUNK) + 2 * (size_t)m + 1;
+        if ((top_p || min_p) && vocab > LGX_SF_LIST)
+            a.slots = (int)std::min<size_t>(m, std::max<size_t>(((size_t)64 << 20) / 8 / slot, 1));
+        const size_t eights = ns + m + (size_t)a.slots * slot;
+        const size_t fours = ns * (1 + LGX_SF_SLICE / LGX_SF_CHUNK) + 2 * (size_t)m + 1 + a.slots;
         float* ws = nullptr;
-        if ((st = ensure_ws(c, 8 * (ns + m) + a.slots * slot + 4 * fours, stream, &ws)) != LGX_OK) return st;
+        if ((st = ensure_ws(c, 8 * eights + 4 * fours, stream, &ws)) != LGX_OK) return st;
         a.sum = (double*)ws;
         a.wide_all = a.sum + ns;
         a.hist = (uint64_t*)(a.wide_all + m);
-        a.wide_cut = (lgx_filter_cut*)(a.hist + (size_t)a.slots * bins);
-        a.wide_wi = (uint64_t*)(a.wide_cut + a.slots);
-        a.wide_key = (uint32_t*)(a.wide_wi + (size_t)a.slots * LGX_SF_LIST);
-        a.smax = (float*)(a.wide_key + (size_t)a.slots * LGX_SF_LIST);
+        a.smax = (float*)(a.hist + (size_t)a.slots * slot);
         a.cmax = a.smax + ns;
         a.wide_tau = a.cmax + ns * (LGX_SF_SLICE / LGX_SF_CHUNK);
         a.wide_row = (int32_t*)(a.wide_tau + m);
-        a.wide_n = a.wide_row + m;
+        a.wide_done = a.wide_row + m;
+        a.wide_n = a.wide_done + a.slots;
         if ((st = launch(c, K_FILTER_SCAN, dim3((unsigned)a.nslices, (unsigned)m), dim3(256), a, stream)) != LGX_OK) return st;
         if ((st = launch(c, K_FILTER_PICK, dim3((unsigned)m), dim3(1024), a, stream)) != LGX_OK || !a.slots) return st;
-        if ((st = launch(c, K_FILTER_BINS, dim3((unsigned)a.nslices, std::min(m, 64)), dim3(256), a, stream)) != LGX_OK) return st;
-        if ((st = launch(c, K_FILTER_LIST, dim3((unsigned)std::min<size_t>(ns, 1024)), dim3(256), a, stream)) != LGX_OK) return st;
-        return launch(c, K_FILTER_WIDE, dim3((unsigned)std::min(m, 2 * c->ncu)), dim3(1024), a, stream);
+        return launch(c, K_FILTER_WIDE, dim3((unsigned)std::min<size_t>(ns, 2 * (size_t)c->ncu)), dim3(1024), a, stream);
     });
 }
 

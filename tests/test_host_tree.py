@@ -211,16 +211,16 @@ def test_keep_and_copy_go_over_every_layer(host, layers, parts):
 @pytest.mark.parametrize("m,vocab,p,mp", [(1, 1, None, None), (1, 151936, P, None), (512, 152064, P, P), (3, 4097, None, P), (3, 4096, P, P),
                                           (65535, 64, P, None), (65535, 1 << 19, None, None), (7, 1 << 19, P, P)])
 def test_sampling_workspace(host, m, vocab, p, mp):
-    """Slices' sums and maxima, chunks' maxima, the list of wide rows and the bins and
-    lists of as many as 64 MiB hold, one at least."""
+    """Slices' sums and maxima, chunks' maxima, the list of wide rows and the bins of
+    as many as 64 MiB hold, one at least."""
     (st, launches, alloc), = host([sample(m, vocab, p=p, mp=mp, ld=vocab + 3)])
     assert st == "LGX_OK"
     ns = -(-vocab // 4096)
-    names = ["lgx_k_filter_scan", "lgx_k_filter_pick"] + ["lgx_k_filter_bins", "lgx_k_filter_list", "lgx_k_filter_wide"] * bool((p or mp) and vocab > 4096)
+    names = ["lgx_k_filter_scan", "lgx_k_filter_pick"] + ["lgx_k_filter_wide"] * bool((p or mp) and vocab > 4096)
     assert [x[0] for x in launches] == names and launches[0][1:3] == (ns, m) and launches[1][1] == m
-    slot = ns * 256 * 8 + 24 + 4096 * 12
+    slot = ns * 256 * 8
     slots = min(m, max((64 << 20) // slot, 1)) if (p or mp) and vocab > 4096 else 0
-    assert alloc >= m * ns * (8 + 4 + 64 * 4) + m * (8 + 4 + 4) + 4 + slots * slot
+    assert alloc >= m * ns * (8 + 4 + 64 * 4) + m * (8 + 4 + 4) + 4 + slots * (slot + 4)
 
 
 def test_reserve_lists_no_more_pages_than_there_are(host):
