@@ -13,19 +13,21 @@
 // logit tau below which no token can be kept, reads again only the runs of 64 whose largest
 // reaches it, and selects among those tokens, in LDS.  A row without filters needs the
 // sums and one run of 4096.  Rows of which top-p or min-p keep more tokens than that list
-// holds (wide) are left to three more launches: bins of the weights by 4096 logits, the
-// tokens of the bins that are neither kept nor cut whole, and the choice among those.
+// holds (wide) are left to one more launch: bins of the weights by 4096 logits, and by the
+// workgroup that brings a row's last bins the choice from them.
 //
-// What bounds it, at 151936 logits: many rows the scan, which reads at 4.1 to 4.9 TB/s
-// (512 rows of all kinds 60 us of 127; 256 rows without sums 38), and its weights where
-// top-p or no filter needs their sums (another 24 us of 256 rows: binary64 arithmetic).  One
-// row its chain of memory rounds and barriers: scan 3.7 us, pick 6 to 10 us, 1 us each for
-// the launches that find no wide row; 58 us for a row of which 100000 tokens are kept.
+// What bounds it, at 151936 logits: many rows the scan, which reads at 4.1 to 5.2 TB/s
+// (512 rows of all kinds 60 us of 138; 256 rows without sums 35), and its weights where
+// top-p or no filter needs their sums (another 25 us of 256 rows: binary64 arithmetic).  One
+// row its chain of memory rounds and barriers: scan 3.5 us, pick 4 to 10 us, 1 us for the
+// launch that finds no wide row; 71 us for a row of which 100000 tokens are kept.
 //   One pass over the row by its own workgroup in place of scan and pick: 152064 logits at
 //   one compute unit's rate are 20 us or more a pass, and small batches need all of them.
 //   Tokens read by the runs' maxima: a row with top-k 50 reads 60 to 100 runs of 2374.
-//   Wide rows by their own workgroup: 100 us against 58 for one row, 74 against 50 at
-//   temperature 1.4; but 207 against 237 for 256 of them, which fill the device by themselves.
+//   Wide rows in three launches (bins, the deciding tokens listed by all slices, choice): one
+//   58 against 71 us, 256 of them 237 against 245, 512 mixed rows 127 against 138; but 3 us
+//   more for every call without a wide row (top-k 50 and top-p 17.9 against 14.9), and 2 to
+//   3 us of the host's.
 //
 // Sums decide between tokens, so they are exact or nearly: the weights that a
 // selection adds up are whole multiples of 2^-42 in 64-bit integers, whose sums
