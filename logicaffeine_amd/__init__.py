@@ -481,6 +481,7 @@ class Context:
         self.device = device
         self.dev = torch.device("cuda", device)
         self.where = str(self.dev)
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         h = C.c_void_p()
         _check(lib().lgx_ctx_create(device, hsaco.encode() if hsaco else None, C.byref(h)))
         self.handle = h
@@ -510,7 +511,8 @@ class Context:
         return lib().lgx_ctx_arch(self.handle).decode()
 
     def _s(self):
-        return _stream(self.torch, self.dev)
+        raw = self._raw_stream
+        return raw(self.device) if raw else _stream(self.torch, self.dev)
 
     def kernel_timing(self, enable: bool) -> None:
         """Time every launch by its own dispatch (fresh window when enabled)."""
@@ -842,18 +844,21 @@ class Context:
         """(path [B][N], count [B], next token [B], seq_len + count or None): the nodes from
         node 0 on whose tokens were picked behind their parents."""
         t = self.torch
-        _tensor("tokens", tokens, t.int32, (None, None), self.dev)
-        B, N = tokens.shape
-        _tensor("parent", parent, t.int32, (B, N), self.dev)
-        _tensor("picked", picked, t.int32, (B, N), self.dev)
+        i32, dev = t.int32, self.dev
+        if tokens.dim() != 2:
+            raise ValueError(f"tokens {tuple(tokens.shape)} is not [sequences][nodes]")
+        B, N = shape = tokens.shape
+        _tensor("tokens", tokens, i32, shape, dev)
+        _tensor("parent", parent, i32, shape, dev)
+        _tensor("picked", picked, i32, shape, dev)
         for name, x in (("seq_len", seq_len), ("n_nodes", n_nodes), ("next_tokens", next_tokens)):
             if x is not None:
-                _tensor(name, x, t.int32, (B,), self.dev)
-        path = t.empty((B, N), dtype=t.int32, device=self.dev)
-        count = t.empty(B, dtype=t.int32, device=self.dev)
+                _tensor(name, x, i32, (B,), dev)
+        path = t.empty(shape, dtype=i32, device=dev)
+        count = t.empty(B, dtype=i32, device=dev)
         if next_tokens is None:
-            next_tokens = (t.empty if n_nodes is None else t.zeros)(B, dtype=t.int32, device=self.dev)
-        lens = t.empty(B, dtype=t.int32, device=self.dev) if seq_len is not None else None
+            next_tokens = (t.empty if n_nodes is None else t.zeros)(B, dtype=i32, device=dev)
+        lens = t.empty(B, dtype=i32, device=dev) if seq_len is not None else None
         _check(lib().lgx_tree_accept(self.handle, tokens.data_ptr(), parent.data_ptr(), picked.data_ptr(),
                                      _ptr_or_none(n_nodes), _ptr_or_none(seq_len), B, N, path.data_ptr(), count.data_ptr(),
                                      next_tokens.data_ptr(), _ptr_or_none(lens), self._s()))
@@ -866,8 +871,10 @@ class Context:
         caches = list(caches)
         if not caches:
             raise ValueError("no caches")
-        _tensor("keep", keep, t.int32, (page_table.shape[0], None), self.dev)
+        if keep.dim() != 2:
+            raise ValueError(f"keep {tuple(keep.shape)} is not [sequences][rows]")
         B, N = keep.shape
+        _tensor("keep", keep, t.int32, (page_table.shape[0], N), self.dev)
         # dozens of layers: strings compare in a fifth of the time of torch's devices
         if {kv.where for kv in caches} != {self.where}:
             raise ValueError(f"caches on {sorted({kv.where for kv in caches})}, the context on {self.dev}")
@@ -901,29 +908,31 @@ class Context:
 
     # ---- pages of a cache ------------------------------------------------
     def _pool(self, pool, page_table, **lengths):
-        if pool.device != self.dev:
-            raise ValueError(f"the pool is on {pool.device}, the context on {self.dev}")
-        i32 = self.torch.int32
-        _tensor("page_table", page_table, i32, (None, None), self.dev)
+        dev, i32 = self.dev, self.torch.int32
+        if pool.device != dev:
+            raise ValueError(f"the pool is on {pool.device}, the context on {dev}")
+        if page_table.dim() != 2:
+            raise ValueError(f"page_table {tuple(page_table.shape)} is not [sequences][pages]")
+        shape = page_table.shape
+        _tensor("page_table", page_table, i32, shape, dev)
         for name, x in lengths.items():
-            _tensor(name, x, i32, (page_table.shape[0],), self.dev)
+            _tensor(name, x, i32, shape[:1], dev)
+        return shape
 
     def pages_fork(self, pool: PagePool, page_table, seq_len, src, dst) -> None:
         """Sequence dst[i] becomes a copy of sequence src[i], sharing its pages."""
-        self._pool(pool, page_table, seq_len=seq_len)
-        S, maxp = page_table.shape
-        i32 = self.torch.int32
-        _tensor("src", src, i32, (None,), self.dev)
-        _tensor("dst", dst, i32, src.shape, self.dev)
+        S, maxp = self._pool(pool, page_table, seq_len=seq_len)
+        i32, n = self.torch.int32, src.numel()
+        _tensor("src", src, i32, (n,), self.dev)
+        _tensor("dst", dst, i32, (n,), self.dev)
         _check(lib().lgx_pages_fork(self.handle, pool.cstruct, page_table.data_ptr(), seq_len.data_ptr(), src.data_ptr(),
-                                    dst.data_ptr(), S, src.shape[0], maxp, self._s()))
+                                    dst.data_ptr(), S, n, maxp, self._s()))
 
     def pages_reserve(self, pool: PagePool, page_table, seq_len, need, out=None):
         """Room for need[b] tokens behind seq_len[b]: (copies [B][2], n_copies [1],
         lacking [1]); the copies are pages_copy's."""
-        self._pool(pool, page_table, seq_len=seq_len, need=need)
+        B, maxp = self._pool(pool, page_table, seq_len=seq_len, need=need)
         t = self.torch
-        B, maxp = page_table.shape
         shapes = ((B, 2), (1,), (1,))
         if out is None:
             out = tuple(t.zeros(s, dtype=t.int32, device=self.dev) for s in shapes)
@@ -937,16 +946,15 @@ class Context:
         """Copies page copies[i][0] to copies[i][1], i < n_copies[0], in every plane."""
         if planes.device != self.dev:
             raise ValueError(f"the planes are on {planes.device}, the context on {self.dev}")
-        i32 = self.torch.int32
-        _tensor("copies", copies, i32, (None, 2), self.dev)
+        i32, n = self.torch.int32, copies.numel() // 2
+        _tensor("copies", copies, i32, (n, 2), self.dev)
         _tensor("n_copies", n_copies, i32, (1,), self.dev)
         _check(lib().lgx_pages_copy(self.handle, planes.carray, planes.count, planes.num_pages, copies.data_ptr(),
-                                    n_copies.data_ptr(), copies.shape[0], self._s()))
+                                    n_copies.data_ptr(), n, self._s()))
 
     def pages_free(self, pool: PagePool, page_table, keep) -> None:
         """Gives back the pages past each sequence's first keep[b] tokens."""
-        self._pool(pool, page_table, keep=keep)
-        B, maxp = page_table.shape
+        B, maxp = self._pool(pool, page_table, keep=keep)
         _check(lib().lgx_pages_free(self.handle, pool.cstruct, page_table.data_ptr(), keep.data_ptr(), B, maxp, self._s()))
 
     def q8_gemm(self, W: Q8Matrix, xq, xd, y=None):
