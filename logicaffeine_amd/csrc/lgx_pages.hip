@@ -17,17 +17,13 @@
 // Exclusive sums over the workgroup's threads; total: of all.  sums: one per wave.
 template <int NT>
 __device__ __forceinline__ int block_scan(int v, int* sums, int& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int upto = wave_scan(v);
     if (lane == 63) sums[wave] = upto;
     __syncthreads();
-    int before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 64; ++w) {
-        before += w < wave ? sums[w] : 0;
-        total += sums[w];
-    }
+    const int w = wave_scan(lane < NT / 64 ? sums[lane] : 0);
+    total = __builtin_amdgcn_readlane(w, 63);
+    const int before = wave ? __builtin_amdgcn_readlane(w, wave - 1) : 0;
     __syncthreads();
     return before + upto - v;
 }
