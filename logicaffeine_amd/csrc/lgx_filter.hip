@@ -214,7 +214,6 @@ struct SfLds {
     double dwave[SF_NT / 64];
     double roots[SF_ROOTS];                       // 2^(j / 64)
     uint64_t below;
-    uint32_t at;
     int found, count;
 };
 static_assert(sizeof(SfLds) <= 81920, "two workgroups per compute unit");
@@ -885,9 +884,8 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
     const int most = r.k ? r.k : SF_GUESS;
     float high = tau;
     if (guess || (r.k && r.k <= nruns)) {
-        // a bin of the runs' maxima by which so many of them are reached, and its lowest
+        // a bin of the runs' maxima by which so many of them are reached
         s.bins[tid] = 0;
-        if (tid == 0) s.at = 0;
         __syncthreads();
         const SfBins bin(M, fmaxf(tau, -3e38f));
 #pragma unroll
@@ -901,16 +899,9 @@ extern "C" __global__ __launch_bounds__(SF_NT) void lgx_k_filter_pick(const lgx_
         if (total >= (uint64_t)most) {            // uniform
             if (upto >= (uint64_t)most && upto - mine < (uint64_t)most) s.found = tid;
             __syncthreads();
-            const int at = s.found;
-            uint32_t low = 0;
-#pragma unroll
-            for (int j = 0; j < CM; ++j)
-                if (cm[j] >= tau && bin(sf_key(cm[j])) <= at) low = max(low, sf_key(cm[j]));
-            low = wave_max_u32(low);
-            if (lane == 0) __hip_atomic_fetch_max(&s.at, low, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            __syncthreads();
-            const uint32_t key = s.at;
-            high = fmaxf(tau, sf_logit(key));
+            // no run of that bin or an earlier one is below the bin's end (with its roundings)
+            const float end = M - (float)(s.found + 1) / bin.scale * 1.000001f;
+            if (bin.scale > 0.0f) high = fmaxf(tau, end - fmaxf(fabsf(M), fabsf(end)) * 1e-6f);
         }
     }
     const double all = S * SF_ONE;
