@@ -7,7 +7,7 @@
 // entries and of free pages, not by the order of workgroups.
 //
 // All but the copy are a launch and a few dependent rounds: fork 2.4 to 4.1 us, free 1.8 to
-// 4.0, reserve 4.1 for 2 sequences and 7.2 for 96 of 1728 pages.  The reserve is one
+// 4.0, reserve 3.4 for 2 sequences and 6.9 for 96 of 1728 pages.  The reserve is one
 // workgroup because its order is the result: split over several it would have to pass the
 // counts of needs and of free pages on, each a launch of its own.  The copy is bound by
 // memory: 83 MB (45 pages in 56 planes, read and written) in 15.7 to 17.9 us, 4.6 to 5.3 TB/s.
