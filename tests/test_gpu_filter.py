@@ -218,3 +218,23 @@ def test_more_wide_rows_than_there_is_room_for(ctx):
         want, share = ref_.choose(row, float(u[i]), p=np.float32(0.9))
         assert int(out[i]) == want and abs(float(prob[i]) - share) <= 2.0 ** -24 * share + 1e-12
     assert (out[1:] >= out[:-1]).all()
+
+
+@pytest.mark.parametrize("m,V,scale", [(7, 151937, 0.1), (96, 152064, 0.1), (64, 4097, 0.01), (200, 60000, 1.0)])
+def test_wide_rows_give_the_same_again(ctx, m, V, scale):
+    """Which workgroup goes on with a wide row depends on their order, its token does not:
+    again and again, with another call's values in the workspace between, and alone."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x, other = (scale * torch.randn(m, V, device="cuda", generator=g) for _ in range(2))
+    u, p, mp = (torch.rand(m, device="cuda", generator=g) for _ in range(3))
+    p, mp = 0.5 + 0.5 * p, 0.2 * mp
+    first = [y.clone() for y in ctx.sample_filtered(x, u, top_p=p, min_p=mp)]
+    for i in range(30):
+        if i % 2:
+            ctx.sample_filtered(other, u, top_p=p, min_p=mp)
+        for a, b in zip(first, ctx.sample_filtered(x, u, top_p=p, min_p=mp)):
+            assert torch.equal(a, b)
+    for i in range(0, m, 7):
+        one = slice(i, i + 1)
+        for a, b in zip(first, ctx.sample_filtered(x[one], u[one], top_p=p[one], min_p=mp[one])):
+            assert torch.equal(a[one], b)
