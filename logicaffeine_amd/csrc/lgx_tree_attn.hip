@@ -359,7 +359,7 @@ __device__ __forceinline__ void tree_weights(const Tree& w, float (&S)[16], Tree
 }
 
 // Column c over its run of tiles, token by token, by one wave: only seen tokens are
-// multiplied.  m, l: the column's reference and sum.
+// multiplied.  m, l: the column's reference and sum (> 0).
 template <int D, bool X>
 __device__ void tree_column(const Tree& w, int c, float m, float l, float* dst) {
     constexpr float kLog2e = 1.44269504088896341f;
@@ -406,12 +406,15 @@ __device__ __forceinline__ void tree_store(const Tree& w, int c, const TreeCol& 
     const bool part = w.ns > 1, on = c < w.ncols;
     const int64_t at = part ? ((int64_t)w.pos * a.hkv + w.g) * LGX_TREE_COLS + c - w.c0 : w.orow(on ? c : 0);
     float* dst = (part ? a.part : a.out) + at * D;
-    const float r = k.l == 0.0f ? 0.0f : 1.0f / k.l, l = k.l * (1.0f / (1 << TREE_UP));   // nothing seen gives zeros
+    const float r = 1.0f / k.l, l = k.l * (1.0f / (1 << TREE_UP));
+    // Nothing seen (here: another split may see some) gives zeros by selection, not by a factor:
+    // o is NaN where an unseen token's V is not finite, and so would be the joined result.
+    const bool none = k.l == 0.0f;
     bool bad = false;
     if (on) {
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
-            const v4f x = o[i] * r;
+            const v4f x = none ? (v4f){0.0f, 0.0f, 0.0f, 0.0f} : o[i] * r;
             *(float4*)(dst + 16 * i + 4 * kg) = make_float4(x[0], x[1], x[2], x[3]);
             bad = bad || !(fabsf(x[0]) + fabsf(x[1]) + fabsf(x[2]) + fabsf(x[3]) < __builtin_inff());
         }

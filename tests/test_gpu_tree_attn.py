@@ -222,6 +222,89 @@ def test_infinities_and_nan_where_a_row_does_not_see(ctx, d, window):
         assert np.isposinf(got[b][only_v][..., ::3]).all() and np.isfinite(got[b][only_v][..., 1::3]).all()
 
 
+def spoil(s, b, tokens, step=1):
+    """Infinities and NaN in the keys and values of a sequence's tokens; the cache on the device anew."""
+    for i, t in enumerate(tokens):
+        at = s["table"][b, t // 16], slice(None), t % 16, slice(None, None, step)
+        s["k"][at] = (np.nan, np.inf, -np.inf)[i % 3]
+        s["v"][at] = (np.inf, np.nan, -np.inf)[i % 3]
+    s["kv"] = lgx.KvCacheF16(*(torch.as_tensor(s[x]).to(s["kv"].device) for x in "kv"))
+
+
+def check_unseen(s, got, sees, depth, bad, **more):
+    """Rows that see no bad token equal the definition's over finite ones (those that see nothing
+    at all are zeros); bad: tokens by sequence."""
+    B, N, hq, d = got.shape
+    finite = [np.nan_to_num(s[x], nan=0, posinf=0, neginf=0) for x in "kv"]
+    for b in range(B):
+        n, sl = min(max(s["n"][b], 0), N), int(s["lens"][b])
+        pos = np.concatenate([np.arange(sl), sl + depth[b][:n]])
+        on = np.concatenate([np.ones((n, sl), bool), sees[b][:n, :n]], 1)
+        if more.get("window"):
+            on &= sl + depth[b][:n, None] - pos < more["window"]
+        clean = ~on[:, [t for t in bad[b] if t < sl + n]].any(1)
+        assert clean.any(), b
+        want, tol = reference(s["q"].reshape(B, N, hq, d)[b, :n], *finite, s["table"][b], sl, n, sees[b], depth[b], **more)
+        off = np.abs(got[b, :n] - want)
+        assert np.isfinite(got[b, :n][clean]).all(), (b, np.flatnonzero(clean & ~np.isfinite(got[b, :n]).all((1, 2))))
+        assert (off <= tol[..., None])[clean].all(), b
+        assert not got[b, :n][~on.any(1)].any()
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (8, 2, 128), (6, 6, 128)])
+@pytest.mark.parametrize("N,lens", [(24, [250]), (100, [448]), (24, [250, 1000, 63]), (100, [448, 30, 2000]), (256, [700])])
+@pytest.mark.parametrize("window", [0, 60])
+def test_bad_drafts_behind_a_split(ctx, hq, hkv, d, N, lens, window):
+    """A context of more than four tiles is split: of the last run, with later nodes alone, the
+    first nodes see nothing, whatever stands there."""
+    rng = np.random.default_rng(N + len(lens))
+    s = make(ctx, rng, len(lens), N, hq, hkv, d, lens, span=5)
+    s["parent"][:, 3] = 0                         # node 2 is no one's parent
+    for j in range(4, N):
+        s["parent"][:, j] = np.where(s["parent"][:, j] == 2, 1, s["parent"][:, j])
+    bad = [[int(L) + i for i in (2, N - 3, N - 2, N - 1)] for L in lens]
+    for b in range(len(lens)):
+        spoil(s, b, bad[b], step=3)
+    o, more = (lgx.AttnOpts(window=window), dict(window=window)) if window else (None, {})
+    tree = [ref_.ancestors(p) for p in s["parent"]]
+    check_unseen(s, run(ctx, s, o), [t[0] for t in tree], [t[1] for t in tree], bad, **more)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens", [[0, 0, 0], [0, 900, 1], [300, 0, 64]])
+def test_rows_that_see_nothing_over_bad_slots(ctx, d, lens):
+    """Empty masks, nothing cached, every slot of the nodes an infinity or a NaN: zeros; and
+    rows that see a few finite nodes only."""
+    rng = np.random.default_rng(d + sum(lens))
+    B, N = 3, 70
+    s = make(ctx, rng, B, N, 10, 2, d, lens, n=[N, N - 1, N - 5])
+    sees = np.zeros((B, N, N), bool)
+    finite = np.arange(N) % 9 == 4
+    sees[:, 1::2] = finite
+    bad = [[int(lens[b]) + i for i in range(N) if not finite[i]] for b in range(B)]
+    for b in range(B):
+        spoil(s, b, bad[b])
+    got = run(ctx, s, plan=False, mask=ctx.to_device(ref_.words(sees)))
+    check_unseen(s, got, sees, [np.arange(N)] * B, bad)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window", [400, 900])
+def test_bad_tokens_ahead_of_the_windows_of_deep_nodes(ctx, d, window):
+    """The first runs of tiles lie in the windows of the shallow nodes alone."""
+    rng = np.random.default_rng(window)
+    N, L = 20, 1500
+    s = make(ctx, rng, 1, N, 4, 2, d, [L])
+    depth = np.where(np.arange(N) < 5, 0, 350 + 3 * np.arange(N))
+    sees = np.tril(np.ones((1, N, N), bool))
+    bad = [list(range(L - window + 1, L - window + 300, 7))]
+    spoil(s, 0, bad[0])
+    out = torch.full((N, 4, d), 7.0, device=ctx.dev)
+    ctx.gqa_tree_attn(ctx.to_device(s["q"]), s["kv"], ctx.to_device(s["table"]), ctx.to_device(s["lens"]), N, L,
+                      depth=ctx.to_device(depth[None].astype(I32)), opts=lgx.AttnOpts(window=window), out=out)
+    check_unseen(s, out.cpu().numpy().reshape(1, N, 4, d), sees, [depth], bad, window=window)
+
+
 def test_bad_queries_and_far_scales(ctx):
     """NaN or infinite query rows give NaN and nothing else does; rows of 2^-60 and 2^40 keep
     their bits; scores of thousands."""
