@@ -384,7 +384,7 @@ lgx_status lgx_rope_kv_append_rows(lgx_ctx* ctx, const float* qkv, const float* 
  * (clamped to [0, max_seq_len], max_seq_len + N <= 16 maxp) and those nodes i < n_nodes[b] whose
  * bit is set in mask[b][j] (lgx_tree_plan's words, or any others; NULL: nodes 0 .. j), cache
  * slots seq_len[b] + i.  opts as above, by positions: node j stands at seq_len[b] +
- * depth[b][j] (NULL: j; below 0: 0).  q and out [B*N][hq][d], 16-byte aligned, apart from
+ * depth[b][j] (NULL: j; below 0: 0), or at 2^31 - 1 if that is more.  q and out [B*N][hq][d], 16-byte aligned, apart from
  * each other; hq/hkv in 1..16; page ids are clamped to [0, num_pages).  A node that sees nothing gives zeros.  With
  * N = 1 and neither mask nor depth a decode step whose token is already cached.
  * Not the canonical schedule: products of binary16 keys and values with queries and

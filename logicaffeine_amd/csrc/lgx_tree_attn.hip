@@ -178,7 +178,10 @@ struct Tree {
     }
     __device__ __forceinline__ int64_t row(int c) const { return (int64_t)b * a.N + c / G; }
     __device__ __forceinline__ int64_t orow(int c) const { return row(c) * a.hq + g * G + c % G; }
-    __device__ __forceinline__ int depth(int i) const { return a.depth ? max(a.depth[(int64_t)b * a.N + i], 0) : i; }
+    // positions end at 2^31 - 1, so that their distances have 31 bits
+    __device__ __forceinline__ int depth(int i) const {
+        return a.depth ? min(max(a.depth[(int64_t)b * a.N + i], 0), 0x7fffffff - sl) : i;
+    }
     // bit i: node j sees token t0 + i (but for a window among the nodes: in_window)
     __device__ __forceinline__ uint64_t sees(int t0, int j, int dj) const {
         const int base = t0 - sl;                 // node of bit 0

@@ -305,6 +305,28 @@ def test_bad_tokens_ahead_of_the_windows_of_deep_nodes(ctx, d, window):
     check_unseen(s, out.cpu().numpy().reshape(1, N, 4, d), sees, [depth], bad, window=window)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window", [0, 50, 2**31 - 1])
+def test_depths_up_to_the_last_position(ctx, d, window):
+    """Positions end at 2^31 - 1: nodes that would stand behind it stand there, with the
+    distances and the window of that position."""
+    rng = np.random.default_rng(d)
+    B, N, hq, lens = 3, 9, 4, [400, 70, 0]
+    s = make(ctx, rng, B, N, hq, 2, d, lens)
+    most = 2**31 - 1
+    depth = np.array([0, 1, most, 2**30, most - 399, most - 400, most - 10, 2**31 - 70, -5])
+    slopes = (2.0 ** -np.arange(29, 29 + hq)).astype(np.float32)
+    sees = np.tril(np.ones((N, N), bool))
+    out = torch.full((B * N, hq, d), 7.0, device=ctx.dev)
+    ctx.gqa_tree_attn(ctx.to_device(s["q"]), s["kv"], ctx.to_device(s["table"]), ctx.to_device(s["lens"]), N, 400,
+                      depth=ctx.to_device(np.tile(depth.astype(I32), (B, 1))),
+                      opts=lgx.AttnOpts(window=window, slopes=ctx.to_device(slopes)), out=out)
+    # each sequence by itself: the last position is as far behind its length as that leaves
+    got = out.cpu().numpy().reshape(B, N, hq, d)
+    for b in range(B):
+        check(s, got, sees=[sees] * B, depth=np.clip(depth, 0, most - lens[b]), only=[b], window=window, slopes=slopes)
+
+
 def test_bad_queries_and_far_scales(ctx):
     """NaN or infinite query rows give NaN and nothing else does; rows of 2^-60 and 2^40 keep
     their bits; scores of thousands."""
