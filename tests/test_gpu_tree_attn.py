@@ -347,6 +347,20 @@ def test_bad_queries_and_far_scales(ctx):
         assert (off <= tol[..., None]).all()
 
 
+def test_queries_far_above_one(ctx):
+    """Rows of 2^40 and 2^100 beside ordinary ones, and rows of 2^-60, with scales that leave
+    moderate scores."""
+    rng = np.random.default_rng(15)
+    for d in (64, 128):
+        for up in (40, 100, -60):
+            s = make(ctx, rng, 2, 5, 4, 2, d, [70, 300])
+            s["q"].reshape(2, 5, -1)[:, ::2 if up > 0 else 1] *= 2.0 ** up
+            scale = 2.0 ** (-3 - up)
+            for more in (dict(), dict(cap=10.0), dict(window=33)):
+                o = lgx.AttnOpts(scale=scale, softcap=more.get("cap", 0.0), window=more.get("window", 0))
+                check(s, run(ctx, s, o), scale=scale, **more)
+
+
 def test_constant_values_and_one_token(ctx):
     """Weights sum to one: constant V comes out as it is, one seen token as its V row."""
     rng = np.random.default_rng(10)
