@@ -428,10 +428,13 @@ lgx_status lgx_kv_keep(lgx_ctx* ctx, const lgx_kv_f16* kv, int32_t layers, const
  *            their whole weight
  * A temperature of 0 (or less, or NaN) takes the first in order.  out[i] = the token,
  * prob[i] (nullable) = its share of the kept weight.  A row without any token gives 0 and
- * 0.  u below 0 or NaN counts as 0, from 1 on as the last.  Weights are summed in units of
- * 2^-42 or in binary64, so that equal inputs give equal tokens in any batch, and a choice
- * differs from the definition's only where two sums are within about 1e-12 of each
- * other.  vocab <= 2^19, m <= 65535.  Intermediates live in the ctx workspace. */
+ * 0.  u below 0 or NaN counts as 0, from 1 on as the last.  Equal inputs give equal tokens in
+ * any batch.  A row with filters rounds each weight to a multiple of 2^-42 (below
+ * 2^-43 to nothing): a sum over n tokens is off by up to n 2^-43 and by 2^-41 of itself,
+ * which for 2^19 tokens of a long tail is 6e-8, the step of binary32 numbers u; one without
+ * filters by the latter alone.  A choice differs from the definition's only where two
+ * numbers that it compares are that near to each other.  vocab <= 2^19, m <= 65535.
+ * Intermediates live in the ctx workspace. */
 lgx_status lgx_sample_filtered(lgx_ctx* ctx, const float* logits, int64_t ld, int32_t m, int32_t vocab,
                                const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                                const float* u, int32_t* out, float* prob, void* stream);

@@ -29,9 +29,13 @@
 //   more for every call without a wide row (top-k 50 and top-p 17.9 against 14.9), and 2 to
 //   3 us of the host's.
 //
-// Sums decide between tokens, so they are exact or nearly: the weights that a
-// selection adds up are whole multiples of 2^-42 in 64-bit integers, whose sums
-// do not depend on any order; the scan's are binary64.  exp is computed in binary64.
+// Sums decide between tokens, so they must not depend on their order: the weights that a
+// selection adds up are whole multiples of 2^-42 in 64-bit integers, each rounded by 2^-43
+// at most (the smaller ones to nothing); the scan's are binary64.  exp is binary64
+// arithmetic with a relative error of 1.5e-13 (sf_root_exp).  A sum over n tokens is
+// so off by n 2^-43 at most and by 2^-41 of itself: 6e-8 for half a million tokens of
+// 2^-43 each behind one of 1, some 1e-12 for a few.  A finer unit that holds 1e-12 over 2^19
+// tokens would take sums of 80 bits.
 // ---------------------------------------------------------------------------
 #define SF_ONE 0x1p42                             // 2^19 weights stay below 2^62
 #define SF_LIST LGX_SF_LIST                       // tokens kept in LDS

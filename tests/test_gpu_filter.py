@@ -83,6 +83,41 @@ def test_ties_at_the_border(ctx):
         check(ctx, x, rng.random(24, dtype=np.float32), mp=0.2, p=0.99)
 
 
+def test_tails_of_weights_near_the_unit(ctx):
+    """Half a million tokens that weigh about as much as a weight is rounded to, 2^-43 (those
+    below it weigh nothing).  A sum over n of them is off by e = n 2^-43 at most, and by 2^-41 of
+    it for exp and for binary64.  So a token is right if the definition's draw falls within 2 e
+    of its interval; with top-p, whose cut may be 2 e off as well, which moves both ends and
+    the draw by up to 4 e, within 6 e."""
+    V = 1 << 19
+    rng = np.random.default_rng(19)
+    u = np.array([0.0, 2.0 ** -30, 2.0 ** -25, 2.0 ** -24, 1.5 * 2.0 ** -24, 2.0 ** -23, 2.0 ** -22, 0.5], np.float32)
+    m = len(u)
+    for tail in (np.full(V, np.log(1.49 * 2.0 ** -42)), np.full(V, np.log(0.49 * 2.0 ** -42)),
+                 rng.uniform(np.log(2.0 ** -45), np.log(2.0 ** -40), V)):
+        row = tail.astype(np.float32)
+        row[V - 1] = 0.0
+        x = torch.as_tensor(row).to(ctx.dev).expand(m, V).contiguous()
+        w = np.exp(row.astype(np.longdouble))
+        for k, p in ((V - 1, 1.0), (300000, 1.0), (0, 1 - 2.0 ** -24), (0, 1 - 2.0 ** -23), (V - 1, 1 - 2.0 ** -24)):
+            f = lambda v, t: torch.full((m,), v, dtype=t, device=ctx.dev)  # noqa: E731
+            out, prob = (y.cpu().numpy() for y in ctx.sample_filtered(x, torch.as_tensor(u).to(ctx.dev), top_k=f(k, torch.int32),
+                                                                      top_p=f(p, torch.float32)))
+            order = np.argsort(-row, kind="stable")[:k or V]
+            up = np.cumsum(w[order])
+            e = len(order) * 2.0 ** -43 + up[-1] * 2.0 ** -41
+            room = 2 * e if p >= 1 else 6 * e
+            cut = len(order) if p >= 1 else int((up - w[order] < np.longdouble(np.float32(p)) * up[-1] + 2 * e).sum())
+            kept = np.sort(order[:cut])
+            c = np.cumsum(w[kept])
+            for i in range(m):
+                at = int(np.searchsorted(kept, out[i]))
+                assert at < cut and kept[at] == out[i], (k, p, u[i], out[i])
+                t = np.longdouble(u[i]) * c[-1]
+                assert c[at] - w[out[i]] - room <= t <= c[at] + room, (k, p, u[i], out[i])
+                assert abs(prob[i] - w[out[i]] / c[-1]) <= 2.0 ** -24 * prob[i] + room + 2.0 ** -43
+
+
 def test_infinities_nan_and_masked_rows(ctx):
     inf, nan = np.inf, np.nan
     rng = np.random.default_rng(1)
