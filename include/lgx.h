@@ -466,8 +466,11 @@ lgx_status lgx_pages_fork(lgx_ctx* ctx, const lgx_page_pool* pool, int32_t* page
  * entries name too, the sequence leaves that page to them for a new one and (old, new) is
  * added to copies [B][2]; n_copies[0] of them are written.  New pages are the
  * lowest free ones in the order of (sequence, entry).  If there are too few, nothing
- * changes, n_copies[0] is 0 and lacking[0], else 0, says how many more it would take.  The
- * copies have to be made (lgx_pages_copy) before the old pages change hands again.
+ * changes, n_copies[0] is 0 and lacking[0], else 0, says how many more it would take.
+ * Nothing may then be appended: the sequences' pages may be others' too.  (Work enqueued
+ * behind it without looking takes need[b] * (lacking[0] == 0) as its numbers of rows: the
+ * calls above leave a sequence of 0 rows alone.)  The copies have to be made
+ * (lgx_pages_copy) before the old pages change hands again.
  * B (maxp + 1) < 2^31. */
 lgx_status lgx_pages_reserve(lgx_ctx* ctx, const lgx_page_pool* pool, int32_t* page_table, const int32_t* seq_len,
                              const int32_t* need, int32_t B, int32_t maxp, int32_t* copies, int32_t* n_copies,

@@ -930,7 +930,8 @@ class Context:
 
     def pages_reserve(self, pool: PagePool, page_table, seq_len, need, out=None):
         """Room for need[b] tokens behind seq_len[b]: (copies [B][2], n_copies [1],
-        lacking [1]); the copies are pages_copy's."""
+        lacking [1]); the copies are pages_copy's.  If lacking[0] is not 0 no sequence
+        got room, and none may be appended to."""
         B, maxp = self._pool(pool, page_table, seq_len=seq_len, need=need)
         t = self.torch
         shapes = ((B, 2), (1,), (1,))

@@ -1,6 +1,9 @@
 """Drafts, sampling and a cache's pages together, as a server uses them: sequences of a
 small network go on by trees of drafts, share pages where one forks from another, and
 yield the tokens that they would yield one at a time."""
+import os
+import re
+
 import numpy as np
 import pytest
 import torch
@@ -278,3 +281,63 @@ def test_two_graphs_share_a_workspace_that_grows(ctx):
     del graphs, g, result
     torch.cuda.synchronize()
     own.close()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_the_documented_round_where_pages_run_out(ctx, captured):
+    """INTEGRATION.md's round as it stands there: three sequences share a partly filled page, and
+    the pool lacks a page for their drafts.  The round changes nothing, however often it
+    runs; once a page is free it goes on, each sequence in a page of its own."""
+    with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")) as f:
+        block = re.search(r"```python\n(layers = \[lgx\.KvCacheF16.*?)```", f.read(), re.S).group(1)
+    setup, body = block[:block.index("# tokens, parent")], compile(block[block.index("# tokens, parent"):], "round", "exec")
+    S, N, pages, held, hq, hkv, d, vocab = 3, 5, 4, 21, 28, 4, 128, 64
+    rng = np.random.default_rng(21)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    qkv = torch.tensor(rng.standard_normal((S * N, (hq + 2 * hkv) * d)), dtype=torch.float32, device="cuda")
+    names = dict(
+        lgx=lgx, torch=torch, ctx=ctx, num_pages=pages, S=S, N=N, weights=range(28), qkv=qkv, bias=None, max_len=4 * PAGE - N,
+        rope=lgx.Rope.tables(ctx, 4 * PAGE, d), table=torch.full((S, 4), -1, **i32), seq_len=torch.zeros(S, **i32),
+        tokens=torch.zeros((S, N), **i32), parent=torch.arange(-1, N - 1, **i32).repeat(S, 1), n=torch.full((S,), N, **i32),
+        logits=torch.tensor(rng.standard_normal((S * N, vocab)), dtype=torch.float32, device="cuda"),
+        u=torch.full((S * N,), 0.5, device="cuda"), temperature=None, top_k=None, top_p=None, min_p=None,
+        src=torch.zeros(1, **i32), dst=torch.zeros(1, **i32))
+    exec(setup, names)
+    table, lens, ref = names["table"], names["seq_len"], names["pool"].ref
+    ref.copy_(torch.tensor([S, 0, S, 1]))         # page 3 is held elsewhere
+    table[:, :2] = torch.tensor([2, 0])
+    lens.fill_(held)
+    for x in names["planes"].tensors:
+        x.copy_(torch.tensor(rng.standard_normal(x.shape), dtype=x.dtype))
+
+    def state():
+        return [x.clone() for x in (table, lens, ref, *names["planes"].tensors)]
+
+    before = state()
+    if captured:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            exec(body, names)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            exec(body, names)
+    go = graph.replay if captured else lambda: exec(body, names)
+    for _ in range(3):
+        go()
+        assert int(names["lacking"]) == 1 and int(names["count"].abs().sum()) == 0
+        for x, y in zip(before, state()):
+            assert torch.equal(x, y)
+    ref[3] = 0
+    go()
+    assert int(names["lacking"]) == 0
+    rows = table[:, 1].cpu().numpy()
+    assert sorted(rows) == [0, 1, 3] and (table[:, 0] == 2).all() and ref.tolist() == [1, 1, S, 1]
+    count = names["count"]
+    assert (count >= 1).all() and torch.equal(lens, held + count)
+    v = qkv.view(S, N, hq + 2 * hkv, d)[:, 0, hq + hkv:].half()
+    for kv, old in zip(names["layers"], before[3:][1::2]):
+        for s in range(S):
+            at = held % PAGE                      # what the page held, then node 0's row
+            assert torch.equal(kv.v[rows[s], :, :at], old[0, :, :at]) and torch.equal(kv.v[rows[s], :, at], v[s])
