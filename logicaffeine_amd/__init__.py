@@ -796,7 +796,8 @@ class Context:
                             n_new=None, q_out=None):
         """Rotates and appends rows [B*N][(hq + 2 hkv) d] (row b*N + j: slot seq_len[b] + j,
         position seq_len[b] + depth[b][j], or + j) to the binary16 cache; returns the rotated
-        queries [B*N][hq][d]."""
+        queries [B*N][hq][d].  Rows of padding (n_new) are q_out's own; without q_out they
+        hold anything."""
         t = self.torch
         B, maxp = page_table.shape
         d, hkv = kv.d, kv.hkv
@@ -823,7 +824,8 @@ class Context:
                       n_nodes=None, opts: AttnOpts = None, out=None):
         """q [B*N][hq][d]: row b*N + j is node j of sequence b, whose keys and values are
         in slot seq_len[b] + j of the binary16 cache; it sees the first seq_len[b] tokens
-        and the nodes of mask [B][N][ceil(N / 64)] (int64 words; None: nodes 0 .. j)."""
+        and the nodes of mask [B][N][ceil(N / 64)] (int64 words; None: nodes 0 .. j).  Rows of
+        padding (n_nodes) are out's own; without out they hold anything."""
         t = self.torch
         (B, maxp), (rows, hq, d) = page_table.shape, q.shape
         if rows != B * N or d != kv.d:

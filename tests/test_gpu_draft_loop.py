@@ -287,7 +287,8 @@ def test_two_graphs_share_a_workspace_that_grows(ctx):
 def test_the_documented_round_where_pages_run_out(ctx, captured):
     """INTEGRATION.md's round as it stands there: three sequences share a partly filled page, and
     the pool lacks a page for their drafts.  The round changes nothing, however often it
-    runs; once a page is free it goes on, each sequence in a page of its own."""
+    runs; once a page is free it goes on, each sequence in a page of its own.  Rows of
+    padding stay zeros."""
     with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")) as f:
         block = re.search(r"```python\n(layers = \[lgx\.KvCacheF16.*?)```", f.read(), re.S).group(1)
     setup, body = block[:block.index("# tokens, parent")], compile(block[block.index("# tokens, parent"):], "round", "exec")
@@ -298,7 +299,7 @@ def test_the_documented_round_where_pages_run_out(ctx, captured):
     names = dict(
         lgx=lgx, torch=torch, ctx=ctx, num_pages=pages, S=S, N=N, weights=range(28), qkv=qkv, bias=None, max_len=4 * PAGE - N,
         rope=lgx.Rope.tables(ctx, 4 * PAGE, d), table=torch.full((S, 4), -1, **i32), seq_len=torch.zeros(S, **i32),
-        tokens=torch.zeros((S, N), **i32), parent=torch.arange(-1, N - 1, **i32).repeat(S, 1), n=torch.full((S,), N, **i32),
+        tokens=torch.zeros((S, N), **i32), parent=torch.arange(-1, N - 1, **i32).repeat(S, 1), n=torch.tensor([N, N - 2, N], **i32),
         logits=torch.tensor(rng.standard_normal((S * N, vocab)), dtype=torch.float32, device="cuda"),
         u=torch.full((S * N,), 0.5, device="cuda"), temperature=None, top_k=None, top_p=None, min_p=None,
         src=torch.zeros(1, **i32), dst=torch.zeros(1, **i32))
@@ -327,6 +328,7 @@ def test_the_documented_round_where_pages_run_out(ctx, captured):
     for _ in range(3):
         go()
         assert int(names["lacking"]) == 1 and int(names["count"].abs().sum()) == 0
+        assert not names["q"].any() and not names["out"].any()
         for x, y in zip(before, state()):
             assert torch.equal(x, y)
     ref[3] = 0
@@ -341,3 +343,6 @@ def test_the_documented_round_where_pages_run_out(ctx, captured):
         for s in range(S):
             at = held % PAGE                      # what the page held, then node 0's row
             assert torch.equal(kv.v[rows[s], :, :at], old[0, :, :at]) and torch.equal(kv.v[rows[s], :, at], v[s])
+    for x in (names["q"], names["out"]):
+        used = x.view(S, N, -1).any(-1).tolist()
+        assert used == [[True] * N, [True] * (N - 2) + [False] * 2, [True] * N]
