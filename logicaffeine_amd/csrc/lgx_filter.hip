@@ -216,7 +216,7 @@ struct SfLds {
     uint32_t few_key[SF_FEW];
     uint64_t wave[SF_NT / 64];
     double dwave[SF_NT / 64];
-    double roots[SF_ROOTS];                       // 2^(j / 64)
+    double roots[SF_ROOTS];                       // 2^(j / 256)
     uint64_t below;
     int found, count;
 };

@@ -514,7 +514,7 @@ typedef struct {
     int32_t* copies;           // [B][2]
     int32_t* n_copies;         // [1]
     int32_t* lacking;          // [1]
-    int32_t* found;            // [min(num_pages, B * maxp)] free pages in order
+    int32_t* found;            // [min(num_pages, B * (maxp + 1))] free pages in order: entries and one copy per row
     int32_t num_pages, B, maxp;
 } lgx_reserve_args;
 
