@@ -59,14 +59,11 @@ def _compile_kernels(source: str) -> str:
     return stem + ".o"
 
 
-def build_kernels(only=None) -> str:
-    """The code object of all kernel files, compiled side by side.  only: compile
-    these again and link them with the others' objects of an earlier build."""
+def build_kernels() -> str:
+    """The code object of all kernel files, compiled side by side."""
     os.makedirs(BUILD_DIR, exist_ok=True)
-    todo = [s for s in KERNEL_SOURCES if only is None or s in only]
-    with concurrent.futures.ThreadPoolExecutor(len(todo)) as pool:
-        list(pool.map(_compile_kernels, todo))
-    objects = [os.path.join(BUILD_DIR, os.path.splitext(s)[0] + ".o") for s in KERNEL_SOURCES]
+    with concurrent.futures.ThreadPoolExecutor(len(KERNEL_SOURCES)) as pool:
+        objects = list(pool.map(_compile_kernels, KERNEL_SOURCES))
     tmp = HSACO + ".tmp"
     _run([os.path.join(ROCM, "llvm", "bin", "ld.lld"), "-shared", "--no-undefined", "-o", tmp, *objects])
     os.replace(tmp, HSACO)
