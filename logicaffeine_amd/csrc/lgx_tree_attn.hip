@@ -37,9 +37,12 @@
 //     36.8 against 34.2 us, 100 nodes of 8 sequences of 1000 55 against 44; only 200 nodes
 //     of 2 sequences of 5200 gain (113 against 136), where 22 blocks read the same K and V.
 // What bounds it: few nodes, the cache's bytes (one token of 64 sequences: 4.2 TB/s of
-// the 4.7 that a copy reaches); many, the way of a tile from memory through LDS into the
-// matrix unit, which is busy 32 to 43 % of the time (without the products 53 us become
-// 35 for 100 nodes of 8 sequences); short calls, the launch and the splits' join.
+// the 4.7 that a copy reaches); many, that a wave's LDS reads, products and softmax follow
+// each other and the SIMD's other wave does not fill the gaps: of the compute units' busy
+// cycles the matrix unit is busy in 31 to 32 %, VALU instructions are under way in 42 to 48
+// % (64 nodes over 8000 tokens, 32 x 16 over up to 4096, 8 x 100 over 1000; no LDS bank
+// conflicts), and with capped scores in 16 and 57 % (9 x 201 over 1500); short calls, the
+// launch and the splits' join.
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) uint16_t lds_u16;
 typedef __attribute__((address_space(4))) const int32_t const_i32;
