@@ -115,8 +115,11 @@ extern "C" __global__ __launch_bounds__(256) void lgx_k_append_rows_d128(const l
 
 // ---------------------------------------------------------------------------
 // Trees.  parent[j] < j, or -1 where node j hangs from the sequence's last token; any
-// other value counts as -1.  A plan or a walk is a few dependent steps of one wave:
-// 2.5 us for the walk of one tree of 6 nodes, 5.0 for 32 of 24.
+// other value counts as -1.  Bound by chains of dependent steps, one for each generation.
+// The plan, an LDS read a step: 1.6 us for a chain of 6 nodes, 3.1 for 32 trees of 24, 5.5 for a
+// chain of 64, 18 for one of 256 (19.6 for 64 of them; 4.6 for a tree of 256 nodes with
+// parents among the last 12).  The walk, some VALU operations a step: 2.5 us for one tree of 6
+// nodes, 5.0 for 32 of 24.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int tree_parent(int p, int j) { return p >= 0 && p < j ? p : -1; }
 
