@@ -1,9 +1,6 @@
 """Drafts, sampling and a cache's pages together, as a server uses them: sequences of a
 small network go on by trees of drafts, share pages where one forks from another, and
 yield the tokens that they would yield one at a time."""
-import os
-import re
-
 import numpy as np
 import pytest
 import torch
@@ -284,65 +281,80 @@ def test_two_graphs_share_a_workspace_that_grows(ctx):
 
 
 @pytest.mark.parametrize("captured", [False, True])
-def test_the_documented_round_where_pages_run_out(ctx, captured):
-    """INTEGRATION.md's round as it stands there: three sequences share a partly filled page, and
-    the pool lacks a page for their drafts.  The round changes nothing, however often it
-    runs; once a page is free it goes on, each sequence in a page of its own.  Rows of
+def test_a_round_where_pages_run_out(ctx, captured):
+    """Three sequences share a partly filled page, and the pool lacks a page for their drafts: a
+    round that takes its numbers of nodes times (lacking == 0) changes nothing, however often
+    it runs; once a page is free it goes on, each sequence in a page of its own.  Rows of
     padding stay zeros."""
-    with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")) as f:
-        block = re.search(r"```python\n(layers = \[lgx\.KvCacheF16.*?)```", f.read(), re.S).group(1)
-    setup, body = block[:block.index("# tokens, parent")], compile(block[block.index("# tokens, parent"):], "round", "exec")
     S, N, pages, held, hq, hkv, d, vocab = 3, 5, 4, 21, 28, 4, 128, 64
     rng = np.random.default_rng(21)
     i32 = dict(dtype=torch.int32, device="cuda")
+    layers = [lgx.KvCacheF16.empty(ctx, pages, hkv, d) for _ in range(28)]
+    planes = lgx.PagePlanes([x for kv in layers for x in (kv.k, kv.v)])
+    pool = lgx.PagePool.empty(ctx, pages)
+    q, out = (torch.zeros(S * N, hq, d, device="cuda") for _ in range(2))
     qkv = torch.tensor(rng.standard_normal((S * N, (hq + 2 * hkv) * d)), dtype=torch.float32, device="cuda")
-    names = dict(
-        lgx=lgx, torch=torch, ctx=ctx, num_pages=pages, S=S, N=N, weights=range(28), qkv=qkv, bias=None, max_len=4 * PAGE - N,
-        rope=lgx.Rope.tables(ctx, 4 * PAGE, d), table=torch.full((S, 4), -1, **i32), seq_len=torch.zeros(S, **i32),
-        tokens=torch.zeros((S, N), **i32), parent=torch.arange(-1, N - 1, **i32).repeat(S, 1), n=torch.tensor([N, N - 2, N], **i32),
-        logits=torch.tensor(rng.standard_normal((S * N, vocab)), dtype=torch.float32, device="cuda"),
-        u=torch.full((S * N,), 0.5, device="cuda"), temperature=None, top_k=None, top_p=None, min_p=None,
-        src=torch.zeros(1, **i32), dst=torch.zeros(1, **i32))
-    exec(setup, names)
-    table, lens, ref = names["table"], names["seq_len"], names["pool"].ref
-    ref.copy_(torch.tensor([S, 0, S, 1]))         # page 3 is held elsewhere
+    logits = torch.tensor(rng.standard_normal((S * N, vocab)), dtype=torch.float32, device="cuda")
+    u, rope = torch.full((S * N,), 0.5, device="cuda"), lgx.Rope.tables(ctx, 4 * PAGE, d)
+    tokens, parent = torch.zeros((S, N), **i32), torch.arange(-1, N - 1, **i32).repeat(S, 1)
+    n, none = torch.tensor([N, N - 2, N], **i32), torch.zeros(1, **i32)
+    table, lens = torch.full((S, 4), -1, **i32), torch.full((S,), held, **i32)
     table[:, :2] = torch.tensor([2, 0])
-    lens.fill_(held)
-    for x in names["planes"].tensors:
+    pool.ref.copy_(torch.tensor([S, 0, S, 1]))    # page 3 is held elsewhere
+    for x in planes.tensors:
         x.copy_(torch.tensor(rng.standard_normal(x.shape), dtype=x.dtype))
 
+    def work():
+        copies, n_copies, lacking = ctx.pages_reserve(pool, table, lens, n)
+        live = n * (lacking == 0)
+        ctx.pages_copy(planes, copies, n_copies)
+        depth, mask = ctx.tree_plan(parent, live)
+        for kv in layers:
+            ctx.rope_kv_append_rows(qkv, None, rope, lens, table, kv, N, depth, live, q_out=q)
+            ctx.gqa_tree_attn(q, kv, table, lens, N, 4 * PAGE - N, mask, depth, live, out=out)
+        picked, _ = ctx.sample_filtered(logits, u)
+        path, count, _, new = ctx.tree_accept(tokens, parent, picked.view(S, N), lens, live)
+        ctx.kv_keep(layers, table, lens, path, count)
+        lens.copy_(new)
+        ctx.pages_free(pool, table, lens)
+        ctx.pages_fork(pool, table, lens, none, none)     # onto itself: left out
+        return lacking, count
+
     def state():
-        return [x.clone() for x in (table, lens, ref, *names["planes"].tensors)]
+        return [x.clone() for x in (table, lens, pool.ref, *planes.tensors)]
 
     before = state()
     if captured:
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
-            exec(body, names)
+            work()
         torch.cuda.current_stream().wait_stream(side)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            exec(body, names)
-    go = graph.replay if captured else lambda: exec(body, names)
+            result = work()
+
+    def go():
+        if not captured:
+            return work()
+        graph.replay()
+        return result
+
     for _ in range(3):
-        go()
-        assert int(names["lacking"]) == 1 and int(names["count"].abs().sum()) == 0
-        assert not names["q"].any() and not names["out"].any()
+        lacking, count = go()
+        assert int(lacking) == 1 and not count.any() and not q.any() and not out.any()
         for x, y in zip(before, state()):
             assert torch.equal(x, y)
-    ref[3] = 0
-    go()
-    assert int(names["lacking"]) == 0
+    pool.ref[3] = 0
+    lacking, count = go()
+    assert int(lacking) == 0
     rows = table[:, 1].cpu().numpy()
-    assert sorted(rows) == [0, 1, 3] and (table[:, 0] == 2).all() and ref.tolist() == [1, 1, S, 1]
-    count = names["count"]
+    assert sorted(rows) == [0, 1, 3] and (table[:, 0] == 2).all() and pool.ref.tolist() == [1, 1, S, 1]
     assert (count >= 1).all() and torch.equal(lens, held + count)
     v = qkv.view(S, N, hq + 2 * hkv, d)[:, 0, hq + hkv:].half()
-    for kv, old in zip(names["layers"], before[3:][1::2]):
+    for kv, old in zip(layers, before[3:][1::2]):
         for s in range(S):
             at = held % PAGE                      # what the page held, then node 0's row
             assert torch.equal(kv.v[rows[s], :, :at], old[0, :, :at]) and torch.equal(kv.v[rows[s], :, at], v[s])
-    for x in (names["q"], names["out"]):
-        used = x.view(S, N, -1).any(-1).tolist()
-        assert used == [[True] * N, [True] * (N - 2) + [False] * 2, [True] * N]
+    for x in (q, out):
+        assert x.view(S, N, -1).any(-1).tolist() == [[True] * N, [True] * (N - 2) + [False] * 2, [True] * N]
